@@ -1432,7 +1432,7 @@ FIE_DEV void finish_row(FinSmem& S, const KParams& P, const int row)
     float rep = 1.0f, pres = 0.0f, freq = 0.0f;
     if (pen) { rep = a.repetition[row]; pres = a.presence[row]; freq = a.frequency[row]; }
     // the row's draw: on-device counter-based, or the caller's
-    const double urow = greedy ? 0.0 : (a.rng ? philox_uniform(a.rng + 3 * (size_t)row) : a.uniform[row]);
+    const double urow = greedy ? 0.0 : row_uniform(a, row, fl);
     int32_t status = 0;
     if (pen && P.w.bad[row] && !a.hist_invalid) status |= FIE_ROW_UNCOUNTED_IDS;
 
@@ -1831,7 +1831,7 @@ FIE_DEV RowSet row_settings(const KParams& P, int row)
         r.pen = fl & FIE_FLAG_PENALTY;
         if (r.pen) { r.rep = rep; r.pres = pres; r.freq = freq; }
     }
-    r.u = a.rng ? philox_uniform(a.rng + 3 * (size_t)row) : a.uniform[row];
+    r.u = row_uniform(a, row, fl);
     if (fl & FIE_FLAG_GREEDY) { r.s = 1.0f; r.tp = 1.0f; r.mp = 0.0f; r.topk = 0; }
     return r;
 }
@@ -1867,13 +1867,14 @@ FIE_DEV void window_row(FinSmem& S, const KParams& P, int row, const bool hd)
     asm("" : "+s"(row));        // not finish_row's row, for the optimizer
     const fie_sampler_args& a = P.a;
     RowSet r;                   // never a greedy row: what the windows need, and no more
-    r.pen = a.apply_penalties && (a.flags[row] & FIE_FLAG_PENALTY);
+    const int32_t fl = a.flags[row];
+    r.pen = a.apply_penalties && (fl & FIE_FLAG_PENALTY);
     r.s = a.scale[row];
     r.tp = a.top_p[row];
     r.rep = 1.0f;
     r.pres = r.freq = 0.0f;
     if (r.pen) { r.rep = a.repetition[row]; r.pres = a.presence[row]; r.freq = a.frequency[row]; }
-    r.u = a.rng ? philox_uniform(a.rng + 3 * (size_t)row) : a.uniform[row];
+    r.u = row_uniform(a, row, fl);
     const u128 sall = S.dfr.sall;
     const float M = S.dfr.M;
     const uint32_t k0 = S.dfr.k0;

@@ -205,7 +205,7 @@ __global__ void k_cexp(const float* in, float* out, int64_t n)
 // ---------------------------------------------------------------- host side
 static thread_local char g_err[512];
 
-static int fail(int code, const char* msg)
+int fail(int code, const char* msg)
 {
     snprintf(g_err, sizeof g_err, "%s", msg);
     return code;
@@ -327,7 +327,7 @@ static int check_args(const fie_sampler_args* a)
         }                                                                               \
     } while (0)
 
-static int launch_status(hipError_t e, const char* what)
+int launch_status(hipError_t e, const char* what)
 {
     if (e == hipSuccess) return FIE_OK;
     snprintf(g_err, sizeof g_err, "%s: %s", what, hipGetErrorString(e));
@@ -336,7 +336,7 @@ static int launch_status(hipError_t e, const char* what)
 
 // Compute units of the current device (queried once per device; 0 when unknown,
 // which selects the narrow k_finish).
-static int cu_count()
+int cu_count()
 {
     static int cus[64];
     int dev = 0;
@@ -491,6 +491,29 @@ int fie_sampler_lmhead_stage(const fie_sampler_args* args, const void* hidden, c
                              int32_t hidden_dim, const fie_workspace* ws, void* stream)
 {
     return lmhead_run(args, hidden, weight, hidden_dim, ws, stream, false);
+}
+
+int fie_sampler_verify(const fie_sampler_args* args, const fie_verify_args* v, const fie_workspace* ws, void* stream)
+{
+    if (!args || !v) return fail(FIE_E_ARG, "args is NULL");
+    if (v->requests < 0 || v->max_drafts < 0 || v->max_drafts > FIE_MAX_DRAFTS)
+        return fail(FIE_E_ARG, "requests or max_drafts out of range");
+    if (args->rows < v->requests || (int64_t)args->rows > (int64_t)v->requests * (1 + v->max_drafts))
+        return fail(FIE_E_ARG, "rows do not fit the requests and their drafts");
+    if (args->rows > v->requests) {
+        if (!v->draft_ids) return fail(FIE_E_ARG, "draft_ids is NULL");
+        if (v->draft_probs && (v->draft_dtype < FIE_F32 || v->draft_dtype > FIE_BF16))
+            return fail(FIE_E_ARG, "unknown draft dtype");
+        if (v->draft_probs && v->draft_stride < args->vocab) return fail(FIE_E_ARG, "draft_stride < vocab");
+    }
+    if (v->requests > 0 && (!v->draft_offsets || !v->tokens || !v->accepted))
+        return fail(FIE_E_ARG, "a required pointer is NULL");
+    KParams P;
+    int rc = prepare(args, ws, &P);
+    if (rc != FIE_OK || args->rows == 0) return rc;
+    rc = fie_sampler_sample(args, ws, stream);
+    if (rc != FIE_OK) return rc;
+    return launch_status(launch_verify(P, *v, (hipStream_t)stream), "k_verify");
 }
 
 int fie_sampler_stage(const fie_sampler_args* args, const fie_workspace* ws, int32_t stage, void* stream)

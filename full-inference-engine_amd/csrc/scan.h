@@ -174,6 +174,13 @@ FIE_DEV int64_t hist_end(const fie_sampler_args& a, int row)
     return a.hist_ends ? a.hist_ends[row] : a.hist_offsets[row + 1];
 }
 
+// The row's draw: the caller's, or counter-based on the device; 0 where none is wanted.
+FIE_DEV double row_uniform(const fie_sampler_args& a, int row, int32_t flags)
+{
+    if (flags & FIE_FLAG_NO_DRAW) return 0.0;
+    return a.rng ? philox_uniform(a.rng + 3 * (size_t)row) : a.uniform[row];
+}
+
 // Token idx of a row, as fp32.
 template <int DT>
 FIE_DEV float load_elem(const char* rowp, uint32_t idx)

@@ -15,13 +15,14 @@ LIB_PATH = os.path.join(_HERE, "_native", "libfie_sampler.so")
 FIE_OK = 0
 FIE_E_ARG, FIE_E_WORKSPACE, FIE_E_LAUNCH = -1, -2, -3
 FIE_F32, FIE_F16, FIE_BF16 = 0, 1, 2
-FIE_FLAG_GREEDY, FIE_FLAG_PENALTY = 1, 2
+FIE_FLAG_GREEDY, FIE_FLAG_PENALTY, FIE_FLAG_NO_DRAW = 1, 2, 4
 FIE_ROW_EXACT_PATH = 1
 FIE_ROW_UNCOUNTED_IDS = 2
 FIE_STAGE_PREP, FIE_STAGE_SCAN, FIE_STAGE_FINISH, FIE_STAGE_DEEP = 0, 1, 2, 3
 LP_COLS = 20
 TILE = 8192
 MAX_VOCAB = 64 * TILE
+MAX_DRAFTS = 255
 
 _vp = ctypes.c_void_p
 
@@ -43,6 +44,16 @@ class SamplerArgs(ctypes.Structure):
     ]
 
 
+class VerifyArgs(ctypes.Structure):
+    """Mirror of ``fie_verify_args``."""
+
+    _fields_ = [
+        ("requests", ctypes.c_int32), ("max_drafts", ctypes.c_int32), ("draft_offsets", _vp), ("draft_ids", _vp),
+        ("draft_probs", _vp), ("draft_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("draft_stride", ctypes.c_int64), ("tokens", _vp), ("accepted", _vp), ("target_probs", _vp),
+    ]
+
+
 class Workspace(ctypes.Structure):
     """Mirror of ``fie_workspace``."""
 
@@ -55,7 +66,7 @@ EXPORTS = (
     "fie_sampler_workspace_size", "fie_sampler_sample", "fie_sampler_stage",
     "fie_sampler_argmax", "fie_sampler_kept", "fie_sampler_cexp", "fie_sampler_last_error",
     "fie_sampler_sample_noalloc", "fie_sampler_uniforms", "fie_sampler_history_write",
-    "fie_sampler_lmhead_sample", "fie_sampler_lmhead_stage",
+    "fie_sampler_lmhead_sample", "fie_sampler_lmhead_stage", "fie_sampler_verify",
 )
 SCRATCH_BYTES = 64 << 20
 
@@ -100,6 +111,8 @@ def bind(lib) -> None:
     lib.fie_sampler_history_write.argtypes = [_vp, _vp, _vp, ctypes.c_int64, _vp]
     for name in ("fie_sampler_lmhead_sample", "fie_sampler_lmhead_stage"):
         getattr(lib, name).argtypes = [ctypes.POINTER(SamplerArgs), _vp, _vp, ctypes.c_int32,
+                                       ctypes.POINTER(Workspace), _vp]
+    lib.fie_sampler_verify.argtypes = [ctypes.POINTER(SamplerArgs), ctypes.POINTER(VerifyArgs),
                                        ctypes.POINTER(Workspace), _vp]
     lib.fie_sampler_last_error.restype = ctypes.c_char_p
     for name in EXPORTS:

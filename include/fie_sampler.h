@@ -46,6 +46,9 @@ enum { FIE_F32 = 0, FIE_F16 = 1, FIE_BF16 = 2 };
 enum {
     FIE_FLAG_GREEDY = 1,    /* SamplingParams.greedy (sampling.py:71-74) */
     FIE_FLAG_PENALTY = 2,   /* SamplingParams.has_penalties (sampling.py:76-79) */
+    FIE_FLAG_NO_DRAW = 4,   /* the row's draw is not wanted: its token is its most likely one (a
+                               draw of 0), its thresholds and masses are what they are.  For rows
+                               that fie_sampler_verify tests a draft on */
 };
 
 /* Per-row status bits written to fie_sampler_args.status (informational). */
@@ -195,6 +198,44 @@ int fie_sampler_argmax(const void* logits, int32_t dtype, int32_t rows, int32_t 
    NULL. */
 int fie_sampler_kept(const fie_sampler_args* args, uint8_t* kept, float* probs,
                      const fie_workspace* ws, void* stream);
+
+/* Verification of drafted tokens.  The reference accepts drafts of greedy requests only
+   (engine/speculative/acceptance.py); here a draft is tested against the distribution that
+   fie_sampler_sample draws from, so that what comes out is distributed as if every token had
+   been sampled one by one.
+
+   Request r has k_r = draft_offsets[r + 1] - draft_offsets[r] drafts d_0 .. d_{k-1} and
+   k_r + 1 rows of logits, one after another from row draft_offsets[r] + r on: row j is the
+   model's answer after j drafts.  The sampler's args describe these rows (its rows = drafts
+   + requests), with FIE_FLAG_NO_DRAW on every row but a request's last, and one draw u a row.
+   With p the row's kept distribution (weights over kept mass, fp32) and q the draft's (all
+   on d_j without draft_probs):
+     d_j is kept iff u_j * q(d_j) < p(d_j), a product in double, and every draft before it was
+     a refusal at n gives the first token whose sum of floor(max(p - q, 0) * 2^48), in token
+       order, exceeds floor(u * total), u the request's last draw (the row's most likely token
+       where p has nothing over q)
+     no refusal gives the last row's own token
+   A q below 0 or NaN counts as 0; a draft id outside the vocabulary is refused.  A request
+   whose offsets do not fit (below 0, more than max_drafts, past the rows) gets accepted = -1
+   and no tokens. */
+typedef struct fie_verify_args {
+    int32_t requests;
+    int32_t max_drafts;            /* the most drafts of one request, 0..FIE_MAX_DRAFTS */
+    const int64_t* draft_offsets;  /* [requests + 1], from 0 to the number of drafts */
+    const int64_t* draft_ids;      /* [drafts] (NULL without drafts) */
+    const void* draft_probs;       /* [drafts, vocab], rows draft_stride elements apart, or NULL */
+    int32_t draft_dtype;           /* FIE_F32 / FIE_F16 / FIE_BF16 */
+    int32_t reserved;
+    int64_t draft_stride;
+    int64_t* tokens;               /* [requests, max_drafts + 1]: kept drafts, one more token, -1 */
+    int32_t* accepted;             /* [requests] kept drafts */
+    float* target_probs;           /* [drafts] p(d_j), or NULL */
+} fie_verify_args;
+#define FIE_MAX_DRAFTS 255
+
+/* fie_sampler_sample on the rows, then the verification, on one stream. */
+int fie_sampler_verify(const fie_sampler_args* args, const fie_verify_args* verify,
+                       const fie_workspace* ws, void* stream);
 
 /* The build's canonical fp32 exponential on n device values (verification aid). */
 int fie_sampler_cexp(const float* in, float* out, int64_t n, void* stream);
