@@ -1,0 +1,69 @@
+// Block norms behind the C ABI of include/fie_ops.h: instantiations of norm.h's kernel and
+// the choice among them.
+#include "norm.h"
+
+namespace fie {
+
+template <int DX, int DR>
+static hipError_t norm_of(const fie_norm_args& a, hipStream_t st)
+{
+    const int vecs = (a.width + 7) / 8;
+    if (vecs <= 64) {
+        k_norm<DX, DR, 1, true><<<(unsigned)((a.tokens + 3) / 4), 256, 0, st>>>(a);
+        return hipGetLastError();
+    }
+    const int vpt = vecs <= 256 ? 1 : vecs <= 1024 ? 2 : vecs <= 2048 ? 4 : 8;
+    const int threads = ((vecs + vpt - 1) / vpt + 63) / 64 * 64;
+    const unsigned grid = (unsigned)a.tokens;
+    switch (vpt) {
+    case 1: k_norm<DX, DR, 1, false><<<grid, threads, 0, st>>>(a); break;
+    case 2: k_norm<DX, DR, 2, false><<<grid, threads, 0, st>>>(a); break;
+    case 4: k_norm<DX, DR, 4, false><<<grid, threads, 0, st>>>(a); break;
+    default: k_norm<DX, DR, 8, false><<<grid, threads, 0, st>>>(a); break;
+    }
+    return hipGetLastError();
+}
+
+static int norm_check(const fie_norm_args* a)
+{
+    if (!a) return fail(FIE_E_ARG, "args is NULL");
+    if (a->tokens < 0 || a->tokens > 0x7FFFFFFF) return fail(FIE_E_ARG, "tokens out of range");
+    if (a->width < 1 || a->width > FIE_MAX_WIDTH) return fail(FIE_E_ARG, "width out of range [1, 65536]");
+    if (a->x_dtype < FIE_F32 || a->x_dtype > FIE_BF16 || a->residual_dtype < FIE_F32 || a->residual_dtype > FIE_BF16)
+        return fail(FIE_E_ARG, "unknown dtype");
+    if (a->x && a->residual_dtype != a->x_dtype && a->residual_dtype != FIE_F32)
+        return fail(FIE_E_ARG, "residual is in x's type or fp32");
+    if (a->y && a->y_dtype != a->x_dtype && a->y_dtype != FIE_I8) return fail(FIE_E_ARG, "y is in x's type or int8");
+    if (a->kind < FIE_NORM_RMS || a->kind > FIE_NORM_NONE) return fail(FIE_E_ARG, "unknown kind of norm");
+    if (a->post_norm && (a->kind == FIE_NORM_NONE || !a->x)) return fail(FIE_E_ARG, "post_norm needs x and a kind of norm");
+    if (a->gate && (!a->x || (a->gate_step != 0 && a->gate_step != 1))) return fail(FIE_E_ARG, "a gate needs x and a step of 0 or 1");
+    if (a->tokens == 0) return FIE_OK;
+    if (!a->residual) return fail(FIE_E_ARG, "residual is NULL");
+    if (a->y && a->y_dtype == FIE_I8 && !a->y_scale) return fail(FIE_E_ARG, "int8 output without y_scale");
+    if (!a->y && !a->residual_out) return fail(FIE_E_ARG, "no output");
+    return FIE_OK;
+}
+
+}  // namespace fie
+
+using namespace fie;
+
+extern "C" int fie_block_norm(const fie_norm_args* a, void* stream)
+{
+    const int rc = norm_check(a);
+    if (rc != FIE_OK || a->tokens == 0) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    hipError_t e;
+    switch (a->x_dtype * 3 + a->residual_dtype) {
+    case FIE_F32 * 3 + FIE_F32: e = norm_of<FIE_F32, FIE_F32>(*a, st); break;
+    case FIE_F32 * 3 + FIE_F16: e = norm_of<FIE_F32, FIE_F16>(*a, st); break;
+    case FIE_F32 * 3 + FIE_BF16: e = norm_of<FIE_F32, FIE_BF16>(*a, st); break;
+    case FIE_F16 * 3 + FIE_F32: e = norm_of<FIE_F16, FIE_F32>(*a, st); break;
+    case FIE_F16 * 3 + FIE_F16: e = norm_of<FIE_F16, FIE_F16>(*a, st); break;
+    case FIE_F16 * 3 + FIE_BF16: e = norm_of<FIE_F16, FIE_BF16>(*a, st); break;
+    case FIE_BF16 * 3 + FIE_F32: e = norm_of<FIE_BF16, FIE_F32>(*a, st); break;
+    case FIE_BF16 * 3 + FIE_F16: e = norm_of<FIE_BF16, FIE_F16>(*a, st); break;
+    default: e = norm_of<FIE_BF16, FIE_BF16>(*a, st); break;
+    }
+    return launch_status(e, "k_norm");
+}

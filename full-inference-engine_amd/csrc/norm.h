@@ -1,0 +1,277 @@
+// Block norms (fie_block_norm): the end of one block and the norm in front of the next.
+//
+// A row is held in registers, 8 neighbouring elements a vector, from its loads to its
+// stores; each norm costs one reduction over the row's threads (a layer norm two, its
+// squares taken about the mean).  Bound by HBM: x, residual and gate read once, residual
+// and y written once.
+#pragma once
+
+#include "launchers.h"
+#include "fie_ops.h"
+
+namespace fie {
+
+// 8 elements from e0 on, as loaded; those at or past `width` are 0.
+template <int DT> struct Vec8 { uint4 r[DT == FIE_F32 ? 2 : 1]; };
+
+template <int DT>
+FIE_DEV Vec8<DT> load8(const char* rowp, int e0, int width)
+{
+    Vec8<DT> v;
+    v.r[0] = load_group<DT>(rowp, e0, width);
+    if constexpr (DT == FIE_F32) v.r[1] = load_group<DT>(rowp, e0 + 4, width);
+    return v;
+}
+
+template <int DT>
+FIE_DEV float get8(const Vec8<DT>& v, int e)
+{
+    if constexpr (DT == FIE_F32) return lane_get<DT>(v.r[e >> 2], e & 3);
+    else return lane_get<DT>(v.r[0], e);
+}
+
+// A parameter vector: in DT, or in fp32.
+template <int DT>
+FIE_DEV void load_param(float (&w)[8], const void* p, bool f32, int e0, int width)
+{
+    if (DT == FIE_F32 || f32) {
+        const Vec8<FIE_F32> v = load8<FIE_F32>((const char*)p, e0, width);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = get8<FIE_F32>(v, e);
+    } else {
+        const Vec8<DT> v = load8<DT>((const char*)p, e0, width);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = get8<DT>(v, e);
+    }
+}
+
+// fp32 to 16 bits, round to nearest even (NaN stays NaN).
+template <int DT>
+FIE_DEV uint32_t half_bits(float v)
+{
+    if constexpr (DT == FIE_BF16) {
+        const __bf16 h = (__bf16)v;
+        return __builtin_bit_cast(uint16_t, h);
+    } else {
+        const _Float16 h = (_Float16)v;
+        return __builtin_bit_cast(uint16_t, h);
+    }
+}
+
+template <int DT>
+FIE_DEV void store8(char* rowp, int e0, int width, const float (&v)[8])
+{
+    typedef typename Raw16<DTy<DT>::SZ>::T raw;
+    if constexpr (DT == FIE_F32) {
+        float* p = (float*)rowp + e0;
+        if (e0 + 8 <= width) {
+            *(raw*)p = raw{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+            *(raw*)(p + 4) = raw{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e0 + e < width) p[e] = v[e];
+        }
+    } else {
+        uint16_t* p = (uint16_t*)rowp + e0;
+        uint32_t h[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = half_bits<DT>(v[e]);
+        if (e0 + 8 <= width) {
+            *(raw*)p = raw{h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e0 + e < width) p[e] = (uint16_t)h[e];
+        }
+    }
+}
+
+FIE_DEV void store8_i8(char* rowp, int e0, int width, const float (&v)[8])
+{
+    typedef uint32_t raw __attribute__((ext_vector_type(2), aligned(1)));
+    uint32_t b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = (uint32_t)(int32_t)v[e] & 0xFFu;
+    if (e0 + 8 <= width) {
+        *(raw*)(rowp + e0) = raw{b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24), b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24)};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e0 + e < width) rowp[e0 + e] = (char)b[e];
+    }
+}
+
+FIE_DEV float dwave_sum_f32(float x)
+{
+    auto step = [](float v, auto mv) { return v + __uint_as_float(mv(__float_as_uint(v))); };
+    x = step(x, [](uint32_t a) { return dpp_mov<kDppXor1>(a); });
+    x = step(x, [](uint32_t a) { return dpp_mov<kDppXor2>(a); });
+    x = step(x, [](uint32_t a) { return dpp_mov<kDppHalfMirror>(a); });
+    x = step(x, [](uint32_t a) { return dpp_mov<kDppMirror>(a); });
+    const uint32_t b = __float_as_uint(x);
+    return (__uint_as_float(rl(b, 0)) + __uint_as_float(rl(b, 16))) + (__uint_as_float(rl(b, 32)) + __uint_as_float(rl(b, 48)));
+}
+
+// Over a row's threads: a wave's (ONE), or the workgroup's.  `slot` is a scratch area that
+// no other reduction of the row uses, so one barrier is enough.
+template <bool ONE>
+FIE_DEV float row_sum(float x, float* slot)
+{
+    x = dwave_sum_f32(x);
+    if (ONE) return x;
+    const int waves = blockDim.x >> 6;
+    if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = x;
+    __syncthreads();
+    float t = 0.0f;
+    for (int w = 0; w < waves; ++w) t += slot[w];
+    return t;
+}
+
+template <bool ONE>
+FIE_DEV float row_max(float x, float* slot)     // of values >= 0: their bits order them
+{
+    x = __uint_as_float(dwave_max_u32(__float_as_uint(x)));
+    if (ONE) return x;
+    const int waves = blockDim.x >> 6;
+    if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = x;
+    __syncthreads();
+    float t = 0.0f;
+    for (int w = 0; w < waves; ++w) t = slot[w] > t ? slot[w] : t;
+    return t;
+}
+
+// DX: x and y; DR: residual.  A row's thread t holds vectors t, t + T, ..: VPT of them, 0 past
+// the row's end (parameters load as 0 there).
+// ONE: a wave a row, four rows a workgroup.
+template <int DX, int DR, int VPT, bool ONE>
+__global__ __launch_bounds__(ONE ? 256 : (VPT > 4 ? 1024 : 512)) void k_norm(const fie_norm_args a)
+{
+    __shared__ float red[5][16];
+    const int T = ONE ? 64 : blockDim.x;
+    const int t = ONE ? threadIdx.x & 63 : threadIdx.x;
+    const int64_t row = ONE ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
+    if (ONE && row >= a.tokens) return;
+    const int H = a.width;
+    const float inv = 1.0f / (float)H;
+    constexpr int SX = DTy<DX>::SZ, SR = DTy<DR>::SZ;
+    const char* xp = (const char*)a.x + row * a.x_stride * SX;
+    const char* rp = (const char*)a.residual + row * a.residual_stride * SR;
+    const char* gp = (const char*)a.gate + row * a.gate_stride * (a.gate_f32 ? 4 : SX);
+
+    float v[VPT][8];
+    Vec8<DR> res[VPT];
+    Vec8<DX> xs[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int e0 = (i * T + t) * 8;
+        res[i] = load8<DR>(rp, e0, H);
+        if (a.x) xs[i] = load8<DX>(xp, e0, H);
+    }
+    // (v - mean) / sqrt(mean((v - mean)^2) + eps) * weight + bias, in place
+    auto norm = [&](const void* weight, const void* bias, int slot) {
+        if (a.kind == FIE_NORM_LAYER) {
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s += v[i][e];
+            const float mean = row_sum<ONE>(s, red[slot]) * inv;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    v[i][e] = (i * T + t) * 8 + e < H ? v[i][e] - mean : 0.0f;
+        }
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += v[i][e] * v[i][e];
+        const float rstd = 1.0f / __builtin_sqrtf(row_sum<ONE>(s, red[slot + 1]) * inv + a.eps);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int e0 = (i * T + t) * 8;
+            float w[8], b[8];
+            if (weight) {
+                load_param<DX>(w, weight, a.weight_f32, e0, H);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] += a.weight_offset;
+            }
+            if (bias) load_param<DX>(b, bias, a.weight_f32, e0, H);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[i][e] *= rstd;
+                if (weight) v[i][e] *= w[e];
+                if (bias) v[i][e] += b[e];
+            }
+        }
+    };
+    if (a.x) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = get8<DX>(xs[i], e);
+        if (a.post_norm) norm(a.post_weight, a.post_bias, 0);
+        if (a.gate) {
+            if (a.gate_step) {
+#pragma unroll
+                for (int i = 0; i < VPT; ++i) {
+                    float g[8];
+                    load_param<DX>(g, gp, a.gate_f32, (i * T + t) * 8, H);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[i][e] *= g[e];
+                }
+            } else {
+                const float g = DX == FIE_F32 || a.gate_f32 ? *(const float*)gp : load_elem<DX>(gp, 0);
+#pragma unroll
+                for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[i][e] *= g;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = get8<DR>(res[i], e) + a.scale * v[i][e];
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = get8<DR>(res[i], e);
+    }
+    if (a.residual_out) {
+        char* op = (char*)a.residual_out + row * a.residual_out_stride * SR;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) store8<DR>(op, (i * T + t) * 8, H, v[i]);
+    }
+    if (!a.y) return;
+    if (a.kind != FIE_NORM_NONE) norm(a.weight, a.bias, 2);
+    if (a.y_dtype != FIE_I8) {
+        char* yp = (char*)a.y + row * a.y_stride * SX;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) store8<DX>(yp, (i * T + t) * 8, H, v[i]);
+        return;
+    }
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = __builtin_fmaxf(m, __builtin_fabsf(v[i][e]));
+    // IEEE quotients: what a plain x / (max|x| / 127) rounds to
+    const float s = row_max<ONE>(m, red[4]) / 127.0f;
+    if (t == 0) a.y_scale[row] = s;
+    char* yp = (char*)a.y + row * a.y_stride;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        float q[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float u = __builtin_rintf(v[i][e] / s);
+            q[e] = u >= -127.0f && u <= 127.0f ? u : 0.0f;       // 0 / 0 and NaN: 0
+        }
+        store8_i8(yp, (i * T + t) * 8, H, q);
+    }
+}
+
+}  // namespace fie

@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/fie_sampler.h.
+"""ctypes binding of the C ABI in include/fie_sampler.h and include/fie_ops.h.
 
 The shared library is built in-tree by ``fie_amd.build`` into ``fie_amd/_native``.
 There is no fallback: if the library cannot be loaded, every entry point raises.
@@ -6,6 +6,7 @@ There is no fallback: if the library cannot be loaded, every entry point raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -14,7 +15,7 @@ LIB_PATH = os.path.join(_HERE, "_native", "libfie_sampler.so")
 
 FIE_OK = 0
 FIE_E_ARG, FIE_E_WORKSPACE, FIE_E_LAUNCH = -1, -2, -3
-FIE_F32, FIE_F16, FIE_BF16 = 0, 1, 2
+FIE_F32, FIE_F16, FIE_BF16, FIE_I8 = 0, 1, 2, 3
 FIE_FLAG_GREEDY, FIE_FLAG_PENALTY, FIE_FLAG_NO_DRAW = 1, 2, 4
 FIE_ROW_EXACT_PATH = 1
 FIE_ROW_UNCOUNTED_IDS = 2
@@ -54,6 +55,32 @@ class VerifyArgs(ctypes.Structure):
     ]
 
 
+class NormArgs(ctypes.Structure):
+    """Mirror of ``fie_norm_args``."""
+
+    _fields_ = [
+        ("x", _vp), ("residual", _vp), ("residual_out", _vp), ("y", _vp), ("y_scale", _vp),
+        ("weight", _vp), ("bias", _vp), ("post_weight", _vp), ("post_bias", _vp), ("gate", _vp),
+        ("tokens", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("residual_stride", ctypes.c_int64),
+        ("residual_out_stride", ctypes.c_int64), ("y_stride", ctypes.c_int64), ("gate_stride", ctypes.c_int64),
+        ("gate_step", ctypes.c_int32), ("width", ctypes.c_int32), ("x_dtype", ctypes.c_int32),
+        ("residual_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32), ("weight_f32", ctypes.c_int32),
+        ("gate_f32", ctypes.c_int32), ("kind", ctypes.c_int32), ("post_norm", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float),
+    ]
+
+
+class Int8Args(ctypes.Structure):
+    """Mirror of ``fie_int8_args``."""
+
+    _fields_ = [
+        ("x", _vp), ("w", _vp), ("x_scale", _vp), ("w_scale", _vp), ("bias", _vp), ("y", _vp),
+        ("m", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("w_stride", ctypes.c_int64),
+        ("y_stride", ctypes.c_int64), ("n", ctypes.c_int32), ("k", ctypes.c_int32),
+        ("y_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
 class Workspace(ctypes.Structure):
     """Mirror of ``fie_workspace``."""
 
@@ -68,6 +95,8 @@ EXPORTS = (
     "fie_sampler_sample_noalloc", "fie_sampler_uniforms", "fie_sampler_history_write",
     "fie_sampler_lmhead_sample", "fie_sampler_lmhead_stage", "fie_sampler_verify",
 )
+# Every symbol include/fie_ops.h declares.
+OPS_EXPORTS = ("fie_block_norm", "fie_int8_linear")
 SCRATCH_BYTES = 64 << 20
 
 _lib = None
@@ -115,9 +144,20 @@ def bind(lib) -> None:
     lib.fie_sampler_verify.argtypes = [ctypes.POINTER(SamplerArgs), ctypes.POINTER(VerifyArgs),
                                        ctypes.POINTER(Workspace), _vp]
     lib.fie_sampler_last_error.restype = ctypes.c_char_p
-    for name in EXPORTS:
+    lib.fie_block_norm.argtypes = [ctypes.POINTER(NormArgs), _vp]
+    lib.fie_int8_linear.argtypes = [ctypes.POINTER(Int8Args), _vp]
+    for name in EXPORTS + OPS_EXPORTS:
         if name not in ("fie_sampler_workspace_size", "fie_sampler_last_error"):
             getattr(lib, name).restype = ctypes.c_int
+
+
+def on_device(device):
+    """The context in which launches go to ``device``: nothing to do where it is current."""
+    import torch
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def check(rc: int, what: str) -> None:

@@ -1,7 +1,7 @@
 """Builds the HIP sampler library in-tree for gfx950 (no JIT cache, no pip install).
 
 The kernels live in several translation units (the C ABI and small kernels in
-sampler.hip; k_scan, k_finish per dtype, k_lmhead and k_verify in their own files), compiled
+sampler.hip; k_scan, k_finish per dtype, k_lmhead, k_verify, k_norm and k_int8 in their own files), compiled
 to objects in parallel and linked into one shared library."""
 
 from __future__ import annotations
@@ -19,7 +19,7 @@ OUT = os.path.join(_HERE, "_native", "libfie_sampler.so")
 OBJ_DIR = os.path.join(_HERE, "_native", "obj")
 
 SOURCES = ("sampler.hip", "k_scan.hip", "k_finish_f32.hip", "k_finish_f16.hip", "k_finish_bf16.hip",
-           "k_lmhead.hip", "k_verify.hip")
+           "k_lmhead.hip", "k_verify.hip", "k_norm.hip", "k_int8.hip")
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
