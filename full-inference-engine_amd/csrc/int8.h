@@ -2,6 +2,8 @@
 // (fie_int8_linear): y = x_scale w_scale sum_k x w + bias.
 #pragma once
 
+#include <type_traits>
+
 #include "launchers.h"
 #include "fie_ops.h"
 
@@ -59,86 +61,285 @@ constexpr int kI8K = 128;               // bytes of k a stage
 // cycle serves read eight rows' chunk c from eight distinct bank groups.
 FIE_DEV int i8_slot(int n, int c) { return n * 8 + (c ^ (n & 7)); }
 
-// 16 bytes of a row from k0 on; those at or past K are 0.
-FIE_DEV i32x4_t load_k(const int8_t* rowp, int k0, int K)
+// 16 bytes at any address: a load of the 16 from the word that holds the first, one of the word
+// after them, and a shift.  (One load at the byte's own address takes 3 times as long: 16 x
+// 50001 at k 4097 151 us.)  Only words that hold some of the 16 bytes are touched.
+FIE_DEV i32x4_t load_any(const int8_t* p)
 {
-    typedef int32_t raw __attribute__((ext_vector_type(4), aligned(1)));
-    if (k0 + 16 <= K) {
-        const raw r = *(const raw*)(rowp + k0);
-        return i32x4_t{r.x, r.y, r.z, r.w};
-    }
-    i32x4_t r{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (k0 + i < K) r[i / 4] |= (int32_t)((uint32_t)(uint8_t)rowp[k0 + i] << (8 * (i % 4)));
-    return r;
+    typedef uint32_t raw __attribute__((ext_vector_type(4), aligned(4)));
+    const uint32_t sh = (uint32_t)(uintptr_t)p & 3u;
+    const int8_t* b = p - sh;
+    const raw r = *(const raw*)b;
+    const uint32_t e = *(const uint32_t*)(b + (sh ? 16 : 12));
+    return i32x4_t{(int32_t)__builtin_amdgcn_alignbyte(r.y, r.x, sh), (int32_t)__builtin_amdgcn_alignbyte(r.z, r.y, sh),
+                   (int32_t)__builtin_amdgcn_alignbyte(r.w, r.z, sh), (int32_t)__builtin_amdgcn_alignbyte(e, r.w, sh)};
 }
 
-// 64 WM tokens by 64 WN channels a workgroup of WM x WN waves, 64 x 64 each; k in stages of
-// 128 through two LDS buffers, the next stage in registers meanwhile.  Grid: 8 * ceil(tiles /
-// 8) * nrb, dealt to the XCDs so that a channel tile's token blocks follow one another on one.
-template <int DT, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_int8_tile(const fie_int8_args a, int nrb, int wide)
+// 16 bytes of a row from k0 on; those at or past K are 0.  Where the row ends inside them, its
+// last 16 bytes are loaded and shifted down.
+FIE_DEV i32x4_t load_k(const int8_t* rowp, int k0, int K)
 {
-    constexpr int BM = 64 * WM, BN = 64 * WN, TH = 64 * WM * WN;
-    constexpr int NC = (BM + BN) * (kI8K / 16) / TH;            // 16-byte chunks per thread and stage
-    __shared__ i32x4_t L[2][(BM + BN) * (kI8K / 16)];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int xcd = blockIdx.x & 7, kb = blockIdx.x >> 3;
-    const int t0 = (8 * (kb / nrb) + xcd) * BN;
-    const int64_t r0 = (int64_t)(kb % nrb) * BM;
-    if (t0 >= a.n) return;
-    const int8_t* src[NC];
-    int dst[NC], off[NC];
+    if (k0 >= K) return i32x4_t{0, 0, 0, 0};
+    if (K < 16) {                               // shorter than one load
+        i32x4_t r{0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-        const int p = j * TH + tid, n = p >> 3, c = p & 7;
-        src[j] = n < BM ? a.x + min(r0 + n, a.m - 1) * a.x_stride : a.w + (int64_t)min(t0 + n - BM, a.n - 1) * a.w_stride;
-        off[j] = 16 * c;
-        dst[j] = i8_slot(n, c);
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t b = (uint8_t)rowp[min(k0 + i, K - 1)];
+            r[i / 4] |= (int32_t)((k0 + i < K ? b : 0u) << (8 * (i % 4)));
+        }
+        return r;
     }
-    const int ns = (a.k + kI8K - 1) / kI8K;
-    i32x4_t r[NC];
-    auto load = [&](int s) {
+    const int past = max(k0 + 16 - K, 0);
+    const i32x4_t r = load_any(rowp + k0 - past);
+    const u128 v = ((u128)(uint32_t)r.w << 96) | ((u128)(uint32_t)r.z << 64) | ((u128)(uint32_t)r.y << 32) | (uint32_t)r.x;
+    const u128 t = v >> (8 * past);
+    return i32x4_t{(int32_t)(uint32_t)t, (int32_t)(uint32_t)(t >> 32), (int32_t)(uint32_t)(t >> 64), (int32_t)(uint32_t)(t >> 96)};
+}
+
+// Rows at any address into rows of whole stages at aligned ones, 0 past k: what the pipe kernel
+// needs.  A wave a row; a lane makes a word from the two that hold its bytes, so that every
+// load and store of a wave is one piece of 256 bytes (16 bytes a lane at odd addresses take
+// four times as long: 250 x 16384 at k 4097 122 us without this).
+__global__ __launch_bounds__(256) void k_align_rows(const int8_t* src, int64_t stride, int64_t rows, int K, int8_t* dst, int64_t pitch)
+{
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int8_t* p = src + row * stride;
+    const uint32_t sh = (uint32_t)(uintptr_t)p & 3u;
+    const uint32_t* b = (const uint32_t*)(p - sh);
+    const int words = (int)((sh + K + 3) / 4);          // that hold some of the row
+    uint32_t* out = (uint32_t*)(dst + row * pitch);
+    for (int j = lane; j < (int)(pitch / 4); j += 64) {
+        const uint32_t lo = b[min(j, words - 1)], hi = b[min(j + 1, words - 1)];
+        uint32_t v = __builtin_amdgcn_alignbyte(hi, lo, sh);
+        const int left = K - 4 * j;                     // bytes of the row from this word on
+        if (left < 4) v = left > 0 ? v & ((1u << (8 * left)) - 1u) : 0u;
+        out[j] = v;
+    }
+}
+
+// Few tokens: bound by the weights' way from memory.  A workgroup takes 16 NW channels and all
+// tokens, 16 MT at most; its S waves take k in turn, 128 bytes each (whole lines of 16 NW rows),
+// U of them loaded at once straight into the matrix instructions' operands, with no LDS and no
+// barrier before the waves' sums meet.  Unaligned rows load as aligned ones do.
+template <int DT, int MT, int NW, int S, int U>
+__global__ __launch_bounds__(64 * S) void k_int8_rows(const fie_int8_args a, int wide)
+{
+    __shared__ i32x4_t red[S][MT * NW][64];
+    const int lane = threadIdx.x & 63, K = a.k;
+    const int s = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * (16 * NW);
+    const int8_t* wp[NW];
+    const int8_t* xp[MT];
 #pragma unroll
-        for (int j = 0; j < NC; ++j) r[j] = load_k(src[j], s * kI8K + off[j], a.k);
+    for (int q = 0; q < NW; ++q) wp[q] = a.w + (int64_t)min(n0 + 16 * q + (lane & 15), a.n - 1) * a.w_stride + 16 * (lane >> 4);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) xp[m] = a.x + min((int64_t)(16 * m + (lane & 15)), a.m - 1) * a.x_stride + 16 * (lane >> 4);
+    i32x4_t acc[MT][NW];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int q = 0; q < NW; ++q) acc[m][q] = i32x4_t{0, 0, 0, 0};
+    auto steps = [&](int k0, auto count) {          // chunks k0, k0 + 128 S, ..
+        constexpr int N = decltype(count)::value;
+        i32x4_t fw[N][2][NW], fx[N][2][MT];
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int q = 0; q < NW; ++q) fw[u][h][q] = load_any(wp[q] + k0 + u * (128 * S) + 64 * h);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) fx[u][h][m] = load_any(xp[m] + k0 + u * (128 * S) + 64 * h);
+            }
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int q = 0; q < NW; ++q) acc[m][q] = mfma_i8(fw[u][h][q], fx[u][h][m], acc[m][q]);
     };
-    const int wr = wave % WM, wn = wave / WM;
-    i32x4_t acc[4][4];
+    const int full = K / 128;                       // whole chunks
+    int c = s;
+    for (; c + (U - 1) * S < full; c += U * S) steps(c * 128, std::integral_constant<int, U>{});
+    for (; c < full; c += S) steps(c * 128, std::integral_constant<int, 1>{});
+    if (c == full && K % 128) {                     // the rest, by the wave whose turn it is
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+        for (int h = 0; h < 2; ++h) {
+            const int k0 = full * 128 + 64 * h, r = K - 16 * (lane >> 4);       // what is left from wp, xp on
+            i32x4_t fx[MT];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[m][q] = i32x4_t{0, 0, 0, 0};
-    load(0);
-    for (int s = 0; s < ns; ++s) {
-        const int b = s & 1;
+            for (int m = 0; m < MT; ++m) fx[m] = load_k(xp[m], k0, r);
 #pragma unroll
-        for (int j = 0; j < NC; ++j) L[b][dst[j]] = r[j];
-        __syncthreads();                        // the buffer's readers of two stages ago are behind it
-        if (s + 1 < ns) load(s + 1);
+            for (int q = 0; q < NW; ++q) {
+                const i32x4_t fw = load_k(wp[q], k0, r);
 #pragma unroll
-        for (int kk = 0; kk < kI8K / 64; ++kk) {
-            const int c = kk * 4 + (lane >> 4);
-            i32x4_t fx[4], fw[4];
-#pragma unroll
-            for (int m = 0; m < 4; ++m) fx[m] = L[b][i8_slot(64 * wr + 16 * m + (lane & 15), c)];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) fw[q] = L[b][i8_slot(BM + 64 * wn + 16 * q + (lane & 15), c)];
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) acc[m][q] = mfma_i8(fw[q], fx[m], acc[m][q]);
+                for (int m = 0; m < MT; ++m) acc[m][q] = mfma_i8(fw, fx[m], acc[m][q]);
+            }
         }
     }
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-        const int64_t row = r0 + 64 * wr + 16 * m + (lane & 15);
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int q = 0; q < NW; ++q) red[s][m * NW + q][lane] = acc[m][q];
+    __syncthreads();
+    for (int f = s; f < MT * NW; f += S) {
+        i32x4_t t = red[0][f][lane];
+#pragma unroll
+        for (int i = 1; i < S; ++i) t += red[i][f][lane];
+        const int64_t row = 16 * (f / NW) + (lane & 15);
+        const int n = n0 + 16 * (f % NW) + 4 * (lane >> 4);
+        if (row < a.m && n < a.n) store_scaled<DT>(a, row, n, t, a.x_scale[row], wide);
+    }
+}
+
+// Many tokens: BM tokens by BN channels a workgroup of WM x WN waves.  k goes in stages of 128
+// bytes through NB LDS buffers that the loads fill by themselves (16 bytes a lane, no registers
+// between), NB - 1 stages ahead; a stage costs one barrier.  A wave's instruction fills eight
+// rows of 128 bytes in lane order, so the swizzle of i8_slot is in the addresses it loads from.
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+// Workgroup b's tile of nrb x ncb.  Workgroups are dealt to the eight XCDs round robin: each
+// XCD takes an eighth of the tiles, in bands of kBand token blocks down and then across, so
+// that the tiles it works on at a time share their rows in its L2.  Grid: tile_grid().
+constexpr int kBand = 4;
+FIE_DEV bool tile_at(int b, int nrb, int ncb, int* rb, int* cb)
+{
+    const int total = nrb * ncb, share = (total + 7) / 8;
+    const int j = b >> 3, id = (b & 7) * share + j;
+    if (j >= share || id >= total) return false;
+    const int band = id / (kBand * ncb), in = id - band * (kBand * ncb);
+    const int h = min(kBand, nrb - band * kBand);
+    *rb = band * kBand + in % h;
+    *cb = in / h;
+    return true;
+}
+
+template <int N> FIE_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+FIE_DEV void meet()             // a barrier that waits for no load
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// KG groups of WM x WN waves take the stages in turn, each in buffers of its own, and their sums
+// meet at the end: more of them in flight where there are few tiles.
+template <int DT, int BM, int BN, int WM, int WN, int NB, int KG, int OCC>
+__global__ __launch_bounds__(64 * WM * WN * KG, OCC) void k_int8_pipe(const fie_int8_args a, int nrb, int wide)
+{
+    constexpr int NWV = WM * WN;                                // waves of a group
+    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;         // 16 x 16 results of a wave
+    constexpr int ROWS = BM + BN, NI = ROWS / 8 / NWV;          // loads of a wave a stage
+    static_assert(ROWS % (8 * NWV) == 0 && BM % 8 == 0, "whole loads");
+    static_assert(NB * ROWS * kI8K >= BM * BN * 4 || KG == 1, "a group's sums fit its buffers");
+    __shared__ __attribute__((aligned(1024))) int8_t L[KG][NB][ROWS * kI8K];
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grp = wv / NWV, wave = wv % NWV;
+    int rb, cb;
+    if (!tile_at(blockIdx.x, nrb, (a.n + BN - 1) / BN, &rb, &cb)) return;
+    const int t0 = cb * BN;
+    const int64_t r0 = (int64_t)rb * BM;
+    // load i of this wave: rows 8 (wave + NWV i) .. +7 of the stage (tokens, then channels)
+    uint32_t off[NI];
+    const int8_t* const xb = a.x + r0 * a.x_stride;
+    const int8_t* const wb = a.w + (int64_t)t0 * a.w_stride;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int r = 8 * (wave + NWV * i) + (lane >> 3), c = (lane & 7) ^ (r & 7);
+        const int rm = (int)min((int64_t)r, a.m - 1 - r0), rn = min(r - BM, a.n - 1 - t0);
+        off[i] = (r < BM ? (uint32_t)rm * (uint32_t)a.x_stride : (uint32_t)rn * (uint32_t)a.w_stride) + 16u * c;
+    }
+    auto issue = [&](int s) {                                   // the group's s-th stage
+        int8_t* to = L[grp][s % NB];
+        const int64_t k0 = (int64_t)(s * KG + grp) * kI8K;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int at = wave + NWV * i;
+            const int8_t* b = (8 * at < BM ? xb : wb) + k0;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(b + off[i]), (lds_ptr)(to + at * 1024), 16, 0, 0);
+        }
+    };
+    const int wr = wave % WM, wn = wave / WM;
+    i32x4_t acc[FM][FN];
+#pragma unroll
+    for (int m = 0; m < FM; ++m)
+#pragma unroll
+        for (int q = 0; q < FN; ++q) acc[m][q] = i32x4_t{0, 0, 0, 0};
+    auto mul = [&](const int8_t* b) {
+        const i32x4_t* l = (const i32x4_t*)b;
+#pragma unroll
+        for (int kk = 0; kk < kI8K / 64; ++kk) {
+            const int c = kk * 4 + (lane >> 4);
+            i32x4_t fx[FM], fw[FN];
+#pragma unroll
+            for (int m = 0; m < FM; ++m) fx[m] = l[i8_slot((BM / WM) * wr + 16 * m + (lane & 15), c)];
+#pragma unroll
+            for (int q = 0; q < FN; ++q) fw[q] = l[i8_slot(BM + (BN / WN) * wn + 16 * q + (lane & 15), c)];
+#pragma unroll
+            for (int m = 0; m < FM; ++m)
+#pragma unroll
+                for (int q = 0; q < FN; ++q) acc[m][q] = mfma_i8(fw[q], fx[m], acc[m][q]);
+        }
+    };
+    const int full = a.k / kI8K;                                // whole stages
+    const int ns = (full - grp + KG - 1) / KG;                  // this group's
+    const int most = (full + KG - 1) / KG;                      // the first group's: no group has more
+#pragma unroll
+    for (int s = 0; s < NB - 1; ++s)
+        if (s < ns) issue(s);
+    for (int s = 0; s < most; ++s) {
+        // this stage's loads of every wave are done, and every wave is past the stage before
+        if (s + NB - 1 <= ns) wait_loads<(NB - 2) * NI>();
+        else wait_loads<0>();
+        meet();
+        if (s + NB - 1 < ns) issue(s + NB - 1);
+        if (KG == 1 || s < ns) mul(L[grp][s % NB]);
+    }
+    if (a.k % kI8K) {                                           // the rest of k, 0 past its end
+        meet();
+        if (grp == 0) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int r = 8 * (wave + NWV * i) + (lane >> 3), c = (lane & 7) ^ (r & 7);
+                const int8_t* row = (8 * (wave + NWV * i) < BM ? xb : wb) + (off[i] - 16u * c);
+                *(i32x4_t*)(L[0][0] + (wave + NWV * i) * 1024 + lane * 16) = load_k(row, full * kI8K + 16 * c, a.k);
+            }
+        }
+        __syncthreads();
+        if (grp == 0) mul(L[0][0]);
+    }
+    if constexpr (KG > 1) {                                     // the groups' sums
+        __syncthreads();
+        i32x4_t* mine = (i32x4_t*)L[grp][0];
+        if (grp)
+#pragma unroll
+            for (int m = 0; m < FM; ++m)
+#pragma unroll
+                for (int q = 0; q < FN; ++q) mine[((wave * FM + m) * FN + q) * 64 + lane] = acc[m][q];
+        __syncthreads();
+        if (grp) return;
+#pragma unroll
+        for (int g = 1; g < KG; ++g) {
+            const i32x4_t* other = (const i32x4_t*)L[g][0];
+#pragma unroll
+            for (int m = 0; m < FM; ++m)
+#pragma unroll
+                for (int q = 0; q < FN; ++q) acc[m][q] += other[((wave * FM + m) * FN + q) * 64 + lane];
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+        const int64_t row = r0 + (BM / WM) * wr + 16 * m + (lane & 15);
         if (row >= a.m) continue;
         const float xs = a.x_scale[row];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int n = t0 + 64 * wn + 16 * q + 4 * (lane >> 4);
+        for (int q = 0; q < FN; ++q) {
+            const int n = t0 + (BN / WN) * wn + 16 * q + 4 * (lane >> 4);
             if (n < a.n) store_scaled<DT>(a, row, n, acc[m][q], xs, wide);
         }
     }

@@ -4,22 +4,116 @@
 
 namespace fie {
 
-template <int DT, int WM, int WN>
-static hipError_t tile_of(const fie_int8_args& a, int wide, hipStream_t st)
+template <int DT, int MT, int NW, int S, int U>
+static hipError_t rows_of(const fie_int8_args& a, int wide, hipStream_t st)
 {
-    constexpr int BM = 64 * WM, BN = 64 * WN;
-    const int64_t nrb = (a.m + BM - 1) / BM, tiles = (a.n + BN - 1) / BN;
-    k_int8_tile<DT, WM, WN><<<(unsigned)(8 * ((tiles + 7) / 8) * nrb), 64 * WM * WN, 0, st>>>(a, (int)nrb, wide);
+    k_int8_rows<DT, MT, NW, S, U><<<(a.n + 16 * NW - 1) / (16 * NW), 64 * S, 0, st>>>(a, wide);
+    return hipGetLastError();
+}
+
+template <int DT, int BM, int BN, int WM, int WN, int NB, int KG, int OCC>
+static hipError_t pipe_of(const fie_int8_args& a, int wide, hipStream_t st)
+{
+    const int64_t nrb = (a.m + BM - 1) / BM, ncb = (a.n + BN - 1) / BN;
+    k_int8_pipe<DT, BM, BN, WM, WN, NB, KG, OCC><<<(unsigned)(8 * ((nrb * ncb + 7) / 8)), 64 * WM * WN * KG, 0, st>>>(a, (int)nrb, wide);
+    return hipGetLastError();
+}
+
+// The pipe kernel's tiles, and what a CU takes for one of each, as measured at k 4096 (us over
+// the launch's own 3, tiles as many as CUs; the other tiles on the same product beside it):
+//   32 x 32, k in four groups    4.6   64 x 4096  7.4 (32 x 64 10.0, 64 x 64 12.6)
+//   32 x 64                      6.5   16 x 151936  113 (64 x 64 124, 64 x 128 126)
+//   64 x 64                     10.5   250 x 4096  13.1 (32 x 64 14.0, 64 x 128 17.3)
+//   64 x 128                    17     128 x 16384  22.1 (64 x 64 26.2, 128 x 128 26.5)
+//   128 x 128                   26     250 x 16384  29.0 (64 x 128 34.6, 256 x 128 38.5)
+//   256 x 128                   40     256 x 151936  226 (256 x 256 254, 128 x 128 261)
+//   256 x 256                   73     4096 x 4096 at k 16384  221 (256 x 128 261, 128 x 128 306)
+// A product takes the tile with the least cost times rounds of the CUs; all of them go over k
+// alike.
+struct Tile { int bm, bn; float cost; };
+constexpr Tile kTiles[] = {{32, 32, 4.6f}, {32, 64, 6.5f}, {64, 64, 10.5f}, {64, 128, 17.0f},
+                           {128, 128, 26.0f}, {256, 128, 40.0f}, {256, 256, 73.0f}};
+
+static int cheapest(int64_t m, int64_t n)
+{
+    const int64_t cus = cu_count() > 0 ? cu_count() : 256;
+    int best = 0;
+    float least = 0.0f;
+    for (int i = 0; i < (int)(sizeof kTiles / sizeof kTiles[0]); ++i) {
+        const Tile& t = kTiles[i];
+        const int64_t tiles = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
+        const float c = t.cost * (float)((tiles + cus - 1) / cus);
+        if (i == 0 || c < least) { best = i; least = c; }
+    }
+    return best;
+}
+
+// Rows that the pipe kernel's loads take: 16 bytes at aligned addresses, 32-bit offsets from a
+// tile's first row.
+static bool aligned_rows(const void* p, int64_t stride)
+{
+    return (((uintptr_t)p | (uint64_t)stride) & 15) == 0 && stride < (1 << 23);
+}
+
+// Tokens few enough to go with the weights at whatever address, straight to registers: up to
+// 32, or 96 where the channels are few (77 x 5001 at k 1003).
+static bool by_rows(int64_t m, int n) { return m <= (n >= 512 * 16 ? 32 : 96); }
+
+static int64_t pitch_of(int k) { return ((int64_t)k + kI8K - 1) / kI8K * kI8K; }
+
+static size_t int8_workspace(const fie_int8_args& a)
+{
+    const bool ax = aligned_rows(a.x, a.x_stride), aw = aligned_rows(a.w, a.w_stride);
+    if ((ax && aw) || by_rows(a.m, a.n)) return 0;
+    return (size_t)((ax ? 0 : a.m) + (aw ? 0 : (int64_t)a.n)) * (size_t)pitch_of(a.k);
+}
+
+static hipError_t align_rows(const int8_t* src, int64_t stride, int64_t rows, int k, int8_t* dst, hipStream_t st)
+{
+    k_align_rows<<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(src, stride, rows, k, dst, pitch_of(k));
     return hipGetLastError();
 }
 
 template <int DT>
-static hipError_t int8_dt(const fie_int8_args& a, hipStream_t st)
+static hipError_t int8_dt(fie_int8_args a, hipStream_t st)
 {
     constexpr int SZ = DT == FIE_F32 ? 4 : 2;
     const int wide = ((uintptr_t)a.y % (4 * SZ)) == 0 && a.y_stride % 4 == 0;
-    if (a.m <= 64) return tile_of<DT, 1, 4>(a, wide, st);
-    return tile_of<DT, 2, 2>(a, wide, st);
+    const bool ax = aligned_rows(a.x, a.x_stride), aw = aligned_rows(a.w, a.w_stride);
+    if (!(ax && aw)) {
+        if (by_rows(a.m, a.n)) {
+            // from 512 workgroups on with more channels a wave (fewer loads of the tokens: 16 x
+            // 50001 at k 4096 52 us against 63, and at 4096 channels 8.2 against 6.5)
+            const bool many = a.n >= 512 * 16;
+            if (a.m <= 16) return many ? rows_of<DT, 1, 2, 8, 2>(a, wide, st) : rows_of<DT, 1, 1, 16, 2>(a, wide, st);
+            if (a.m <= 32) return many ? rows_of<DT, 2, 4, 8, 1>(a, wide, st) : rows_of<DT, 2, 1, 8, 2>(a, wide, st);
+            return a.m <= 64 ? rows_of<DT, 4, 1, 8, 1>(a, wide, st) : rows_of<DT, 6, 1, 8, 1>(a, wide, st);
+        }
+        int8_t* to = (int8_t*)a.workspace;
+        hipError_t e = hipSuccess;
+        if (!ax) {
+            e = align_rows(a.x, a.x_stride, a.m, a.k, to, st);
+            a.x = to;
+            a.x_stride = pitch_of(a.k);
+            to += a.m * a.x_stride;
+        }
+        if (e == hipSuccess && !aw) {
+            e = align_rows(a.w, a.w_stride, a.n, a.k, to, st);
+            a.w = to;
+            a.w_stride = pitch_of(a.k);
+        }
+        if (e != hipSuccess) return e;
+        if (!ax && !aw) a.k = (int)pitch_of(a.k);           // zeros on both sides: no last piece
+    }
+    switch (cheapest(a.m, a.n)) {
+    case 0: return pipe_of<DT, 32, 32, 1, 2, 4, 4, 2>(a, wide, st);
+    case 1: return pipe_of<DT, 32, 64, 1, 4, 4, 1, 3>(a, wide, st);
+    case 2: return pipe_of<DT, 64, 64, 2, 2, 4, 1, 2>(a, wide, st);
+    case 3: return pipe_of<DT, 64, 128, 2, 4, 3, 1, 4>(a, wide, st);
+    case 4: return pipe_of<DT, 128, 128, 4, 4, 4, 1, 4>(a, wide, st);
+    case 5: return pipe_of<DT, 256, 128, 4, 4, 3, 1, 4>(a, wide, st);
+    default: return pipe_of<DT, 256, 256, 4, 4, 2, 1, 4>(a, wide, st);
+    }
 }
 
 static int int8_check(const fie_int8_args* a)
@@ -29,15 +123,24 @@ static int int8_check(const fie_int8_args* a)
     if (a->k < 1 || a->k > FIE_MAX_K) return fail(FIE_E_ARG, "k out of range [1, 131071]");
     if (a->y_dtype < FIE_F32 || a->y_dtype > FIE_BF16) return fail(FIE_E_ARG, "unknown dtype");
     if (a->x_stride < a->k || a->w_stride < a->k || a->y_stride < a->n) return fail(FIE_E_ARG, "a row stride is shorter than its row");
-    if ((a->m + 63) / 64 * ((a->n + 63) / 64) > 0x0FFFFFFF) return fail(FIE_E_ARG, "m x n too large for one launch");
+    if ((a->m + 31) / 32 * ((a->n + 31) / 32) > 0x0FFFFFFF) return fail(FIE_E_ARG, "m x n too large for one launch");
     if (a->m == 0) return FIE_OK;
     if (!a->x || !a->w || !a->x_scale || !a->w_scale || !a->y) return fail(FIE_E_ARG, "a required pointer is NULL");
+    if (const size_t need = int8_workspace(*a)) {
+        if (!a->workspace || a->workspace_bytes < need) return fail(FIE_E_WORKSPACE, "workspace too small for unaligned rows");
+        if (((uintptr_t)a->workspace & 15) != 0) return fail(FIE_E_WORKSPACE, "workspace not 16-byte aligned");
+    }
     return FIE_OK;
 }
 
 }  // namespace fie
 
 using namespace fie;
+
+extern "C" size_t fie_int8_workspace_size(const fie_int8_args* a)
+{
+    return a && a->m > 0 && a->n > 0 && a->k > 0 ? int8_workspace(*a) : 0;
+}
 
 extern "C" int fie_int8_linear(const fie_int8_args* a, void* stream)
 {

@@ -77,7 +77,8 @@ class Int8Args(ctypes.Structure):
         ("x", _vp), ("w", _vp), ("x_scale", _vp), ("w_scale", _vp), ("bias", _vp), ("y", _vp),
         ("m", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("w_stride", ctypes.c_int64),
         ("y_stride", ctypes.c_int64), ("n", ctypes.c_int32), ("k", ctypes.c_int32),
-        ("y_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("y_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32), ("workspace", _vp),
+        ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -96,7 +97,7 @@ EXPORTS = (
     "fie_sampler_lmhead_sample", "fie_sampler_lmhead_stage", "fie_sampler_verify",
 )
 # Every symbol include/fie_ops.h declares.
-OPS_EXPORTS = ("fie_block_norm", "fie_int8_linear")
+OPS_EXPORTS = ("fie_block_norm", "fie_int8_linear", "fie_int8_workspace_size")
 SCRATCH_BYTES = 64 << 20
 
 _lib = None
@@ -149,6 +150,8 @@ def bind(lib) -> None:
     for name in EXPORTS + OPS_EXPORTS:
         if name not in ("fie_sampler_workspace_size", "fie_sampler_last_error"):
             getattr(lib, name).restype = ctypes.c_int
+    lib.fie_int8_workspace_size.argtypes = [ctypes.POINTER(Int8Args)]
+    lib.fie_int8_workspace_size.restype = ctypes.c_size_t
 
 
 def on_device(device):

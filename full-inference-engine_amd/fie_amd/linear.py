@@ -35,7 +35,9 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
 
     x is int8 with ``x_scale`` (float32, one a token), or float32, float16 or bfloat16, which is
     quantised for each token first.  ``out_dtype``: float32, float16 or bfloat16; by default x's own
-    (bfloat16 for int8).  ``out`` [tokens, n] is written instead of a new tensor: unit element
+    (bfloat16 for int8).  Weights whose rows begin at multiples of 16 bytes are read in place at
+    any number of tokens (pad the rows of a storage: ``w = room[:, :k]``); others are laid out anew
+    in every call past 32 tokens.  ``out`` [tokens, n] is written instead of a new tensor: unit element
     stride, any row stride.  Runs on the current stream; nothing waits for it."""
     if weight.ndim != 2 or weight.dtype != torch.int8:
         raise ValueError("weight must be int8 [channels, k]")
@@ -87,6 +89,10 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         a.m, a.n, a.k = tokens, n, k
         a.x_stride, a.w_stride, a.y_stride = max(x.stride(0), k), max(weight.stride(0), k), max(y.stride(0), n)
         lib = _lib.load()
+        if (a.x | a.w | a.x_stride | a.w_stride) & 15 or max(a.x_stride, a.w_stride) >= 1 << 23:
+            a.workspace_bytes = lib.fie_int8_workspace_size(ctypes.byref(a))
+            room = torch.empty(a.workspace_bytes, dtype=torch.int8, device=device)
+            a.workspace = room.data_ptr() if a.workspace_bytes else None
         with _lib.on_device(device):
             _lib.check(lib.fie_int8_linear(ctypes.byref(a), torch.cuda.current_stream(device).cuda_stream),
                        "fie_int8_linear")

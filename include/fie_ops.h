@@ -72,8 +72,15 @@ typedef struct fie_int8_args {
     int32_t n, k;               /* 1 <= k <= FIE_MAX_K (the sums stay in 32 bits) */
     int32_t y_dtype;            /* FIE_F32, FIE_F16, FIE_BF16 */
     int32_t reserved;
+    void* workspace;            /* fie_int8_workspace_size() bytes, 16-byte aligned (NULL: none) */
+    size_t workspace_bytes;
 } fie_int8_args;
 #define FIE_MAX_K 131071
+
+/* Bytes that a call with these pointers and sizes needs beside its operands: 0 where the rows
+   of x and w begin at multiples of 16 bytes (and for few tokens); otherwise the unaligned
+   operand is laid out there first.  Weights whose rows are padded to 16 bytes avoid that. */
+size_t fie_int8_workspace_size(const fie_int8_args* args);
 
 int fie_int8_linear(const fie_int8_args* args, void* stream);
 
