@@ -6,7 +6,6 @@ There is no fallback: if the library cannot be loaded, every entry point raises.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 
@@ -55,31 +54,11 @@ class VerifyArgs(ctypes.Structure):
     ]
 
 
-class NormArgs(ctypes.Structure):
-    """Mirror of ``fie_norm_args``."""
-
-    _fields_ = [
-        ("x", _vp), ("residual", _vp), ("residual_out", _vp), ("y", _vp), ("y_scale", _vp),
-        ("weight", _vp), ("bias", _vp), ("post_weight", _vp), ("post_bias", _vp), ("gate", _vp),
-        ("tokens", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("residual_stride", ctypes.c_int64),
-        ("residual_out_stride", ctypes.c_int64), ("y_stride", ctypes.c_int64), ("gate_stride", ctypes.c_int64),
-        ("gate_step", ctypes.c_int32), ("width", ctypes.c_int32), ("x_dtype", ctypes.c_int32),
-        ("residual_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32), ("weight_f32", ctypes.c_int32),
-        ("gate_f32", ctypes.c_int32), ("kind", ctypes.c_int32), ("post_norm", ctypes.c_int32),
-        ("scale", ctypes.c_float), ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float),
-    ]
-
-
-class Int8Args(ctypes.Structure):
-    """Mirror of ``fie_int8_args``."""
-
-    _fields_ = [
-        ("x", _vp), ("w", _vp), ("x_scale", _vp), ("w_scale", _vp), ("bias", _vp), ("y", _vp),
-        ("m", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("w_stride", ctypes.c_int64),
-        ("y_stride", ctypes.c_int64), ("n", ctypes.c_int32), ("k", ctypes.c_int32),
-        ("y_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32), ("workspace", _vp),
-        ("workspace_bytes", ctypes.c_size_t),
-    ]
+# ``fie_norm_args`` and ``fie_int8_args`` as struct formats, native sizes and alignment (filling
+# a ctypes structure of as many fields takes four times as long): pointers and sizes as P and q,
+# a trailing 0 quad pads to the structure's alignment.
+NORM_ARGS = "@10P6q9i3f0q"
+INT8_ARGS = "@6P4q4iPN0q"
 
 
 class Workspace(ctypes.Structure):
@@ -145,22 +124,37 @@ def bind(lib) -> None:
     lib.fie_sampler_verify.argtypes = [ctypes.POINTER(SamplerArgs), ctypes.POINTER(VerifyArgs),
                                        ctypes.POINTER(Workspace), _vp]
     lib.fie_sampler_last_error.restype = ctypes.c_char_p
-    lib.fie_block_norm.argtypes = [ctypes.POINTER(NormArgs), _vp]
-    lib.fie_int8_linear.argtypes = [ctypes.POINTER(Int8Args), _vp]
+    lib.fie_block_norm.argtypes = [ctypes.c_char_p, _vp]
+    lib.fie_int8_linear.argtypes = [ctypes.c_char_p, _vp]
     for name in EXPORTS + OPS_EXPORTS:
         if name not in ("fie_sampler_workspace_size", "fie_sampler_last_error"):
             getattr(lib, name).restype = ctypes.c_int
-    lib.fie_int8_workspace_size.argtypes = [ctypes.POINTER(Int8Args)]
+    lib.fie_int8_workspace_size.argtypes = [ctypes.c_char_p]
     lib.fie_int8_workspace_size.restype = ctypes.c_size_t
 
 
-def on_device(device):
-    """The context in which launches go to ``device``: nothing to do where it is current."""
-    import torch
+class on_device:
+    """Launches inside go to device ``index``, on its current stream, the context's value (the
+    interpreter's own calls for both take a tenth of the time of torch.cuda's wrappers)."""
 
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    __slots__ = ("index", "before")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self) -> int:
+        import torch
+
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.before != self.index:
+            import torch
+
+            torch._C._cuda_setDevice(self.before)
 
 
 def check(rc: int, what: str) -> None:

@@ -8,15 +8,16 @@ nn.Linear's [channels, k] layout.
 
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
 from . import _lib
-from ._lib import FIE_BF16, FIE_F16, FIE_F32, Int8Args
+from ._lib import FIE_BF16, FIE_F16, FIE_F32
 from .norm import block_norm
 
 _DTYPES = {torch.float32: FIE_F32, torch.float16: FIE_F16, torch.bfloat16: FIE_BF16}
+_pack = struct.Struct(_lib.INT8_ARGS).pack
 MAX_K = 131071          # the sums of longer products could pass 32 bits
 
 
@@ -42,13 +43,14 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     if weight.ndim != 2 or weight.dtype != torch.int8:
         raise ValueError("weight must be int8 [channels, k]")
     n, k = weight.shape
-    if x.ndim < 1 or x.shape[-1] != k or n < 1 or not 1 <= k <= MAX_K:
+    shape = x.shape
+    if not shape or shape[-1] != k or n < 1 or not 1 <= k <= MAX_K:
         raise ValueError(f"x [..., k] and weight [channels, k] must agree on k in [1, {MAX_K}]")
-    device = weight.device
-    if device.type != "cuda":
+    index = weight.get_device()
+    if index < 0:
         raise ValueError("int8_linear runs on a HIP device")
     for t in (x, weight_scale, x_scale, bias, out):
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError("every tensor must be on the weight's device")
     if x.dtype == torch.int8:
         if x_scale is None:
@@ -60,40 +62,40 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         dtype = out_dtype or x.dtype
     else:
         raise ValueError("x must be int8, float32, float16 or bfloat16")
-    if dtype not in _DTYPES:
+    y_dtype = _DTYPES.get(dtype)
+    if y_dtype is None:
         raise ValueError("out_dtype must be float32, float16 or bfloat16")
-    shape = x.shape[:-1]
     tokens = x.numel() // k
     for t, name, size in ((weight_scale, "weight_scale", n), (bias, "bias", n), (x_scale, "x_scale", tokens)):
         if t is not None and (t.dtype != torch.float32 or t.numel() != size or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous float32 of {size}")
     if out is None:
-        y = torch.empty((tokens, n), dtype=dtype, device=device)
+        y, y_stride = torch.empty((tokens, n), dtype=dtype, device=weight.device), n
     else:
         if out.ndim != 2 or out.shape != (tokens, n) or out.dtype != dtype or (n > 1 and out.stride(1) != 1) \
                 or (tokens > 1 and out.stride(0) < n):
             raise ValueError(f"out must be [{tokens}, {n}] in {dtype} with unit element stride")
-        y = out
+        y, y_stride = out, max(out.stride(0), n)
     if tokens:
         if x.dtype != torch.int8:
             x, x_scale = quantize_rows(x)
-        x = x if x.ndim == 2 else x.reshape(-1, k)
-        if (k > 1 and x.stride(1) != 1) or (tokens > 1 and x.stride(0) < k):
-            x = x.contiguous()
-        if (k > 1 and weight.stride(1) != 1) or (n > 1 and weight.stride(0) < k):
-            weight = weight.contiguous()
-        a = Int8Args()
-        a.x, a.w, a.x_scale, a.w_scale = x.data_ptr(), weight.data_ptr(), x_scale.data_ptr(), weight_scale.data_ptr()
-        a.bias = None if bias is None else bias.data_ptr()
-        a.y, a.y_dtype = y.data_ptr(), _DTYPES[dtype]
-        a.m, a.n, a.k = tokens, n, k
-        a.x_stride, a.w_stride, a.y_stride = max(x.stride(0), k), max(weight.stride(0), k), max(y.stride(0), n)
+        if len(shape) != 2:
+            x = x.reshape(-1, k)
+        x_stride, step = x.stride()
+        if (k > 1 and step != 1) or (tokens > 1 and x_stride < k):
+            x, x_stride = x.contiguous(), k
+        w_stride, step = weight.stride()
+        if (k > 1 and step != 1) or (n > 1 and w_stride < k):
+            weight, w_stride = weight.contiguous(), k
+        xp, wp, x_stride, w_stride = x.data_ptr(), weight.data_ptr(), max(x_stride, k), max(w_stride, k)
+        args = [xp, wp, x_scale.data_ptr(), weight_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr(),
+                tokens, x_stride, w_stride, y_stride, n, k, y_dtype, 0, 0, 0]
         lib = _lib.load()
-        if (a.x | a.w | a.x_stride | a.w_stride) & 15 or max(a.x_stride, a.w_stride) >= 1 << 23:
-            a.workspace_bytes = lib.fie_int8_workspace_size(ctypes.byref(a))
-            room = torch.empty(a.workspace_bytes, dtype=torch.int8, device=device)
-            a.workspace = room.data_ptr() if a.workspace_bytes else None
-        with _lib.on_device(device):
-            _lib.check(lib.fie_int8_linear(ctypes.byref(a), torch.cuda.current_stream(device).cuda_stream),
-                       "fie_int8_linear")
-    return y.view(*shape, n) if out is None else out
+        with _lib.on_device(index) as stream:
+            if (xp | wp | x_stride | w_stride) & 15 or max(x_stride, w_stride) >= 1 << 23:
+                args[-1] = lib.fie_int8_workspace_size(_pack(*args))
+                if args[-1]:
+                    room = torch.empty(args[-1], dtype=torch.int8, device=y.device)
+                    args[-2] = room.data_ptr()
+            _lib.check(lib.fie_int8_linear(_pack(*args), stream), "fie_int8_linear")
+    return y.view(*shape[:-1], n) if out is None and len(shape) != 2 else y

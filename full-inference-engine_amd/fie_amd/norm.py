@@ -11,16 +11,17 @@ the stores; ``y`` optionally in 8-bit integers with a scale for each token, as
 
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from ._lib import FIE_BF16, FIE_F16, FIE_F32, FIE_I8, NormArgs
+from ._lib import FIE_BF16, FIE_F16, FIE_F32, FIE_I8
 
 _DTYPES = {torch.float32: FIE_F32, torch.float16: FIE_F16, torch.bfloat16: FIE_BF16}
 _KINDS = {"rms": 0, "layer": 1, "none": 2}
+_pack = struct.Struct(_lib.NORM_ARGS).pack
 MAX_WIDTH = 65536
 
 
@@ -35,17 +36,6 @@ def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     if t.ndim != 2:
         t = t.reshape(-1, width)
     return t if t.stride(1) == 1 or width == 1 else t.contiguous()
-
-
-def _vector(t: torch.Tensor | None, name: str, width: int, dtype: torch.dtype, f32: list) -> int | None:
-    if t is None:
-        return None
-    if t.ndim != 1 or t.shape[0] != width or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous vector of {width}")
-    if t.dtype != dtype and t.dtype != torch.float32:
-        raise ValueError(f"{name} must be in {dtype} or float32")
-    f32.append(t.dtype == torch.float32)
-    return t.data_ptr()
 
 
 def block_norm(residual: torch.Tensor, x: torch.Tensor | None = None, weight: torch.Tensor | None = None, *,
@@ -63,87 +53,98 @@ def block_norm(residual: torch.Tensor, x: torch.Tensor | None = None, weight: to
     "layer" or "none" (y is r itself).  ``weight_offset`` is added to both weights.  Parameters
     are in x's type or float32 (weights and biases all in one).  ``inplace`` writes the new
     residual over the old.  Runs on the current stream; nothing waits for it."""
-    shape, width = residual.shape, residual.shape[-1] if residual.ndim else 0
-    if residual.ndim < 1 or not 1 <= width <= MAX_WIDTH:
+    shape = residual.shape
+    width = shape[-1] if shape else 0
+    if not 1 <= width <= MAX_WIDTH:
         raise ValueError(f"residual must be [..., width] with width in [1, {MAX_WIDTH}]")
-    if residual.dtype not in _DTYPES:
+    r_dtype = _DTYPES.get(residual.dtype)
+    if r_dtype is None:
         raise ValueError("residual must be float32, float16 or bfloat16")
-    if kind not in _KINDS:
+    norm = _KINDS.get(kind)
+    if norm is None:
         raise ValueError("kind must be 'rms', 'layer' or 'none'")
-    dtype = residual.dtype if x is None else x.dtype
     if x is None:
-        dtype = out_dtype if out_dtype is not None else dtype
+        dtype = out_dtype if out_dtype is not None else residual.dtype
         if gate is not None or post_norm or post_weight is not None or post_bias is not None or inplace:
             raise ValueError("gate, post norm and inplace need x")
-    elif x.shape != shape:
-        raise ValueError("x and residual must have one shape")
-    elif x.dtype not in _DTYPES or residual.dtype not in (x.dtype, torch.float32):
-        raise ValueError("x must be float32, float16 or bfloat16, and residual in its type or float32")
-    elif out_dtype is not None and out_dtype != dtype:
-        raise ValueError("out_dtype is x's type")
-    if dtype not in _DTYPES:
-        raise ValueError("out_dtype must be float32, float16 or bfloat16")
-    post = post_norm if post_norm is not None else post_weight is not None
-    if kind == "none" and (post or weight is not None or bias is not None):
-        raise ValueError("kind 'none' takes no norm parameters")
-    if not post and (post_weight is not None or post_bias is not None):
-        raise ValueError("post parameters without post_norm")
-    device = residual.device
-    if device.type != "cuda":
+    else:
+        dtype = x.dtype
+        if x.shape != shape:
+            raise ValueError("x and residual must have one shape")
+        if residual.dtype != dtype and residual.dtype != torch.float32:
+            raise ValueError("residual is in x's type or float32")
+        if out_dtype is not None and out_dtype != dtype:
+            raise ValueError("out_dtype is x's type")
+    x_dtype = _DTYPES.get(dtype)
+    if x_dtype is None:
+        raise ValueError("x and out_dtype must be float32, float16 or bfloat16")
+    index = residual.get_device()
+    if index < 0:
         raise ValueError("block_norm runs on a HIP device")
-    for t in (x, weight, bias, post_weight, post_bias, gate):
-        if t is not None and t.device != device:
-            raise ValueError("every tensor must be on the residual's device")
-
-    a = NormArgs()
-    f32: list = []
-    a.weight = _vector(weight, "weight", width, dtype, f32)
-    a.bias = _vector(bias, "bias", width, dtype, f32)
-    a.post_weight = _vector(post_weight, "post_weight", width, dtype, f32)
-    a.post_bias = _vector(post_bias, "post_bias", width, dtype, f32)
-    if f32 and any(f32) != all(f32):
-        raise ValueError("weights and biases must share one type")
-    a.weight_f32 = bool(f32) and f32[0]
+    post = post_norm if post_norm is not None else post_weight is not None
+    # parameter vectors: all in x's type, or all in float32
+    vectors, v_dtype = [0, 0, 0, 0], None
+    for i, t in enumerate((weight, bias, post_weight, post_bias)):
+        if t is None:
+            continue
+        if t.shape != (width,) or not t.is_contiguous():
+            raise ValueError(f"weights and biases must be contiguous vectors of {width}")
+        if v_dtype is None:
+            v_dtype = t.dtype
+            if v_dtype != dtype and v_dtype != torch.float32:
+                raise ValueError(f"weights and biases must be in {dtype} or float32")
+        if t.dtype != v_dtype or t.get_device() != index:
+            raise ValueError("weights and biases must share one type, on the residual's device")
+        if norm == 2:
+            raise ValueError("kind 'none' takes no norm parameters")
+        if i >= 2 and not post:
+            raise ValueError("post parameters without post_norm")
+        vectors[i] = t.data_ptr()
+    if norm == 2 and post:
+        raise ValueError("kind 'none' takes no norm parameters")
     res = _rows(residual, width)
-    tokens = res.shape[0]
-    a.residual, a.residual_stride, a.residual_dtype = res.data_ptr(), res.stride(0), _DTYPES[res.dtype]
-    a.tokens, a.width, a.x_dtype = tokens, width, _DTYPES[dtype]
-    new = None
+    tokens, r_stride = res.shape[0], res.stride(0)
+    device = residual.device
+    new = xs = gp = None
+    xp = x_stride = n_ptr = n_stride = g_ptr = g_stride = g_step = g_f32 = 0
     if x is not None:
         xs = _rows(x, width)
-        a.x, a.x_stride = xs.data_ptr(), xs.stride(0)
+        xp, x_stride = xs.data_ptr(), xs.stride(0)
+        if x.get_device() != index:
+            raise ValueError("x must be on the residual's device")
         if inplace:
-            if res.data_ptr() != residual.data_ptr() or (tokens > 1 and res.stride(0) < width):
+            if res.data_ptr() != residual.data_ptr() or (tokens > 1 and r_stride < width):
                 raise ValueError("inplace needs a residual with unit element stride and rows that do not overlap")
-            new = res
+            new, n_stride = res, r_stride
         else:
-            new = torch.empty((tokens, width), dtype=res.dtype, device=device)
-        a.residual_out, a.residual_out_stride = new.data_ptr(), new.stride(0)
+            new, n_stride = torch.empty((tokens, width), dtype=residual.dtype, device=device), width
+        n_ptr = new.data_ptr()
         if gate is not None:
-            if gate.dtype != dtype and gate.dtype != torch.float32:
-                raise ValueError(f"gate must be in {dtype} or float32")
+            if gate.get_device() != index or (gate.dtype != dtype and gate.dtype != torch.float32):
+                raise ValueError(f"gate must be in {dtype} or float32, on the residual's device")
             if gate.shape == (width,):
-                g = gate.contiguous()
-                a.gate_stride, a.gate_step = 0, 1
+                gp, g_stride, g_step = gate.contiguous(), 0, 1
             elif gate.shape == shape:
-                g = _rows(gate, width)
-                a.gate_stride, a.gate_step = g.stride(0), 1
+                gp = _rows(gate, width)
+                g_stride, g_step = gp.stride(0), 1
             elif gate.shape == (*shape[:-1], 1):
-                g = gate.reshape(-1)
-                a.gate_stride, a.gate_step = g.stride(0), 0
+                gp = gate.reshape(-1)
+                g_stride, g_step = gp.stride(0), 0
             else:
                 raise ValueError("gate must be [width], x's shape, or x's shape with a last dimension of 1")
-            a.gate, a.gate_f32 = g.data_ptr(), gate.dtype == torch.float32
+            g_ptr, g_f32 = gp.data_ptr(), gate.dtype == torch.float32
     y = torch.empty((tokens, width), dtype=torch.int8 if quantize else dtype, device=device)
-    a.y, a.y_stride, a.y_dtype = y.data_ptr(), width, FIE_I8 if quantize else a.x_dtype
-    y_scale = None
-    if quantize:
-        y_scale = torch.empty(tokens, dtype=torch.float32, device=device)
-        a.y_scale = y_scale.data_ptr()
-    a.kind, a.post_norm = _KINDS[kind], post
-    a.scale, a.eps, a.weight_offset = scale, eps, weight_offset
+    y_scale = torch.empty(tokens, dtype=torch.float32, device=device) if quantize else None
     if tokens:
+        args = _pack(xp, res.data_ptr(), n_ptr, y.data_ptr(), y_scale.data_ptr() if quantize else 0, *vectors, g_ptr,
+                     tokens, x_stride, r_stride, n_stride, width, g_stride, g_step, width, x_dtype, r_dtype,
+                     FIE_I8 if quantize else x_dtype, v_dtype == torch.float32, g_f32, norm, post, scale, eps,
+                     weight_offset)
         lib = _lib.load()
-        with _lib.on_device(device):
-            _lib.check(lib.fie_block_norm(ctypes.byref(a), torch.cuda.current_stream(device).cuda_stream), "fie_block_norm")
-    return BlockNorm(residual if inplace else new if new is None else new.view(shape), y.view(shape), y_scale)
+        with _lib.on_device(index) as stream:
+            _lib.check(lib.fie_block_norm(args, stream), "fie_block_norm")
+    if len(shape) != 2:
+        y = y.view(shape)
+        if new is not None and not inplace:
+            new = new.view(shape)
+    return BlockNorm(residual if inplace else new, y, y_scale)

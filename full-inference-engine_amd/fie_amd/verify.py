@@ -59,6 +59,9 @@ class VerifyPlan:
         self.requests, self.vocab = len(params), int(vocab)
         self.drafts, self.max_drafts = int(lens.sum()), int(lens.max()) if lens.size else 0
         self.rows = self.drafts + self.requests
+        # what a call's tensors have to be
+        self.logits_shape, self.probs_shape = (self.rows, self.vocab), (self.drafts, self.vocab)
+        self.ids_shape, self.rows_shape = (self.drafts,), (self.rows,)
         row_params = [p for p, n in zip(params, draft_lens) for _ in range(n + 1)]
         row_contexts = None
         if contexts is not None and any(p.has_penalties for p in params):
@@ -73,6 +76,7 @@ class VerifyPlan:
         self._offsets = torch.zeros(self.requests + 1, dtype=torch.int64)
         np.cumsum(lens, out=self._offsets.numpy()[1:])
         self._offsets = self._offsets.to(fused.device)
+        self.index = self._offsets.get_device()
         # the parameter block, uploaded once
         self._buf = DeviceStep(self.rows, hp.tail_ints(), fused.device)
         self._buf.stage(hp)
@@ -118,32 +122,30 @@ class DraftVerifier:
         ``uniforms`` float64 [rows] in [0, 1): a row's test of its draft, and on a request's
         last row its draw.  ``draft_probs`` [drafts, vocab]: the distributions the drafts were
         drawn from; without them a draft counts as certain (prompt lookup, argmax drafts)."""
-        rows, drafts, vocab = plan.rows, plan.drafts, plan.vocab
-        if logits.ndim != 2 or logits.shape[0] != rows or logits.shape[1] != vocab:
+        rows, drafts, vocab, index = plan.rows, plan.drafts, plan.vocab, plan.index
+        if logits.shape != plan.logits_shape:
             raise ValueError(f"logits must be [{rows}, {vocab}], a request's drafts + 1 rows together")
-        if draft_ids.dtype != torch.int64 or draft_ids.ndim != 1 or draft_ids.shape[0] != drafts:
+        if draft_ids.dtype != torch.int64 or draft_ids.shape != plan.ids_shape:
             raise ValueError(f"draft_ids must be int64 [{drafts}]")
         if (uniforms is None) != plan.has_rng:
             raise ValueError("uniforms are required, or a plan that draws on the device, not both")
-        if uniforms is not None and (uniforms.dtype != torch.float64 or uniforms.ndim != 1 or uniforms.shape[0] != rows):
+        if uniforms is not None and (uniforms.dtype != torch.float64 or uniforms.shape != plan.rows_shape):
             raise ValueError(f"uniforms must be float64 [{rows}]")
-        if draft_probs is not None and (draft_probs.ndim != 2 or draft_probs.shape[0] != drafts
-                                        or draft_probs.shape[1] != vocab or draft_probs.dtype not in _DTYPES):
+        if draft_probs is not None and (draft_probs.shape != plan.probs_shape or draft_probs.dtype not in _DTYPES):
             raise ValueError(f"draft_probs must be [{drafts}, {vocab}] in float32, float16 or bfloat16")
         for t in (logits, draft_ids, uniforms, draft_probs):
-            if t is not None and t.device != self._device_of(logits):
-                raise ValueError(f"every tensor must be on {self.device}")
-        tokens = torch.empty((plan.requests, plan.max_drafts + 1), dtype=torch.int64, device=self.device)
-        accepted = torch.empty(plan.requests, dtype=torch.int32, device=self.device)
-        probs = torch.empty(drafts, dtype=torch.float32, device=self.device)
+            if t is not None and t.get_device() != index:
+                raise ValueError(f"every tensor must be on device {index}")
+        device = logits.device
+        tokens = torch.empty((plan.requests, plan.max_drafts + 1), dtype=torch.int64, device=device)
+        accepted = torch.empty(plan.requests, dtype=torch.int32, device=device)
+        probs = torch.empty(drafts, dtype=torch.float32, device=device)
         if plan.requests == 0:
             return Verified(tokens, accepted, probs)
         a, v = plan.args, plan.verify_args
         logits, a.dtype = FusedSampler._logits_info(logits)
         draft_ids = draft_ids.contiguous()
-        a.logits, a.row_stride = logits.data_ptr(), logits.stride(0)
-        if rows == 1:
-            a.row_stride = max(a.row_stride, vocab)
+        a.logits, a.row_stride = logits.data_ptr(), max(logits.stride(0), vocab)
         if uniforms is not None:
             uniforms = uniforms.contiguous()
             a.uniform = uniforms.data_ptr()
@@ -154,13 +156,7 @@ class DraftVerifier:
             v.draft_probs, v.draft_stride = draft_probs.data_ptr(), max(draft_probs.stride(0), vocab)
         v.tokens, v.accepted, v.target_probs = tokens.data_ptr(), accepted.data_ptr(), probs.data_ptr()
         ws = self._fused.ensure_workspace(rows, vocab)
-        rc = self._fused.lib.fie_sampler_verify(ctypes.byref(a), ctypes.byref(v), ctypes.byref(ws),
-                                                self._fused._stream_ptr())
+        with _lib.on_device(index) as stream:
+            rc = self._fused.lib.fie_sampler_verify(ctypes.byref(a), ctypes.byref(v), ctypes.byref(ws), stream)
         _lib.check(rc, "fie_sampler_verify")
         return Verified(tokens, accepted, probs)
-
-    def _device_of(self, logits: torch.Tensor) -> torch.device:
-        d = logits.device
-        if d.type != "cuda" or (self.device.index is not None and d.index != self.device.index):
-            raise ValueError(f"every tensor must be on {self.device}")
-        return d
