@@ -27,20 +27,28 @@ struct RowDist {
     double total;
     const float* mt;
     const uint64_t* ct;
+    float edge;         // tokens above it are kept, those at it up to token `lim`
+    int lim;
 
     FIE_DEV RowDist(const KParams& P, int row)
         : rr(P.w.res[row]), mt(P.w.mt + (size_t)row * (P.NT + 1)), ct(P.w.ct + (size_t)row * (P.NT + 1))
     {
         total = u128_to_double(((u128)rr.khi << 64) | rr.klo);
+        // kept is: key >= tau and (key, index) >= cut in rank order; the later of the two decides
+        const uint32_t ck = comp_k(rr.cut);
+        const bool at_cut = rr.cut != 0 && ck >= rr.tau;
+        const uint32_t k = at_cut ? ck : rr.tau;
+        edge = k > kKeyNegInf ? key_to_float(k) : -__builtin_inff();
+        lim = at_cut ? (int)comp_idx(rr.cut) : 0x7FFFFFFF;
     }
     // a slot's share of the kept mass per unit of weight
     FIE_DEV float share(int slot) const { return total > 0.0 ? (float)((double)ct[slot] / total) : 0.0f; }
-    FIE_DEV bool kept(float y, int idx) const
+    FIE_DEV bool kept(float y, int idx) const { return y > edge || (y == edge && idx <= lim); }
+    // weight20(d) 2^20 floored is the token's weight, below 2^41
+    FIE_DEV float prob(float y, int idx, float m, float sh) const
     {
-        const uint64_t c = comp_key(fkey(y), (uint32_t)idx);
-        return comp_k(c) >= rr.tau && c >= rr.cut;
+        return kept(y, idx) ? __builtin_floorf(weight20(y - m) * 0x1p20f) * sh : 0.0f;
     }
-    FIE_DEV float prob(float y, int idx, float m, float sh) const { return kept(y, idx) ? weight40(y - m) * sh : 0.0f; }
 };
 
 FIE_DEV float row_scale(float x, float s) { return s == 1.0f ? x + 0.0f : scaled(x, s); }
@@ -149,25 +157,40 @@ __global__ __launch_bounds__(kVerThreads) void k_accept(const KParams P, const f
     }
 }
 
-// N tokens of a row of draft probabilities from e0 on; past V: 0.
+// N tokens of a row of draft probabilities from e0 on, as loaded; past V: 0.
 template <int QT, int N>
-FIE_DEV void load_q(float (&q)[N], const char* rowp, int e0, int V)
-{
-    constexpr int EPL = DTy<QT>::EPL;
-    if constexpr (N >= EPL) {
+struct DraftVec {
+    static constexpr int EPL = QT >= 0 ? DTy<QT < 0 ? 0 : QT>::EPL : N, G = N > EPL ? N / EPL : 1;
+    uint4 w[G];
+    FIE_DEV void load(const char* rowp, int e0, int V)
+    {
+        if constexpr (N >= EPL) {
 #pragma unroll
-        for (int g = 0; g < N / EPL; ++g) {
-            const uint4 w = load_group<QT>(rowp, e0 + g * EPL, V);
+            for (int g = 0; g < G; ++g) w[g] = load_group<QT>(rowp, e0 + g * EPL, V);
+        } else {            // four of eight 16-bit values
+            const uint16_t* p = (const uint16_t*)rowp + e0;
+            uint32_t h[4];
 #pragma unroll
-            for (int e = 0; e < EPL; ++e) q[g * EPL + e] = at_least_0(lane_get<QT>(w, e));
+            for (int e = 0; e < 4; ++e) h[e] = e0 + e < V ? p[e] : 0u;
+            w[0] = make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), 0, 0);
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) q[e] = e0 + e < V ? at_least_0(load_elem<QT>(rowp, (uint32_t)(e0 + e))) : 0.0f;
     }
+    FIE_DEV float get(int e) const { return at_least_0(lane_get<QT < 0 ? 0 : QT>(w[N >= EPL ? e / EPL : 0], N >= EPL ? e % EPL : e)); }
+};
+
+// What is left of a token, 2^-48 a unit, as two 24-bit parts: sums of 32 of each stay in 32 bits.
+struct Excess { uint32_t hi, lo; };
+FIE_DEV Excess excess_of(float p, float q)
+{
+    const float t = __builtin_fmaxf(p - q, 0.0f) * 0x1p24f;        // NaN: 0
+    return Excess{(uint32_t)t, (uint32_t)(__builtin_amdgcn_fractf(t) * 0x1p24f)};
 }
 
 // Grid (spans, requests).  QT: the draft's type, -1 without probabilities.
+//
+// Bound by the two rows' way from memory, so what the sampler's tile maxima rule out is not
+// read: a tile whose largest logit is below the row's edge, and q of a wave's tokens when none
+// of them is kept.
 template <int DT, int QT>
 __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const fie_verify_args v, const VerWs vw)
 {
@@ -190,6 +213,11 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
     const char* rowp = (const char*)a.logits + (size_t)row * (size_t)a.row_stride * SZ;
     const char* qp = nullptr;
     if constexpr (QT >= 0) qp = (const char*)v.draft_probs + (size_t)(q.first + n) * (size_t)v.draft_stride * DTy<QT>::SZ;
+    // the divide by Markstein's correction where it is exact, and where neither answer counts
+    // (an infinite logit's weight is 0 either way)
+    const float s = D.rr.s, rs = 1.0f / s;
+    const bool quick = s >= 0x1p-30f && s <= 0x1p30f;
+    const bool all = D.edge == -__builtin_inff() && D.lim == 0x7FFFFFFF;     // no filter
 
     auto count = [&](int lo) {             // the span's penalty counts
         __syncthreads();
@@ -202,65 +230,105 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
         }
         __syncthreads();
     };
-    // the excess of p over q at the EPL tokens from e0 on
-    auto excess = [&](int lo, int e0, uint64_t (&w)[EPL]) {
-        const uint4 raw = load_group<DT>(rowp, e0, V);
-        float qs[EPL];
-        if constexpr (QT >= 0) load_q<QT, EPL>(qs, qp, e0, V);
+    // the tile of the EPL tokens from e0 on holds none that is kept (one tile a workgroup)
+    auto below = [&](int e0) { return e0 >= V || D.mt[1 + e0 / kTile] < D.edge; };
+    // what p has over q at them, from the logits as loaded
+    auto excess = [&](int lo, int e0, uint4 raw, DraftVec<QT, EPL> dv, bool have_q, Excess (&w)[EPL]) {
         const int slot = 1 + min(e0, V - 1) / kTile;
         const float m = D.mt[slot], sh = D.share(slot);
+        float y[EPL];
+        bool odd = false, any = false;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            float x = lane_get<DT>(raw, e);
+            if (pen && e0 + e < V && cnt[e0 + e - lo]) x = penalize(x, rep, pres, freq, cnt[e0 + e - lo]);
+            const float ax = __builtin_fabsf(x);
+            odd |= (DT != FIE_F16 || pen) && ((ax < 0x1p-96f && ax > 0.0f) || (ax > 0x1p96f && ax < __builtin_inff()));
+            y[e] = x;
+        }
+        if (s == 1.0f) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) y[e] += 0.0f;
+        } else if (quick && __ballot(odd) == 0) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) y[e] = div_markstein(y[e], s, rs) + 0.0f;
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) y[e] = scaled(y[e], s);
+        }
+        if (e0 == 0) y[0] = D.mt[0];
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) any |= D.kept(y[e], e0 + e);
+        if (__ballot(any) == 0) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) w[e] = Excess{0, 0};
+            return;
+        }
+        if constexpr (QT >= 0)
+            if (!have_q) dv.load(qp, e0, V);
 #pragma unroll
         for (int e = 0; e < EPL; ++e) {
             const int idx = e0 + e;
-            float x = lane_get<DT>(raw, e);
-            if (pen && idx < V && cnt[idx - lo]) x = penalize(x, rep, pres, freq, cnt[idx - lo]);
-            float p = D.prob(row_scale(x, D.rr.s), idx, m, sh);
-            if (idx == 0) p = D.prob(D.mt[0], 0, D.mt[0], D.share(0));
+            float p = D.prob(y[e], idx, m, sh);
+            if (idx == 0) p = D.prob(y[0], 0, y[0], D.share(0));
             float qv;
-            if constexpr (QT >= 0) qv = qs[e];
+            if constexpr (QT >= 0) qv = dv.get(e);
             else qv = idx == draft ? 1.0f : 0.0f;
-            const float d = p - qv;
-            w[e] = idx < V && d > 0.0f ? (uint64_t)((double)d * 0x1p48) : 0ull;
+            w[e] = excess_of(idx < V ? p : 0.0f, qv);
         }
     };
 
     const int lo = blockIdx.x * kVerSpan;
     if (pen) count(lo);
-    uint64_t part = 0;
-#pragma unroll 1
-    for (int j = 0; j < NL; ++j) {
-        uint64_t w[EPL];
-        excess(lo, lo + (j * kVerThreads + tid) * EPL, w);
+    uint32_t hi = 0, lw = 0;
+    uint4 raw[NL];
+    DraftVec<QT, EPL> qs[NL];
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) part += w[e];
+    for (int j = 0; j < NL; ++j) {
+        const int g0 = lo + j * kVerThreads * EPL;
+        raw[j] = make_uint4(0, 0, 0, 0);
+        if (!below(g0) || g0 == 0) {                // token 0 is a tile of its own
+            raw[j] = load_group<DT>(rowp, g0 + tid * EPL, V);
+            if constexpr (QT >= 0)
+                if (all) qs[j].load(qp, g0 + tid * EPL, V);
+        }
     }
-    part = block_sum_u64<kVerThreads>(part, red);
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+        const int g0 = lo + j * kVerThreads * EPL;
+        if (below(g0) && g0 != 0) continue;
+        Excess w[EPL];
+        excess(lo, g0 + tid * EPL, raw[j], qs[j], all, w);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) { hi += w[e].hi; lw += w[e].lo; }
+    }
+    const uint64_t part = block_sum_u64<kVerThreads>(((uint64_t)hi << 24) + lw, red);
     uint64_t* sums = vw.sum + (size_t)r * spans;
     if (tid == 0) {
-        __hip_atomic_store(&sums[blockIdx.x], part, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last = __hip_atomic_fetch_add(&vw.arrived[r], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)spans - 1;
+        // the sum goes out by an exchange, which is back when it is where every XCD reads it;
+        // then the count.  (A release and acquire at device scope write back and invalidate
+        // whole caches: the kernel took 150 us for 133 refusals with them.)
+        uint64_t before = __hip_atomic_exchange(&sums[blockIdx.x], part, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" : "+v"(before)::"memory");
+        last = __hip_atomic_fetch_add(&vw.arrived[r], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)spans - 1;
     }
     __syncthreads();
     if (!last) return;
 
-    // the last span to arrive: the span the draw lands in, then the token
-    if (tid == 0) {
-        uint64_t total = 0;
-        for (int s = 0; s < spans; ++s) total += __hip_atomic_load(&sums[s], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        found = 0xFFFFFFFFu;
+    // the last span to arrive: the span the draw lands in, then the token (at most 64 spans)
+    if (tid < 64) {
+        const uint64_t x = tid < spans ? __hip_atomic_load(&sums[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0ull;
+        const uint64_t incl = dwave_incl_scan_u64(x);
+        const uint64_t total = shfl_u64(incl, 63);
         if (total) {
             const int32_t fl = a.flags[q.row + q.k] & ~FIE_FLAG_NO_DRAW;
             const double u = row_uniform(a, q.row + q.k, fl);
             uint64_t goal = u > 0.0 ? (uint64_t)(u * (double)total) : 0;
             if (goal >= total) goal = total - 1;
-            int s = 0;
-            for (; s < spans - 1; ++s) {
-                const uint64_t x = __hip_atomic_load(&sums[s], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (x > goal) break;
-                goal -= x;
-            }
-            found = (uint32_t)s;
-            left = goal;
+            const uint64_t over = __ballot(incl > goal);
+            if (tid == (int)__builtin_ctzll(over)) { found = (uint32_t)tid; left = goal - (incl - x); }
+        } else if (tid == 0) {
+            found = 0xFFFFFFFFu;
         }
     }
     __syncthreads();
@@ -272,32 +340,37 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
     const int at = (int)found * kVerSpan;
     if (pen) count(at);
     uint64_t goal = left;
-    for (int j = 0; j < NL; ++j) {
-        uint64_t w[EPL], mine = 0;
-        const int e0 = at + (j * kVerThreads + tid) * EPL;
-        excess(at, e0, w);
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) mine += w[e];
+    for (int j = 0; j < NL; ++j) raw[j] = load_group<DT>(rowp, at + (j * kVerThreads + tid) * EPL, V);
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+        const int e0 = at + (j * kVerThreads + tid) * EPL;
+        Excess w[EPL];
+        excess(at, e0, raw[j], qs[j], false, w);
+        uint64_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) mine += ((uint64_t)w[e].hi << 24) + w[e].lo;
         const uint64_t incl = dwave_incl_scan_u64(mine);
         __syncthreads();
         if ((tid & 63) == 63) red[tid >> 6] = incl;
         __syncthreads();
-        uint64_t before = 0, all = 0;
+        uint64_t before = 0, sum = 0;
         for (int i = 0; i < kVerThreads / 64; ++i) {
             if (i < (tid >> 6)) before += red[i];
-            all += red[i];
+            sum += red[i];
         }
         before += incl - mine;
         if (before <= goal && goal < before + mine) {          // one thread of one round
             uint64_t b = before;
 #pragma unroll
             for (int e = 0; e < EPL; ++e) {
-                if (b <= goal && goal < b + w[e]) *out = e0 + e;
-                b += w[e];
+                const uint64_t x = ((uint64_t)w[e].hi << 24) + w[e].lo;
+                if (b <= goal && goal < b + x) *out = e0 + e;
+                b += x;
             }
         }
-        if (goal < all) return;                                // the same in every thread
-        goal -= all;
+        if (goal < sum) return;                                // the same in every thread
+        goal -= sum;
     }
 }
 
