@@ -455,10 +455,8 @@ FIE_DEV float minp_bound(float mp)
     return key_to_float(hi);
 }
 
-FIE_DEV uint32_t minp_key(float M, float mp)
+FIE_DEV uint32_t minp_key_of(float M, float L)      // L = minp_bound(mp)
 {
-    if (!(mp > 0.0f)) return 0;
-    const float L = minp_bound(mp);
     uint32_t lo = kKeyNegInf, hi = fkey(M);
     if ((key_to_float(lo) - M) >= L) return lo;          // every value passes
     if (!((key_to_float(hi) - M) >= L)) return hi;       // degenerate rows (M not finite)
@@ -469,6 +467,8 @@ FIE_DEV uint32_t minp_key(float M, float mp)
     }
     return hi;
 }
+
+FIE_DEV uint32_t minp_key(float M, float mp) { return mp > 0.0f ? minp_key_of(M, minp_bound(mp)) : 0; }
 
 // ---------------------------------------------------------------- binned full-row path
 // Bins of a row by d = fl(M - y) at kDQ bins per unit (the last bin takes
@@ -1440,7 +1440,8 @@ FIE_DEV void finish_row(FinSmem& S, const KParams& P, const int row)
     // maxima, sums, candidate counts and bounds, token 0's logit and count, and
     // the candidate slots of the first kFinWaves * Q tiles (a tile's count
     // arrives with them, so all its slots are read and the invalid ones dropped).
-    const bool need_cand = !greedy || lp > 0;
+    const bool massonly = mass_only(a, row, fl);
+    const bool need_cand = (!greedy && !massonly) || lp > 0;
     const int lane = tid & 63, wave = tid >> 6;
     const size_t tbase = (size_t)row * NT + tid;
     const uint64_t pf_max = tid < NT ? P.w.maxc[tbase] : 0ull;
@@ -1472,6 +1473,8 @@ FIE_DEV void finish_row(FinSmem& S, const KParams& P, const int row)
         const int t = wave + kFinWaves * q;
         xs[q] = early && t < NT ? P.w.cand[((size_t)row * NT + t) * kCapW + lane] : 0ull;
     }
+    // min-p's bound, while the loads are on their way (its bisection is 3 us)
+    const float mpL = mp > 0.0f ? minp_bound(mp) : 0.0f;
     // Round 1: the row maximum, the safety bound and the candidate count, per wave.
     {
         const uint64_t wm = dwave_max_u64(pf_max);
@@ -1603,6 +1606,10 @@ FIE_DEV void finish_row(FinSmem& S, const KParams& P, const int row)
         token = comp_idx(best);
         tok_comp = best;
         T = comp_weight(S, best);
+    } else if (massonly) {
+        // the first of the largest logits before scaling, which may make others equal to it
+        token = kxm > k0 ? comp_idx(xm) : 0;
+        T = sall;
     }
 
     // Candidates as y-domain composites, sorted: every token whose scaled key
@@ -1639,6 +1646,12 @@ FIE_DEV void finish_row(FinSmem& S, const KParams& P, const int row)
                 // selections can reach go to S.cand (narrowing is cheap here, so
                 // rows narrow from kNarrowRegs candidates on)
                 int bs = kPassBins;
+                if (nv > kNarrowRegs && mp > 0.0f && topk == 0 && cnt == 0) {
+                    // min-p alone: what it drops is not sorted (where it drops nothing that
+                    // may lie past the candidates)
+                    const uint32_t tmp = minp_key_of(M, mpL);
+                    if (tmp > safe) bs = dbin_key(M, tmp);
+                }
                 if (nv > kNarrowRegs && (cnt > 0 || by_mass) && !(mp > 0.0f) && !(by_mass && sall == 0)) {
                     const int b = binned_bound(S, cnt, by_mass, g);
                     if (b >= 0) bs = b;
@@ -1671,7 +1684,7 @@ FIE_DEV void finish_row(FinSmem& S, const KParams& P, const int row)
     // narrowed prefix holds every crossing by construction; should a cut or draw
     // still miss it, that is not a verdict: every candidate is then loaded and
     // sorted and the selection runs again.
-    if (!greedy && !deep) {
+    if (!greedy && !massonly && !deep) {
         for (;;) {
             const bool partial = nv < nvall;
             bool miss = false;
@@ -1681,7 +1694,7 @@ FIE_DEV void finish_row(FinSmem& S, const KParams& P, const int row)
                 if (nv < topk) deep = true;
                 else tk = comp_k(S.cand[topk - 1]);
             }
-            const uint32_t tmp = minp_key(M, mp);
+            const uint32_t tmp = mp > 0.0f ? minp_key_of(M, mpL) : 0;
             tau = tk > tmp ? tk : tmp;
             if (!deep && tau != 0 && tau <= safe) deep = true;
             if (!deep) {
@@ -2013,7 +2026,8 @@ static_assert(kHBins == kPassBins && kHBins == 2 * kFinThreads, "two bins per th
 
 FIE_DEV bool helped_row(const KParams& P, int row)
 {
-    if (P.a.flags[row] & FIE_FLAG_GREEDY) return false;
+    const int32_t fl = P.a.flags[row];
+    if ((fl & FIE_FLAG_GREEDY) || mass_only(P.a, row, fl)) return false;
     const int k = P.a.top_k[row];
     return k == 0 || k > kHelpTopK;
 }

@@ -149,9 +149,8 @@ __global__ __launch_bounds__(kVerThreads) void k_accept(const KParams P, const f
     if (tid == 0) {
         v.accepted[r] = n;
         vw.arrived[r] = 0;
-        // no draw left: every draft kept, a greedy row, or a row without mass
-        const RowRes& rr = P.w.res[q.row + n];
-        const bool done = n == q.k || rr.greedy || (rr.klo | rr.khi) == 0;
+        // no draw left: every draft kept, or a greedy row
+        const bool done = n == q.k || P.w.res[q.row + n].greedy;
         vw.at[r] = done ? -1 : n;
         if (done) out[n] = a.tokens[q.row + n];
     }
@@ -334,7 +333,22 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
     __syncthreads();
     int64_t* out = v.tokens + (size_t)r * (v.max_drafts + 1) + n;
     if (found == 0xFFFFFFFFu) {
-        if (tid == 0) *out = a.tokens[row];
+        // nothing: the most likely token, as FINISH has it, or the first of those that a row
+        // settled by its mass alone has at its largest scaled logit
+        uint32_t best = 0xFFFFFFFFu;
+        if (mass_only(a, row, a.flags[row])) {
+            if (tid == 0 && D.mt[0] == D.rr.M) best = 0;
+            for (int l = 0; l < V; l += kVerSpan) {
+                if (pen) count(l);
+                for (int i = l + tid; i < min(l + kVerSpan, V); i += kVerThreads) {
+                    float x = load_elem<DT>(rowp, (uint32_t)i);
+                    if (pen && cnt[i - l]) x = penalize(x, rep, pres, freq, cnt[i - l]);
+                    if (i > 0 && row_scale(x, s) == D.rr.M && (uint32_t)i < best) best = (uint32_t)i;
+                }
+            }
+            best = block_min_u32<kVerThreads>(best, (uint32_t*)red);
+        }
+        if (tid == 0) *out = best < (uint32_t)V ? (int64_t)best : a.tokens[row];
         return;
     }
     const int at = (int)found * kVerSpan;

@@ -47,8 +47,9 @@ enum {
     FIE_FLAG_GREEDY = 1,    /* SamplingParams.greedy (sampling.py:71-74) */
     FIE_FLAG_PENALTY = 2,   /* SamplingParams.has_penalties (sampling.py:76-79) */
     FIE_FLAG_NO_DRAW = 4,   /* the row's draw is not wanted: its token is its most likely one (a
-                               draw of 0), its thresholds and masses are what they are.  For rows
-                               that fie_sampler_verify tests a draft on */
+                               draw of 0; without filters, one of those that scaling makes equal
+                               to it), its thresholds and masses are what they are.  For rows that
+                               fie_sampler_verify tests a draft on */
 };
 
 /* Per-row status bits written to fie_sampler_args.status (informational). */

@@ -232,6 +232,31 @@ def test_odd_draft_values(verifier):
     check(verifier, x, [SamplingParams(temperature=1.0)] * 8, lens, ids, q, 42)
 
 
+def test_nothing_left_gives_the_first_of_equal_tokens(verifier):
+    """p never over q on rows without filters, where the divide by the temperature makes two
+    logits equal: the lower index, though its logit is the smaller."""
+    V, s = 20000, np.float32(1.7)
+    hi = np.float32(7.0)                 # 7 / 1.7 is past 4: its unit is hi's own
+    for _ in range(100):
+        if hi / s == np.nextafter(hi, np.float32(0)) / s:
+            break
+        hi = np.nextafter(hi, np.float32(8))
+    assert hi / s == np.nextafter(hi, np.float32(0)) / s
+    lo = np.nextafter(hi, np.float32(0))
+    gen = torch.Generator().manual_seed(4)
+    x = torch.randn(8, V, generator=gen)
+    for r, (i, j) in enumerate([(12000, 300), (19999, 0), (0, 7), (9000, 8999)]):
+        x[2 * r, i], x[2 * r, j] = float(hi), float(lo)
+    q = torch.full((4, V), 2.0)
+    pen = SamplingParams(temperature=1.7, presence_penalty=0.5)
+    for params, ctx in (([SamplingParams(temperature=1.7)] * 4, None), ([pen] * 4, [[50, 51]] * 4)):
+        plan = verifier.plan(params, [1] * 4, V, ctx, [[5]] * 4)
+        got = verifier.verify(plan, x.to(DEV), torch.full((4,), 5, device=DEV), torch.full((8,), 0.6, dtype=torch.float64, device=DEV),
+                              q.to(DEV))
+        assert got.accepted.tolist() == [0] * 4
+        assert got.tokens[:, 0].tolist() == [300, 0, 0, 8999]
+
+
 def test_strides_and_alignment(verifier):
     V = 4099
     x, ids, q = make(51, 12, LENS, V, torch.bfloat16, True)
