@@ -14,42 +14,52 @@ namespace fie {
 constexpr int kVerThreads = 256;
 constexpr int kVerSpan = 8192;             // tokens a workgroup of k_refused
 
-// What k_accept leaves for k_refused, in workspace arrays that the sampler is done with.
-struct VerWs {
-    int32_t* at;        // [requests] the refused draft, -1: nothing left to draw
-    uint32_t* arrived;  // [requests]
-    uint64_t* sum;      // [requests * spans]
+// A draw that k_accept leaves for k_refused: all that its workgroups need, in one place (they
+// are a chain of dependent loads otherwise: 2 refusals took 16-22 us, the draws themselves 8).
+struct VerJob {
+    double total;       // the row's kept mass
+    double u;
+    int64_t draft;      // the refused draft, of all drafts
+    int64_t id;
+    int64_t* out;       // where the token goes
+    int32_t row;        // -1: nothing to draw
+    int32_t lim;
+    float edge, s;
 };
 
-// A row's distribution as the sampler left it.
-struct RowDist {
-    RowRes rr;
-    double total;
-    const float* mt;
-    const uint64_t* ct;
-    float edge;         // tokens above it are kept, those at it up to token `lim`
-    int lim;
+// In workspace arrays that the sampler is done with.
+struct VerWs {
+    VerJob* job;        // [requests]
+    uint32_t* arrived;  // [requests]
+    uint64_t* sum;      // [requests * tiles]
+};
+static_assert(sizeof(VerJob) <= sizeof(DeferRec), "jobs go where the deferred rows' records were");
 
-    FIE_DEV RowDist(const KParams& P, int row)
-        : rr(P.w.res[row]), mt(P.w.mt + (size_t)row * (P.NT + 1)), ct(P.w.ct + (size_t)row * (P.NT + 1))
+// What of a row is kept: tokens above `edge`, and those at it up to token `lim`.  (The sampler's
+// rule is key >= tau and (key, index) >= cut in rank order; the later of the two decides.)
+struct Kept {
+    float edge;
+    int lim;
+    FIE_DEV Kept(float e, int l) : edge(e), lim(l) {}
+    FIE_DEV explicit Kept(const RowRes& rr)
     {
-        total = u128_to_double(((u128)rr.khi << 64) | rr.klo);
-        // kept is: key >= tau and (key, index) >= cut in rank order; the later of the two decides
         const uint32_t ck = comp_k(rr.cut);
         const bool at_cut = rr.cut != 0 && ck >= rr.tau;
         const uint32_t k = at_cut ? ck : rr.tau;
         edge = k > kKeyNegInf ? key_to_float(k) : -__builtin_inff();
         lim = at_cut ? (int)comp_idx(rr.cut) : 0x7FFFFFFF;
     }
-    // a slot's share of the kept mass per unit of weight
-    FIE_DEV float share(int slot) const { return total > 0.0 ? (float)((double)ct[slot] / total) : 0.0f; }
-    FIE_DEV bool kept(float y, int idx) const { return y > edge || (y == edge && idx <= lim); }
-    // weight20(d) 2^20 floored is the token's weight, below 2^41
-    FIE_DEV float prob(float y, int idx, float m, float sh) const
-    {
-        return kept(y, idx) ? __builtin_floorf(weight20(y - m) * 0x1p20f) * sh : 0.0f;
-    }
+    FIE_DEV bool operator()(float y, int idx) const { return y > edge || (y == edge && idx <= lim); }
+    FIE_DEV bool all() const { return edge == -__builtin_inff() && lim == 0x7FFFFFFF; }
 };
+
+FIE_DEV double mass_of(const RowRes& rr) { return u128_to_double(((u128)rr.khi << 64) | rr.klo); }
+
+// A tile's share of the kept mass per unit of weight.
+FIE_DEV float share_of(uint64_t ct, double total) { return total > 0.0 ? (float)((double)ct / total) : 0.0f; }
+
+// A kept token's probability: its weight (below 2^41; weight20 2^20, floored) by the share.
+FIE_DEV float prob_of(float y, float m, float share) { return __builtin_floorf(weight20(y - m) * 0x1p20f) * share; }
 
 FIE_DEV float row_scale(float x, float s) { return s == 1.0f ? x + 0.0f : scaled(x, s); }
 
@@ -102,7 +112,7 @@ __global__ __launch_bounds__(kVerThreads) void k_accept(const KParams P, const f
     Request q;
     if (!request_of(P, v, r, &q)) {                            // the same in every thread
         for (int j = tid; j <= v.max_drafts; j += kVerThreads) out[j] = -1;
-        if (tid == 0) { v.accepted[r] = -1; vw.at[r] = -1; }
+        if (tid == 0) { v.accepted[r] = -1; vw.job[r].row = -1; }
         return;
     }
     if (a.apply_penalties) {
@@ -123,21 +133,20 @@ __global__ __launch_bounds__(kVerThreads) void k_accept(const KParams P, const f
         id = v.draft_ids[q.first + tid];
         float p = 0.0f, qd = 0.0f;
         if (id >= 0 && id < V) {
-            const RowDist D(P, row);
-            if (D.rr.greedy) {
-                p = id == D.rr.token ? 1.0f : 0.0f;
-            } else {
-                float y = D.mt[0];
-                int slot = 0;
-                if (id != 0) {
-                    float x = load_elem<DT>((const char*)a.logits + (size_t)row * (size_t)a.row_stride * DTy<DT>::SZ, (uint32_t)id);
-                    if (a.apply_penalties && cnt[tid]) x = penalize(x, a.repetition[row], a.presence[row], a.frequency[row], cnt[tid]);
-                    y = row_scale(x, D.rr.s);
-                    slot = 1 + (int)id / kTile;
-                }
-                p = D.prob(y, (int)id, D.mt[slot], D.share(slot));
-            }
+            const RowRes rr = P.w.res[row];
+            const size_t slot = (size_t)row * (P.NT + 1) + (id ? 1 + (int)id / kTile : 0);
+            const float m = P.w.mt[slot];
+            const uint64_t ct = P.w.ct[slot];
+            const char* rowp = (const char*)a.logits + (size_t)row * (size_t)a.row_stride * DTy<DT>::SZ;
+            float x = load_elem<DT>(rowp, (uint32_t)id);
             qd = v.draft_probs ? draft_prob(v, q.first + tid, id) : 1.0f;
+            if (rr.greedy) {
+                p = id == rr.token ? 1.0f : 0.0f;
+            } else {
+                if (a.apply_penalties && cnt[tid]) x = penalize(x, a.repetition[row], a.presence[row], a.frequency[row], cnt[tid]);
+                const float y = id ? row_scale(x, rr.s) : m;        // token 0 is a tile of its own
+                p = Kept(rr)(y, (int)id) ? prob_of(y, m, share_of(ct, mass_of(rr))) : 0.0f;
+            }
         }
         if (v.target_probs) v.target_probs[q.first + tid] = p;
         const double u = row_uniform(a, row, fl & ~FIE_FLAG_NO_DRAW);
@@ -150,9 +159,25 @@ __global__ __launch_bounds__(kVerThreads) void k_accept(const KParams P, const f
         v.accepted[r] = n;
         vw.arrived[r] = 0;
         // no draw left: every draft kept, or a greedy row
-        const bool done = n == q.k || P.w.res[q.row + n].greedy;
-        vw.at[r] = done ? -1 : n;
-        if (done) out[n] = a.tokens[q.row + n];
+        const RowRes rr = P.w.res[q.row + n];
+        VerJob job{};
+        job.row = -1;
+        if (n == q.k || rr.greedy) {
+            out[n] = a.tokens[q.row + n];
+        } else {
+            const Kept kept(rr);
+            const int last = q.row + q.k;
+            job.total = mass_of(rr);
+            job.u = row_uniform(a, last, a.flags[last] & ~FIE_FLAG_NO_DRAW);
+            job.draft = q.first + n;
+            job.id = v.draft_ids[job.draft];
+            job.out = out + n;
+            job.row = q.row + n;
+            job.lim = kept.lim;
+            job.edge = kept.edge;
+            job.s = rr.s;
+        }
+        vw.job[r] = job;
     }
 }
 
@@ -195,28 +220,28 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
 {
     constexpr int EPL = DTy<DT>::EPL, SZ = DTy<DT>::SZ, NL = kVerSpan / kVerThreads / EPL;
     __shared__ uint32_t cnt[kVerSpan];
-    __shared__ uint64_t red[kVerThreads / 64];
+    constexpr int WV = kVerThreads / 64;
+    __shared__ uint64_t red[WV], tile_part[kVerSpan / kTile][WV];
     __shared__ uint64_t left;
     __shared__ uint32_t found, last;
     const fie_sampler_args& a = P.a;
     const int r = blockIdx.y, tid = threadIdx.x, V = a.vocab, spans = gridDim.x;
-    const int n = vw.at[r];
-    if (n < 0) return;
-    Request q;
-    request_of(P, v, r, &q);
-    const int row = q.row + n;
-    const RowDist D(P, row);
+    const VerJob J = vw.job[r];
+    if (J.row < 0) return;
+    const int row = J.row;
+    const Kept kept(J.edge, J.lim);
+    const float* mt = P.w.mt + (size_t)row * (P.NT + 1);
+    const uint64_t* ct = P.w.ct + (size_t)row * (P.NT + 1);
     const bool pen = a.apply_penalties && (a.flags[row] & FIE_FLAG_PENALTY);
     const float rep = pen ? a.repetition[row] : 1.0f, pres = pen ? a.presence[row] : 0.0f, freq = pen ? a.frequency[row] : 0.0f;
-    const int64_t draft = v.draft_ids[q.first + n];
     const char* rowp = (const char*)a.logits + (size_t)row * (size_t)a.row_stride * SZ;
     const char* qp = nullptr;
-    if constexpr (QT >= 0) qp = (const char*)v.draft_probs + (size_t)(q.first + n) * (size_t)v.draft_stride * DTy<QT>::SZ;
+    if constexpr (QT >= 0) qp = (const char*)v.draft_probs + (size_t)J.draft * (size_t)v.draft_stride * DTy<QT>::SZ;
     // the divide by Markstein's correction where it is exact, and where neither answer counts
     // (an infinite logit's weight is 0 either way)
-    const float s = D.rr.s, rs = 1.0f / s;
+    const float s = J.s, rs = 1.0f / s;
     const bool quick = s >= 0x1p-30f && s <= 0x1p30f;
-    const bool all = D.edge == -__builtin_inff() && D.lim == 0x7FFFFFFF;     // no filter
+    const bool all = kept.all();            // no filter
 
     auto count = [&](int lo) {             // the span's penalty counts
         __syncthreads();
@@ -229,12 +254,28 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
         }
         __syncthreads();
     };
-    // the tile of the EPL tokens from e0 on holds none that is kept (one tile a workgroup)
-    auto below = [&](int e0) { return e0 >= V || D.mt[1 + e0 / kTile] < D.edge; };
-    // what p has over q at them, from the logits as loaded
-    auto excess = [&](int lo, int e0, uint4 raw, DraftVec<QT, EPL> dv, bool have_q, Excess (&w)[EPL]) {
-        const int slot = 1 + min(e0, V - 1) / kTile;
-        const float m = D.mt[slot], sh = D.share(slot);
+    // a span's tiles: their largest scaled logits and their shares
+    constexpr int TPS = kVerSpan / kTile;
+    struct Tiles { float m[TPS], share[TPS]; };
+    auto tiles_of = [&](int lo) {
+        Tiles t;
+        uint64_t c[TPS];
+#pragma unroll
+        for (int i = 0; i < TPS; ++i) {
+            const int slot = min(1 + lo / kTile + i, P.NT);
+            t.m[i] = mt[slot];
+            c[i] = ct[slot];
+        }
+#pragma unroll
+        for (int i = 0; i < TPS; ++i) t.share[i] = share_of(c[i], J.total);
+        return t;
+    };
+    const float m0 = mt[0];
+    const uint64_t c0 = ct[0];
+    constexpr int GPT = kTile / (kVerThreads * EPL);       // groups of the workgroup a tile
+    // what p has over q at the EPL tokens from e0 on, in a tile with maximum m, from the logits
+    // as loaded
+    auto excess = [&](int lo, int e0, float m, float sh, uint4 raw, DraftVec<QT, EPL> dv, bool have_q, Excess (&w)[EPL]) {
         float y[EPL];
         bool odd = false, any = false;
 #pragma unroll
@@ -255,9 +296,9 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
 #pragma unroll
             for (int e = 0; e < EPL; ++e) y[e] = scaled(y[e], s);
         }
-        if (e0 == 0) y[0] = D.mt[0];
+        if (e0 == 0) y[0] = m0;             // token 0 is a tile of its own
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) any |= D.kept(y[e], e0 + e);
+        for (int e = 0; e < EPL; ++e) any |= kept(y[e], e0 + e);
         if (__ballot(any) == 0) {
 #pragma unroll
             for (int e = 0; e < EPL; ++e) w[e] = Excess{0, 0};
@@ -268,99 +309,127 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
 #pragma unroll
         for (int e = 0; e < EPL; ++e) {
             const int idx = e0 + e;
-            float p = D.prob(y[e], idx, m, sh);
-            if (idx == 0) p = D.prob(y[0], 0, y[0], D.share(0));
+            float p = prob_of(y[e], m, sh);
+            if (idx == 0) p = prob_of(m0, m0, share_of(c0, J.total));
+            if (!kept(y[e], idx)) p = 0.0f;
             float qv;
             if constexpr (QT >= 0) qv = dv.get(e);
-            else qv = idx == draft ? 1.0f : 0.0f;
+            else qv = idx == J.id ? 1.0f : 0.0f;
             w[e] = excess_of(idx < V ? p : 0.0f, qv);
         }
     };
 
     const int lo = blockIdx.x * kVerSpan;
     if (pen) count(lo);
-    uint32_t hi = 0, lw = 0;
-    uint4 raw[NL];
-    DraftVec<QT, EPL> qs[NL];
+    {
+        const Tiles t = tiles_of(lo);
+        // a tile all below the edge holds nothing (token 0's own tile aside)
+        auto skip = [&](int i) { return lo + i * kTile >= V || (t.m[i] < kept.edge && lo + i * kTile != 0); };
+        uint4 raw[NL];
+        DraftVec<QT, EPL> qs[NL];
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-        const int g0 = lo + j * kVerThreads * EPL;
-        raw[j] = make_uint4(0, 0, 0, 0);
-        if (!below(g0) || g0 == 0) {                // token 0 is a tile of its own
-            raw[j] = load_group<DT>(rowp, g0 + tid * EPL, V);
-            if constexpr (QT >= 0)
-                if (all) qs[j].load(qp, g0 + tid * EPL, V);
+        for (int j = 0; j < NL; ++j) {
+            const int e0 = lo + (j * kVerThreads + tid) * EPL;
+            raw[j] = make_uint4(0, 0, 0, 0);
+            if (!skip(j / GPT)) {
+                raw[j] = load_group<DT>(rowp, e0, V);
+                if constexpr (QT >= 0)
+                    if (all) qs[j].load(qp, e0, V);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < TPS; ++i) {
+            uint64_t part = 0;
+            if (!skip(i)) {
+                uint32_t hi = 0, lw = 0;
+#pragma unroll
+                for (int j = i * GPT; j < (i + 1) * GPT; ++j) {
+                    Excess w[EPL];
+                    excess(lo, lo + (j * kVerThreads + tid) * EPL, t.m[i], t.share[i], raw[j], qs[j], all, w);
+#pragma unroll
+                    for (int e = 0; e < EPL; ++e) { hi += w[e].hi; lw += w[e].lo; }
+                }
+                part = dwave_sum_u64(((uint64_t)hi << 24) + lw);
+            }
+            if ((tid & 63) == 0) tile_part[i][tid >> 6] = part;
         }
     }
+    __syncthreads();
+    uint64_t* sums = vw.sum + (size_t)r * P.NT;
+    if (tid < 64) {
+        // the tiles' sums go out by exchanges, which are back when they are where every XCD
+        // reads them; then the count.  (A release and acquire at device scope write back and
+        // invalidate whole caches: the kernel took 150 us for 133 refusals with them.)
+        const int tile = lo / kTile + tid;
+        if (tid < TPS && tile < P.NT) {
+            uint64_t part = 0;
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-        const int g0 = lo + j * kVerThreads * EPL;
-        if (below(g0) && g0 != 0) continue;
-        Excess w[EPL];
-        excess(lo, g0 + tid * EPL, raw[j], qs[j], all, w);
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) { hi += w[e].hi; lw += w[e].lo; }
-    }
-    const uint64_t part = block_sum_u64<kVerThreads>(((uint64_t)hi << 24) + lw, red);
-    uint64_t* sums = vw.sum + (size_t)r * spans;
-    if (tid == 0) {
-        // the sum goes out by an exchange, which is back when it is where every XCD reads it;
-        // then the count.  (A release and acquire at device scope write back and invalidate
-        // whole caches: the kernel took 150 us for 133 refusals with them.)
-        uint64_t before = __hip_atomic_exchange(&sums[blockIdx.x], part, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        asm volatile("s_waitcnt vmcnt(0)" : "+v"(before)::"memory");
-        last = __hip_atomic_fetch_add(&vw.arrived[r], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)spans - 1;
+            for (int i = 0; i < WV; ++i) part += tile_part[tid][i];
+            uint64_t before = __hip_atomic_exchange(&sums[tile], part, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            asm volatile("s_waitcnt vmcnt(0)" : "+v"(before)::"memory");
+        }
+        if (tid == 0)
+            last = __hip_atomic_fetch_add(&vw.arrived[r], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)spans - 1;
     }
     __syncthreads();
     if (!last) return;
 
-    // the last span to arrive: the span the draw lands in, then the token (at most 64 spans)
-    if (tid < 64) {
-        const uint64_t x = tid < spans ? __hip_atomic_load(&sums[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0ull;
-        const uint64_t incl = dwave_incl_scan_u64(x);
-        const uint64_t total = shfl_u64(incl, 63);
-        if (total) {
-            const int32_t fl = a.flags[q.row + q.k] & ~FIE_FLAG_NO_DRAW;
-            const double u = row_uniform(a, q.row + q.k, fl);
-            uint64_t goal = u > 0.0 ? (uint64_t)(u * (double)total) : 0;
-            if (goal >= total) goal = total - 1;
-            const uint64_t over = __ballot(incl > goal);
-            if (tid == (int)__builtin_ctzll(over)) { found = (uint32_t)tid; left = goal - (incl - x); }
-        } else if (tid == 0) {
-            found = 0xFFFFFFFFu;
+    // the last span to arrive: the tile the draw lands in, then the token
+    {
+        static_assert(kMaxTiles <= kVerThreads, "a thread a tile");
+        const uint64_t x = tid < P.NT ? __hip_atomic_load(&sums[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0ull;
+        uint64_t incl = dwave_incl_scan_u64(x);
+        if ((tid & 63) == 63) red[tid >> 6] = incl;
+        if (tid == 0) found = 0xFFFFFFFFu;
+        __syncthreads();
+        uint64_t total = 0;
+#pragma unroll
+        for (int i = 0; i < WV; ++i) {
+            if (i < (tid >> 6)) incl += red[i];
+            total += red[i];
         }
+        uint64_t goal = J.u > 0.0 ? (uint64_t)(J.u * (double)total) : 0;
+        if (goal >= total) goal = total - 1;
+        if (total && incl - x <= goal && goal < incl) { found = (uint32_t)tid; left = goal - (incl - x); }
     }
     __syncthreads();
-    int64_t* out = v.tokens + (size_t)r * (v.max_drafts + 1) + n;
     if (found == 0xFFFFFFFFu) {
         // nothing: the most likely token, as FINISH has it, or the first of those that a row
         // settled by its mass alone has at its largest scaled logit
         uint32_t best = 0xFFFFFFFFu;
         if (mass_only(a, row, a.flags[row])) {
-            if (tid == 0 && D.mt[0] == D.rr.M) best = 0;
+            const float M = P.w.res[row].M;
+            if (tid == 0 && m0 == M) best = 0;
             for (int l = 0; l < V; l += kVerSpan) {
                 if (pen) count(l);
                 for (int i = l + tid; i < min(l + kVerSpan, V); i += kVerThreads) {
                     float x = load_elem<DT>(rowp, (uint32_t)i);
                     if (pen && cnt[i - l]) x = penalize(x, rep, pres, freq, cnt[i - l]);
-                    if (i > 0 && row_scale(x, s) == D.rr.M && (uint32_t)i < best) best = (uint32_t)i;
+                    if (i > 0 && row_scale(x, s) == M && (uint32_t)i < best) best = (uint32_t)i;
                 }
             }
             best = block_min_u32<kVerThreads>(best, (uint32_t*)red);
         }
-        if (tid == 0) *out = best < (uint32_t)V ? (int64_t)best : a.tokens[row];
+        if (tid == 0) *J.out = best < (uint32_t)V ? (int64_t)best : a.tokens[row];
         return;
     }
-    const int at = (int)found * kVerSpan;
+    const int at = (int)found * kTile;
     if (pen) count(at);
+    const float m = mt[1 + found], share = share_of(ct[1 + found], J.total);
+    uint4 raw[GPT];
+    DraftVec<QT, EPL> qs[GPT];
+#pragma unroll
+    for (int j = 0; j < GPT; ++j) {
+        const int e0 = at + (j * kVerThreads + tid) * EPL;
+        raw[j] = load_group<DT>(rowp, e0, V);
+        if constexpr (QT >= 0) qs[j].load(qp, e0, V);
+    }
     uint64_t goal = left;
 #pragma unroll
-    for (int j = 0; j < NL; ++j) raw[j] = load_group<DT>(rowp, at + (j * kVerThreads + tid) * EPL, V);
-#pragma unroll
-    for (int j = 0; j < NL; ++j) {
+    for (int j = 0; j < GPT; ++j) {
         const int e0 = at + (j * kVerThreads + tid) * EPL;
         Excess w[EPL];
-        excess(at, e0, raw[j], qs[j], false, w);
+        excess(at, e0, m, share, raw[j], qs[j], true, w);
         uint64_t mine = 0;
 #pragma unroll
         for (int e = 0; e < EPL; ++e) mine += ((uint64_t)w[e].hi << 24) + w[e].lo;
@@ -368,18 +437,17 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
         __syncthreads();
         if ((tid & 63) == 63) red[tid >> 6] = incl;
         __syncthreads();
-        uint64_t before = 0, sum = 0;
-        for (int i = 0; i < kVerThreads / 64; ++i) {
-            if (i < (tid >> 6)) before += red[i];
+        uint64_t b = incl - mine, sum = 0;
+#pragma unroll
+        for (int i = 0; i < WV; ++i) {
+            if (i < (tid >> 6)) b += red[i];
             sum += red[i];
         }
-        before += incl - mine;
-        if (before <= goal && goal < before + mine) {          // one thread of one round
-            uint64_t b = before;
+        if (b <= goal && goal < b + mine) {                    // one thread
 #pragma unroll
             for (int e = 0; e < EPL; ++e) {
                 const uint64_t x = ((uint64_t)w[e].hi << 24) + w[e].lo;
-                if (b <= goal && goal < b + x) *out = e0 + e;
+                if (b <= goal && goal < b + x) *J.out = e0 + e;
                 b += x;
             }
         }
