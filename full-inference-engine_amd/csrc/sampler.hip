@@ -506,6 +506,7 @@ int fie_sampler_verify(const fie_sampler_args* args, const fie_verify_args* v, c
             return fail(FIE_E_ARG, "unknown draft dtype");
         if (v->draft_probs && v->draft_stride < args->vocab) return fail(FIE_E_ARG, "draft_stride < vocab");
     }
+    if (v->draws && args->vocab <= FIE_VERIFY_DRAWS_VOCAB) return fail(FIE_E_ARG, "draws of the last rows need a larger vocabulary");
     if (v->requests > 0 && (!v->draft_offsets || !v->tokens || !v->accepted))
         return fail(FIE_E_ARG, "a required pointer is NULL");
     KParams P;

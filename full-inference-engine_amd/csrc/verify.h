@@ -23,15 +23,17 @@ struct VerJob {
     int64_t id;
     int64_t* out;       // where the token goes
     int32_t row;        // -1: nothing to draw
-    int32_t lim;
-    float edge, s;
+    int32_t lim;        // a refusal's; kRankDraw: a draw of the row in rank order instead
+    float edge, s;      // edge: a rank draw's bins a unit
 };
+constexpr int kRankDraw = -1;
 
 // In workspace arrays that the sampler is done with.
 struct VerWs {
     VerJob* job;        // [requests]
     uint32_t* arrived;  // [requests]
     uint64_t* sum;      // [requests * tiles]
+    uint64_t* sum_hi;   // [requests * tiles]
 };
 static_assert(sizeof(VerJob) <= sizeof(DeferRec), "jobs go where the deferred rows' records were");
 
@@ -99,6 +101,102 @@ FIE_DEV uint32_t history_count(const fie_sampler_args& a, int row, uint32_t id, 
     return dwave_sum_u32(n);
 }
 
+// A row as the kernels that go over it by spans see it.
+template <int DT>
+struct SpanRow {
+    static constexpr int EPL = DTy<DT>::EPL;
+    static constexpr int TPS = kVerSpan / kTile;                    // tiles a span
+    static constexpr int GPT = kTile / (kVerThreads * EPL);         // groups of the workgroup a tile
+    static constexpr int NL = TPS * GPT;                            // ... a span
+    const KParams& P;
+    int row;
+    bool pen, quick;
+    float rep, pres, freq, s, rs;
+    const char* rowp;
+    const float* mt;        // the tiles' largest scaled logits, token 0's first
+    const uint64_t* ct;     // their scales
+    float m0;
+    uint32_t* cnt;          // kVerSpan of the workgroup's LDS: a span's penalty counts
+
+    FIE_DEV SpanRow(const KParams& P_, int row_, float s_, uint32_t* cnt_) : P(P_), row(row_), s(s_), cnt(cnt_)
+    {
+        const fie_sampler_args& a = P.a;
+        mt = P.w.mt + (size_t)row * (P.NT + 1);
+        ct = P.w.ct + (size_t)row * (P.NT + 1);
+        m0 = mt[0];
+        pen = a.apply_penalties && (a.flags[row] & FIE_FLAG_PENALTY);
+        rep = pen ? a.repetition[row] : 1.0f;
+        pres = pen ? a.presence[row] : 0.0f;
+        freq = pen ? a.frequency[row] : 0.0f;
+        rowp = (const char*)a.logits + (size_t)row * (size_t)a.row_stride * DTy<DT>::SZ;
+        // the divide by Markstein's correction where it is exact, and where neither answer
+        // counts (an infinite logit's weight is 0 either way)
+        rs = 1.0f / s;
+        quick = s >= 0x1p-30f && s <= 0x1p30f;
+    }
+    FIE_DEV uint4 load(int e0) const { return load_group<DT>(rowp, e0, P.a.vocab); }
+
+    FIE_DEV void count(int lo) const
+    {
+        const fie_sampler_args& a = P.a;
+        __syncthreads();
+        for (int i = threadIdx.x; i < kVerSpan; i += kVerThreads) cnt[i] = 0;
+        __syncthreads();
+        const int64_t h1 = hist_end(a, row);
+        for (int64_t h = a.hist_offsets[row] + threadIdx.x; h < h1; h += kVerThreads) {
+            const uint32_t id = (uint32_t)a.hist_ids[h];
+            if (id >= (uint32_t)lo && id - (uint32_t)lo < (uint32_t)kVerSpan && id < (uint32_t)a.vocab) atomicAdd(&cnt[id - lo], 1u);
+        }
+        __syncthreads();
+    }
+    // The scaled logits of the EPL tokens from e0 on, as loaded, of the span (or tile) from lo
+    // on that was counted last.
+    FIE_DEV void values(int lo, int e0, const uint4& raw, float (&y)[EPL]) const
+    {
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            float x = lane_get<DT>(raw, e);
+            if (pen && e0 + e < P.a.vocab && cnt[e0 + e - lo]) x = penalize(x, rep, pres, freq, cnt[e0 + e - lo]);
+            const float ax = __builtin_fabsf(x);
+            odd |= (DT != FIE_F16 || pen) && ((ax < 0x1p-96f && ax > 0.0f) || (ax > 0x1p96f && ax < __builtin_inff()));
+            y[e] = x;
+        }
+        if (s == 1.0f) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) y[e] += 0.0f;
+        } else if (quick && __ballot(odd) == 0) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) y[e] = div_markstein(y[e], s, rs) + 0.0f;
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) y[e] = scaled(y[e], s);
+        }
+        if (e0 == 0) y[0] = m0;             // token 0 is a tile of its own
+    }
+};
+
+// After its own stores and atomics at device scope, a workgroup counts itself in; true in every
+// thread of the last of `all`.
+FIE_DEV bool arrive_last(uint32_t* count, uint32_t all, uint32_t* flag)
+{
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0)
+        *flag = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1;
+    __syncthreads();
+    return *flag != 0;
+}
+
+template <typename T> FIE_DEV T from_all(const T* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename T> FIE_DEV void to_all(T* p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+}  // namespace fie
+
+#include "verify_draw.h"
+
+namespace fie {
+
 // One workgroup a request: draft j by thread j; on rows with penalties the draft's
 // occurrences in the row's history are counted first, a wave a draft.
 template <int DT>
@@ -155,27 +253,36 @@ __global__ __launch_bounds__(kVerThreads) void k_accept(const KParams P, const f
     const int n = (int)min(block_min_u32<kVerThreads>(refused, red), (uint32_t)q.k);
     if (tid < n) out[tid] = id;
     if (tid > n && tid <= v.max_drafts) out[tid] = -1;
+    // A request that keeps every draft and whose last row carries FIE_FLAG_NO_DRAW is drawn from
+    // by the passes of verify_draw.h.
+    const int end = q.row + q.k;
+    const bool rank = v.draws && n == q.k && mass_only(a, end, a.flags[end]);
+    if (rank) rank_begin(P, end, red);
     if (tid == 0) {
         v.accepted[r] = n;
         vw.arrived[r] = 0;
-        // no draw left: every draft kept, or a greedy row
+        // no draw left: every draft kept (and the last row drawn from), or a greedy row
         const RowRes rr = P.w.res[q.row + n];
+        const bool none = rank ? (rr.klo | rr.khi) == 0 : n == q.k || rr.greedy;
         VerJob job{};
         job.row = -1;
-        if (n == q.k || rr.greedy) {
+        if (none) {
             out[n] = a.tokens[q.row + n];
         } else {
             const Kept kept(rr);
-            const int last = q.row + q.k;
             job.total = mass_of(rr);
-            job.u = row_uniform(a, last, a.flags[last] & ~FIE_FLAG_NO_DRAW);
-            job.draft = q.first + n;
-            job.id = v.draft_ids[job.draft];
+            job.u = row_uniform(a, end, a.flags[end] & ~FIE_FLAG_NO_DRAW);
             job.out = out + n;
             job.row = q.row + n;
-            job.lim = kept.lim;
-            job.edge = kept.edge;
             job.s = rr.s;
+            if (rank) {
+                job.lim = kRankDraw;
+            } else {
+                job.draft = q.first + n;
+                job.id = v.draft_ids[job.draft];
+                job.lim = kept.lim;
+                job.edge = kept.edge;
+            }
         }
         vw.job[r] = job;
     }
@@ -219,7 +326,7 @@ template <int DT, int QT>
 __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const fie_verify_args v, const VerWs vw)
 {
     constexpr int EPL = DTy<DT>::EPL, SZ = DTy<DT>::SZ, NL = kVerSpan / kVerThreads / EPL;
-    __shared__ uint32_t cnt[kVerSpan];
+    extern __shared__ uint32_t cnt[];       // kVerSpan with penalties
     constexpr int WV = kVerThreads / 64;
     __shared__ uint64_t red[WV], tile_part[kVerSpan / kTile][WV];
     __shared__ uint64_t left;
@@ -228,34 +335,19 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
     const int r = blockIdx.y, tid = threadIdx.x, V = a.vocab, spans = gridDim.x;
     const VerJob J = vw.job[r];
     if (J.row < 0) return;
+    if (J.lim == kRankDraw) {
+        rank_pass<DT, 1>(P, vw, r, J, cnt);
+        return;
+    }
     const int row = J.row;
     const Kept kept(J.edge, J.lim);
-    const float* mt = P.w.mt + (size_t)row * (P.NT + 1);
-    const uint64_t* ct = P.w.ct + (size_t)row * (P.NT + 1);
-    const bool pen = a.apply_penalties && (a.flags[row] & FIE_FLAG_PENALTY);
-    const float rep = pen ? a.repetition[row] : 1.0f, pres = pen ? a.presence[row] : 0.0f, freq = pen ? a.frequency[row] : 0.0f;
-    const char* rowp = (const char*)a.logits + (size_t)row * (size_t)a.row_stride * SZ;
+    const SpanRow<DT> R(P, row, J.s, cnt);
     const char* qp = nullptr;
     if constexpr (QT >= 0) qp = (const char*)v.draft_probs + (size_t)J.draft * (size_t)v.draft_stride * DTy<QT>::SZ;
-    // the divide by Markstein's correction where it is exact, and where neither answer counts
-    // (an infinite logit's weight is 0 either way)
-    const float s = J.s, rs = 1.0f / s;
-    const bool quick = s >= 0x1p-30f && s <= 0x1p30f;
     const bool all = kept.all();            // no filter
 
-    auto count = [&](int lo) {             // the span's penalty counts
-        __syncthreads();
-        for (int i = tid; i < kVerSpan; i += kVerThreads) cnt[i] = 0;
-        __syncthreads();
-        const int64_t h1 = hist_end(a, row);
-        for (int64_t h = a.hist_offsets[row] + tid; h < h1; h += kVerThreads) {
-            const uint32_t id = (uint32_t)a.hist_ids[h];
-            if (id >= (uint32_t)lo && id - (uint32_t)lo < (uint32_t)kVerSpan && id < (uint32_t)V) atomicAdd(&cnt[id - lo], 1u);
-        }
-        __syncthreads();
-    };
     // a span's tiles: their largest scaled logits and their shares
-    constexpr int TPS = kVerSpan / kTile;
+    constexpr int TPS = SpanRow<DT>::TPS, GPT = SpanRow<DT>::GPT;
     struct Tiles { float m[TPS], share[TPS]; };
     auto tiles_of = [&](int lo) {
         Tiles t;
@@ -263,40 +355,21 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
 #pragma unroll
         for (int i = 0; i < TPS; ++i) {
             const int slot = min(1 + lo / kTile + i, P.NT);
-            t.m[i] = mt[slot];
-            c[i] = ct[slot];
+            t.m[i] = R.mt[slot];
+            c[i] = R.ct[slot];
         }
 #pragma unroll
         for (int i = 0; i < TPS; ++i) t.share[i] = share_of(c[i], J.total);
         return t;
     };
-    const float m0 = mt[0];
-    const uint64_t c0 = ct[0];
-    constexpr int GPT = kTile / (kVerThreads * EPL);       // groups of the workgroup a tile
+    const float m0 = R.m0;
+    const uint64_t c0 = R.ct[0];
     // what p has over q at the EPL tokens from e0 on, in a tile with maximum m, from the logits
     // as loaded
     auto excess = [&](int lo, int e0, float m, float sh, uint4 raw, DraftVec<QT, EPL> dv, bool have_q, Excess (&w)[EPL]) {
         float y[EPL];
-        bool odd = false, any = false;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            float x = lane_get<DT>(raw, e);
-            if (pen && e0 + e < V && cnt[e0 + e - lo]) x = penalize(x, rep, pres, freq, cnt[e0 + e - lo]);
-            const float ax = __builtin_fabsf(x);
-            odd |= (DT != FIE_F16 || pen) && ((ax < 0x1p-96f && ax > 0.0f) || (ax > 0x1p96f && ax < __builtin_inff()));
-            y[e] = x;
-        }
-        if (s == 1.0f) {
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) y[e] += 0.0f;
-        } else if (quick && __ballot(odd) == 0) {
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) y[e] = div_markstein(y[e], s, rs) + 0.0f;
-        } else {
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) y[e] = scaled(y[e], s);
-        }
-        if (e0 == 0) y[0] = m0;             // token 0 is a tile of its own
+        bool any = false;
+        R.values(lo, e0, raw, y);
 #pragma unroll
         for (int e = 0; e < EPL; ++e) any |= kept(y[e], e0 + e);
         if (__ballot(any) == 0) {
@@ -320,7 +393,7 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
     };
 
     const int lo = blockIdx.x * kVerSpan;
-    if (pen) count(lo);
+    if (R.pen) R.count(lo);
     {
         const Tiles t = tiles_of(lo);
         // a tile all below the edge holds nothing (token 0's own tile aside)
@@ -332,7 +405,7 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
             const int e0 = lo + (j * kVerThreads + tid) * EPL;
             raw[j] = make_uint4(0, 0, 0, 0);
             if (!skip(j / GPT)) {
-                raw[j] = load_group<DT>(rowp, e0, V);
+                raw[j] = R.load(e0);
                 if constexpr (QT >= 0)
                     if (all) qs[j].load(qp, e0, V);
             }
@@ -366,18 +439,15 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
 #pragma unroll
             for (int i = 0; i < WV; ++i) part += tile_part[tid][i];
             uint64_t before = __hip_atomic_exchange(&sums[tile], part, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            asm volatile("s_waitcnt vmcnt(0)" : "+v"(before)::"memory");
+            asm volatile("" : "+v"(before));
         }
-        if (tid == 0)
-            last = __hip_atomic_fetch_add(&vw.arrived[r], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)spans - 1;
     }
-    __syncthreads();
-    if (!last) return;
+    if (!arrive_last(&vw.arrived[r], (uint32_t)spans, &last)) return;
 
     // the last span to arrive: the tile the draw lands in, then the token
     {
         static_assert(kMaxTiles <= kVerThreads, "a thread a tile");
-        const uint64_t x = tid < P.NT ? __hip_atomic_load(&sums[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0ull;
+        const uint64_t x = tid < P.NT ? from_all(&sums[tid]) : 0ull;
         uint64_t incl = dwave_incl_scan_u64(x);
         if ((tid & 63) == 63) red[tid >> 6] = incl;
         if (tid == 0) found = 0xFFFFFFFFu;
@@ -401,11 +471,11 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
             const float M = P.w.res[row].M;
             if (tid == 0 && m0 == M) best = 0;
             for (int l = 0; l < V; l += kVerSpan) {
-                if (pen) count(l);
+                if (R.pen) R.count(l);
                 for (int i = l + tid; i < min(l + kVerSpan, V); i += kVerThreads) {
-                    float x = load_elem<DT>(rowp, (uint32_t)i);
-                    if (pen && cnt[i - l]) x = penalize(x, rep, pres, freq, cnt[i - l]);
-                    if (i > 0 && row_scale(x, s) == M && (uint32_t)i < best) best = (uint32_t)i;
+                    float x = load_elem<DT>(R.rowp, (uint32_t)i);
+                    if (R.pen && cnt[i - l]) x = penalize(x, R.rep, R.pres, R.freq, cnt[i - l]);
+                    if (i > 0 && row_scale(x, J.s) == M && (uint32_t)i < best) best = (uint32_t)i;
                 }
             }
             best = block_min_u32<kVerThreads>(best, (uint32_t*)red);
@@ -414,14 +484,14 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
         return;
     }
     const int at = (int)found * kTile;
-    if (pen) count(at);
-    const float m = mt[1 + found], share = share_of(ct[1 + found], J.total);
+    if (R.pen) R.count(at);
+    const float m = R.mt[1 + found], share = share_of(R.ct[1 + found], J.total);
     uint4 raw[GPT];
     DraftVec<QT, EPL> qs[GPT];
 #pragma unroll
     for (int j = 0; j < GPT; ++j) {
         const int e0 = at + (j * kVerThreads + tid) * EPL;
-        raw[j] = load_group<DT>(rowp, e0, V);
+        raw[j] = R.load(e0);
         if constexpr (QT >= 0) qs[j].load(qp, e0, V);
     }
     uint64_t goal = left;

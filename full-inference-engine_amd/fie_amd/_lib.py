@@ -23,6 +23,7 @@ LP_COLS = 20
 TILE = 8192
 MAX_VOCAB = 64 * TILE
 MAX_DRAFTS = 255
+VERIFY_DRAWS_VOCAB = 63488
 
 _vp = ctypes.c_void_p
 
@@ -49,7 +50,7 @@ class VerifyArgs(ctypes.Structure):
 
     _fields_ = [
         ("requests", ctypes.c_int32), ("max_drafts", ctypes.c_int32), ("draft_offsets", _vp), ("draft_ids", _vp),
-        ("draft_probs", _vp), ("draft_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("draft_probs", _vp), ("draft_dtype", ctypes.c_int32), ("draws", ctypes.c_int32),
         ("draft_stride", ctypes.c_int64), ("tokens", _vp), ("accepted", _vp), ("target_probs", _vp),
     ]
 

@@ -22,7 +22,7 @@ import torch
 from . import _lib
 from ._lib import VerifyArgs
 from .batching.sampler import resolve_params
-from .kernel import _DTYPES, DeviceStep, FusedSampler
+from .kernel import _DTYPES, FLAG_GREEDY, HELP_ROWS, DeviceStep, FusedSampler
 from .runtime.sampling import SamplingParams
 
 FLAG_NO_DRAW = _lib.FIE_FLAG_NO_DRAW
@@ -72,6 +72,13 @@ class VerifyPlan:
         last = np.cumsum(lens + 1) - 1
         no_draw = np.full(self.rows, FLAG_NO_DRAW, dtype=np.int32)
         no_draw[last] = 0
+        # last rows without filters: the verification draws from them (the sampler's own kernels
+        # do better on the few rows that get span helpers, and on small vocabularies)
+        draws = self.rows > HELP_ROWS and vocab > _lib.VERIFY_DRAWS_VOCAB
+        if draws:
+            plain = ((hp.flags[last] & FLAG_GREEDY) == 0) & (hp.top_k[last] == 0) & (hp.top_p[last] >= 1.0) & (hp.min_p[last] <= 0.0)
+            no_draw[last[plain]] = FLAG_NO_DRAW
+            draws = bool(plain.any())
         hp.flags = hp.flags | no_draw
         self._offsets = torch.zeros(self.requests + 1, dtype=torch.int64)
         np.cumsum(lens, out=self._offsets.numpy()[1:])
@@ -93,7 +100,7 @@ class VerifyPlan:
         self.args = a
         v = VerifyArgs()
         v.requests, v.max_drafts = self.requests, self.max_drafts
-        v.draft_offsets = self._offsets.data_ptr()
+        v.draft_offsets, v.draws = self._offsets.data_ptr(), int(draws)
         self.verify_args = v
 
 

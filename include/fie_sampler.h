@@ -208,7 +208,8 @@ int fie_sampler_kept(const fie_sampler_args* args, uint8_t* kept, float* probs,
    Request r has k_r = draft_offsets[r + 1] - draft_offsets[r] drafts d_0 .. d_{k-1} and
    k_r + 1 rows of logits, one after another from row draft_offsets[r] + r on: row j is the
    model's answer after j drafts.  The sampler's args describe these rows (its rows = drafts
-   + requests), with FIE_FLAG_NO_DRAW on every row but a request's last, and one draw u a row.
+   + requests), with FIE_FLAG_NO_DRAW on every row but a request's last (and see `draws`), and
+   one draw u a row.
    With p the row's kept distribution (weights over kept mass, fp32) and q the draft's (all
    on d_j without draft_probs):
      d_j is kept iff u_j * q(d_j) < p(d_j), a product in double, and every draft before it was
@@ -226,13 +227,17 @@ typedef struct fie_verify_args {
     const int64_t* draft_ids;      /* [drafts] (NULL without drafts) */
     const void* draft_probs;       /* [drafts, vocab], rows draft_stride elements apart, or NULL */
     int32_t draft_dtype;           /* FIE_F32 / FIE_F16 / FIE_BF16 */
-    int32_t reserved;
+    int32_t draws;                 /* 1: last rows without filters may carry FIE_FLAG_NO_DRAW too, and
+                                      are drawn from after the test, spans side by side (vocab past
+                                      FIE_VERIFY_DRAWS_VOCAB); with more than 16 rows much faster
+                                      where such a draw lies deep */
     int64_t draft_stride;
     int64_t* tokens;               /* [requests, max_drafts + 1]: kept drafts, one more token, -1 */
     int32_t* accepted;             /* [requests] kept drafts */
     float* target_probs;           /* [drafts] p(d_j), or NULL */
 } fie_verify_args;
 #define FIE_MAX_DRAFTS 255
+#define FIE_VERIFY_DRAWS_VOCAB 63488
 
 /* fie_sampler_sample on the rows, then the verification, on one stream. */
 int fie_sampler_verify(const fie_sampler_args* args, const fie_verify_args* verify,

@@ -257,6 +257,95 @@ def test_nothing_left_gives_the_first_of_equal_tokens(verifier):
         assert got.tokens[:, 0].tolist() == [300, 0, 0, 8999]
 
 
+def kept_drafts(x, lens):
+    """Draft ids and certain-to-be-kept uniforms: the argmax of each drafted row, u = 0."""
+    last = np.zeros(len(x), bool)
+    last[np.cumsum(np.array(lens) + 1) - 1] = True
+    return last, x.float().argmax(1)[torch.from_numpy(~last)]
+
+
+@pytest.mark.parametrize("kind", ["peaked", "flat", "flatter", "grid", "equal", "two", "masked", "one", "steep", "tiles"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_draws_without_filters(verifier, kind, dtype):
+    """Every draft kept, then the draw in rank order over the whole row: the canonical draw, bit
+    for bit, at places all over the row, where the spans are counted side by side."""
+    V, R = 70001, 24
+    lens = [1, 0] * (R // 2)
+    gen = torch.Generator().manual_seed(len(kind))
+    x = torch.randn(sum(lens) + R, V, generator=gen)
+    if kind == "peaked":
+        x = 0.5 * x - 1.1 * torch.log(1.0 + torch.argsort(torch.rand(len(x), V, generator=gen), 1).float())
+    elif kind == "flat":
+        x = 0.3 * x
+    elif kind == "flatter":
+        x = 0.01 * x
+    elif kind == "grid":
+        x = torch.round(2.0 * x)
+    elif kind == "equal":
+        x = torch.full_like(x, -3.25)
+    elif kind == "two":
+        x = torch.where(x > 0.5, 1.0, 1.0 - 2.0 ** -6)
+    elif kind == "masked":
+        x[torch.rand(len(x), V, generator=gen) < 0.9] = float("-inf")
+        x[::2, :40000] = torch.finfo(dtype).min
+    elif kind == "one":
+        x[:] = float("-inf")
+        x[:, 51111] = 2.0
+    elif kind == "steep":
+        x = 12.0 * x
+    elif kind == "tiles":                        # one tile far above the rest
+        x[:, 4096:6144] += 25.0
+    x = x.to(dtype)
+    last, ids = kept_drafts(x, lens)
+    params = [SamplingParams(temperature=t) for t in (1.0, 0.7, 1.7)] * (R // 3)
+    rows = [p for p, n in zip(params, lens) for _ in range(n + 1)]
+    u = np.zeros(len(rows))
+    spots = np.concatenate([[0.0, 1.0 - 2.0 ** -53, 0.5, 1e-9, 1.0 - 1e-9], np.random.default_rng(5).random(R - 5)])
+    u[last] = spots
+    want = O.canonical_step(x.float().numpy(), O.resolve(rows, V), u)
+    plan = verifier.plan(params, lens, V)
+    assert plan.verify_args.draws == 1
+    got = verifier.verify(plan, x.to(DEV), ids.to(DEV), torch.from_numpy(u).to(DEV))
+    assert got.accepted.tolist() == lens
+    drawn = got.tokens.gather(1, got.accepted.long()[:, None])[:, 0].cpu().numpy()
+    np.testing.assert_array_equal(drawn, want.tokens[last])
+
+
+def test_draws_without_filters_count_penalties(verifier):
+    V, R = 80000, 20
+    lens = [2, 0] * (R // 2)
+    gen = torch.Generator().manual_seed(77)
+    x = (0.5 * torch.randn(sum(lens) + R, V, generator=gen)).to(torch.bfloat16)
+    rng = np.random.default_rng(6)
+    contexts = [rng.integers(0, V, 3000).tolist() + [0] for _ in range(R)]
+    pen = [SamplingParams(temperature=0.9, repetition_penalty=1.3, frequency_penalty=0.4)] * R
+    last = np.zeros(len(x), bool)
+    last[np.cumsum(np.array(lens) + 1) - 1] = True
+    ids = torch.from_numpy(rng.integers(0, V, sum(lens)))
+    u, tokens, accepted, _ = plain(x.float().numpy(), pen, lens, ids.numpy(), None, rng, contexts)
+    plan = verifier.plan(pen, lens, V, contexts, [ids[2 * (i // 2):2 * (i // 2) + n].tolist() for i, n in enumerate(lens)])
+    assert plan.verify_args.draws == 1
+    got = verifier.verify(plan, x.to(DEV), ids.to(DEV), torch.from_numpy(u).to(DEV))
+    np.testing.assert_array_equal(got.accepted.cpu().numpy(), accepted)
+    np.testing.assert_array_equal(got.tokens.cpu().numpy(), tokens)
+
+
+def test_a_draw_past_the_candidates_at_a_middle_key(verifier):
+    """Many tokens of a few keys in one part of one bin: the search over the keys."""
+    V, R = 66000, 20
+    x = torch.zeros(R, V)
+    base = torch.tensor(5.0)
+    for i in range(6):                                    # six neighbouring fp32 values
+        x[:, i::6] = base
+        base = torch.nextafter(base, torch.tensor(0.0))
+    u = np.random.default_rng(8).random(R)
+    params = [SamplingParams(temperature=1.0)] * R
+    want = O.canonical_step(x.numpy(), O.resolve(params, V), u)
+    plan = verifier.plan(params, [0] * R, V)
+    got = verifier.verify(plan, x.to(DEV), torch.zeros(0, dtype=torch.int64, device=DEV), torch.from_numpy(u).to(DEV))
+    np.testing.assert_array_equal(got.tokens[:, 0].cpu().numpy(), want.tokens)
+
+
 def test_strides_and_alignment(verifier):
     V = 4099
     x, ids, q = make(51, 12, LENS, V, torch.bfloat16, True)
