@@ -2,9 +2,9 @@
 //
 // k_accept tests a request's drafts: p(d_j) from the row's thresholds, tile maxima and kept
 // mass, which the sampler left in the workspace.  k_refused draws the token of a refusal from
-// what the row's p has over the draft's q, over one row of logits and one of q a request:
-// 8192-token spans sum the excess as whole numbers (fixed point, 2^-48: sums have no order),
-// and the last span of a request to arrive finds the span and the token the draw lands in.
+// what the row's p has over the draft's q, over one row of logits and one of q a request: spans
+// sum the excess as whole numbers (fixed point, 2^-48: sums have no order), and the last span
+// of a request to arrive finds the tile and the token the draw lands in.
 #pragma once
 
 #include "launchers.h"
@@ -12,7 +12,7 @@
 namespace fie {
 
 constexpr int kVerThreads = 256;
-constexpr int kVerSpan = 8192;             // tokens a workgroup of k_refused
+constexpr int kVerTiles = 4;               // tiles a workgroup of k_refused and k_rank, or one
 
 // A draw that k_accept leaves for k_refused: all that its workgroups need, in one place (they
 // are a chain of dependent loads otherwise: 2 refusals took 16-22 us, the draws themselves 8).
@@ -102,10 +102,9 @@ FIE_DEV uint32_t history_count(const fie_sampler_args& a, int row, uint32_t id, 
 }
 
 // A row as the kernels that go over it by spans see it.
-template <int DT>
+template <int DT, int TPS_>
 struct SpanRow {
-    static constexpr int EPL = DTy<DT>::EPL;
-    static constexpr int TPS = kVerSpan / kTile;                    // tiles a span
+    static constexpr int EPL = DTy<DT>::EPL, TPS = TPS_, kSpanV = TPS * kTile;     // tiles, tokens a span
     static constexpr int GPT = kTile / (kVerThreads * EPL);         // groups of the workgroup a tile
     static constexpr int NL = TPS * GPT;                            // ... a span
     const KParams& P;
@@ -116,7 +115,7 @@ struct SpanRow {
     const float* mt;        // the tiles' largest scaled logits, token 0's first
     const uint64_t* ct;     // their scales
     float m0;
-    uint32_t* cnt;          // kVerSpan of the workgroup's LDS: a span's penalty counts
+    uint32_t* cnt;          // the workgroup's LDS: a span's penalty counts
 
     FIE_DEV SpanRow(const KParams& P_, int row_, float s_, uint32_t* cnt_) : P(P_), row(row_), s(s_), cnt(cnt_)
     {
@@ -140,12 +139,12 @@ struct SpanRow {
     {
         const fie_sampler_args& a = P.a;
         __syncthreads();
-        for (int i = threadIdx.x; i < kVerSpan; i += kVerThreads) cnt[i] = 0;
+        for (int i = threadIdx.x; i < kSpanV; i += kVerThreads) cnt[i] = 0;
         __syncthreads();
         const int64_t h1 = hist_end(a, row);
         for (int64_t h = a.hist_offsets[row] + threadIdx.x; h < h1; h += kVerThreads) {
             const uint32_t id = (uint32_t)a.hist_ids[h];
-            if (id >= (uint32_t)lo && id - (uint32_t)lo < (uint32_t)kVerSpan && id < (uint32_t)a.vocab) atomicAdd(&cnt[id - lo], 1u);
+            if (id >= (uint32_t)lo && id - (uint32_t)lo < (uint32_t)kSpanV && id < (uint32_t)a.vocab) atomicAdd(&cnt[id - lo], 1u);
         }
         __syncthreads();
     }
@@ -322,13 +321,13 @@ FIE_DEV Excess excess_of(float p, float q)
 // Bound by the two rows' way from memory, so what the sampler's tile maxima rule out is not
 // read: a tile whose largest logit is below the row's edge, and q of a wave's tokens when none
 // of them is kept.
-template <int DT, int QT>
+template <int DT, int QT, int TPS>
 __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const fie_verify_args v, const VerWs vw)
 {
-    constexpr int EPL = DTy<DT>::EPL, SZ = DTy<DT>::SZ, NL = kVerSpan / kVerThreads / EPL;
-    extern __shared__ uint32_t cnt[];       // kVerSpan with penalties
+    constexpr int EPL = DTy<DT>::EPL, SZ = DTy<DT>::SZ, NL = TPS * kTile / kVerThreads / EPL;
+    extern __shared__ uint32_t cnt[];       // a span's, with penalties
     constexpr int WV = kVerThreads / 64;
-    __shared__ uint64_t red[WV], tile_part[kVerSpan / kTile][WV];
+    __shared__ uint64_t red[WV], tile_part[TPS][WV];
     __shared__ uint64_t left;
     __shared__ uint32_t found, last;
     const fie_sampler_args& a = P.a;
@@ -336,18 +335,18 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
     const VerJob J = vw.job[r];
     if (J.row < 0) return;
     if (J.lim == kRankDraw) {
-        rank_pass<DT, 1>(P, vw, r, J, cnt);
+        rank_pass<DT, 1, TPS>(P, vw, r, J, cnt);
         return;
     }
     const int row = J.row;
     const Kept kept(J.edge, J.lim);
-    const SpanRow<DT> R(P, row, J.s, cnt);
+    const SpanRow<DT, TPS> R(P, row, J.s, cnt);
     const char* qp = nullptr;
     if constexpr (QT >= 0) qp = (const char*)v.draft_probs + (size_t)J.draft * (size_t)v.draft_stride * DTy<QT>::SZ;
     const bool all = kept.all();            // no filter
 
     // a span's tiles: their largest scaled logits and their shares
-    constexpr int TPS = SpanRow<DT>::TPS, GPT = SpanRow<DT>::GPT;
+    constexpr int GPT = SpanRow<DT, TPS>::GPT, kSpanV = TPS * kTile;
     struct Tiles { float m[TPS], share[TPS]; };
     auto tiles_of = [&](int lo) {
         Tiles t;
@@ -392,7 +391,7 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
         }
     };
 
-    const int lo = blockIdx.x * kVerSpan;
+    const int lo = blockIdx.x * kSpanV;
     if (R.pen) R.count(lo);
     {
         const Tiles t = tiles_of(lo);
@@ -470,9 +469,9 @@ __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const 
         if (mass_only(a, row, a.flags[row])) {
             const float M = P.w.res[row].M;
             if (tid == 0 && m0 == M) best = 0;
-            for (int l = 0; l < V; l += kVerSpan) {
+            for (int l = 0; l < V; l += kSpanV) {
                 if (R.pen) R.count(l);
-                for (int i = l + tid; i < min(l + kVerSpan, V); i += kVerThreads) {
+                for (int i = l + tid; i < min(l + kSpanV, V); i += kVerThreads) {
                     float x = load_elem<DT>(R.rowp, (uint32_t)i);
                     if (R.pen && cnt[i - l]) x = penalize(x, R.rep, R.pres, R.freq, cnt[i - l]);
                     if (i > 0 && row_scale(x, J.s) == M && (uint32_t)i < best) best = (uint32_t)i;

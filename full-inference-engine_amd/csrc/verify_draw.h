@@ -127,10 +127,10 @@ FIE_DEV void rank_find(RankState& S, u128 goal, u128* red)
 }
 
 // One pass of one span; grid (spans, requests).
-template <int DT, int PASS>
+template <int DT, int PASS, int TPS>
 FIE_DEV void rank_pass(const KParams& P, const VerWs& vw, int r, const VerJob& J, uint32_t* cnt)
 {
-    typedef SpanRow<DT> Row;
+    typedef SpanRow<DT, TPS> Row;
     constexpr int EPL = Row::EPL, WV = kVerThreads / 64, GPT = Row::GPT;
     __shared__ uint64_t blo[kRankBins], bhi[kRankBins];     // the last pass: the list, and its masses
     __shared__ u128 red[WV], left;
@@ -141,7 +141,7 @@ FIE_DEV void rank_pass(const KParams& P, const VerWs& vw, int r, const VerJob& J
     const float M = S.M, f = S.f;
     const int b1 = S.b1;
     const RankRange in = rank_range(PASS, f, b1, S.b2);
-    const int lo = blockIdx.x * kVerSpan;
+    const int lo = blockIdx.x * Row::kSpanV;
     if (PASS < 3)
         for (int i = tid; i < kRankBins; i += kVerThreads) { blo[i] = 0; bhi[i] = 0; }
     if (tid < Row::TPS) tiles[tid] = 0;
@@ -329,13 +329,13 @@ FIE_DEV void rank_pass(const KParams& P, const VerWs& vw, int r, const VerJob& J
     }
 }
 
-template <int DT, int PASS>
+template <int DT, int PASS, int TPS>
 __global__ __launch_bounds__(kVerThreads) void k_rank(const KParams P, const VerWs vw)
 {
-    extern __shared__ uint32_t cnt[];       // kVerSpan with penalties
+    extern __shared__ uint32_t cnt[];       // a span's, with penalties
     const VerJob J = vw.job[blockIdx.y];
     if (J.row < 0 || J.lim != kRankDraw) return;
-    rank_pass<DT, PASS>(P, vw, blockIdx.y, J, cnt);
+    rank_pass<DT, PASS, TPS>(P, vw, blockIdx.y, J, cnt);
 }
 
 }  // namespace fie

@@ -207,6 +207,31 @@ def test_penalised_rows_count_their_drafts(verifier):
         check(verifier, x, pen, lens, ids, probs, 22, contexts)
 
 
+@pytest.mark.parametrize("V, times", [(20001, 40), (70001, 12)])
+@pytest.mark.parametrize("penalties", [False, True])
+def test_large_batches_answer_as_small_ones(verifier, V, times, penalties):
+    """The same requests many times over (another split of the rows over workgroups), the small
+    batch checked against 64 bits."""
+    params = [SamplingParams(temperature=1.0), SamplingParams(temperature=0.7, top_p=0.9)] * 6
+    if penalties:
+        params = [SamplingParams(temperature=p.temperature, top_p=p.top_p, presence_penalty=0.3, repetition_penalty=1.2)
+                  for p in params]
+    x, ids, q = make(V, 12, LENS, V, torch.bfloat16, True)
+    rng = np.random.default_rng(V)
+    contexts = [rng.integers(1, V, 200).tolist() for _ in range(12)] if penalties else None
+    u, tokens, accepted, _ = plain(x.float().numpy(), params, LENS, ids.numpy(), q.numpy(), rng, contexts)
+    drafts, at = [], 0
+    for n in LENS:
+        drafts.append(ids[at:at + n].tolist())
+        at += n
+    g = [x.to(DEV), ids.to(DEV), torch.from_numpy(u).to(DEV), q.to(DEV)]
+    for n in (1, times):
+        plan = verifier.plan(params * n, LENS * n, V, None if contexts is None else contexts * n, drafts * n)
+        got = verifier.verify(plan, g[0].repeat(n, 1), g[1].repeat(n), g[2].repeat(n), g[3].repeat(n, 1))
+        np.testing.assert_array_equal(got.accepted.cpu().numpy(), np.tile(accepted, n))
+        np.testing.assert_array_equal(got.tokens.cpu().numpy(), np.tile(tokens, (n, 1)))
+
+
 def test_longest_drafts(verifier):
     lens = [MAX_DRAFTS, 0, 200]
     x, ids, q = make(31, 3, lens, 300, torch.float32, True)
