@@ -11,6 +11,25 @@
 
 namespace fie {
 
+// One 16-byte group of elements [e0, e0 + EPL) of a row, those at or past `width` 0.  Where the
+// row ends inside it, the row's last 16 bytes are loaded and shifted down (element by element
+// this one group cost a row of 2050 as much as all others: 9.0 us for 333 of them).
+template <int DT>
+FIE_DEV uint4 load_row16(const char* rowp, int e0, int width)
+{
+    constexpr int EPL = DTy<DT>::EPL, SZ = DTy<DT>::SZ;
+    if (width < EPL) return load_group<DT>(rowp, e0, width);
+    // the load itself on no branch, so that all of a thread's are on their way together
+    uint4 r = load16<DT>(rowp + (int64_t)min(e0, width - EPL) * SZ);
+    if (e0 + EPL > width) {
+        const int past = min(e0 + EPL - width, EPL);
+        const u128 v = ((u128)r.w << 96) | ((u128)r.z << 64) | ((u128)r.y << 32) | r.x;
+        const u128 t = past < EPL ? v >> (8 * SZ * past) : 0;
+        r = make_uint4((uint32_t)t, (uint32_t)(t >> 32), (uint32_t)(t >> 64), (uint32_t)(t >> 96));
+    }
+    return r;
+}
+
 // 8 elements from e0 on, as loaded; those at or past `width` are 0.
 template <int DT> struct Vec8 { uint4 r[DT == FIE_F32 ? 2 : 1]; };
 
@@ -18,8 +37,8 @@ template <int DT>
 FIE_DEV Vec8<DT> load8(const char* rowp, int e0, int width)
 {
     Vec8<DT> v;
-    v.r[0] = load_group<DT>(rowp, e0, width);
-    if constexpr (DT == FIE_F32) v.r[1] = load_group<DT>(rowp, e0 + 4, width);
+    v.r[0] = load_row16<DT>(rowp, e0, width);
+    if constexpr (DT == FIE_F32) v.r[1] = load_row16<DT>(rowp, e0 + 4, width);
     return v;
 }
 
@@ -30,7 +49,7 @@ FIE_DEV float get8(const Vec8<DT>& v, int e)
     else return lane_get<DT>(v.r[0], e);
 }
 
-// A parameter vector: in DT, or in fp32.
+// 8 elements of a parameter row, in DT or in fp32.
 template <int DT>
 FIE_DEV void load_param(float (&w)[8], const void* p, bool f32, int e0, int width)
 {
@@ -142,10 +161,11 @@ FIE_DEV float row_max(float x, float* slot)     // of values >= 0: their bits or
 }
 
 // DX: x and y; DR: residual.  A row's thread t holds vectors t, t + T, ..: VPT of them, 0 past
-// the row's end (parameters load as 0 there).
+// the row's end (where parameters load as 0, and a weight's offset meets a 0).
 // ONE: a wave a row, four rows a workgroup.
-template <int DX, int DR, int VPT, bool ONE>
-__global__ __launch_bounds__(ONE ? 256 : (VPT > 4 ? 1024 : 512)) void k_norm(const fie_norm_args a)
+// EARLY: every load at once, parameters in DX (a wave's chain is the kernel's time for few tokens).
+template <int DX, int DR, int VPT, bool ONE, bool EARLY>
+__global__ __launch_bounds__(ONE ? 256 : (VPT > 2 ? 1024 : 512)) void k_norm(const fie_norm_args a)
 {
     __shared__ float red[5][16];
     const int T = ONE ? 64 : blockDim.x;
@@ -162,14 +182,34 @@ __global__ __launch_bounds__(ONE ? 256 : (VPT > 4 ? 1024 : 512)) void k_norm(con
     float v[VPT][8];
     Vec8<DR> res[VPT];
     Vec8<DX> xs[VPT];
+    constexpr int PN = EARLY ? VPT : 1;
+    Vec8<DX> pw[PN], pb[PN], gt[PN], nw[PN], nb[PN];
+    const bool wf = a.weight_f32, gf = a.gate_f32, gate_row = a.gate && a.gate_step;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         const int e0 = (i * T + t) * 8;
         res[i] = load8<DR>(rp, e0, H);
         if (a.x) xs[i] = load8<DX>(xp, e0, H);
+        if constexpr (EARLY) {
+            if (a.post_weight) pw[i] = load8<DX>((const char*)a.post_weight, e0, H);
+            if (a.post_bias) pb[i] = load8<DX>((const char*)a.post_bias, e0, H);
+            if (gate_row) gt[i] = load8<DX>(gp, e0, H);
+            if (a.weight) nw[i] = load8<DX>((const char*)a.weight, e0, H);
+            if (a.bias) nb[i] = load8<DX>((const char*)a.bias, e0, H);
+        }
     }
+    float g1 = 1.0f;
+    if (a.gate && !a.gate_step) g1 = DX == FIE_F32 || gf ? *(const float*)gp : load_elem<DX>(gp, 0);
     // (v - mean) / sqrt(mean((v - mean)^2) + eps) * weight + bias, in place
-    auto norm = [&](const void* weight, const void* bias, int slot) {
+    auto param = [&](float (&w)[8], const void* p, bool f32, const Vec8<DX>& early, int e0) {
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = get8<DX>(early, e);
+        } else {
+            load_param<DX>(w, p, f32, e0, H);
+        }
+    };
+    auto norm = [&](const void* weight, const void* bias, const Vec8<DX> (&ew)[PN], const Vec8<DX> (&eb)[PN], int slot) {
         if (a.kind == FIE_NORM_LAYER) {
             float s = 0.0f;
 #pragma unroll
@@ -193,16 +233,12 @@ __global__ __launch_bounds__(ONE ? 256 : (VPT > 4 ? 1024 : 512)) void k_norm(con
         for (int i = 0; i < VPT; ++i) {
             const int e0 = (i * T + t) * 8;
             float w[8], b[8];
-            if (weight) {
-                load_param<DX>(w, weight, a.weight_f32, e0, H);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] += a.weight_offset;
-            }
-            if (bias) load_param<DX>(b, bias, a.weight_f32, e0, H);
+            if (weight) param(w, weight, wf, ew[EARLY ? i : 0], e0);
+            if (bias) param(b, bias, wf, eb[EARLY ? i : 0], e0);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 v[i][e] *= rstd;
-                if (weight) v[i][e] *= w[e];
+                if (weight) v[i][e] *= w[e] + a.weight_offset;
                 if (bias) v[i][e] += b[e];
             }
         }
@@ -212,22 +248,14 @@ __global__ __launch_bounds__(ONE ? 256 : (VPT > 4 ? 1024 : 512)) void k_norm(con
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = get8<DX>(xs[i], e);
-        if (a.post_norm) norm(a.post_weight, a.post_bias, 0);
+        if (a.post_norm) norm(a.post_weight, a.post_bias, pw, pb, 0);
         if (a.gate) {
-            if (a.gate_step) {
 #pragma unroll
-                for (int i = 0; i < VPT; ++i) {
-                    float g[8];
-                    load_param<DX>(g, gp, a.gate_f32, (i * T + t) * 8, H);
+            for (int i = 0; i < VPT; ++i) {
+                float g[8];
+                if (gate_row) param(g, gp, gf, gt[EARLY ? i : 0], (i * T + t) * 8);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[i][e] *= g[e];
-                }
-            } else {
-                const float g = DX == FIE_F32 || a.gate_f32 ? *(const float*)gp : load_elem<DX>(gp, 0);
-#pragma unroll
-                for (int i = 0; i < VPT; ++i)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[i][e] *= g;
+                for (int e = 0; e < 8; ++e) v[i][e] *= gate_row ? g[e] : g1;
             }
         }
 #pragma unroll
@@ -246,7 +274,7 @@ __global__ __launch_bounds__(ONE ? 256 : (VPT > 4 ? 1024 : 512)) void k_norm(con
         for (int i = 0; i < VPT; ++i) store8<DR>(op, (i * T + t) * 8, H, v[i]);
     }
     if (!a.y) return;
-    if (a.kind != FIE_NORM_NONE) norm(a.weight, a.bias, 2);
+    if (a.kind != FIE_NORM_NONE) norm(a.weight, a.bias, nw, nb, 2);
     if (a.y_dtype != FIE_I8) {
         char* yp = (char*)a.y + row * a.y_stride * SX;
 #pragma unroll

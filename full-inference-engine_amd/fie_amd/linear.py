@@ -18,6 +18,7 @@ from .norm import block_norm
 
 _DTYPES = {torch.float32: FIE_F32, torch.float16: FIE_F16, torch.bfloat16: FIE_BF16}
 _pack = struct.Struct(_lib.INT8_ARGS).pack
+_run = None             # the library's entry, loaded with the first call
 MAX_K = 131071          # the sums of longer products could pass 32 bits
 
 
@@ -90,12 +91,13 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         xp, wp, x_stride, w_stride = x.data_ptr(), weight.data_ptr(), max(x_stride, k), max(w_stride, k)
         args = [xp, wp, x_scale.data_ptr(), weight_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr(),
                 tokens, x_stride, w_stride, y_stride, n, k, y_dtype, 0, 0, 0]
-        lib = _lib.load()
-        with _lib.on_device(index) as stream:
-            if (xp | wp | x_stride | w_stride) & 15 or max(x_stride, w_stride) >= 1 << 23:
-                args[-1] = lib.fie_int8_workspace_size(_pack(*args))
-                if args[-1]:
-                    room = torch.empty(args[-1], dtype=torch.int8, device=y.device)
-                    args[-2] = room.data_ptr()
-            _lib.check(lib.fie_int8_linear(_pack(*args), stream), "fie_int8_linear")
+        global _run
+        if _run is None:
+            _run = _lib.launcher("fie_int8_linear")
+        if (xp | wp | x_stride | w_stride) & 15 or x_stride >= 1 << 23 or w_stride >= 1 << 23:
+            args[-1] = _lib.load().fie_int8_workspace_size(_pack(*args))
+            if args[-1]:
+                room = torch.empty(args[-1], dtype=torch.int8, device=y.device)
+                args[-2] = room.data_ptr()
+        _run(index, _pack(*args))
     return y.view(*shape[:-1], n) if out is None and len(shape) != 2 else y

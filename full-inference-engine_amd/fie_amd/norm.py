@@ -22,6 +22,7 @@ from ._lib import FIE_BF16, FIE_F16, FIE_F32, FIE_I8
 _DTYPES = {torch.float32: FIE_F32, torch.float16: FIE_F16, torch.bfloat16: FIE_BF16}
 _KINDS = {"rms": 0, "layer": 1, "none": 2}
 _pack = struct.Struct(_lib.NORM_ARGS).pack
+_run = None             # the library's entry, loaded with the first call
 MAX_WIDTH = 65536
 
 
@@ -87,7 +88,7 @@ def block_norm(residual: torch.Tensor, x: torch.Tensor | None = None, weight: to
     for i, t in enumerate((weight, bias, post_weight, post_bias)):
         if t is None:
             continue
-        if t.shape != (width,) or not t.is_contiguous():
+        if t.ndim != 1 or t.shape[0] != width or not t.is_contiguous():
             raise ValueError(f"weights and biases must be contiguous vectors of {width}")
         if v_dtype is None:
             v_dtype = t.dtype
@@ -102,13 +103,14 @@ def block_norm(residual: torch.Tensor, x: torch.Tensor | None = None, weight: to
         vectors[i] = t.data_ptr()
     if norm == 2 and post:
         raise ValueError("kind 'none' takes no norm parameters")
-    res = _rows(residual, width)
+    flat = len(shape) == 2
+    res = residual if flat and (residual.stride(1) == 1 or width == 1) else _rows(residual, width)
     tokens, r_stride = res.shape[0], res.stride(0)
     device = residual.device
     new = xs = gp = None
     xp = x_stride = n_ptr = n_stride = g_ptr = g_stride = g_step = g_f32 = 0
     if x is not None:
-        xs = _rows(x, width)
+        xs = x if flat and (x.stride(1) == 1 or width == 1) else _rows(x, width)
         xp, x_stride = xs.data_ptr(), xs.stride(0)
         if x.get_device() != index:
             raise ValueError("x must be on the residual's device")
@@ -117,7 +119,8 @@ def block_norm(residual: torch.Tensor, x: torch.Tensor | None = None, weight: to
                 raise ValueError("inplace needs a residual with unit element stride and rows that do not overlap")
             new, n_stride = res, r_stride
         else:
-            new, n_stride = torch.empty((tokens, width), dtype=residual.dtype, device=device), width
+            new = torch.empty_like(res) if r_stride == width else torch.empty((tokens, width), dtype=residual.dtype, device=device)
+            n_stride = width
         n_ptr = new.data_ptr()
         if gate is not None:
             if gate.get_device() != index or (gate.dtype != dtype and gate.dtype != torch.float32):
@@ -133,17 +136,21 @@ def block_norm(residual: torch.Tensor, x: torch.Tensor | None = None, weight: to
             else:
                 raise ValueError("gate must be [width], x's shape, or x's shape with a last dimension of 1")
             g_ptr, g_f32 = gp.data_ptr(), gate.dtype == torch.float32
-    y = torch.empty((tokens, width), dtype=torch.int8 if quantize else dtype, device=device)
+    like = res if xs is None else xs
+    if not quantize and like.dtype == dtype and like.stride(0) == width:
+        y = torch.empty_like(like)
+    else:
+        y = torch.empty((tokens, width), dtype=torch.int8 if quantize else dtype, device=device)
     y_scale = torch.empty(tokens, dtype=torch.float32, device=device) if quantize else None
     if tokens:
-        args = _pack(xp, res.data_ptr(), n_ptr, y.data_ptr(), y_scale.data_ptr() if quantize else 0, *vectors, g_ptr,
-                     tokens, x_stride, r_stride, n_stride, width, g_stride, g_step, width, x_dtype, r_dtype,
-                     FIE_I8 if quantize else x_dtype, v_dtype == torch.float32, g_f32, norm, post, scale, eps,
-                     weight_offset)
-        lib = _lib.load()
-        with _lib.on_device(index) as stream:
-            _lib.check(lib.fie_block_norm(args, stream), "fie_block_norm")
-    if len(shape) != 2:
+        global _run
+        if _run is None:
+            _run = _lib.launcher("fie_block_norm")
+        _run(index, _pack(xp, res.data_ptr(), n_ptr, y.data_ptr(), y_scale.data_ptr() if quantize else 0, *vectors, g_ptr,
+                          tokens, x_stride, r_stride, n_stride, width, g_stride, g_step, width, x_dtype, r_dtype,
+                          FIE_I8 if quantize else x_dtype, v_dtype == torch.float32, g_f32, norm, post, scale, eps,
+                          weight_offset))
+    if not flat:
         y = y.view(shape)
         if new is not None and not inplace:
             new = new.view(shape)

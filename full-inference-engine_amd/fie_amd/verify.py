@@ -111,6 +111,7 @@ class DraftVerifier:
     def __init__(self, device: torch.device | str, fused: FusedSampler | None = None):
         self._fused = fused if fused is not None else FusedSampler(device)
         self.device = self._fused.device
+        self._run = _lib.launcher("fie_sampler_verify")
 
     def plan(self, params: list[SamplingParams], draft_lens: list[int], vocab: int,
              contexts: list[list[int]] | None = None, drafts: list[list[int]] | None = None,
@@ -163,7 +164,5 @@ class DraftVerifier:
             v.draft_probs, v.draft_stride = draft_probs.data_ptr(), max(draft_probs.stride(0), vocab)
         v.tokens, v.accepted, v.target_probs = tokens.data_ptr(), accepted.data_ptr(), probs.data_ptr()
         ws = self._fused.ensure_workspace(rows, vocab)
-        with _lib.on_device(index) as stream:
-            rc = self._fused.lib.fie_sampler_verify(ctypes.byref(a), ctypes.byref(v), ctypes.byref(ws), stream)
-        _lib.check(rc, "fie_sampler_verify")
+        self._run(index, ctypes.byref(a), ctypes.byref(v), ctypes.byref(ws))
         return Verified(tokens, accepted, probs)
