@@ -2,9 +2,11 @@
 
 ``fie_amd.batching.sampler.BatchedSampler`` and ``fie_amd.runtime.sampling`` mirror
 ``engine.batching.sampler`` and ``engine.runtime.sampling`` of full-inference-engine.
+Beside them: ``fie_amd.verify`` (drafted tokens), ``fie_amd.linear`` (products in 8-bit
+integers) and ``fie_amd.norm`` (block norms).
 """
 
-from .batching.sampler import BatchedSampler, SampleResult
+from .batching.sampler import BatchedSampler, SampleResult, VerifyResult
 from .runtime.sampling import GREEDY, SamplingParams
 
-__all__ = ["BatchedSampler", "SampleResult", "SamplingParams", "GREEDY"]
+__all__ = ["BatchedSampler", "SampleResult", "VerifyResult", "SamplingParams", "GREEDY"]

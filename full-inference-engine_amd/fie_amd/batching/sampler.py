@@ -38,6 +38,14 @@ class SampleResult:
     logprobs: dict[int, list[tuple[int, float]]]
 
 
+@dataclass
+class VerifyResult:
+    """A request's new tokens (its kept drafts and one more), and how many drafts it kept."""
+
+    token_ids: list[list[int]]
+    accepted: list[int]
+
+
 def pack_history(contexts: list[list[int]], include: np.ndarray, vocab: int):
     """CSR of the penalty contexts of the rows in `include` (sampler.py:136-144 reads
     only penalised rows), plus, per row, the ids >= vocab that the reference's
@@ -318,6 +326,75 @@ class BatchedSampler:
         out, _, _ = self._fused.step(logits, hp)
         tokens = out["tokens"].tolist()
         return SampleResult(tokens, self._logprobs(params, tokens, out) if t.wants_logprobs else {})
+
+    # ------------------------------------------------------------------ drafted tokens
+    def verify(
+        self,
+        logits: torch.Tensor,
+        drafts: list[list[int]],
+        params: list[SamplingParams],
+        draft_probs: torch.Tensor | None = None,
+        context_tokens: list[list[int]] | None = None,
+        request_ids: list[object] | None = None,
+    ) -> VerifyResult:
+        """Keep or replace drafted tokens so that what comes out is distributed as ``sample``
+        would have drawn it token by token (``fie_amd.verify``).
+
+        ``logits`` holds each request's len(drafts[i]) + 1 rows, one request after another; row
+        j is the model's answer after j drafts.  ``draft_probs`` [all drafts, vocab] are the
+        distributions the drafts were drawn from; without them a draft counts as certain.
+        ``context_tokens`` are the requests' contexts without the drafts.  A seeded request
+        takes len(drafts[i]) + 1 draws of its stream, whatever it keeps."""
+        from ..verify import DraftVerifier, VerifyPlan
+
+        if logits.ndim != 2:
+            raise ValueError("logits must have shape [rows, vocab]")
+        lens = [len(d) for d in drafts]
+        if len(params) != len(drafts):
+            raise ValueError("one SamplingParams per list of drafts is required")
+        if logits.shape[0] != sum(lens) + len(lens):
+            raise ValueError("logits must hold one row more than drafts for each request")
+        if context_tokens is not None and len(context_tokens) != len(params):
+            raise ValueError("one context per request is required")
+        if request_ids is not None and len(request_ids) != len(params):
+            raise ValueError("one request id per request is required")
+        flat = [t for d in drafts for t in d]
+        if flat and not (0 <= min(flat) and max(flat) < logits.shape[1]):
+            raise ValueError("drafted tokens must be inside the vocabulary")
+        if not lens:
+            return VerifyResult([], [])
+        if self._verifier is None:
+            self._verifier = DraftVerifier(self.device, self._fused)
+        plan = VerifyPlan(self._fused, params, lens, logits.shape[1], context_tokens, drafts,
+                          self._verify_keys(params, lens, request_ids), shared=True)
+        ids = torch.tensor(flat, dtype=torch.int64).to(logits.device)
+        got = self._verifier.verify(plan, logits, ids, None, draft_probs)
+        accepted = got.accepted.tolist()
+        return VerifyResult([row[:n + 1] for row, n in zip(got.tokens.tolist(), accepted)], accepted)
+
+    _verifier = None
+
+    def _verify_keys(self, params: list[SamplingParams], lens: list[int],
+                     request_ids: list[object] | None) -> np.ndarray:
+        """uint64 [rows, 3]: each row's draw, as _draw_keys gives a batch of these rows."""
+        t = self._params(params)
+        counts = np.asarray(lens, dtype=np.int64) + 1
+        keys = np.zeros((int(counts.sum()), 3), dtype=np.uint64)
+        first = np.cumsum(counts) - counts
+        for r in range(len(params)):
+            if t.greedy[r]:
+                continue
+            rows = slice(int(first[r]), int(first[r] + counts[r]))
+            if t.seeded[r]:
+                rid = request_ids[r] if request_ids is not None else r
+                keys[rows, 0], keys[rows, 1] = int(t.seeds[r]), SEEDED_STREAM
+                keys[rows, 2] = [self._next_draw(rid) for _ in range(int(counts[r]))]
+            else:
+                n = int(counts[r])
+                keys[rows, 0], keys[rows, 1] = self._shared_key, SHARED_STREAM
+                keys[rows, 2] = np.arange(self._shared_draws + 1, self._shared_draws + 1 + n, dtype=np.uint64)
+                self._shared_draws += n
+        return keys
 
     @staticmethod
     def _logprobs(params: list[SamplingParams], chosen: list[int],

@@ -43,7 +43,8 @@ class VerifyPlan:
 
     def __init__(self, fused: FusedSampler, params: list[SamplingParams], draft_lens: list[int], vocab: int,
                  contexts: list[list[int]] | None = None, drafts: list[list[int]] | None = None,
-                 rng: np.ndarray | None = None):
+                 rng: np.ndarray | None = None, shared: bool = False):
+        # shared: the fused sampler's own block of this size, for one call that is waited for
         if len(draft_lens) != len(params):
             raise ValueError("one draft length per request is required")
         lens = np.asarray(draft_lens, dtype=np.int64).reshape(-1)
@@ -85,7 +86,8 @@ class VerifyPlan:
         self._offsets = self._offsets.to(fused.device)
         self.index = self._offsets.get_device()
         # the parameter block, uploaded once
-        self._buf = DeviceStep(self.rows, hp.tail_ints(), fused.device)
+        self._buf = (fused.step_buffers(self.rows, hp.tail_ints()) if shared
+                     else DeviceStep(self.rows, hp.tail_ints(), fused.device))
         self._buf.stage(hp)
         self._buf.upload(torch.cuda.current_stream(fused.device))
         a = self._buf.args_of()
