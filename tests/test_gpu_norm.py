@@ -210,3 +210,18 @@ def test_refusals():
                      ((r.t().contiguous().t(), r, w), dict(inplace=True)), ((r[:1].expand(4, 64), r), dict(inplace=True))]:
         with pytest.raises(ValueError):
             block_norm(*args, **kw)
+
+
+def test_large_offsets():
+    """More than 2^31 elements: the last rows."""
+    T, H = 2 ** 31 // 32768 + 40, 32768
+    x = torch.zeros(T, H, dtype=torch.float16, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x[-5:] = torch.randn(5, H, generator=gen, device=DEV).half()
+    got = block_norm(x, x)
+    r, y = plain(x[-5:], x[-5:], None)
+    near(got.residual[-5:], r, torch.float16, "residual")
+    near(got.y[-5:], y, torch.float16, "y")
+    assert not got.y[:5].any()
+    q, s = quantize_rows(x)
+    assert not q[:-5].any() and s[-1] > 0 and q[-5:].abs().amax() == 127

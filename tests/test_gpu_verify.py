@@ -489,3 +489,31 @@ def test_refusals(verifier):
             verifier.plan(*args)
     none = verifier.verify(verifier.plan([], [], V), x[:0], ids[:0], u[:0])
     assert none.tokens.shape == (0, 1)
+
+
+@pytest.mark.parametrize("V", [300, 70001])
+def test_rows_of_nothing(verifier, V):
+    """Rows of -inf alone, among ordinary ones: the first token, whatever the settings."""
+    lens = [1, 0, 2, 1] * 6
+    x, ids, q = make(V, 24, lens, V, torch.float32, True)
+    x[::2] = float("-inf")
+    x[-3:] = float("-inf")
+    for probs in (q, None):
+        check(verifier, x, (MIXED * 4), lens, ids, probs, 5)
+
+
+def test_large_offsets(verifier):
+    """Rows of logits and draft probabilities 2^31 elements apart."""
+    V, step = 1000, 2 ** 31 + 8
+    x, ids, q = make(91, 1, [1], V, torch.float16, True)
+    far = [torch.empty(step + V, dtype=torch.float16, device=DEV) for _ in range(2)]
+
+    def spread(g):
+        a = torch.as_strided(far[0], (2, V), (step, 1))
+        a.copy_(g[0])
+        b = torch.as_strided(far[1], (2, V), (step, 1))
+        b[1].copy_(g[3][0])
+        b[0].copy_(g[3][0])
+        return [a, g[1], g[2], b[1:2]]
+
+    check(verifier, x, [SamplingParams(temperature=1.0)], [1], ids, q.half(), 92, transform=spread)
