@@ -296,7 +296,9 @@ __global__ __launch_bounds__(ONE ? 256 : (VPT > 2 ? 1024 : 512)) void k_norm(con
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float u = __builtin_rintf(v[i][e] / s);
-            q[e] = u >= -127.0f && u <= 127.0f ? u : 0.0f;       // 0 / 0 and NaN: 0
+            // NaN (0 / 0, inf / inf) and rows without a scale: 0; past 127 where s is a few
+            // denormal units, rounded down
+            q[e] = s > 0.0f && u == u ? __builtin_fminf(__builtin_fmaxf(u, -127.0f), 127.0f) : 0.0f;
         }
         store8_i8(yp, (i * T + t) * 8, H, q);
     }

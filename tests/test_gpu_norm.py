@@ -155,6 +155,17 @@ def test_quantize_rows_is_the_ieee_quotient(dtype, width):
     np.testing.assert_array_equal(q.cpu().numpy(), np.where(np.isnan(t), 0, t).astype(np.int8))
 
 
+@pytest.mark.parametrize("units", [1, 63, 64, 100, 190, 191, 254, 1000, 12345])
+def test_quantize_rows_of_denormals(units):
+    """Rows of a few 2^-149: the scale, itself a denormal, is off by up to half of itself."""
+    x = (np.arange(-8, 9) * units // 8 * 2.0 ** -149).astype(np.float32)
+    q, s = quantize_rows(torch.from_numpy(x[None]).to(DEV))
+    scale = np.float32(np.abs(x).max()) / np.float32(127)
+    assert s.cpu().numpy()[0] == scale
+    want = np.clip(np.rint(x.astype(np.float64) / scale), -127, 127) if scale > 0 else np.zeros(17)
+    np.testing.assert_array_equal(q.cpu().numpy()[0], want.astype(np.int8))
+
+
 def test_strides_inplace_and_streams():
     H, T = 1003, 13
     m = make(8, (T, H), torch.bfloat16, torch.bfloat16)
