@@ -119,7 +119,7 @@ static hipError_t int8_dt(fie_int8_args a, hipStream_t st)
 static int int8_check(const fie_int8_args* a)
 {
     if (!a) return fail(FIE_E_ARG, "args is NULL");
-    if (a->m < 0 || a->m > 0x7FFFFF00 || a->n < 1) return fail(FIE_E_ARG, "sizes out of range");
+    if (a->m < 0 || a->m > 0x7FFFFF00 || a->n < 1 || a->n > 0x7FFFFF00) return fail(FIE_E_ARG, "sizes out of range");
     if (a->k < 1 || a->k > FIE_MAX_K) return fail(FIE_E_ARG, "k out of range [1, 131071]");
     if (a->y_dtype < FIE_F32 || a->y_dtype > FIE_BF16) return fail(FIE_E_ARG, "unknown dtype");
     if (a->x_stride < a->k || a->w_stride < a->k || a->y_stride < a->n) return fail(FIE_E_ARG, "a row stride is shorter than its row");

@@ -20,6 +20,7 @@ _DTYPES = {torch.float32: FIE_F32, torch.float16: FIE_F16, torch.bfloat16: FIE_B
 _pack = struct.Struct(_lib.INT8_ARGS).pack
 _run = None             # the library's entry, loaded with the first call
 MAX_K = 131071          # the sums of longer products could pass 32 bits
+MAX_CHANNELS = 0x7FFFFF00
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -45,7 +46,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         raise ValueError("weight must be int8 [channels, k]")
     n, k = weight.shape
     shape = x.shape
-    if not shape or shape[-1] != k or n < 1 or not 1 <= k <= MAX_K:
+    if not shape or shape[-1] != k or not 1 <= n <= MAX_CHANNELS or not 1 <= k <= MAX_K:
         raise ValueError(f"x [..., k] and weight [channels, k] must agree on k in [1, {MAX_K}]")
     index = weight.get_device()
     if index < 0:

@@ -75,7 +75,8 @@ def int8_args(**kw):
 
 
 @pytest.mark.parametrize("kw, code, text", [
-    (dict(m=-1), _lib.FIE_E_ARG, b"sizes"), (dict(n=0), _lib.FIE_E_ARG, b"sizes"), (dict(k=0), _lib.FIE_E_ARG, b"k out"),
+    (dict(m=-1), _lib.FIE_E_ARG, b"sizes"), (dict(n=0), _lib.FIE_E_ARG, b"sizes"),
+    (dict(n=2 ** 31 - 1, y_stride=2 ** 31), _lib.FIE_E_ARG, b"sizes"), (dict(k=0), _lib.FIE_E_ARG, b"k out"),
     (dict(k=MAX_K + 1), _lib.FIE_E_ARG, b"k out"), (dict(y_dtype=3), _lib.FIE_E_ARG, b"dtype"),
     (dict(x_stride=63), _lib.FIE_E_ARG, b"stride"), (dict(w_stride=1), _lib.FIE_E_ARG, b"stride"),
     (dict(y_stride=31), _lib.FIE_E_ARG, b"stride"), (dict(x=0), _lib.FIE_E_ARG, b"NULL"), (dict(y=0), _lib.FIE_E_ARG, b"NULL"),
