@@ -218,7 +218,8 @@ FIE_DEV bool tile_at(int b, int nrb, int ncb, int* rb, int* cb)
     return true;
 }
 
-template <int N> FIE_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// All but the wave's last N loads into LDS are done, and all that it reads from there.
+template <int N> FIE_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
 
 FIE_DEV void meet()             // a barrier that waits for no load
 {
@@ -301,7 +302,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, OCC) void k_int8_pipe(const fie_
         if (KG == 1 || s < ns) mul(L[grp][s % NB]);
     }
     if (a.k % kI8K) {                                           // the rest of k, 0 past its end
-        meet();
+        __syncthreads();
         if (grp == 0) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
