@@ -99,7 +99,8 @@ FIE_DEV i32x4_t load_k(const int8_t* rowp, int k0, int K)
 // Rows at any address into rows of whole stages at aligned ones, 0 past k: what the pipe kernel
 // needs.  A wave a row; a lane makes a word from the two that hold its bytes, so that every
 // load and store of a wave is one piece of 256 bytes (16 bytes a lane at odd addresses take
-// four times as long: 250 x 16384 at k 4097 122 us without this).
+// four times as long: 250 x 16384 at k 4097 122 us without this).  Bound by HBM: the matrix
+// read and written once, on top of what the product reads.
 __global__ __launch_bounds__(256) void k_align_rows(const int8_t* src, int64_t stride, int64_t rows, int K, int8_t* dst, int64_t pitch)
 {
     const int lane = threadIdx.x & 63;

@@ -2,8 +2,11 @@
 //
 // A row is held in registers, 8 neighbouring elements a vector, from its loads to its
 // stores; each norm costs one reduction over the row's threads (a layer norm two, its
-// squares taken about the mean).  Bound by HBM: x, residual and gate read once, residual
-// and y written once.
+// squares taken about the mean: sum(x^2) - n mean^2 cancels where the mean is large).  Bound
+// by HBM: x, residual and gate read once, residual and y written once.  bf16 8192 x 4096 with
+// norms on both sides 54 us, 268 MB at 5.0 TB/s (a copy of 2 GiB runs at 4.8); few rows are
+// bound by their chain of loads, barriers and stores: 1 x 4096 3.0 us, 333 x 2050 layer norms
+// 7.7, 250 x 4096 to int8 4.2.
 #pragma once
 
 #include "launchers.h"

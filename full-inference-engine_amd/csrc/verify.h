@@ -198,6 +198,10 @@ namespace fie {
 
 // One workgroup a request: draft j by thread j; on rows with penalties the draft's
 // occurrences in the row's history are counted first, a wave a draft.
+//
+// A draft's p from one logit and its tile's maximum and scale: the row is not read again, so
+// the kernel is a chain of three dependent loads (offsets, draft, logit and tile) whatever the
+// vocabulary: 4.7 us for 1 request of 4 drafts, 7.3 for 256 (rank_begin's bins among them).
 template <int DT>
 __global__ __launch_bounds__(kVerThreads) void k_accept(const KParams P, const fie_verify_args v, const VerWs vw)
 {
@@ -320,7 +324,11 @@ FIE_DEV Excess excess_of(float p, float q)
 //
 // Bound by the two rows' way from memory, so what the sampler's tile maxima rule out is not
 // read: a tile whose largest logit is below the row's edge, and q of a wave's tokens when none
-// of them is kept.
+// of them is kept.  A span a workgroup, since a refusal's row and its q (0.9 MB at vocab 151936)
+// are far too much for one CU's loads.  256 requests of
+// 4 drafts, bf16 logits and fp32 q: 39 us, 133 refusals and the first pass of 123 rank draws,
+// 158 MB at most, 4 TB/s.  Few requests wait on the loads and on the last span's second look:
+// 16 without q 16 us.
 template <int DT, int QT, int TPS>
 __global__ __launch_bounds__(kVerThreads) void k_refused(const KParams P, const fie_verify_args v, const VerWs vw)
 {

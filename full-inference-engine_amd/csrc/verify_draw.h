@@ -9,6 +9,12 @@
 // arrive looks for the draw.  What is left in the end is a short list, or one value that many
 // tokens share (16-bit logits lie on a grid), whose tokens are then counted in index order; and
 // for anything else a search over the keys by one workgroup.
+//
+// Three passes rather than one that keeps every token by bin: the row is 0.3 MB and stays in the
+// caches, a list of its keys would be written and read at four times that.  The second and third
+// read only tiles whose largest value reaches into the part.  Bound by latency and by the vector
+// instructions of the masses (two 41-bit limbs a token): 123 draws of 151936 bf16 logits, the
+// first pass within k_refused's 39 us, the second 11.6, the third 25.
 #pragma once
 
 namespace fie {
