@@ -1,8 +1,7 @@
 /*
  * fie_ops.h -- C ABI of the operators in front of the output layer and of the output layer
  * in 8-bit integers: block norms, per-token quantisation, the integer product.  No
- * counterpart on the reference's sampler path; its engine runs these as separate Triton
- * kernels (engine/kernels/).
+ * counterpart on the reference's sampler path.
  *
  * Conventions are fie_sampler.h's: device pointers, work enqueued on `stream`, nothing
  * synchronises or allocates, FIE_OK or a negative FIE_E* code, and
