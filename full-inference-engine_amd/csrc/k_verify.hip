@@ -35,7 +35,7 @@ hipError_t launch_verify(const KParams& P, const fie_verify_args& v, hipStream_t
 {
     // the candidates' and deferred rows' arrays are free once the rows are settled: a request has at least one
     // row, and a row at least as many tiles as spans
-    const VerWs vw{(VerJob*)P.w.dfr, P.w.ncand, P.w.sw, P.w.maxc};
+    const VerWs vw{(VerJob*)P.w.dfr, P.w.ncand, P.w.sw};
     switch (P.a.dtype) {
     case FIE_F32: verify_dt<FIE_F32>(P, v, vw, st); break;
     case FIE_F16: verify_dt<FIE_F16>(P, v, vw, st); break;

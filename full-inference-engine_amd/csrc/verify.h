@@ -33,7 +33,6 @@ struct VerWs {
     VerJob* job;        // [requests]
     uint32_t* arrived;  // [requests]
     uint64_t* sum;      // [requests * tiles]
-    uint64_t* sum_hi;   // [requests * tiles]
 };
 static_assert(sizeof(VerJob) <= sizeof(DeferRec), "jobs go where the deferred rows' records were");
 

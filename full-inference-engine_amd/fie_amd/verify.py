@@ -27,6 +27,7 @@ from .runtime.sampling import SamplingParams
 
 FLAG_NO_DRAW = _lib.FIE_FLAG_NO_DRAW
 MAX_DRAFTS = _lib.MAX_DRAFTS
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 class Verified(NamedTuple):
@@ -104,11 +105,25 @@ class VerifyPlan:
         v.requests, v.max_drafts = self.requests, self.max_drafts
         v.draft_offsets, v.draws = self._offsets.data_ptr(), int(draws)
         self.verify_args = v
+        self.stream = _raw_stream(self.index)
+        self._ready = torch.cuda.Event()
+        self._ready.record(torch.cuda.current_stream(fused.device))
+
+    def use_on(self, stream: torch.cuda.Stream) -> None:
+        """The settings' upload comes before what ``stream`` runs next, and their memory is kept
+        for it.  (A stream that captures waits for nothing outside: the upload is then long done.)"""
+        if torch.cuda.is_current_stream_capturing():
+            return
+        stream.wait_event(self._ready)
+        for t in (self._buf.dev, self._offsets):
+            t.record_stream(stream)
 
 
 class DraftVerifier:
     """Verifies drafts on one device; calls of one verifier share a workspace and go on one
-    stream at a time."""
+    stream at a time.  A captured call keeps its plan's and the verifier's buffers by address:
+    both outlive the graph, plans are made well before the capture, and the largest call (rows,
+    vocabulary) goes before it, so that the workspace grows no more."""
 
     def __init__(self, device: torch.device | str, fused: FusedSampler | None = None):
         self._fused = fused if fused is not None else FusedSampler(device)
@@ -147,6 +162,8 @@ class DraftVerifier:
             if t is not None and t.get_device() != index:
                 raise ValueError(f"every tensor must be on device {index}")
         device = logits.device
+        if _raw_stream(index) != plan.stream:
+            plan.use_on(torch.cuda.current_stream(index))
         tokens = torch.empty((plan.requests, plan.max_drafts + 1), dtype=torch.int64, device=device)
         accepted = torch.empty(plan.requests, dtype=torch.int32, device=device)
         probs = torch.empty(drafts, dtype=torch.float32, device=device)

@@ -406,6 +406,22 @@ def test_another_stream_and_a_reused_plan(verifier):
     torch.cuda.current_stream().wait_stream(side)
 
 
+def test_a_plan_made_on_a_busy_stream(verifier):
+    V = 3000
+    params = (MIXED * 2)[:12]
+    x, ids, q = make(63, 12, LENS, V, torch.float32, True)
+    u, want, _, _ = plain(x.float().numpy(), params, LENS, ids.numpy(), q.numpy(), np.random.default_rng(64))
+    g = [x.to(DEV), ids.to(DEV), torch.from_numpy(u).to(DEV), q.to(DEV)]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)           # some 20 ms in front of the settings' upload
+        plan = verifier.plan(params, LENS, V)
+    got = verifier.verify(plan, *g)
+    del plan
+    np.testing.assert_array_equal(got.tokens.cpu().numpy(), want)
+
+
 def test_graph_replay(verifier):
     V = 20000
     params = (MIXED * 2)[:12]
