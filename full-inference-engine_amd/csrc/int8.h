@@ -61,40 +61,83 @@ constexpr int kI8K = 128;               // bytes of k a stage
 // cycle serves read eight rows' chunk c from eight distinct bank groups.
 FIE_DEV int i8_slot(int n, int c) { return n * 8 + (c ^ (n & 7)); }
 
-// 16 bytes at any address: a load of the 16 from the word that holds the first, one of the word
-// after them, and a shift.  (One load at the byte's own address takes 3 times as long: 16 x
-// 50001 at k 4097 151 us.)  Only words that hold some of the 16 bytes are touched.
-FIE_DEV i32x4_t load_any(const int8_t* p)
-{
+// 16 bytes at any address: the 16 from the word that holds the first, the word after them, and a
+// shift.  (One load at the byte's own address takes 3 times as long: 16 x 50001 at k 4097 151 us.)
+// Only words that hold some of the 16 bytes are touched.
+struct Any16 {
     typedef uint32_t raw __attribute__((ext_vector_type(4), aligned(4)));
-    const uint32_t sh = (uint32_t)(uintptr_t)p & 3u;
-    const int8_t* b = p - sh;
-    const raw r = *(const raw*)b;
-    const uint32_t e = *(const uint32_t*)(b + (sh ? 16 : 12));
-    return i32x4_t{(int32_t)__builtin_amdgcn_alignbyte(r.y, r.x, sh), (int32_t)__builtin_amdgcn_alignbyte(r.z, r.y, sh),
-                   (int32_t)__builtin_amdgcn_alignbyte(r.w, r.z, sh), (int32_t)__builtin_amdgcn_alignbyte(e, r.w, sh)};
+    raw r;
+    uint32_t e;
+    FIE_DEV void load(const int8_t* p, uint32_t sh)         // sh: the low two bits of p
+    {
+        const int8_t* b = p - sh;
+        r = *(const raw*)b;
+        e = *(const uint32_t*)(b + (sh ? 16 : 12));
+    }
+    FIE_DEV i32x4_t get(uint32_t sh) const
+    {
+        return i32x4_t{(int32_t)__builtin_amdgcn_alignbyte(r.y, r.x, sh), (int32_t)__builtin_amdgcn_alignbyte(r.z, r.y, sh),
+                       (int32_t)__builtin_amdgcn_alignbyte(r.w, r.z, sh), (int32_t)__builtin_amdgcn_alignbyte(e, r.w, sh)};
+    }
+};
+FIE_DEV uint32_t low2(const int8_t* p) { return (uint32_t)(uintptr_t)p & 3u; }
+
+// 16 bytes of a row of at least 16 from k0 on; those at or past K are 0.  Where the row ends inside
+// them, its last 16 bytes are loaded and shifted down, on no branch.
+struct Last16 {
+    Any16 v;
+    uint32_t sh;
+    int past;
+    FIE_DEV void load(const int8_t* rowp, int k0, int K)
+    {
+        const int8_t* p = rowp + min(k0, K - 16);
+        past = min(max(k0 + 16 - K, 0), 16);
+        sh = low2(p);
+        v.load(p, sh);
+    }
+    FIE_DEV i32x4_t get() const
+    {
+        const i32x4_t r = v.get(sh);
+        const u128 x = ((u128)(uint32_t)r.w << 96) | ((u128)(uint32_t)r.z << 64) | ((u128)(uint32_t)r.y << 32) | (uint32_t)r.x;
+        const u128 t = past < 16 ? x >> (8 * past) : 0;
+        return i32x4_t{(int32_t)(uint32_t)t, (int32_t)(uint32_t)(t >> 32), (int32_t)(uint32_t)(t >> 64), (int32_t)(uint32_t)(t >> 96)};
+    }
+};
+
+// The same of a row shorter than 16.
+FIE_DEV i32x4_t load_short(const int8_t* rowp, int k0, int K)
+{
+    i32x4_t r{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t b = (uint8_t)rowp[min(k0 + i, K - 1)];
+        r[i / 4] |= (int32_t)((k0 + i < K ? b : 0u) << (8 * (i % 4)));
+    }
+    return r;
 }
 
-// 16 bytes of a row from k0 on; those at or past K are 0.  Where the row ends inside them, its
-// last 16 bytes are loaded and shifted down.
-FIE_DEV i32x4_t load_k(const int8_t* rowp, int k0, int K)
-{
-    if (k0 >= K) return i32x4_t{0, 0, 0, 0};
-    if (K < 16) {                               // shorter than one load
-        i32x4_t r{0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const uint32_t b = (uint8_t)rowp[min(k0 + i, K - 1)];
-            r[i / 4] |= (int32_t)((k0 + i < K ? b : 0u) << (8 * (i % 4)));
-        }
-        return r;
+// A wave's 128 bytes of 16 rows at any address: lane l holds bytes 64 h + 16 (l / 16) .. +15 of
+// row l % 16.  Each lane loads the 16 from the word that holds its first; the word after them is
+// the first of the lane 16 further on (or of the other half, or one more load), so that no byte is
+// loaded twice: with a load of its own for each such word the lines were out of the L1 again
+// before it came (16 x 50001 at k 4097 73 us against 60).
+struct Chunk {
+    Any16::raw r[2];
+    uint32_t e;
+    FIE_DEV void load(const int8_t* p, const int8_t* past)      // p: a multiple of 4
+    {
+        r[0] = *(const Any16::raw*)p;
+        r[1] = *(const Any16::raw*)(p + 64);
+        e = *(const uint32_t*)past;
     }
-    const int past = max(k0 + 16 - K, 0);
-    const i32x4_t r = load_any(rowp + k0 - past);
-    const u128 v = ((u128)(uint32_t)r.w << 96) | ((u128)(uint32_t)r.z << 64) | ((u128)(uint32_t)r.y << 32) | (uint32_t)r.x;
-    const u128 t = v >> (8 * past);
-    return i32x4_t{(int32_t)(uint32_t)t, (int32_t)(uint32_t)(t >> 32), (int32_t)(uint32_t)(t >> 64), (int32_t)(uint32_t)(t >> 96)};
-}
+    template <int H> FIE_DEV i32x4_t get(uint32_t sh, int lane) const
+    {
+        const uint32_t x = lane < 16 ? (H == 0 ? r[1].x : e) : r[H].x;
+        const uint32_t n = (uint32_t)__builtin_amdgcn_ds_bpermute(((lane + 16) & 63) * 4, (int)x);
+        const Any16 v{r[H], n};
+        return v.get(sh);
+    }
+};
 
 // Rows at any address into rows of whole stages at aligned ones, 0 past k: what the pipe kernel
 // needs.  A wave a row; a lane makes a word from the two that hold its bytes, so that every
@@ -123,7 +166,10 @@ __global__ __launch_bounds__(256) void k_align_rows(const int8_t* src, int64_t s
 // Few tokens: bound by the weights' way from memory.  A workgroup takes 16 NW channels and all
 // tokens, 16 MT at most; its S waves take k in turn, 128 bytes each (whole lines of 16 NW rows),
 // U of them loaded at once straight into the matrix instructions' operands, with no LDS and no
-// barrier before the waves' sums meet.  Unaligned rows load as aligned ones do.
+// barrier before the waves' sums meet.  For rows that the pipe kernel's loads do not take: 16
+// bytes at any address take shifts and a word of a neighbour's, and rows straddle lines, so it stays below
+// the memory's rate (16 x 50001 at k 4097 52 us, 4.0 TB/s; at k 4096 in aligned rows the pipe kernel
+// takes 35).
 template <int DT, int MT, int NW, int S, int U>
 __global__ __launch_bounds__(64 * S) void k_int8_rows(const fie_int8_args a, int wide)
 {
@@ -142,43 +188,71 @@ __global__ __launch_bounds__(64 * S) void k_int8_rows(const fie_int8_args a, int
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int q = 0; q < NW; ++q) acc[m][q] = i32x4_t{0, 0, 0, 0};
+    const int at = 16 * (lane >> 4);
+    uint32_t ws[NW], xs[MT];
+    const int8_t *we[NW], *xe[MT];                  // the word past the row's 128 bytes that holds some of them, or the last
+    auto past = [&](const int8_t* p, uint32_t sh) { return p - at - sh + (sh ? 128 : 124); };
+#pragma unroll
+    for (int q = 0; q < NW; ++q) { ws[q] = low2(wp[q]); we[q] = past(wp[q], ws[q]); }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) { xs[m] = low2(xp[m]); xe[m] = past(xp[m], xs[m]); }
+    // Loads first, then what uses them: left to itself the compiler waits for each before the next.
     auto steps = [&](int k0, auto count) {          // chunks k0, k0 + 128 S, ..
         constexpr int N = decltype(count)::value;
-        i32x4_t fw[N][2][NW], fx[N][2][MT];
+        Chunk fw[N][NW], fx[N][MT];
 #pragma unroll
-        for (int u = 0; u < N; ++u)
+        for (int u = 0; u < N; ++u) {
+            const int k = k0 + u * (128 * S);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int q = 0; q < NW; ++q) fw[u][q].load(wp[q] - ws[q] + k, we[q] + k);
 #pragma unroll
-                for (int q = 0; q < NW; ++q) fw[u][h][q] = load_any(wp[q] + k0 + u * (128 * S) + 64 * h);
+            for (int m = 0; m < MT; ++m) fx[u][m].load(xp[m] - xs[m] + k, xe[m] + k);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        auto half = [&](auto which, int u) {
+            constexpr int H = decltype(which)::value;
+            i32x4_t w[NW];
 #pragma unroll
-                for (int m = 0; m < MT; ++m) fx[u][h][m] = load_any(xp[m] + k0 + u * (128 * S) + 64 * h);
+            for (int q = 0; q < NW; ++q) w[q] = fw[u][q].template get<H>(ws[q], lane);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const i32x4_t x = fx[u][m].template get<H>(xs[m], lane);
+#pragma unroll
+                for (int q = 0; q < NW; ++q) acc[m][q] = mfma_i8(w[q], x, acc[m][q]);
             }
+        };
 #pragma unroll
-        for (int u = 0; u < N; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int q = 0; q < NW; ++q) acc[m][q] = mfma_i8(fw[u][h][q], fx[u][h][m], acc[m][q]);
+        for (int u = 0; u < N; ++u) {
+            half(std::integral_constant<int, 0>{}, u);
+            half(std::integral_constant<int, 1>{}, u);
+        }
     };
     const int full = K / 128;                       // whole chunks
     int c = s;
     for (; c + (U - 1) * S < full; c += U * S) steps(c * 128, std::integral_constant<int, U>{});
     for (; c < full; c += S) steps(c * 128, std::integral_constant<int, 1>{});
-    if (c == full && K % 128) {                     // the rest, by the wave whose turn it is
+    if (c == full && K < 16) {                      // the rest, by the wave whose turn it is
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int k0 = full * 128 + 64 * h, r = K - 16 * (lane >> 4);       // what is left from wp, xp on
-            i32x4_t fx[MT];
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int m = 0; m < MT; ++m) fx[m] = load_k(xp[m], k0, r);
+            for (int q = 0; q < NW; ++q) acc[m][q] = mfma_i8(load_short(wp[q] - at, at, K), load_short(xp[m] - at, at, K), acc[m][q]);
+    } else if (c == full) {
+#pragma unroll 1
+        for (int k0 = full * 128; k0 < K; k0 += 64) {
+            Last16 fw[NW], fx[MT];
 #pragma unroll
-            for (int q = 0; q < NW; ++q) {
-                const i32x4_t fw = load_k(wp[q], k0, r);
+            for (int q = 0; q < NW; ++q) fw[q].load(wp[q] - at, k0 + at, K);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) acc[m][q] = mfma_i8(fw, fx[m], acc[m][q]);
+            for (int m = 0; m < MT; ++m) fx[m].load(xp[m] - at, k0 + at, K);
+            __builtin_amdgcn_sched_barrier(0);
+            i32x4_t w[NW];
+#pragma unroll
+            for (int q = 0; q < NW; ++q) w[q] = fw[q].get();
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const i32x4_t x = fx[m].get();
+#pragma unroll
+                for (int q = 0; q < NW; ++q) acc[m][q] = mfma_i8(w[q], x, acc[m][q]);
             }
         }
     }
@@ -305,11 +379,25 @@ __global__ __launch_bounds__(64 * WM * WN * KG, OCC) void k_int8_pipe(const fie_
     if (a.k % kI8K) {                                           // the rest of k, 0 past its end
         __syncthreads();
         if (grp == 0) {
+            const int8_t* row[NI];
+            int k0[NI];
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int r = 8 * (wave + NWV * i) + (lane >> 3), c = (lane & 7) ^ (r & 7);
-                const int8_t* row = (8 * (wave + NWV * i) < BM ? xb : wb) + (off[i] - 16u * c);
-                *(i32x4_t*)(L[0][0] + (wave + NWV * i) * 1024 + lane * 16) = load_k(row, full * kI8K + 16 * c, a.k);
+                row[i] = (8 * (wave + NWV * i) < BM ? xb : wb) + (off[i] - 16u * c);
+                k0[i] = full * kI8K + 16 * c;
+            }
+            auto put = [&](int i, i32x4_t v) { *(i32x4_t*)(L[0][0] + (wave + NWV * i) * 1024 + lane * 16) = v; };
+            if (a.k < 16) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i) put(i, load_short(row[i], k0[i], a.k));
+            } else {                                            // the loads together
+                Last16 v[NI];
+#pragma unroll
+                for (int i = 0; i < NI; ++i) v[i].load(row[i], k0[i], a.k);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < NI; ++i) put(i, v[i].get());
             }
         }
         __syncthreads();

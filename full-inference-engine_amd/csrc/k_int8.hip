@@ -34,15 +34,16 @@ struct Tile { int bm, bn; float cost; };
 constexpr Tile kTiles[] = {{32, 32, 4.6f}, {32, 64, 6.5f}, {64, 64, 10.5f}, {64, 128, 17.0f},
                            {128, 128, 26.0f}, {256, 128, 40.0f}, {256, 256, 73.0f}};
 
+static int cus() { return cu_count() > 0 ? cu_count() : 256; }
+
 static int cheapest(int64_t m, int64_t n)
 {
-    const int64_t cus = cu_count() > 0 ? cu_count() : 256;
     int best = 0;
     float least = 0.0f;
     for (int i = 0; i < (int)(sizeof kTiles / sizeof kTiles[0]); ++i) {
         const Tile& t = kTiles[i];
         const int64_t tiles = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
-        const float c = t.cost * (float)((tiles + cus - 1) / cus);
+        const float c = t.cost * (float)((tiles + cus() - 1) / cus());
         if (i == 0 || c < least) { best = i; least = c; }
     }
     return best;
@@ -55,9 +56,10 @@ static bool aligned_rows(const void* p, int64_t stride)
     return (((uintptr_t)p | (uint64_t)stride) & 15) == 0 && stride < (1 << 23);
 }
 
-// Tokens few enough to go with the weights at whatever address, straight to registers: up to
-// 32, or 96 where the channels are few (77 x 5001 at k 1003).
-static bool by_rows(int64_t m, int n) { return m <= (n >= 512 * 16 ? 32 : 96); }
+// Tokens few enough to go with the weights at whatever address, straight to registers: us so and
+// laid out first, 96 x 50001 at k 4097 159, 168; 128 x 5001 at k 1003 11.9, 16.0; but 128 x 20001 at
+// k 4097 92, 75.
+static bool by_rows(int64_t m, int n) { return m <= (n <= 2 * 16 * cus() ? 128 : 96); }
 
 static int64_t pitch_of(int k) { return ((int64_t)k + kI8K - 1) / kI8K * kI8K; }
 
@@ -82,12 +84,26 @@ static hipError_t int8_dt(fie_int8_args a, hipStream_t st)
     const bool ax = aligned_rows(a.x, a.x_stride), aw = aligned_rows(a.w, a.w_stride);
     if (!(ax && aw)) {
         if (by_rows(a.m, a.n)) {
-            // from 512 workgroups on with more channels a wave (fewer loads of the tokens: 16 x
-            // 50001 at k 4096 52 us against 63, and at 4096 channels 8.2 against 6.5)
-            const bool many = a.n >= 512 * 16;
-            if (a.m <= 16) return many ? rows_of<DT, 1, 2, 8, 2>(a, wide, st) : rows_of<DT, 1, 1, 16, 2>(a, wide, st);
-            if (a.m <= 32) return many ? rows_of<DT, 2, 4, 8, 1>(a, wide, st) : rows_of<DT, 2, 1, 8, 2>(a, wide, st);
-            return a.m <= 64 ? rows_of<DT, 4, 1, 8, 1>(a, wide, st) : rows_of<DT, 6, 1, 8, 1>(a, wide, st);
+            // 16 channels a workgroup up to one for each CU, where that is the shorter way; past it
+            // 32, which save a round (and loads of the tokens), past two for each CU 64.  us, 16,
+            // 32 and 64 channels:
+            //    16 tokens   4096 at k 4097   7.8,  9.6         8190 at k 4097  13.8, 10.6
+            //    32          4096 at k 4097  10.2, 12.6         9001 at k 4097  25.1, 23.7, 19.3
+            //    64          4096 at k 1003   5.4,  6.4        20001 at k 4097  64.7, 52.3, 49.5
+            //    77          4096 at k 1003   6.2,  7.5         5001 at k 4097  35.4, 21.7
+            //   128          2000 at k 1003   7.5, 12.0         5001 at k 4097  47.6, 31.2
+            const int per = (a.n - 1) / (16 * cus());
+            if (a.m <= 16) return per ? rows_of<DT, 1, 2, 8, 1>(a, wide, st) : rows_of<DT, 1, 1, 8, 2>(a, wide, st);
+            if (a.m <= 32)
+                return per > 1 ? rows_of<DT, 2, 4, 8, 1>(a, wide, st)
+                     : per     ? rows_of<DT, 2, 2, 8, 1>(a, wide, st)
+                               : rows_of<DT, 2, 1, 8, 1>(a, wide, st);
+            if (a.m <= 64)
+                return per > 1 ? rows_of<DT, 4, 4, 8, 1>(a, wide, st)
+                     : per     ? rows_of<DT, 4, 2, 8, 1>(a, wide, st)
+                               : rows_of<DT, 4, 1, 8, 1>(a, wide, st);
+            if (a.m <= 96) return per ? rows_of<DT, 6, 2, 8, 1>(a, wide, st) : rows_of<DT, 6, 1, 8, 1>(a, wide, st);
+            return per ? rows_of<DT, 8, 2, 8, 1>(a, wide, st) : rows_of<DT, 8, 1, 8, 1>(a, wide, st);
         }
         int8_t* to = (int8_t*)a.workspace;
         hipError_t e = hipSuccess;

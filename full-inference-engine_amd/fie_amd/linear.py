@@ -40,7 +40,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     quantised for each token first.  ``out_dtype``: float32, float16 or bfloat16; by default x's own
     (bfloat16 for int8).  Weights whose rows begin at multiples of 16 bytes are read in place at
     any number of tokens (pad the rows of a storage: ``w = room[:, :k]``); others are laid out anew
-    in every call past 32 tokens.  ``out`` [tokens, n] is written instead of a new tensor: unit element
+    in every call past 96 tokens.  ``out`` [tokens, n] is written instead of a new tensor: unit element
     stride, any row stride.  Runs on the current stream; nothing waits for it."""
     if weight.ndim != 2 or weight.dtype != torch.int8:
         raise ValueError("weight must be int8 [channels, k]")

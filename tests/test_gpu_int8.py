@@ -62,6 +62,14 @@ def test_every_batch_of_a_decode_step(m):
         check(int8_linear(x, w, ws, x_scale=xs, out_dtype=torch.bfloat16), x, w, xs, ws)
 
 
+@pytest.mark.parametrize("m", [1, 16, 17, 32, 33, 64, 65, 77, 96, 97, 128, 129])
+@pytest.mark.parametrize("n", [4096, 4097, 8193, 9001])
+def test_unaligned_rows_of_few_tokens(m, n):
+    for k in (1003, 13, 2177):
+        x, w, xs, ws, bias = make(m + n + k, m, n, k)
+        check(int8_linear(x, w, ws, x_scale=xs, bias=bias, out_dtype=torch.float32), x, w, xs, ws, bias)
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_longest_sums_stay_exact(m):
     """The most negative products at the largest k: 2^14 each, just inside 32 bits."""
