@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import FIE_BF16, FIE_F16, FIE_F32
-from .norm import block_norm
+from .norm import quantized
 
 _DTYPES = {torch.float32: FIE_F32, torch.float16: FIE_F16, torch.bfloat16: FIE_BF16}
 _pack = struct.Struct(_lib.INT8_ARGS).pack
@@ -27,8 +27,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(q, scale) of x [..., k]: scale = max|row| / 127 (float32 [rows]), q = round(row / scale) in
     int8, ties to even; a row of zeros gives 0 and scale 0.  For a weight [channels, k] it gives
     the scales of its channels, for activations those of the tokens."""
-    got = block_norm(x, kind="none", quantize=True)
-    return got.y, got.scale
+    q, scale = quantized(x)
+    return q if x.ndim == 2 else q.view(x.shape), scale
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
@@ -80,8 +80,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         y, y_stride = out, max(out.stride(0), n)
     if tokens:
         if x.dtype != torch.int8:
-            x, x_scale = quantize_rows(x)
-        if len(shape) != 2:
+            x, x_scale = quantized(x)
+        elif len(shape) != 2:
             x = x.reshape(-1, k)
         x_stride, step = x.stride()
         if (k > 1 and step != 1) or (tokens > 1 and x_stride < k):

@@ -32,6 +32,13 @@ class BlockNorm(NamedTuple):
     scale: torch.Tensor | None          # float32 [tokens] with int8
 
 
+def _launch(index: int, args: bytes) -> None:
+    global _run
+    if _run is None:
+        _run = _lib.launcher("fie_block_norm")
+    _run(index, args)
+
+
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     """[tokens, width] with unit element stride (a copy where the view has none)."""
     if t.ndim != 2:
@@ -143,15 +150,34 @@ def block_norm(residual: torch.Tensor, x: torch.Tensor | None = None, weight: to
         y = torch.empty((tokens, width), dtype=torch.int8 if quantize else dtype, device=device)
     y_scale = torch.empty(tokens, dtype=torch.float32, device=device) if quantize else None
     if tokens:
-        global _run
-        if _run is None:
-            _run = _lib.launcher("fie_block_norm")
-        _run(index, _pack(xp, res.data_ptr(), n_ptr, y.data_ptr(), y_scale.data_ptr() if quantize else 0, *vectors, g_ptr,
-                          tokens, x_stride, r_stride, n_stride, width, g_stride, g_step, width, x_dtype, r_dtype,
-                          FIE_I8 if quantize else x_dtype, v_dtype == torch.float32, g_f32, norm, post, scale, eps,
-                          weight_offset))
+        _launch(index, _pack(xp, res.data_ptr(), n_ptr, y.data_ptr(), y_scale.data_ptr() if quantize else 0, *vectors, g_ptr,
+                             tokens, x_stride, r_stride, n_stride, width, g_stride, g_step, width, x_dtype, r_dtype,
+                             FIE_I8 if quantize else x_dtype, v_dtype == torch.float32, g_f32, norm, post, scale, eps,
+                             weight_offset))
     if not flat:
         y = y.view(shape)
         if new is not None and not inplace:
             new = new.view(shape)
     return BlockNorm(residual if inplace else new, y, y_scale)
+
+
+def quantized(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """x [..., width] in int8 [tokens, width], and its rows' scales: what ``block_norm`` of kind "none"
+    gives with ``quantize``, without its other arguments' checks."""
+    shape = x.shape
+    width = shape[-1] if shape else 0
+    if not 1 <= width <= MAX_WIDTH:
+        raise ValueError(f"x must be [..., width] with width in [1, {MAX_WIDTH}]")
+    dtype, index = _DTYPES.get(x.dtype), x.get_device()
+    if dtype is None:
+        raise ValueError("x must be float32, float16 or bfloat16")
+    if index < 0:
+        raise ValueError("quantisation runs on a HIP device")
+    rows = x if len(shape) == 2 and (x.stride(1) == 1 or width == 1) else _rows(x, width)
+    tokens, device = rows.shape[0], rows.device
+    y = torch.empty((tokens, width), dtype=torch.int8, device=device)
+    scale = torch.empty(tokens, dtype=torch.float32, device=device)
+    if tokens:
+        _launch(index, _pack(0, rows.data_ptr(), 0, y.data_ptr(), scale.data_ptr(), 0, 0, 0, 0, 0, tokens, 0, rows.stride(0), 0,
+                             width, 0, 0, width, dtype, dtype, FIE_I8, 0, 0, 2, 0, 1.0, 0.0, 0.0))
+    return y, scale
