@@ -34,17 +34,22 @@ struct Tile { int bm, bn; float cost; };
 constexpr Tile kTiles[] = {{32, 32, 4.6f}, {32, 64, 6.5f}, {64, 64, 10.5f}, {64, 128, 17.0f},
                            {128, 128, 26.0f}, {256, 128, 40.0f}, {256, 256, 73.0f}};
 
-static int cus() { return cu_count() > 0 ? cu_count() : 256; }
+static int cus()
+{
+    const int n = cu_count();
+    return n > 0 ? n : 256;
+}
 
 static int cheapest(int64_t m, int64_t n)
 {
+    const int64_t c = cus();
     int best = 0;
     float least = 0.0f;
     for (int i = 0; i < (int)(sizeof kTiles / sizeof kTiles[0]); ++i) {
         const Tile& t = kTiles[i];
         const int64_t tiles = ((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
-        const float c = t.cost * (float)((tiles + cus() - 1) / cus());
-        if (i == 0 || c < least) { best = i; least = c; }
+        const float cost = t.cost * (float)((tiles + c - 1) / c);
+        if (i == 0 || cost < least) { best = i; least = cost; }
     }
     return best;
 }

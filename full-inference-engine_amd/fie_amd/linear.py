@@ -31,6 +31,15 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return q if x.ndim == 2 else q.view(x.shape), scale
 
 
+def _vector(t: torch.Tensor, name: str, size: int, index: int) -> int:
+    """Its address, if it is a contiguous float32 of that size on that device."""
+    if t.dtype != torch.float32 or t.numel() != size or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous float32 of {size}")
+    if t.get_device() != index:
+        raise ValueError("every tensor must be on the weight's device")
+    return t.data_ptr()
+
+
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
                 x_scale: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                 out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -51,9 +60,12 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     index = weight.get_device()
     if index < 0:
         raise ValueError("int8_linear runs on a HIP device")
-    for t in (x, weight_scale, x_scale, bias, out):
-        if t is not None and t.get_device() != index:
-            raise ValueError("every tensor must be on the weight's device")
+    if x.get_device() != index or (out is not None and out.get_device() != index):
+        raise ValueError("every tensor must be on the weight's device")
+    tokens = x.numel() // k
+    ws = _vector(weight_scale, "weight_scale", n, index)
+    xs = _vector(x_scale, "x_scale", tokens, index) if x_scale is not None else 0
+    bs = _vector(bias, "bias", n, index) if bias is not None else 0
     if x.dtype == torch.int8:
         if x_scale is None:
             raise ValueError("int8 tokens need x_scale")
@@ -67,10 +79,6 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     y_dtype = _DTYPES.get(dtype)
     if y_dtype is None:
         raise ValueError("out_dtype must be float32, float16 or bfloat16")
-    tokens = x.numel() // k
-    for t, name, size in ((weight_scale, "weight_scale", n), (bias, "bias", n), (x_scale, "x_scale", tokens)):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != size or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous float32 of {size}")
     if out is None:
         y, y_stride = torch.empty((tokens, n), dtype=dtype, device=weight.device), n
     else:
@@ -81,6 +89,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     if tokens:
         if x.dtype != torch.int8:
             x, x_scale = quantized(x)
+            xs = x_scale.data_ptr()
         elif len(shape) != 2:
             x = x.reshape(-1, k)
         x_stride, step = x.stride()
@@ -90,8 +99,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         if (k > 1 and step != 1) or (n > 1 and w_stride < k):
             weight, w_stride = weight.contiguous(), k
         xp, wp, x_stride, w_stride = x.data_ptr(), weight.data_ptr(), max(x_stride, k), max(w_stride, k)
-        args = [xp, wp, x_scale.data_ptr(), weight_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr(),
-                tokens, x_stride, w_stride, y_stride, n, k, y_dtype, 0, 0, 0]
+        args = [xp, wp, xs, ws, bs, y.data_ptr(), tokens, x_stride, w_stride, y_stride, n, k, y_dtype, 0, 0, 0]
         global _run
         if _run is None:
             _run = _lib.launcher("fie_int8_linear")
