@@ -286,6 +286,11 @@ __global__ __launch_bounds__(64 * S) void k_int8_rows(const fie_int8_args a, int
 // bytes through NB LDS buffers that the loads fill by themselves (16 bytes a lane, no registers
 // between), NB - 1 stages ahead; a stage costs one barrier.  A wave's instruction fills eight
 // rows of 128 bytes in lane order, so the swizzle of i8_slot is in the addresses it loads from.
+// Large products are bound by the matrix cores and the LDS that feeds them (4096 x 4096 at k 16384
+// 217-225 us, 2.4-2.5 Pop/s, 16 waves of 64 x 64: 8 waves 242, 128 x 128 306), few tokens by the
+// weights' way from memory (16 x 151936 at k 4096 109-113 us, 5.6 TB/s), and what lies between by
+// the loads into LDS, 55-60 GB/s a CU (250 x 16384 at k 4096 25-28 us, where operations and
+// bytes alone take 14; more buffers, fewer waves, two stages a barrier took as long or longer).
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
 // Workgroup b's tile of nrb x ncb.  Workgroups are dealt to the eight XCDs round robin: each
