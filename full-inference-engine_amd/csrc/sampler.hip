@@ -389,6 +389,8 @@ static int prepare(const fie_sampler_args* args, const fie_workspace* ws, KParam
     P->NT = (args->vocab + kTile - 1) / kTile;
     P->NS = (P->NT + kWavesPerWG - 1) / kWavesPerWG;
     P->helpers = 0;
+    P->requests = 0;
+    P->draft_offsets = nullptr;
     if (args->rows == 0) return FIE_OK;
     rc = ws_of(ws, args->rows, args->vocab, &P->w);
     if (rc != FIE_OK) return rc;
@@ -438,19 +440,23 @@ size_t fie_sampler_workspace_size(int32_t max_rows, int32_t vocab)
     return layout_of(max_rows, vocab, &L) ? L.total : 0;
 }
 
-int fie_sampler_sample(const fie_sampler_args* args, const fie_workspace* ws, void* stream)
+static int sample_run(const KParams& P, hipStream_t st)
 {
-    KParams P;
-    int rc = prepare(args, ws, &P);
-    if (rc != FIE_OK || args->rows == 0) return rc;
-    hipStream_t st = (hipStream_t)stream;
-    rc = run_stage(P, FIE_STAGE_PREP, st);
+    int rc = run_stage(P, FIE_STAGE_PREP, st);
     if (rc != FIE_OK) return rc;
     rc = run_stage(P, FIE_STAGE_SCAN, st);
     if (rc != FIE_OK) return rc;
     rc = run_stage(P, FIE_STAGE_FINISH, st);
     if (rc != FIE_OK || finish_in_place(P)) return rc;
     return run_stage(P, FIE_STAGE_DEEP, st);
+}
+
+int fie_sampler_sample(const fie_sampler_args* args, const fie_workspace* ws, void* stream)
+{
+    KParams P;
+    int rc = prepare(args, ws, &P);
+    if (rc != FIE_OK || args->rows == 0) return rc;
+    return sample_run(P, (hipStream_t)stream);
 }
 
 static int lmhead_run(const fie_sampler_args* args, const void* hidden, const void* weight, int32_t hidden_dim,
@@ -512,7 +518,9 @@ int fie_sampler_verify(const fie_sampler_args* args, const fie_verify_args* v, c
     KParams P;
     int rc = prepare(args, ws, &P);
     if (rc != FIE_OK || args->rows == 0) return rc;
-    rc = fie_sampler_sample(args, ws, stream);
+    P.requests = v->requests;
+    P.draft_offsets = v->draft_offsets;
+    rc = sample_run(P, (hipStream_t)stream);
     if (rc != FIE_OK) return rc;
     return launch_status(launch_verify(P, *v, (hipStream_t)stream), "k_verify");
 }

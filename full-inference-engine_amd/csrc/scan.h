@@ -105,6 +105,8 @@ struct KParams {
     int NT;
     int NS;              // spans of kSpan tokens per row
     int helpers;         // 1: k_finish runs one helper workgroup per span of each sampled row
+    int requests;        // of a verification, whose drafts begin at draft_offsets; 0: every row is a step's own
+    const int64_t* draft_offsets;
 };
 
 // ---------------------------------------------------------------- element access

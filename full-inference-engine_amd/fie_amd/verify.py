@@ -5,7 +5,9 @@ A request's drafts are tested, in order, against the distribution the sampler dr
 kept iff ``u * q(d) < p(d)``; the first refusal is replaced by a draw from what ``p`` has over
 ``q``, and after the last kept draft the model's next answer is drawn as ``sample`` draws it.
 What comes out is distributed as if every token had been sampled one by one, and is at
-least one token a request.
+least one token a request.  Where ``sample`` lets a row's answer depend on its batch (token 0
+keeps its penalty only in the widest row), the batch is the rows after as many drafts: those
+that one step of ``sample`` would hold.
 
 The reference accepts drafts by argmax only (engine/speculative/acceptance.py); a request
 with temperature 0 gives exactly that here.

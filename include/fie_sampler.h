@@ -209,7 +209,8 @@ int fie_sampler_kept(const fie_sampler_args* args, uint8_t* kept, float* probs,
    k_r + 1 rows of logits, one after another from row draft_offsets[r] + r on: row j is the
    model's answer after j drafts.  The sampler's args describe these rows (its rows = drafts
    + requests), with FIE_FLAG_NO_DRAW on every row but a request's last (and see `draws`), and
-   one draw u a row.
+   one draw u a row.  Where a row's answer depends on the batch (token 0 keeps its penalty only
+   in the widest row), its batch is the rows after as many drafts, as in a step of sampling.
    With p the row's kept distribution (weights over kept mass, fp32) and q the draft's (all
    on d_j without draft_probs):
      d_j is kept iff u_j * q(d_j) < p(d_j), a product in double, and every draft before it was
@@ -239,7 +240,7 @@ typedef struct fie_verify_args {
 #define FIE_MAX_DRAFTS 255
 #define FIE_VERIFY_DRAWS_VOCAB 63488
 
-/* fie_sampler_sample on the rows, then the verification, on one stream. */
+/* The sampler's step on the rows, then the verification, on one stream. */
 int fie_sampler_verify(const fie_sampler_args* args, const fie_verify_args* verify,
                        const fie_workspace* ws, void* stream);
 
