@@ -150,17 +150,21 @@ FIE_DEV float row_sum(float x, float* slot)
     return t;
 }
 
+// The largest |v|, by bits: those of values >= 0 order them, and NaN's lie past infinity's, so that
+// a row with a NaN gives NaN (a float maximum drops it).
+FIE_DEV uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
 template <bool ONE>
-FIE_DEV float row_max(float x, float* slot)     // of values >= 0: their bits order them
+FIE_DEV float row_max(uint32_t x, float* slot)
 {
-    x = __uint_as_float(dwave_max_u32(__float_as_uint(x)));
-    if (ONE) return x;
+    x = dwave_max_u32(x);
+    if (ONE) return __uint_as_float(x);
     const int waves = blockDim.x >> 6;
-    if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = x;
+    if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = __uint_as_float(x);
     __syncthreads();
-    float t = 0.0f;
-    for (int w = 0; w < waves; ++w) t = slot[w] > t ? slot[w] : t;
-    return t;
+    uint32_t t = 0;
+    for (int w = 0; w < waves; ++w) t = max(t, __float_as_uint(slot[w]));
+    return __uint_as_float(t);
 }
 
 // DX: x and y; DR: residual.  A row's thread t holds vectors t, t + T, ..: VPT of them, 0 past
@@ -284,11 +288,11 @@ __global__ __launch_bounds__(ONE ? 256 : (VPT > 2 ? 1024 : 512)) void k_norm(con
         for (int i = 0; i < VPT; ++i) store8<DX>(yp, (i * T + t) * 8, H, v[i]);
         return;
     }
-    float m = 0.0f;
+    uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = __builtin_fmaxf(m, __builtin_fabsf(v[i][e]));
+        for (int e = 0; e < 8; ++e) m = max(m, abs_bits(v[i][e]));
     // IEEE quotients: what a plain x / (max|x| / 127) rounds to
     const float s = row_max<ONE>(m, red[4]) / 127.0f;
     if (t == 0) a.y_scale[row] = s;
@@ -299,8 +303,8 @@ __global__ __launch_bounds__(ONE ? 256 : (VPT > 2 ? 1024 : 512)) void k_norm(con
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float u = __builtin_rintf(v[i][e] / s);
-            // NaN (0 / 0, inf / inf) and rows without a scale: 0; past 127 where s is a few
-            // denormal units, rounded down
+            // 0 in rows without a scale (0) or with a NaN (its scale), and for inf / inf; past 127
+            // where s is a few denormal units, rounded down
             q[e] = s > 0.0f && u == u ? __builtin_fminf(__builtin_fmaxf(u, -127.0f), 127.0f) : 0.0f;
         }
         store8_i8(yp, (i * T + t) * 8, H, q);

@@ -25,8 +25,9 @@ MAX_CHANNELS = 0x7FFFFF00
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(q, scale) of x [..., k]: scale = max|row| / 127 (float32 [rows]), q = round(row / scale) in
-    int8, ties to even; a row of zeros gives 0 and scale 0.  For a weight [channels, k] it gives
-    the scales of its channels, for activations those of the tokens."""
+    int8, ties to even; a row of zeros gives 0 and scale 0, a row with a NaN 0 and scale NaN (its
+    products are then NaN).  For a weight [channels, k] it gives the scales of its channels, for
+    activations those of the tokens."""
     q, scale = quantized(x)
     return q if x.ndim == 2 else q.view(x.shape), scale
 

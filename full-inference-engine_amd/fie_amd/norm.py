@@ -6,7 +6,8 @@
 
 with the norm over the last dimension (RMS or layer), everything in fp32 between the loads and
 the stores; ``y`` optionally in 8-bit integers with a scale for each token, as
-``fie_amd.linear.int8_linear`` takes it.
+``fie_amd.linear.int8_linear`` takes it (a token with a NaN has the scale NaN, and its products are
+NaN).
 """
 
 from __future__ import annotations

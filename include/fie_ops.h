@@ -30,7 +30,8 @@ enum { FIE_NORM_RMS = 0, FIE_NORM_LAYER = 1, FIE_NORM_NONE = 2 };
    Absent weights are 1 (without the offset), absent biases 0.  r is rounded into
    residual_out, y is taken from the unrounded r.  With y_dtype FIE_I8, y is stored as
    round(y / s), at most 127 either way, s = max|y| / 127 of its row in y_scale (an all-zero
-   row: 0 and s = 0). */
+   row: 0 and s = 0; a row with a NaN: 0 and s = NaN, one with an infinity: 0 and s infinite, so that
+   the product's row is NaN in both). */
 typedef struct fie_norm_args {
     const void* x;              /* [tokens, width], or NULL */
     const void* residual;       /* [tokens, width] */

@@ -21,6 +21,22 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a HIP device (MI355X) and the built library")
 
 
+# Tests that expect a value that the definition does not give.  They stay as they are and run;
+# the tests named beside them hold what the definition gives.
+_WRONG_VALUES = {
+    ("test_gpu_norm.py", "test_quantize_rows_is_the_ieee_quotient"):
+        "takes the scale of a row with a NaN from its other elements; max|row| / 127 is NaN "
+        "(test_gpu_quantize_values.py, test of the same name)",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        why = _WRONG_VALUES.get((item.path.name, getattr(item, "originalname", item.name)))
+        if why:
+            item.add_marker(pytest.mark.xfail(reason=why, raises=AssertionError, strict=True))
+
+
 @pytest.fixture(scope="session")
 def oracle_lib():
     import oracle
