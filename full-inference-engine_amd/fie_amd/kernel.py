@@ -19,6 +19,8 @@ from ._lib import LP_COLS, SamplerArgs, Workspace
 _DTYPES = {torch.float32: _lib.FIE_F32, torch.float16: _lib.FIE_F16,
            torch.bfloat16: _lib.FIE_BF16}
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
 # Per-row parameter arrays in upload order: (name, dtype, values per row).
 PARAM_FIELDS = (
     ("scale", np.float32, 1), ("top_k", np.int32, 1), ("top_p", np.float32, 1),
@@ -231,16 +233,22 @@ class FusedSampler:
         # Two workspaces: batches of at most HELP_ROWS rows use one sized for
         # HELP_ROWS, which also holds the span helpers' arrays (the library runs
         # k_finish's helpers only in such a workspace); larger batches use one that
-        # grows with the largest batch seen.
-        self._wss: dict[bool, tuple[torch.Tensor | None, Workspace, tuple[int, int]]] = {
-            True: (None, Workspace(), (0, 0)), False: (None, Workspace(), (0, 0))}
+        # grows with the largest batch seen.  With each the stream it was allocated on.
+        self._wss: dict[bool, tuple[torch.Tensor | None, Workspace, tuple[int, int], int]] = {
+            True: (None, Workspace(), (0, 0), 0), False: (None, Workspace(), (0, 0), 0)}
         self._steps: dict[tuple[int, int], DeviceStep] = {}
 
     # ------------------------------------------------------------------ workspace
     def ensure_workspace(self, rows: int, vocab: int) -> Workspace:
+        """A workspace for a call of this size on the current stream.  One that was allocated on
+        another stream is marked as used on this one: when it is replaced or dropped, its memory
+        goes back to the other stream's pool, and is not to be handed out while kernels here
+        still use it.  (A captured call's workspace outlives the graph instead.)"""
         small = rows <= HELP_ROWS
-        tensor, ws, (r0, v0) = self._wss[small]
+        tensor, ws, (r0, v0), made_on = self._wss[small]
         if rows <= r0 and vocab <= v0:
+            if _raw_stream(tensor.get_device()) != made_on and not torch.cuda.is_current_stream_capturing():
+                tensor.record_stream(torch.cuda.current_stream(tensor.device))
             return ws
         rows = HELP_ROWS if small else max(rows, r0, 1)
         vocab = max(vocab, v0)
@@ -250,7 +258,7 @@ class FusedSampler:
                              f"(vocab must be in [1, {_lib.MAX_VOCAB}])")
         tensor = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         ws = Workspace(tensor.data_ptr(), nbytes, rows, vocab)
-        self._wss[small] = (tensor, ws, (rows, vocab))
+        self._wss[small] = (tensor, ws, (rows, vocab), _raw_stream(tensor.get_device()))
         return ws
 
     def _stream_ptr(self) -> int:

@@ -123,7 +123,8 @@ class VerifyPlan:
 
 class DraftVerifier:
     """Verifies drafts on one device; calls of one verifier share a workspace and go on one
-    stream at a time.  A captured call keeps its plan's and the verifier's buffers by address:
+    stream at a time (going over to another stream, with a wait, is fine: the workspace and the plan's
+    memory are kept for both).  A captured call keeps its plan's and the verifier's buffers by address:
     both outlive the graph, plans are made well before the capture, and the largest call (rows,
     vocabulary) goes before it, so that the workspace grows no more."""
 
