@@ -344,7 +344,8 @@ class BatchedSampler:
         j is the model's answer after j drafts.  ``draft_probs`` [all drafts, vocab] are the
         distributions the drafts were drawn from; without them a draft counts as certain.
         ``context_tokens`` are the requests' contexts without the drafts.  A seeded request
-        takes len(drafts[i]) + 1 draws of its stream, whatever it keeps."""
+        takes len(drafts[i]) + 1 draws of its stream, whatever it keeps; a call that is refused
+        takes none."""
         from ..verify import DraftVerifier, VerifyPlan
 
         if logits.ndim != 2:
@@ -365,9 +366,14 @@ class BatchedSampler:
             return VerifyResult([], [])
         if self._verifier is None:
             self._verifier = DraftVerifier(self.device, self._fused)
-        plan = VerifyPlan(self._fused, params, lens, logits.shape[1], context_tokens, drafts,
-                          self._verify_keys(params, lens, request_ids), shared=True)
         ids = torch.tensor(flat, dtype=torch.int64).to(logits.device)
+
+        def keys(plan: VerifyPlan) -> np.ndarray:
+            # a call that is refused takes no draws: they come after every check
+            plan.check(logits, ids, None, draft_probs)
+            return self._verify_keys(params, lens, request_ids)
+
+        plan = VerifyPlan(self._fused, params, lens, logits.shape[1], context_tokens, drafts, keys, shared=True)
         got = self._verifier.verify(plan, logits, ids, None, draft_probs)
         accepted = got.accepted.tolist()
         return VerifyResult([row[:n + 1] for row, n in zip(got.tokens.tolist(), accepted)], accepted)

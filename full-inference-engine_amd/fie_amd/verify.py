@@ -16,7 +16,7 @@ with temperature 0 gives exactly that here.
 from __future__ import annotations
 
 import ctypes
-from typing import NamedTuple
+from typing import Callable, NamedTuple
 
 import numpy as np
 import torch
@@ -46,8 +46,10 @@ class VerifyPlan:
 
     def __init__(self, fused: FusedSampler, params: list[SamplingParams], draft_lens: list[int], vocab: int,
                  contexts: list[list[int]] | None = None, drafts: list[list[int]] | None = None,
-                 rng: np.ndarray | None = None, shared: bool = False):
-        # shared: the fused sampler's own block of this size, for one call that is waited for
+                 rng: np.ndarray | Callable[[VerifyPlan], np.ndarray] | None = None, shared: bool = False):
+        # rng as a function is asked for the draws when everything else has been checked, so that
+        # a plan that is refused takes none.  shared: the fused sampler's own block of this size,
+        # for one call that is waited for
         if len(draft_lens) != len(params):
             raise ValueError("one draft length per request is required")
         lens = np.asarray(draft_lens, dtype=np.int64).reshape(-1)
@@ -72,7 +74,7 @@ class VerifyPlan:
             if drafts is None:
                 raise ValueError("requests with penalties need their drafts on the host")
             row_contexts = [list(c) + list(d[:j]) for c, d in zip(contexts, drafts) for j in range(len(d) + 1)]
-        hp = resolve_params(row_params, vocab, None, row_contexts, rng=rng)
+        hp = resolve_params(row_params, vocab, None, row_contexts, rng=None if callable(rng) else rng)
         last = np.cumsum(lens + 1) - 1
         no_draw = np.full(self.rows, FLAG_NO_DRAW, dtype=np.int32)
         no_draw[last] = 0
@@ -88,6 +90,9 @@ class VerifyPlan:
         np.cumsum(lens, out=self._offsets.numpy()[1:])
         self._offsets = self._offsets.to(fused.device)
         self.index = self._offsets.get_device()
+        self.has_rng = rng is not None
+        if callable(rng):
+            hp.rng = np.ascontiguousarray(rng(self), dtype=np.uint64).reshape(self.rows, 3)
         # the parameter block, uploaded once
         self._buf = (fused.step_buffers(self.rows, hp.tail_ints()) if shared
                      else DeviceStep(self.rows, hp.tail_ints(), fused.device))
@@ -101,7 +106,6 @@ class VerifyPlan:
             a.hist_invalid = self._buf.ptr("hist_invalid")
         if hp.rng is not None:
             a.rng = self._buf.ptr("rng")
-        self.has_rng = hp.rng is not None
         self.args = a
         v = VerifyArgs()
         v.requests, v.max_drafts = self.requests, self.max_drafts
@@ -110,6 +114,24 @@ class VerifyPlan:
         self.stream = _raw_stream(self.index)
         self._ready = torch.cuda.Event()
         self._ready.record(torch.cuda.current_stream(fused.device))
+
+    def check(self, logits: torch.Tensor, draft_ids: torch.Tensor, uniforms: torch.Tensor | None,
+              draft_probs: torch.Tensor | None) -> None:
+        """ValueError where a call's tensors do not fit the plan."""
+        rows, drafts, vocab, index = self.rows, self.drafts, self.vocab, self.index
+        if logits.shape != self.logits_shape:
+            raise ValueError(f"logits must be [{rows}, {vocab}], a request's drafts + 1 rows together")
+        if draft_ids.dtype != torch.int64 or draft_ids.shape != self.ids_shape:
+            raise ValueError(f"draft_ids must be int64 [{drafts}]")
+        if (uniforms is None) != self.has_rng:
+            raise ValueError("uniforms are required, or a plan that draws on the device, not both")
+        if uniforms is not None and (uniforms.dtype != torch.float64 or uniforms.shape != self.rows_shape):
+            raise ValueError(f"uniforms must be float64 [{rows}]")
+        if draft_probs is not None and (draft_probs.shape != self.probs_shape or draft_probs.dtype not in _DTYPES):
+            raise ValueError(f"draft_probs must be [{drafts}, {vocab}] in float32, float16 or bfloat16")
+        for t in (logits, draft_ids, uniforms, draft_probs):
+            if t is not None and t.get_device() != index:
+                raise ValueError(f"every tensor must be on device {index}")
 
     def use_on(self, stream: torch.cuda.Stream) -> None:
         """The settings' upload comes before what ``stream`` runs next, and their memory is kept
@@ -150,20 +172,8 @@ class DraftVerifier:
         ``uniforms`` float64 [rows] in [0, 1): a row's test of its draft, and on a request's
         last row its draw.  ``draft_probs`` [drafts, vocab]: the distributions the drafts were
         drawn from; without them a draft counts as certain (prompt lookup, argmax drafts)."""
+        plan.check(logits, draft_ids, uniforms, draft_probs)
         rows, drafts, vocab, index = plan.rows, plan.drafts, plan.vocab, plan.index
-        if logits.shape != plan.logits_shape:
-            raise ValueError(f"logits must be [{rows}, {vocab}], a request's drafts + 1 rows together")
-        if draft_ids.dtype != torch.int64 or draft_ids.shape != plan.ids_shape:
-            raise ValueError(f"draft_ids must be int64 [{drafts}]")
-        if (uniforms is None) != plan.has_rng:
-            raise ValueError("uniforms are required, or a plan that draws on the device, not both")
-        if uniforms is not None and (uniforms.dtype != torch.float64 or uniforms.shape != plan.rows_shape):
-            raise ValueError(f"uniforms must be float64 [{rows}]")
-        if draft_probs is not None and (draft_probs.shape != plan.probs_shape or draft_probs.dtype not in _DTYPES):
-            raise ValueError(f"draft_probs must be [{drafts}, {vocab}] in float32, float16 or bfloat16")
-        for t in (logits, draft_ids, uniforms, draft_probs):
-            if t is not None and t.get_device() != index:
-                raise ValueError(f"every tensor must be on device {index}")
         device = logits.device
         if _raw_stream(index) != plan.stream:
             plan.use_on(torch.cuda.current_stream(index))
