@@ -36,6 +36,39 @@ static hipError_t norm_of(const fie_norm_args& a, hipStream_t st)
     }
 }
 
+// The rows of one launch: a grid holds fewer than 2^32 threads (past that the launch leaves rows
+// out, without an error), and a row takes 64 of them or at most 1024.
+static int64_t rows_at_once(int width) { return width <= 512 ? 1 << 25 : 1 << 21; }
+
+static fie_norm_args rows_from(fie_norm_args a, int64_t row)
+{
+    auto size = [](int dtype) -> int64_t { return dtype == FIE_I8 ? 1 : dtype == FIE_F32 ? 4 : 2; };
+    auto on = [&](auto* p, int64_t stride, int64_t bytes) { return p ? (decltype(p))((uintptr_t)p + (uintptr_t)(row * stride * bytes)) : p; };
+    a.x = on(a.x, a.x_stride, size(a.x_dtype));
+    a.residual = on(a.residual, a.residual_stride, size(a.residual_dtype));
+    a.residual_out = on(a.residual_out, a.residual_out_stride, size(a.residual_dtype));
+    a.y = on(a.y, a.y_stride, size(a.y_dtype));
+    a.y_scale = on(a.y_scale, 1, 4);
+    a.gate = on(a.gate, a.gate_stride, a.gate_f32 ? 4 : size(a.x_dtype));
+    a.tokens -= row;
+    return a;
+}
+
+static hipError_t norm_run(const fie_norm_args& a, hipStream_t st)
+{
+    switch (a.x_dtype * 3 + a.residual_dtype) {
+    case FIE_F32 * 3 + FIE_F32: return norm_of<FIE_F32, FIE_F32>(a, st);
+    case FIE_F32 * 3 + FIE_F16: return norm_of<FIE_F32, FIE_F16>(a, st);
+    case FIE_F32 * 3 + FIE_BF16: return norm_of<FIE_F32, FIE_BF16>(a, st);
+    case FIE_F16 * 3 + FIE_F32: return norm_of<FIE_F16, FIE_F32>(a, st);
+    case FIE_F16 * 3 + FIE_F16: return norm_of<FIE_F16, FIE_F16>(a, st);
+    case FIE_F16 * 3 + FIE_BF16: return norm_of<FIE_F16, FIE_BF16>(a, st);
+    case FIE_BF16 * 3 + FIE_F32: return norm_of<FIE_BF16, FIE_F32>(a, st);
+    case FIE_BF16 * 3 + FIE_F16: return norm_of<FIE_BF16, FIE_F16>(a, st);
+    default: return norm_of<FIE_BF16, FIE_BF16>(a, st);
+    }
+}
+
 static int norm_check(const fie_norm_args* a)
 {
     if (!a) return fail(FIE_E_ARG, "args is NULL");
@@ -65,17 +98,12 @@ extern "C" int fie_block_norm(const fie_norm_args* a, void* stream)
     const int rc = norm_check(a);
     if (rc != FIE_OK || a->tokens == 0) return rc;
     hipStream_t st = (hipStream_t)stream;
-    hipError_t e;
-    switch (a->x_dtype * 3 + a->residual_dtype) {
-    case FIE_F32 * 3 + FIE_F32: e = norm_of<FIE_F32, FIE_F32>(*a, st); break;
-    case FIE_F32 * 3 + FIE_F16: e = norm_of<FIE_F32, FIE_F16>(*a, st); break;
-    case FIE_F32 * 3 + FIE_BF16: e = norm_of<FIE_F32, FIE_BF16>(*a, st); break;
-    case FIE_F16 * 3 + FIE_F32: e = norm_of<FIE_F16, FIE_F32>(*a, st); break;
-    case FIE_F16 * 3 + FIE_F16: e = norm_of<FIE_F16, FIE_F16>(*a, st); break;
-    case FIE_F16 * 3 + FIE_BF16: e = norm_of<FIE_F16, FIE_BF16>(*a, st); break;
-    case FIE_BF16 * 3 + FIE_F32: e = norm_of<FIE_BF16, FIE_F32>(*a, st); break;
-    case FIE_BF16 * 3 + FIE_F16: e = norm_of<FIE_BF16, FIE_F16>(*a, st); break;
-    default: e = norm_of<FIE_BF16, FIE_BF16>(*a, st); break;
+    hipError_t e = hipSuccess;
+    const int64_t most = rows_at_once(a->width);
+    for (int64_t row = 0; row < a->tokens && e == hipSuccess; row += most) {
+        fie_norm_args part = rows_from(*a, row);
+        if (part.tokens > most) part.tokens = most;
+        e = norm_run(part, st);
     }
     return launch_status(e, "k_norm");
 }
