@@ -1,5 +1,7 @@
 // The 8-bit integer product behind the C ABI of include/fie_ops.h: instantiations of int8.h's
 // kernels and the choice among them.
+#include <algorithm>
+
 #include "int8.h"
 
 namespace fie {
@@ -137,6 +139,39 @@ static hipError_t int8_dt(fie_int8_args a, hipStream_t st)
     }
 }
 
+// A launch holds fewer than 2^32 threads (past that it leaves tiles out, without an error), so
+// larger products go in pieces: channels and tokens whose layout (64 threads a row) and rows' kernel
+// (32 a channel) fit, and tokens, whole tiles of any size, that leave 2^22 tiles of 32 x 32 (512
+// threads each; larger tiles have at most twice the threads and half the tiles).
+constexpr int64_t kMostChannels = 1 << 24, kMostTokens = 1 << 25, kMostTiles = 1 << 22;
+
+static hipError_t int8_run(const fie_int8_args& a, hipStream_t st)
+{
+    const int64_t size = a.y_dtype == FIE_F32 ? 4 : 2;
+    for (int64_t n0 = 0; n0 < a.n; n0 += kMostChannels) {
+        fie_int8_args p = a;
+        p.n = (int)std::min<int64_t>(a.n - n0, kMostChannels);
+        p.w = a.w + n0 * a.w_stride;
+        p.w_scale = a.w_scale + n0;
+        p.bias = a.bias ? a.bias + n0 : nullptr;
+        const int64_t most = std::min(kMostTokens, kMostTiles / ((p.n + 31) / 32) * 32 / 256 * 256);
+        for (int64_t m0 = 0; m0 < a.m; m0 += most) {
+            p.m = std::min(a.m - m0, most);
+            p.x = a.x + m0 * a.x_stride;
+            p.x_scale = a.x_scale + m0;
+            p.y = (char*)a.y + (m0 * a.y_stride + n0) * size;
+            hipError_t e;
+            switch (a.y_dtype) {
+            case FIE_F32: e = int8_dt<FIE_F32>(p, st); break;
+            case FIE_F16: e = int8_dt<FIE_F16>(p, st); break;
+            default: e = int8_dt<FIE_BF16>(p, st); break;
+            }
+            if (e != hipSuccess) return e;
+        }
+    }
+    return hipSuccess;
+}
+
 static int int8_check(const fie_int8_args* a)
 {
     if (!a) return fail(FIE_E_ARG, "args is NULL");
@@ -167,12 +202,5 @@ extern "C" int fie_int8_linear(const fie_int8_args* a, void* stream)
 {
     const int rc = int8_check(a);
     if (rc != FIE_OK || a->m == 0) return rc;
-    hipStream_t st = (hipStream_t)stream;
-    hipError_t e;
-    switch (a->y_dtype) {
-    case FIE_F32: e = int8_dt<FIE_F32>(*a, st); break;
-    case FIE_F16: e = int8_dt<FIE_F16>(*a, st); break;
-    default: e = int8_dt<FIE_BF16>(*a, st); break;
-    }
-    return launch_status(e, "k_int8");
+    return launch_status(int8_run(*a, (hipStream_t)stream), "k_int8");
 }
