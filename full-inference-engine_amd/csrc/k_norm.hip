@@ -20,6 +20,10 @@ template <int DX, int DR>
 static hipError_t norm_of(const fie_norm_args& a, hipStream_t st)
 {
     const int vecs = (a.width + 7) / 8;
+    if (a.width > FIE_MAX_WIDTH) {                      // to int8 alone (norm_check)
+        k_quantise_wide<DR><<<(unsigned)a.tokens, 1024, 0, st>>>(a);
+        return hipGetLastError();
+    }
     if (vecs <= 64) return norm_at<DX, DR, 1, true>(a, (unsigned)((a.tokens + 3) / 4), 256, st);
     // Few rows: a vector a thread, the shorter chain (1 x 4096 4.2 us with two, 3.0; 512 x 4096
     // layer 8.2, 7.9); many: two, more in flight a workgroup (1024 x 4096 7.6 with two, 8.4;
@@ -73,7 +77,10 @@ static int norm_check(const fie_norm_args* a)
 {
     if (!a) return fail(FIE_E_ARG, "args is NULL");
     if (a->tokens < 0 || a->tokens > 0x7FFFFFFF) return fail(FIE_E_ARG, "tokens out of range");
-    if (a->width < 1 || a->width > FIE_MAX_WIDTH) return fail(FIE_E_ARG, "width out of range [1, 65536]");
+    const bool alone = !a->x && !a->residual_out && a->kind == FIE_NORM_NONE && a->y && a->y_dtype == FIE_I8;
+    if (a->width < 1 || a->width > FIE_MAX_WIDTH)
+        if (!alone || a->width < 1 || a->width > FIE_MAX_K)
+            return fail(FIE_E_ARG, "width out of range [1, 65536] (a quantisation alone: 131071)");
     if (a->x_dtype < FIE_F32 || a->x_dtype > FIE_BF16 || a->residual_dtype < FIE_F32 || a->residual_dtype > FIE_BF16)
         return fail(FIE_E_ARG, "unknown dtype");
     if (a->x && a->residual_dtype != a->x_dtype && a->residual_dtype != FIE_F32)

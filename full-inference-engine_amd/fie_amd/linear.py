@@ -2,8 +2,8 @@
 
     y[t, n] = x_scale[t] * w_scale[n] * sum_k x[t, k] * w[n, k]   (+ bias[n])
 
-The sums are exact in 32 bits; scaling is fp32, rounded once to the output's type.  Weights keep
-nn.Linear's [channels, k] layout.
+The sums are exact in 32 bits (k up to MAX_K; those of longer products could pass them); scaling
+is fp32, rounded once to the output's type.  Weights keep nn.Linear's [channels, k] layout.
 """
 
 from __future__ import annotations
@@ -14,12 +14,11 @@ import torch
 
 from . import _lib
 from ._lib import FIE_BF16, FIE_F16, FIE_F32
-from .norm import quantized
+from .norm import MAX_K, quantized
 
 _DTYPES = {torch.float32: FIE_F32, torch.float16: FIE_F16, torch.bfloat16: FIE_BF16}
 _pack = struct.Struct(_lib.INT8_ARGS).pack
 _run = None             # the library's entry, loaded with the first call
-MAX_K = 131071          # the sums of longer products could pass 32 bits
 MAX_CHANNELS = 0x7FFFFF00
 
 

@@ -25,6 +25,7 @@ _KINDS = {"rms": 0, "layer": 1, "none": 2}
 _pack = struct.Struct(_lib.NORM_ARGS).pack
 _run = None             # the library's entry, loaded with the first call
 MAX_WIDTH = 65536
+MAX_K = 131071          # of a quantisation alone: as wide as the 8-bit product takes its rows
 
 
 class BlockNorm(NamedTuple):
@@ -164,11 +165,11 @@ def block_norm(residual: torch.Tensor, x: torch.Tensor | None = None, weight: to
 
 def quantized(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x [..., width] in int8 [tokens, width], and its rows' scales: what ``block_norm`` of kind "none"
-    gives with ``quantize``, without its other arguments' checks."""
+    gives with ``quantize``, without its other arguments' checks, and up to MAX_K wide."""
     shape = x.shape
     width = shape[-1] if shape else 0
-    if not 1 <= width <= MAX_WIDTH:
-        raise ValueError(f"x must be [..., width] with width in [1, {MAX_WIDTH}]")
+    if not 1 <= width <= MAX_K:
+        raise ValueError(f"x must be [..., k] with k in [1, {MAX_K}]")
     dtype, index = _DTYPES.get(x.dtype), x.get_device()
     if dtype is None:
         raise ValueError("x must be float32, float16 or bfloat16")

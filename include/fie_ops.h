@@ -47,7 +47,7 @@ typedef struct fie_norm_args {
     int64_t x_stride, residual_stride, residual_out_stride, y_stride;   /* elements between rows */
     int64_t gate_stride;        /* 0: one row for every token */
     int32_t gate_step;          /* 1, or 0: one value for a whole row */
-    int32_t width;              /* 1..FIE_MAX_WIDTH */
+    int32_t width;              /* 1..FIE_MAX_WIDTH (FIE_MAX_K: kind NONE of a residual alone to FIE_I8) */
     int32_t x_dtype;            /* of x and y (without x: of y's float type); FIE_F32, F16, BF16 */
     int32_t residual_dtype;     /* x_dtype or FIE_F32 (without x: any of the three) */
     int32_t y_dtype;            /* x_dtype or FIE_I8 */
