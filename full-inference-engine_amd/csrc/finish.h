@@ -914,37 +914,14 @@ FIE_DEV int keep_from(FinSmem& S, int nv, uint32_t key)
     return m;
 }
 
-// Token 0 keeps its penalty iff the row is the widest of its step (no pad entry
+// Token 0 keeps its penalty iff the row is the widest of the batch (no pad entry
 // rewrites index 0 after it) and no id >= vocab first occurs after it
-// (sampler.py:148,156-157,174-175 with a sequential scatter).  A step's rows are the batch;
-// in a verification they are the rows after as many drafts, one of each request that has
-// them: what a step of sampling would hold.  (A request's later rows have its drafts in
-// their history and are wider; against all rows only the widest request's last row would
-// keep the penalty.)
+// (sampler.py:148,156-157,174-175 with a sequential scatter).  A verification's rows are
+// not one batch: k_steps settles them.
 FIE_DEV bool q1_keeps(FinSmem& S, const KParams& P, int row)
 {
     const fie_sampler_args& a = P.a;
     const int NT = P.NT, B = a.rows, tid = threadIdx.x;
-    const int64_t* const off = P.requests ? P.draft_offsets : nullptr;
-    const int members = off ? P.requests : B;
-    int64_t place = 0;                          // drafts before the row
-    if (off) {                                  // of the last request to begin at the row or before
-        int lo = 0, hi = P.requests - 1;
-        while (lo < hi) {
-            const int mid = lo + (hi - lo + 1) / 2;
-            if (off[mid] <= (int64_t)row - mid) lo = mid;
-            else hi = mid - 1;
-        }
-        place = (int64_t)row - lo - off[lo];
-    }
-    // member i's row of this step, or -1 (drafts too few, offsets that do not fit)
-    auto row_of = [&](int i) -> int {
-        if (!off) return i;
-        const int64_t first = off[i], end = off[i + 1];
-        if (place < 0 || first < 0 || first > B || end > B || end - first < place) return -1;
-        const int64_t r = first + i + place;
-        return r < B ? (int)r : -1;
-    };
     auto nu_of = [&](int r) -> uint32_t {
         if (!(a.flags[r] & FIE_FLAG_PENALTY)) return 0u;
         uint32_t u = P.w.tok0c[r] ? 1u : 0u;
@@ -952,13 +929,7 @@ FIE_DEV bool q1_keeps(FinSmem& S, const KParams& P, int row)
         return u;
     };
     uint32_t mine = 0, wmax = 0;
-    if (off) {                                  // offsets that do not fit may leave the row out
-        if (tid == 0) S.red32[31] = 0;
-        __syncthreads();
-    }
-    for (int i = tid; i < members; i += kFinThreads) {
-        const int r = row_of(i);
-        if (r < 0) continue;
+    for (int r = tid; r < B; r += kFinThreads) {
         uint32_t u = nu_of(r);
         for (int t = 0; t < NT; ++t) u += P.w.nu[(size_t)r * NT + t];
         wmax = u > wmax ? u : wmax;
@@ -1558,7 +1529,7 @@ FIE_DEV void finish_row(FinSmem& S, const KParams& P, const int row)
 
     // Token 0 (a tile of its own).
     float w0 = x0;
-    if (c0 && q1_keeps(S, P, row)) w0 = penalize(x0, rep, pres, freq, c0);
+    if (c0 && (P.settled0 || q1_keeps(S, P, row))) w0 = penalize(x0, rep, pres, freq, c0);
     const float y0 = s == 1.0f ? w0 + 0.0f : scaled(w0, s);
     const uint32_t k0 = fkey(y0);
 

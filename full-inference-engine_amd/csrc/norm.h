@@ -316,9 +316,9 @@ __global__ __launch_bounds__(ONE ? 256 : (VPT > 2 ? 1024 : 512)) void k_norm(con
     }
 }
 
-// A row wider than the registers of a workgroup, to int8 and nothing else: twice over it, the second
-// time from the L2, where 256 rows of 0.3 MB at a time fit.  bf16 4096 x 131064 446 us, 1.6 GB at
-// 3.6 TB/s; 250 x 131071 35 us, one row 25 (the chain of 32 loads a thread).
+// A row wider than the registers of a workgroup, to int8 and nothing else: twice over it (the rows on
+// their way at a time, 256 of 0.26 MB, are past the L2 but not past the cache behind it).  bf16
+// 4096 x 131064 446 us, 1.6 GB read and written once at 3.6 TB/s; 250 x 131071 35 us, one row 25 (the chain of 32 loads a thread).
 template <int DR>
 __global__ __launch_bounds__(1024) void k_quantise_wide(const fie_norm_args a)
 {

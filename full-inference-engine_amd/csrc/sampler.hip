@@ -1,6 +1,7 @@
 // MI355X fused token sampler: kernels behind the C ABI of include/fie_sampler.h.
 //
 //   k_prep      penalty histories bucketed by span                (here)
+//   k_steps     token 0's penalty in a verification, by steps     (here)
 //   k_scan      one streaming read of the logits, tile partials   (scan.h)
 //   k_finish    one workgroup per row: exact selection and draw   (finish.h)
 //   k_argmax_*  the greedy fast path, logits.argmax(-1)           (sampler.py:106)
@@ -68,6 +69,65 @@ __global__ __launch_bounds__(kPrepThreads) void k_prep(const KParams P)
     if (tid == 0) {
         P.w.tok0c[row] = zc;
         P.w.bad[row] = badc;
+    }
+}
+
+// ---------------------------------------------------------------- k_steps
+// Token 0's penalty in a verification, by steps: the reference's rule (q1_keeps) is one of a
+// step's batch, and a step's rows here are those after as many drafts, one of each request
+// that has them: what a step of sampling would hold.  (A request's later rows have its drafts
+// in their history and are wider: against all rows together only the widest request's last
+// row would keep the penalty.)  A workgroup a step: the rows' widths, a wave four rows at a
+// time, into the first of their tiles' counts; then rows that lose the penalty are left with no
+// token 0 in their history, which FINISH takes as it is.  Two dependent round trips for every
+// 64 requests.
+constexpr int kStepThreads = 1024;
+
+__global__ __launch_bounds__(kStepThreads) void k_steps(const KParams P, const fie_verify_args v)
+{
+    constexpr int W = kStepThreads / 64, U = 4;         // waves, rows of a wave at a time
+    __shared__ uint32_t red[W];
+    const fie_sampler_args& a = P.a;
+    const int place = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, NT = P.NT;
+    const int64_t* off = v.draft_offsets;
+    // request i's row of this step; -1: too few drafts, offsets that do not fit, no penalties
+    auto row_of = [&](int i) -> int {
+        if (i >= v.requests) return -1;
+        const int64_t first = off[i], end = off[i + 1];
+        if (first < 0 || first > a.rows || end > a.rows || end - first < place) return -1;
+        const int64_t r = first + i + place;
+        return r < a.rows && (a.flags[r] & FIE_FLAG_PENALTY) ? (int)r : -1;
+    };
+    uint32_t most = 0;
+    for (int i0 = wave * U; i0 < v.requests; i0 += W * U) {
+        int row[U];
+        uint32_t u[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) row[j] = row_of(i0 + j);
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            u[j] = 0;
+            if (row[j] < 0) continue;
+            const uint32_t* nu = P.w.nu + (size_t)row[j] * NT;
+            for (int t = lane; t < NT; t += 64) u[j] += nu[t];
+            if (lane == 0) u[j] += P.w.tok0c[row[j]] ? 1u : 0u;
+            if (lane == 0 && a.hist_invalid) u[j] += (uint32_t)a.hist_invalid[row[j]] & 0x3FFFFFFFu;
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const uint32_t width = dwave_sum_u32(u[j]);
+            most = max(most, width);
+            if (row[j] >= 0 && lane == 0) P.w.nu[(size_t)row[j] * NT] = width;
+        }
+    }
+    if (lane == 0) red[wave] = most;
+    __syncthreads();
+    for (int w = 0; w < W; ++w) most = max(most, red[w]);
+    for (int i = tid; i < v.requests; i += kStepThreads) {
+        const int r = row_of(i);
+        if (r < 0 || P.w.tok0c[r] == 0) continue;
+        const bool late = a.hist_invalid && (((uint32_t)a.hist_invalid[r] >> 30) & 1u);
+        if (P.w.nu[(size_t)r * NT] != most || late) P.w.tok0c[r] = 0;
     }
 }
 
@@ -389,8 +449,7 @@ static int prepare(const fie_sampler_args* args, const fie_workspace* ws, KParam
     P->NT = (args->vocab + kTile - 1) / kTile;
     P->NS = (P->NT + kWavesPerWG - 1) / kWavesPerWG;
     P->helpers = 0;
-    P->requests = 0;
-    P->draft_offsets = nullptr;
+    P->settled0 = 0;
     if (args->rows == 0) return FIE_OK;
     rc = ws_of(ws, args->rows, args->vocab, &P->w);
     if (rc != FIE_OK) return rc;
@@ -440,12 +499,18 @@ size_t fie_sampler_workspace_size(int32_t max_rows, int32_t vocab)
     return layout_of(max_rows, vocab, &L) ? L.total : 0;
 }
 
-static int sample_run(const KParams& P, hipStream_t st)
+// v: the rows are a verification's.
+static int sample_run(KParams& P, const fie_verify_args* v, hipStream_t st)
 {
     int rc = run_stage(P, FIE_STAGE_PREP, st);
     if (rc != FIE_OK) return rc;
     rc = run_stage(P, FIE_STAGE_SCAN, st);
     if (rc != FIE_OK) return rc;
+    if (v && P.a.apply_penalties) {
+        k_steps<<<v->max_drafts + 1, kStepThreads, 0, st>>>(P, *v);
+        FIE_LAUNCH_CHECK("k_steps");
+        P.settled0 = 1;
+    }
     rc = run_stage(P, FIE_STAGE_FINISH, st);
     if (rc != FIE_OK || finish_in_place(P)) return rc;
     return run_stage(P, FIE_STAGE_DEEP, st);
@@ -456,7 +521,7 @@ int fie_sampler_sample(const fie_sampler_args* args, const fie_workspace* ws, vo
     KParams P;
     int rc = prepare(args, ws, &P);
     if (rc != FIE_OK || args->rows == 0) return rc;
-    return sample_run(P, (hipStream_t)stream);
+    return sample_run(P, nullptr, (hipStream_t)stream);
 }
 
 static int lmhead_run(const fie_sampler_args* args, const void* hidden, const void* weight, int32_t hidden_dim,
@@ -518,9 +583,7 @@ int fie_sampler_verify(const fie_sampler_args* args, const fie_verify_args* v, c
     KParams P;
     int rc = prepare(args, ws, &P);
     if (rc != FIE_OK || args->rows == 0) return rc;
-    P.requests = v->requests;
-    P.draft_offsets = v->draft_offsets;
-    rc = sample_run(P, (hipStream_t)stream);
+    rc = sample_run(P, v, (hipStream_t)stream);
     if (rc != FIE_OK) return rc;
     return launch_status(launch_verify(P, *v, (hipStream_t)stream), "k_verify");
 }

@@ -105,8 +105,7 @@ struct KParams {
     int NT;
     int NS;              // spans of kSpan tokens per row
     int helpers;         // 1: k_finish runs one helper workgroup per span of each sampled row
-    int requests;        // of a verification, whose drafts begin at draft_offsets; 0: every row is a step's own
-    const int64_t* draft_offsets;
+    int settled0;        // 1: rows whose token 0 keeps no penalty have tok0c = 0 already (k_steps)
 };
 
 // ---------------------------------------------------------------- element access
