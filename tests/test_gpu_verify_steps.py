@@ -131,3 +131,24 @@ def test_ids_outside_the_vocabulary_and_requests_without_penalties():
     for r in range(3):
         k = next((j for j in range(2) if steps[j][r] != drafts[r][j]), 2)
         assert got.token_ids[r] == drafts[r][:k] + [steps[k][r]]
+
+
+def test_more_requests_than_a_workgroup_has_threads():
+    """2500 requests of one step after another, their widths all over it, against small batches'
+    answers: the widest row of each step alone keeps the penalty, unless ties share it."""
+    V, n, R = 300, 2, 2500
+    rng = np.random.default_rng(12)
+    x = torch.zeros(R, n + 1, V, device=DEV)
+    x[..., 0], x[..., 8], x[..., 9], x[..., 10] = 3.0, 2.5, 2.2, 2.0
+    pen = SamplingParams(presence_penalty=2.0)
+    contexts = [[0] + rng.integers(20, 200, int(rng.integers(0, 30))).tolist() for _ in range(R)]
+    contexts[1700] = [0] + list(range(20, 90))              # the widest of all, and again
+    contexts[3] = list(contexts[1700])
+    drafts = [[8, 9] if r in (3, 1700) or r % 2 else [0, 8] for r in range(R)]
+    s = BatchedSampler(DEV)
+    steps = [s.sample(x[:, j].contiguous(), [pen] * R, [c + d[:j] for c, d in zip(contexts, drafts)]).token_ids for j in range(n + 1)]
+    assert steps[0][3] == steps[0][1700] == 8 and steps[0].count(0) == R - 2
+    got = s.verify(x.view(R * (n + 1), V), drafts, [pen] * R, context_tokens=contexts)
+    for r in range(R):
+        k = next((j for j in range(n) if steps[j][r] != drafts[r][j]), n)
+        assert got.token_ids[r] == drafts[r][:k] + [steps[k][r]]
