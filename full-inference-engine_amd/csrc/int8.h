@@ -142,7 +142,7 @@ struct Chunk {
 // Rows at any address into rows of whole stages at aligned ones, 0 past k: what the pipe kernel
 // needs.  A wave a row; a lane makes a word from the two that hold its bytes, so that every
 // load and store of a wave is one piece of 256 bytes (16 bytes a lane at odd addresses take
-// four times as long: 250 x 16384 at k 4097 61 us, 122 without this).  Bound by HBM: the matrix
+// four times as long).  250 x 16384 at k 4097 52 us with this, the product alone 29.  Bound by HBM: the matrix
 // read and written once, on top of what the product reads.
 __global__ __launch_bounds__(256) void k_align_rows(const int8_t* src, int64_t stride, int64_t rows, int K, int8_t* dst, int64_t pitch)
 {
@@ -179,8 +179,8 @@ __global__ __launch_bounds__(256) void k_align_rows(const int8_t* src, int64_t s
 // U of them loaded at once straight into the matrix instructions' operands, with no LDS and no
 // barrier before the waves' sums meet.  For rows that the pipe kernel's loads do not take: 16
 // bytes at any address take shifts and a word of a neighbour's, and rows straddle lines, so it stays below
-// the memory's rate (16 x 50001 at k 4097 52 us, 4.0 TB/s; at k 4096 in aligned rows the pipe kernel
-// takes 35).
+// the memory's rate (16 x 50001 at k 4097 50 us, 4.1 TB/s; with the weights' rows padded to 16 bytes
+// 43, and 38 by the pipe kernel with the tokens' as well).
 template <int DT, int MT, int NW, int S, int U>
 __global__ __launch_bounds__(64 * S) void k_int8_rows(const fie_int8_args a, int wide)
 {
@@ -287,10 +287,10 @@ __global__ __launch_bounds__(64 * S) void k_int8_rows(const fie_int8_args a, int
 // between), NB - 1 stages ahead; a stage costs one barrier.  A wave's instruction fills eight
 // rows of 128 bytes in lane order, so the swizzle of i8_slot is in the addresses it loads from.
 // Large products are bound by the matrix cores and the LDS that feeds them (4096 x 4096 at k 16384
-// 217-225 us, 2.4-2.5 Pop/s, 16 waves of 64 x 64: 8 waves 242, 128 x 128 306), few tokens by the
-// weights' way from memory (16 x 151936 at k 4096 109-113 us, 5.6 TB/s), and what lies between by
-// the loads into LDS, 55-60 GB/s a CU (250 x 16384 at k 4096 25-28 us, where operations and
-// bytes alone take 14; more buffers, fewer waves, two stages a barrier took as long or longer).
+// 216-226 us, 2.4-2.5 Pop/s, 16 waves of 64 x 64: 8 waves 242, 128 x 128 306), few tokens by the
+// weights' way from memory (16 x 151936 at k 4096 111-114 us, 5.5 TB/s), and what lies between by
+// the loads into LDS, 55-60 GB/s a CU (250 x 16384 at k 4096 25-26 us a dispatch, 28.6 with the
+// launch, where operations and bytes alone take 14; more buffers, fewer waves, two stages a barrier took as long or longer).
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
 // Workgroup b's tile of nrb x ncb.  Workgroups are dealt to the eight XCDs round robin: each

@@ -21,8 +21,9 @@ static hipError_t pipe_of(const fie_int8_args& a, int wide, hipStream_t st)
     return hipGetLastError();
 }
 
-// The pipe kernel's tiles, and what a CU takes for one of each, as measured at k 4096 (us over
-// the launch's own 3, tiles as many as CUs; the other tiles on the same product beside it):
+// The pipe kernel's tiles, and what a CU takes for one of each, as measured at k 4096 (us, tiles as
+// many as CUs, less the launch's own 3; then products on that tile, back to back with their launches,
+// and in brackets the same on other tiles):
 //   32 x 32, k in four groups    4.6   64 x 4096  7.4 (32 x 64 10.0, 64 x 64 12.6)
 //   32 x 64                      6.5   16 x 151936  113 (64 x 64 124, 64 x 128 126)
 //   64 x 64                     10.5   250 x 4096  13.1 (32 x 64 14.0, 64 x 128 17.3)

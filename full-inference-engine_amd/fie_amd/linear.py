@@ -47,9 +47,10 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
 
     x is int8 with ``x_scale`` (float32, one a token), or float32, float16 or bfloat16, which is
     quantised for each token first.  ``out_dtype``: float32, float16 or bfloat16; by default x's own
-    (bfloat16 for int8).  Weights whose rows begin at multiples of 16 bytes are read in place at
-    any number of tokens (pad the rows of a storage: ``w = room[:, :k]``); others are laid out anew
-    in every call past 96 tokens.  ``out`` [tokens, n] is written instead of a new tensor: unit element
+    (bfloat16 for int8).  Rows of weights and of int8 tokens that begin at multiples of 16 bytes
+    (pad those of a storage where k is none: ``w = room[:, :k]``) are read fastest; others go at their
+    own addresses up to 96 tokens, and past them are laid out anew in every call.  (Tokens that are
+    quantised here or by ``quantize_rows`` have rows of k bytes.)  ``out`` [tokens, n] is written instead of a new tensor: unit element
     stride, any row stride.  Runs on the current stream; nothing waits for it."""
     if weight.ndim != 2 or weight.dtype != torch.int8:
         raise ValueError("weight must be int8 [channels, k]")
