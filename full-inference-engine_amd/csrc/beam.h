@@ -1,0 +1,483 @@
+// Beam search's selection (fie_beam_step): the best continuations of a request's beams.
+#pragma once
+
+#include "launchers.h"
+#include "fie_decode.h"
+
+namespace fie {
+
+constexpr int kBeamThreads = 256, kBeamWaves = kBeamThreads / 64;
+constexpr int kBeamEach = 32;                           // logits of a thread a tile
+constexpr int kBeamTile = kBeamThreads * kBeamEach;
+constexpr int kBeamList = 2048;                         // candidates a workgroup holds
+constexpr int kBeamSpans = 32;                          // most spans of a row
+constexpr float kLog2e = 1.44269502f;
+constexpr float kLargest = 3.40282347e38f;
+
+// A span's results: the largest logit, the sum of exp(x - it), how many candidates.
+struct BeamSpan {
+    double sum;
+    float top;
+    int32_t count;
+};
+
+// The workspace: spans' results, then their candidates, best first.
+struct BeamWork {
+    BeamSpan* span;             // [rows][spans]
+    uint64_t* cand;             // [rows][spans][most]
+    int spans, tiles, most;     // of a row; tiles of a span; candidates of a span
+};
+
+FIE_DEV float beam_clean(float x) { return x != x ? -__builtin_inff() : __builtin_fminf(x, kLargest); }
+
+template <int DT> struct BeamVec {                      // 16 bytes of logits
+    static constexpr int N = DT == FIE_F32 ? 4 : 8;
+    static FIE_DEV void open(const uint4& r, float* x)
+    {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == FIE_F32) x[i] = __uint_as_float(w[i]);
+            else if constexpr (DT == FIE_BF16) {
+                x[2 * i] = __uint_as_float(w[i] << 16);
+                x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            } else {
+                x[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[i]);
+                x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16));
+            }
+        }
+    }
+};
+
+// The largest key T, low 16 bits 0, that at least `rank` lanes of the wave reach.
+FIE_DEV uint32_t beam_reach(uint32_t key, int rank)
+{
+    uint32_t t = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t up = t | (1u << bit);
+        if (__popcll(__ballot(key >= up)) >= rank) t = up;
+    }
+    return t;
+}
+
+FIE_DEV bool beam_dead(const fie_beam_args& a, int row)
+{
+    return a.done[row / a.beams] || !(a.scores[row] > -__builtin_inff());
+}
+
+// A row's logits in vectors at aligned addresses; those of the first and the last vector that
+// are outside the row count as -inf (no vector without some of the row is touched).
+template <int DT> struct BeamRow {
+    static constexpr int N = BeamVec<DT>::N, LOADS = kBeamEach / N;
+    const uint4* base;
+    int shift, vocab, vecs;
+    FIE_DEV BeamRow(const fie_beam_args& a, int row)
+    {
+        constexpr int SZ = 16 / N;
+        const uintptr_t p = (uintptr_t)a.logits + (uintptr_t)((int64_t)row * a.row_stride * SZ);
+        base = (const uint4*)(p & ~(uintptr_t)15);
+        shift = (int)(p & 15) / SZ;
+        vocab = a.vocab;
+        vecs = (shift + vocab + N - 1) / N;
+    }
+    FIE_DEV void load(int tile, uint4 (&r)[LOADS]) const
+    {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) r[j] = base[min((tile * LOADS + j) * kBeamThreads + (int)threadIdx.x, vecs - 1)];
+    }
+    FIE_DEV int index(int tile, int e) const            // of the thread's e-th logit of a tile
+    {
+        return ((tile * LOADS + e / N) * kBeamThreads + (int)threadIdx.x) * N + e % N - shift;
+    }
+    FIE_DEV void open(int tile, const uint4 (&r)[LOADS], float (&x)[kBeamEach]) const
+    {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) BeamVec<DT>::open(r[j], x + j * N);
+        if (tile == 0 || (tile + 1) * LOADS * kBeamThreads >= vecs)
+#pragma unroll
+            for (int e = 0; e < kBeamEach; ++e) {
+                const int i = index(tile, e);
+                if (i < 0 || i >= vocab) x[e] = -__builtin_inff();
+            }
+    }
+};
+
+struct BeamShared {
+    uint64_t list[kBeamList];
+    uint32_t hist[2048];
+    uint32_t wave[kBeamWaves];
+    double sum[kBeamWaves];
+    float top[kBeamWaves];
+    int32_t count;
+    uint32_t above, bin;
+};
+
+// The `need`-th best candidate of a span, exactly: radix passes over (key, index) that read the
+// span again, and at the end the `need` best into the list.  For spans whose candidates do not
+// fit the list (equal logits, or logits in rising order).
+template <int DT>
+__device__ __noinline__ int beam_deep(const BeamRow<DT>& row, int first, int last, int most, BeamShared& S)
+{
+    const int tid = threadIdx.x;
+    auto each = [&](auto&& f) {
+        constexpr int N = BeamRow<DT>::N, LOADS = BeamRow<DT>::LOADS;
+        for (int j = first * LOADS; j < min(last * LOADS, (row.vecs + kBeamThreads - 1) / kBeamThreads); ++j) {
+            const int v = j * kBeamThreads + tid;
+            float x[N];
+            BeamVec<DT>::open(row.base[min(v, row.vecs - 1)], x);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int i = v * N + e - row.shift;
+                const float y = beam_clean(x[e]);
+                if (v < row.vecs && i >= 0 && i < row.vocab && y > -__builtin_inff()) f(comp_key(fkey(y + 0.0f), (uint32_t)i));
+            }
+        }
+    };
+    __syncthreads();
+    if (tid == 0) S.count = 0;
+    __syncthreads();
+    int mine = 0;
+    each([&](uint64_t) { ++mine; });
+    atomicAdd(&S.count, mine);
+    __syncthreads();
+    const int need = min(most, S.count);
+    __syncthreads();
+    if (need == 0) return 0;
+    constexpr int kShift[5] = {53, 42, 32, 10, 0}, kBits[5] = {11, 11, 10, 10, 10};
+    uint64_t prefix = 0;
+    int left = need;
+    for (int p = 0; p < 5; ++p) {
+        const int sh = kShift[p], bits = kBits[p], known = p == 3 ? 32 : sh + bits;     // bits 20..31 are the same in all
+        if (p == 3) prefix |= 0xFFF00000u;
+        for (int i = tid; i < 2048; i += kBeamThreads) S.hist[i] = 0;
+        __syncthreads();
+        const uint64_t want = known >= 64 ? 0 : prefix >> known;
+        each([&](uint64_t c) {
+            if ((known >= 64 ? 0 : c >> known) == want) atomicAdd(&S.hist[(uint32_t)(c >> sh) & ((1u << bits) - 1u)], 1u);
+        });
+        __syncthreads();
+        // bins from the highest down: thread t sums 8 of them
+        uint32_t own = 0;
+        const int top = 2047 - 8 * tid;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) own += S.hist[top - i];
+        const uint32_t incl = wave_incl_scan_u32(own);
+        if ((tid & 63) == 63) S.wave[tid >> 6] = incl;
+        __syncthreads();
+        uint32_t before = incl - own;
+        for (int w = 0; w < (tid >> 6); ++w) before += S.wave[w];
+        if (before < (uint32_t)left && before + own >= (uint32_t)left) {
+            uint32_t sum = before;
+            int b = top;
+            while (sum + S.hist[b] < (uint32_t)left) sum += S.hist[b--];
+            S.above = sum;
+            S.bin = (uint32_t)b;
+        }
+        __syncthreads();
+        left -= (int)S.above;
+        prefix |= (uint64_t)S.bin << sh;
+        __syncthreads();
+    }
+    if (tid == 0) S.count = 0;
+    __syncthreads();
+    each([&](uint64_t c) {
+        if (c >= prefix) S.list[atomicAdd(&S.count, 1)] = c;
+    });
+    __syncthreads();
+    return need;
+}
+
+// grid (spans, rows): a span's largest logit, its sum of exp, and its best candidates in order.
+// One pass over the logits.  The first tile gives a bound: every wave finds what a quarter of the
+// wanted candidates reach among its 64 lanes' maxima, and the least of the four waves' bounds is
+// reached by all of them.  What reaches it is listed, in later tiles too; the list is ranked at
+// the end.
+template <int DT>
+__global__ __launch_bounds__(kBeamThreads) void k_beam_scan(const fie_beam_args a, const BeamWork w)
+{
+    __shared__ BeamShared S;
+    const int row_id = blockIdx.y, span = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (beam_dead(a, row_id)) return;
+    const BeamRow<DT> row(a, row_id);
+    constexpr int LOADS = BeamRow<DT>::LOADS;
+    const int tiles = (row.vecs + LOADS * kBeamThreads - 1) / (LOADS * kBeamThreads);
+    const int first = span * w.tiles, last = min(first + w.tiles, tiles);
+    BeamSpan* out = w.span + (int64_t)row_id * w.spans + span;
+    if (first >= last) {
+        if (tid == 0) *out = BeamSpan{0.0, -kLargest, 0};
+        return;
+    }
+    if (tid == 0) S.count = 0;
+    const int rank = (w.most + kBeamWaves - 1) / kBeamWaves;
+    float top = -kLargest, bound = -__builtin_inff();
+    double sum = 0.0;
+    uint4 raw[LOADS];
+    row.load(first, raw);
+    for (int t = first; t < last; ++t) {
+        float x[kBeamEach];
+        row.open(t, raw, x);
+        if (t + 1 < last) row.load(t + 1, raw);
+        float m = x[0];
+#pragma unroll
+        for (int e = 1; e < kBeamEach; ++e) m = __builtin_fmaxf(m, x[e]);
+        const float high = __builtin_fmaxf(top, m);
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < kBeamEach; ++e) s[e & 3] += __builtin_amdgcn_exp2f((x[e] - high) * kLog2e);
+        float here = (s[0] + s[1]) + (s[2] + s[3]);
+        float up = high;
+        if (!(here == here) || high > kLargest) {       // a NaN or an infinity among them
+            m = -__builtin_inff();
+#pragma unroll
+            for (int e = 0; e < kBeamEach; ++e) {
+                x[e] = beam_clean(x[e]);
+                m = __builtin_fmaxf(m, x[e]);
+            }
+            up = __builtin_fmaxf(top, m);
+            here = 0.0f;
+#pragma unroll
+            for (int e = 0; e < kBeamEach; ++e) here += __builtin_amdgcn_exp2f((x[e] - up) * kLog2e);
+        }
+        if (up > top) sum *= __builtin_amdgcn_exp2f((top - up) * kLog2e);
+        sum += here;
+        top = up;
+        if (t == first) {
+            const uint32_t key = m > -__builtin_inff() ? fkey(m + 0.0f) : 0u;
+            const uint32_t reach = beam_reach(key, rank);
+            if (lane == 0) S.wave[wave] = reach;
+            __syncthreads();
+            uint32_t least = S.wave[0];
+#pragma unroll
+            for (int i = 1; i < kBeamWaves; ++i) least = min(least, S.wave[i]);
+            // a bound that some wave's lanes do not reach: everything is listed
+            bound = least > kKeyNegInf ? key_to_float(least) : -kLargest;
+        }
+        if (m >= bound)
+#pragma unroll
+            for (int e = 0; e < kBeamEach; ++e)
+                if (x[e] >= bound) {
+                    const int at = atomicAdd(&S.count, 1);
+                    if (at < kBeamList) S.list[at] = comp_key(fkey(x[e] + 0.0f), (uint32_t)row.index(t, e));
+                }
+    }
+    // the span's maximum and sum
+    float all = top;
+    for (int d = 32; d; d >>= 1) all = __builtin_fmaxf(all, __shfl_xor(all, d, 64));
+    if (lane == 0) S.top[wave] = all;
+    __syncthreads();
+    all = S.top[0];
+#pragma unroll
+    for (int i = 1; i < kBeamWaves; ++i) all = __builtin_fmaxf(all, S.top[i]);
+    sum *= __builtin_amdgcn_exp2f((top - all) * kLog2e);
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    if (lane == 0) S.sum[wave] = sum;
+    int count = S.count;
+    __syncthreads();
+    // a long list: a bound among what is listed, every lane holding some of it
+    if (count > kBeamThreads && count <= kBeamList) {
+        uint32_t best = 0;
+        for (int i = tid; i < count; i += kBeamThreads) best = max(best, comp_k(S.list[i]));
+        const uint32_t reach = beam_reach(best, rank);
+        if (lane == 0) S.wave[wave] = reach;
+        __syncthreads();
+        uint32_t least = S.wave[0];
+#pragma unroll
+        for (int i = 1; i < kBeamWaves; ++i) least = min(least, S.wave[i]);
+        uint64_t keep[kBeamList / kBeamThreads];
+#pragma unroll
+        for (int i = 0; i < kBeamList / kBeamThreads; ++i) keep[i] = tid + i * kBeamThreads < count ? S.list[tid + i * kBeamThreads] : 0;
+        if (tid == 0) S.count = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kBeamList / kBeamThreads; ++i)
+            if (keep[i] && comp_k(keep[i]) >= least) S.list[atomicAdd(&S.count, 1)] = keep[i];
+        __syncthreads();
+        count = S.count;
+        __syncthreads();
+    }
+    if (count > 2 * kBeamThreads) count = beam_deep<DT>(row, first, last, w.most, S);
+    // each entry's place
+    uint64_t* cand = w.cand + ((int64_t)row_id * w.spans + span) * w.most;
+    for (int i = tid; i < count; i += kBeamThreads) {
+        const uint64_t c = S.list[i];
+        int place = 0;
+        for (int j = 0; j < count; ++j) place += S.list[j] > c;
+        if (place < w.most) cand[place] = c;
+    }
+    if (tid == 0) *out = BeamSpan{(S.sum[0] + S.sum[1]) + (S.sum[2] + S.sum[3]), all, min(count, w.most)};
+}
+
+// The order of doubles as that of whole numbers; -inf and NaN are 0, no continuation.
+FIE_DEV uint64_t beam_order(double v)
+{
+    if (!(v > -__builtin_inf())) return 0;
+    const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
+    return b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
+}
+
+FIE_DEV double beam_value(uint64_t k)
+{
+    return __longlong_as_double((int64_t)((k >> 63) ? (k & 0x7FFFFFFFFFFFFFFFull) : ~k));
+}
+
+// A workgroup a request, a wave a row at first: the row's spans' lists are in order, so its best
+// candidates come off their heads one by one; then the request's, off its rows' lists, in one
+// wave with a beam a lane.  Bound by that chain: a few hundred cycles a candidate.
+// Dynamic LDS: [waves][spans][most] spans' lists, [beams][most] rows' lists.
+__global__ __launch_bounds__(1024) void k_beam_pick(const fie_beam_args a, const BeamWork w)
+{
+    extern __shared__ uint64_t L[];
+    __shared__ double lse[FIE_MAX_BEAMS];               // log of a row's sum, less its maximum
+    __shared__ float top[FIE_MAX_BEAMS];
+    __shared__ int32_t counts[FIE_MAX_BEAMS];
+    __shared__ uint64_t live_key[FIE_MAX_BEAMS];
+    __shared__ int32_t live_token[FIE_MAX_BEAMS], live_beam[FIE_MAX_BEAMS];
+    __shared__ float end_value[FIE_MAX_BEAMS], old_value[FIE_MAX_BEAMS];
+    __shared__ int32_t end_token[FIE_MAX_BEAMS], end_beam[FIE_MAX_BEAMS], old_end[FIE_MAX_BEAMS][3];
+    __shared__ int32_t found, ended;
+    const int r = blockIdx.x, K = a.beams, lane = threadIdx.x & 63, most = w.most;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int length = a.lengths[r];
+    const bool was = a.done[r] != 0;
+    uint64_t* heads = L + (int64_t)wave * w.spans * most;
+    uint64_t* rows = L + (int64_t)waves * w.spans * most;
+    for (int b = wave; b < K; b += waves) {
+        const int row = r * K + b;
+        if (beam_dead(a, row)) {
+            if (lane == 0) counts[b] = 0;
+            continue;
+        }
+        const bool in = lane < w.spans;
+        const BeamSpan sp = in ? w.span[(int64_t)row * w.spans + lane] : BeamSpan{0.0, -kLargest, 0};
+        float m = sp.top;
+        for (int d = 32; d; d >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d, 64));
+        double s = sp.sum > 0.0 ? sp.sum * exp((double)sp.top - (double)m) : 0.0;
+        for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
+        const uint64_t* from = w.cand + (int64_t)row * w.spans * most;
+        for (int i = lane; i < w.spans * most; i += 64) heads[i] = from[i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        int at = 0, n = 0;
+        uint64_t head = sp.count > 0 ? heads[lane * most] : 0;
+        for (; n < most; ++n) {
+            const uint64_t best = dwave_max_u64(head);
+            if (best == 0) break;
+            if (lane == 0) rows[b * most + n] = best;
+            if (head == best) {
+                ++at;
+                head = at < sp.count ? heads[lane * most + at] : 0;
+            }
+        }
+        if (lane == 0) {
+            counts[b] = n;
+            top[b] = m;
+            lse[b] = log(s);
+        }
+    }
+    if ((int)threadIdx.x < K) {
+        const float p = a.pool[r * K + threadIdx.x];
+        old_value[threadIdx.x] = p == p ? p : -__builtin_inff();
+        for (int i = 0; i < 3; ++i) old_end[threadIdx.x][i] = a.ends[(r * K + threadIdx.x) * 3 + i];
+    }
+    __syncthreads();
+    const double scale = pow((double)max(was ? length : length + 1, 1), a.length_penalty);
+    if (wave == 0) {
+        const bool mine = lane < K && counts[lane] > 0;
+        const double prior = mine ? (double)a.scores[r * K + lane] : 0.0;
+        const int n = mine ? counts[lane] : 0;
+        int at = 0;
+        auto look = [&]() {
+            if (at >= n) return (uint64_t)0;
+            const float x = key_to_float(comp_k(rows[lane * most + at]));
+            return beam_order(prior + ((double)(x - top[lane]) - lse[lane]));
+        };
+        uint64_t head = look();
+        int live = 0, ends = 0, rank = 0;
+        const bool last = a.max_tokens > 0 && length + 1 >= a.max_tokens;     // all end
+        while (live < K && !(last && rank >= K)) {
+            const uint64_t best = dwave_max_u64(head);
+            if (best == 0) break;
+            const int who = (int)__builtin_ctzll(__ballot(head == best));     // ties: the lower beam
+            const int token = (int)comp_idx(rows[who * most + __builtin_amdgcn_readlane(at, who)]);
+            bool eos = false;
+            for (int i = 0; i < a.eos_count; ++i) eos |= token == a.eos[i];
+            if (lane == who) {
+                ++at;
+                head = look();
+            }
+            if (eos && length + 1 < a.min_tokens) continue;                   // does not exist
+            eos |= last;
+            if (lane == 0) {
+                if (!eos) {
+                    live_key[live] = best;
+                    live_token[live] = token;
+                    live_beam[live] = who;
+                } else if (rank < K) {
+                    end_value[ends] = (float)(beam_value(best) / scale);
+                    end_token[ends] = token;
+                    end_beam[ends] = who;
+                }
+            }
+            if (!eos) ++live;
+            else if (rank < K) ++ends;
+            ++rank;
+        }
+        if (lane == 0) {
+            found = live;
+            ended = ends;
+        }
+    }
+    __syncthreads();
+    if (wave) return;
+    // the pool: its own and the new ones by value, the older first; both are held before the writes
+    const int E = ended, live = found;
+    const float mine = lane < K ? old_value[lane] : -__builtin_inff();
+    int place = 64;
+    if (lane < K) {
+        place = 0;
+        for (int j = 0; j < K; ++j) place += old_value[j] > mine || (old_value[j] == mine && j < lane);
+        for (int j = 0; j < E; ++j) place += end_value[j] > mine;
+    }
+    int fresh = 64;
+    if (lane < E) {
+        fresh = 0;
+        const float v = end_value[lane];
+        for (int j = 0; j < K; ++j) fresh += old_value[j] >= v;
+        for (int j = 0; j < E; ++j) fresh += end_value[j] > v || (end_value[j] == v && j < lane);
+    }
+    auto put = [&](int to, float v, int e0, int e1, int e2) {
+        a.next_pool[r * K + to] = v;
+        int32_t* e = a.next_ends + (int64_t)(r * K + to) * 3;
+        e[0] = e0;
+        e[1] = e1;
+        e[2] = e2;
+    };
+    if (place < K) put(place, mine, old_end[lane][0], old_end[lane][1], old_end[lane][2]);
+    if (fresh < K) put(fresh, end_value[lane], length + 1, r * K + end_beam[lane], end_token[lane]);
+    // the pool's worst
+    float worst = __builtin_inff();
+    if (place == K - 1) worst = mine;
+    if (fresh == K - 1) worst = end_value[lane];
+    for (int d = 32; d; d >>= 1) worst = __builtin_fminf(worst, __shfl_xor(worst, d, 64));
+    bool done = was || live == 0;
+    if (!done && worst > -__builtin_inff()) done = a.early_stopping || worst >= (float)(beam_value(live_key[0]) / scale);
+    if (lane < K) {
+        const int row = r * K + lane;
+        const bool goes = !done && lane < live;
+        const int token = goes ? live_token[lane] : a.pad, parent = goes ? r * K + live_beam[lane] : row;
+        a.next_scores[row] = goes ? (float)beam_value(live_key[lane]) : -__builtin_inff();
+        a.tokens[row] = token;
+        a.parents[row] = parent;
+        if (a.history_tokens && !was && length >= 0 && length < a.history_steps) {
+            const int64_t to = (int64_t)length * a.requests * K + row;
+            a.history_tokens[to] = token;
+            a.history_parents[to] = parent;
+        }
+    }
+    if (lane == 0) {
+        a.next_lengths[r] = was ? length : length + 1;
+        a.next_done[r] = done;
+    }
+}
+
+}  // namespace fie

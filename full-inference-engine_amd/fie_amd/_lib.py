@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/fie_sampler.h and include/fie_ops.h.
+"""ctypes binding of the C ABI in include/fie_sampler.h, include/fie_ops.h and include/fie_decode.h.
 
 The shared library is built in-tree by ``fie_amd.build`` into ``fie_amd/_native``.
 There is no fallback: if the library cannot be loaded, every entry point raises.
@@ -60,6 +60,8 @@ class VerifyArgs(ctypes.Structure):
 # a trailing 0 quad pads to the structure's alignment.
 NORM_ARGS = "@10P6q9i3f0q"
 INT8_ARGS = "@6P4q4iPN0q"
+BEAM_ARGS = "@15PqPNd8i18i0q"
+STATES_ARGS, STATE_ARGS = "@P2i", "2P4q"        # the head, and as many states as there are
 
 
 class Workspace(ctypes.Structure):
@@ -78,6 +80,8 @@ EXPORTS = (
 )
 # Every symbol include/fie_ops.h declares.
 OPS_EXPORTS = ("fie_block_norm", "fie_int8_linear", "fie_int8_workspace_size")
+# Every symbol include/fie_decode.h declares.
+DECODE_EXPORTS = ("fie_beam_workspace_size", "fie_beam_step", "fie_reorder_states")
 SCRATCH_BYTES = 64 << 20
 
 _lib = None
@@ -127,9 +131,13 @@ def bind(lib) -> None:
     lib.fie_sampler_last_error.restype = ctypes.c_char_p
     lib.fie_block_norm.argtypes = [ctypes.c_char_p, _vp]
     lib.fie_int8_linear.argtypes = [ctypes.c_char_p, _vp]
-    for name in EXPORTS + OPS_EXPORTS:
+    for name in ("fie_beam_step", "fie_reorder_states"):
+        getattr(lib, name).argtypes = [ctypes.c_char_p, _vp]
+    for name in EXPORTS + OPS_EXPORTS + DECODE_EXPORTS:
         if name not in ("fie_sampler_workspace_size", "fie_sampler_last_error"):
             getattr(lib, name).restype = ctypes.c_int
+    lib.fie_beam_workspace_size.argtypes = [ctypes.c_char_p]
+    lib.fie_beam_workspace_size.restype = ctypes.c_size_t
     lib.fie_int8_workspace_size.argtypes = [ctypes.c_char_p]
     lib.fie_int8_workspace_size.restype = ctypes.c_size_t
 

@@ -1,0 +1,276 @@
+"""Beam search on the device: the selection over beams and vocabulary, the pool of ended answers,
+and the states that go with the beams.
+
+A request's beams are rows next to each other: beam b of request r is row r * beams + b of the
+logits and of every state.  ``beam_step`` is one step of all requests; ``reorder_states`` gathers
+dense states by the parents it returns, ``fie_amd.pages.CachePages.step`` the pages of a cache.
+``BeamSearch`` keeps a batch's beams from step to step and the way back to their tokens.
+"""
+
+from __future__ import annotations
+
+import struct
+from typing import NamedTuple, Sequence
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import FIE_BF16, FIE_F16, FIE_F32
+
+_DTYPES = {torch.float32: FIE_F32, torch.float16: FIE_F16, torch.bfloat16: FIE_BF16}
+_pack = struct.Struct(_lib.BEAM_ARGS).pack
+_run = None             # the library's entry, loaded with the first call
+_size = None
+_reorder = None
+MAX_STATES = 48         # tensors of one launch
+MAX_BEAMS = 64
+MAX_EOS = 16
+MAX_ROWS = 65535
+
+
+class Beams(NamedTuple):
+    """The beams of some requests between two steps, on the device."""
+
+    scores: torch.Tensor        # float32 [requests, beams] sums of log-probabilities; -inf: no such beam
+    lengths: torch.Tensor       # int32 [requests] tokens chosen so far
+    done: torch.Tensor          # bool [requests]
+    pool: torch.Tensor          # float32 [requests, beams] ended answers' values, the best first; -inf: none
+    ends: torch.Tensor          # int32 [requests, beams, 3] theirs: length, parent row, eos token
+
+
+class BeamStep(NamedTuple):
+    beams: Beams
+    tokens: torch.Tensor        # int64 [rows] the token each row goes on with
+    parents: torch.Tensor       # int32 [rows] the row that it went on from
+
+
+def first_beams(requests: int, beams: int, device: torch.device | str) -> Beams:
+    """Before the first step: a request's first row is its only beam."""
+    scores = torch.full((requests, beams), float("-inf"), device=device)
+    scores[:, :1] = 0.0
+    return Beams(scores, torch.zeros(requests, dtype=torch.int32, device=device),
+                 torch.zeros(requests, dtype=torch.bool, device=device),
+                 torch.full((requests, beams), float("-inf"), device=device),
+                 torch.full((requests, beams, 3), -1, dtype=torch.int32, device=device))
+
+
+_FIELDS = (("scores", torch.float32), ("lengths", torch.int32), ("done", torch.bool), ("pool", torch.float32),
+           ("ends", torch.int32))
+
+
+def beam_step(logits: torch.Tensor, beams: Beams, *, eos: Sequence[int] = (), length_penalty: float = 1.0,
+              early_stopping: bool = False, min_tokens: int = 0, max_tokens: int = 0, pad: int = 0, inplace: bool = False,
+              history: tuple[torch.Tensor, torch.Tensor] | None = None) -> BeamStep:
+    """One step of beam search: ``logits`` [requests * beams, vocab] (float32, float16, bfloat16).
+
+    A continuation's score is its beam's and the token's log-probability, in 64 bits and rounded
+    once; continuations rank by score, then lower beam, larger logit, lower token.  The best
+    ``beams`` of a request that are not in ``eos`` go on.  An ending one among its best ``beams``
+    of all joins the request's pool at score / (length + 1) ** ``length_penalty``; before
+    ``min_tokens`` tokens none exists, and with ``max_tokens`` those of that many tokens all end.  A request is done when its pool is full and, unless
+    ``early_stopping``, the best that goes on is no better than the pool's worst; or when nothing
+    goes on.  Rows of a request that is done, and rows beside its last beam, come out with score
+    -inf, token ``pad`` and themselves as parent, and their logits are not read at the next step.
+
+    A NaN logit counts as -inf, +inf as the largest float32; tokens masked with -inf do not exist.
+    ``inplace`` writes the new beams over the old.  ``history``: int32 [steps, rows] tokens and
+    parents; a step's are kept at its request's length.  Runs on the current stream; nothing waits
+    for it."""
+    scores = beams.scores
+    if scores.ndim != 2:
+        raise ValueError("scores must be [requests, beams]")
+    requests, count = scores.shape
+    rows = requests * count
+    if not 1 <= count <= MAX_BEAMS or rows > MAX_ROWS:
+        raise ValueError(f"beams must be in [1, {MAX_BEAMS}], rows at most {MAX_ROWS}")
+    index = scores.get_device()
+    if index < 0:
+        raise ValueError("beam_step runs on a HIP device")
+    shapes = ((requests, count), (requests,), (requests,), (requests, count), (requests, count, 3))
+    for t, (name, dtype), shape in zip(beams, _FIELDS, shapes):
+        if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {dtype} {list(shape)}")
+        if t.get_device() != index:
+            raise ValueError("every tensor must be on the scores' device")
+    if logits.ndim != 2 or logits.shape[0] != rows:
+        raise ValueError(f"logits must be [{rows}, vocab], a request's beams together")
+    vocab = logits.shape[1]
+    code = _DTYPES.get(logits.dtype)
+    if code is None:
+        raise ValueError("logits must be float32, float16 or bfloat16")
+    if not 1 <= vocab <= _lib.MAX_VOCAB:
+        raise ValueError(f"vocab must be in [1, {_lib.MAX_VOCAB}]")
+    if logits.get_device() != index:
+        raise ValueError("every tensor must be on the scores' device")
+    eos = tuple(eos)
+    if len(eos) > MAX_EOS or any(not 0 <= e < vocab for e in eos):
+        raise ValueError(f"eos: at most {MAX_EOS} tokens of the vocabulary")
+    if not length_penalty == length_penalty or not 0 <= pad < 1 << 31 or not 0 <= min_tokens < 1 << 31 \
+            or not 0 <= max_tokens < 1 << 31:
+        raise ValueError("length_penalty must be a number, pad, min_tokens and max_tokens whole numbers of 31 bits")
+    h_tokens = h_parents = h_steps = 0
+    if history is not None:
+        for t in history:
+            if t.dtype != torch.int32 or t.ndim != 2 or t.shape[1] != rows or t.shape != history[0].shape \
+                    or not t.is_contiguous() or t.get_device() != index:
+                raise ValueError(f"history must be two contiguous int32 [steps, {rows}] on the scores' device")
+        h_tokens, h_parents, h_steps = history[0].data_ptr(), history[1].data_ptr(), history[0].shape[0]
+    if (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+        logits = logits.contiguous()
+    device = scores.device
+    new = beams if inplace else Beams(*(torch.empty_like(t) for t in beams))
+    tokens = torch.empty(rows, dtype=torch.int64, device=device)
+    parents = torch.empty(rows, dtype=torch.int32, device=device)
+    if rows:
+        global _run, _size
+        if _run is None:
+            _run, _size = _lib.launcher("fie_beam_step"), _lib.load().fie_beam_workspace_size
+        args = [logits.data_ptr(), *(t.data_ptr() for t in beams), *(t.data_ptr() for t in new), tokens.data_ptr(),
+                parents.data_ptr(), h_tokens, h_parents, max(logits.stride(0), vocab), 0, 0, float(length_penalty), requests, count,
+                vocab, code, bool(early_stopping), min_tokens, pad, h_steps, len(eos), *eos, *(0,) * (MAX_EOS - len(eos)), max_tokens]
+        args[17] = _size(_pack(*args))
+        room = torch.empty(args[17], dtype=torch.uint8, device=device)
+        args[16] = room.data_ptr()
+        _run(index, _pack(*args))
+    return BeamStep(new, tokens, parents)
+
+
+def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor,
+                   out: Sequence[torch.Tensor] | None = None) -> list[torch.Tensor]:
+    """``[s[parents] for s in states]`` in one launch: states [rows, ...] of any types, ``parents`` int32
+    [n] rows (one outside [0, rows) stands for the row's own number, which has to be one of the
+    states').  ``out``: as many tensors [n, ...] to write into, apart from the states.  Runs on the
+    current stream; nothing waits for it."""
+    if parents.dtype != torch.int32 or parents.ndim != 1:
+        raise ValueError("parents must be int32 [rows]")
+    index = parents.get_device()
+    if index < 0:
+        raise ValueError("reorder_states runs on a HIP device")
+    n = parents.shape[0]
+    parents = parents.contiguous()
+    if out is not None and len(out) != len(states):
+        raise ValueError("as many outputs as states")
+    got, parts, held = [], [], []                    # held: copies, until the launch
+    for i, s in enumerate(states):
+        if s.ndim < 1 or s.get_device() != index:
+            raise ValueError("states must be [rows, ...] on the parents' device")
+        rows = s.shape[0]
+        if n > rows:
+            raise ValueError(f"{n} parents of {rows} rows")
+        if rows and not s[0].is_contiguous():
+            s = s.contiguous()
+            held.append(s)
+        if out is None:
+            t = torch.empty((n, *s.shape[1:]), dtype=s.dtype, device=s.device)
+        else:
+            t = out[i]
+            if t.dtype != s.dtype or t.shape != (n, *s.shape[1:]) or t.get_device() != index:
+                raise ValueError(f"output {i} must be [{n}, ...] as its state")
+            if n and not t[0].is_contiguous() or (n > 1 and t.numel() and t.stride(0) < t[0].numel()):
+                raise ValueError("outputs need contiguous rows that do not overlap")
+            if s.numel() and t.numel() and _meet(s, t):
+                raise ValueError("an output overlaps its state")
+        got.append(t)
+        size = s.element_size()
+        width = t[0].numel() * size if n else 0
+        if width:
+            parts.append((s.data_ptr(), t.data_ptr(), s.stride(0) * size, t.stride(0) * size, width, rows))
+    global _reorder
+    if parts and _reorder is None:
+        _reorder = _lib.launcher("fie_reorder_states")
+    for at in range(0, len(parts), MAX_STATES):
+        some = parts[at:at + MAX_STATES]
+        flat = [v for p in some for v in p]
+        _reorder(index, struct.pack(_lib.STATES_ARGS + _lib.STATE_ARGS * len(some), parents.data_ptr(), n, len(some), *flat))
+    return got
+
+
+def _meet(s: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether the memory from the first to the last element of one has any of the other's."""
+    def span(x):
+        last = sum((n - 1) * st for n, st in zip(x.shape, x.stride()))
+        return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
+    (a, b), (c, d) = span(s), span(t)
+    return a < d and c < b
+
+
+class Answer(NamedTuple):
+    value: float                # score / length ** length_penalty
+    tokens: list[int]           # its eos among them, if it ended with one
+    ended: bool
+
+
+class BeamSearch:
+    """The beams of up to ``requests`` requests from step to step on one device; ``step`` takes a model's
+    logits and says which token each row goes on with and which row it went on from.
+
+        search = BeamSearch(device, requests, beams, max_tokens=200, eos=[2])
+        while not search.all_done():                     # or so many steps: nothing else waits
+            got = search.step(model(tokens, caches))
+            pages.step(pages.lengths + 1, got.parents)   # fie_amd.pages: the beams' caches
+            tokens = got.tokens
+        best = search.answers(0)[0]
+
+    A request's slot is used again after ``restart``.  Calls of one search go on one stream at a
+    time."""
+
+    def __init__(self, device: torch.device | str, requests: int, beams: int, *, max_tokens: int,
+                 eos: Sequence[int] = (), length_penalty: float = 1.0, early_stopping: bool = False, min_tokens: int = 0,
+                 pad: int = 0):
+        if requests < 1 or not 1 <= beams <= MAX_BEAMS or requests * beams > MAX_ROWS:
+            raise ValueError(f"beams must be in [1, {MAX_BEAMS}], rows in [1, {MAX_ROWS}]")
+        if max_tokens < 1:
+            raise ValueError("max_tokens must be at least 1")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError("BeamSearch runs on a HIP device")
+        self.requests, self.count, self.max_tokens = requests, beams, max_tokens
+        self._settings = dict(eos=tuple(eos), length_penalty=length_penalty, early_stopping=early_stopping,
+                              min_tokens=min_tokens, max_tokens=max_tokens, pad=pad)
+        self.beams = first_beams(requests, beams, self.device)
+        rows = requests * beams
+        self._history = (torch.zeros((max_tokens, rows), dtype=torch.int32, device=self.device),
+                         torch.zeros((max_tokens, rows), dtype=torch.int32, device=self.device))
+
+    def step(self, logits: torch.Tensor) -> BeamStep:
+        """One step of every request (``beam_step``); the beams are written over."""
+        return beam_step(logits, self.beams, inplace=True, history=self._history, **self._settings)
+
+    def restart(self, requests: Sequence[int]) -> None:
+        """These requests' slots begin anew."""
+        if not len(requests):
+            return
+        if any(not 0 <= r < self.requests for r in requests):
+            raise ValueError(f"requests must be in [0, {self.requests})")
+        at = torch.tensor(list(requests), dtype=torch.int64).to(self.device)
+        for t, fresh in zip(self.beams, first_beams(len(requests), self.count, self.device)):
+            t[at] = fresh
+
+    def all_done(self) -> bool:
+        """Whether every request is done (waits for the device)."""
+        return bool(self.beams.done.all())
+
+    def answers(self, request: int) -> list[Answer]:
+        """A request's ended answers, the best first, and while it is not done its beams behind them
+        (waits for the device)."""
+        if not 0 <= request < self.requests:
+            raise ValueError(f"request must be in [0, {self.requests})")
+        scores, length, done, pool, ends = (t[request].cpu().numpy() for t in self.beams)
+        rows = slice(request * self.count, (request + 1) * self.count)
+        steps = min(int(length), self.max_tokens)
+        tokens, parents = (t[:steps, rows].cpu().numpy() for t in self._history)
+
+        def way(row: int, n: int) -> list[int]:
+            got = []
+            for t in range(n - 1, -1, -1):
+                got.append(int(tokens[t, row]))
+                row = int(parents[t, row]) - rows.start
+            return got[::-1]
+
+        got = [Answer(float(v), way(int(p) - rows.start, int(n) - 1) + [int(t)], True)
+               for v, (n, p, t) in zip(pool, ends) if v > -np.inf]
+        if not done and length:
+            scale = float(length) ** self._settings["length_penalty"]
+            got += [Answer(float(s) / scale, way(b, steps), False) for b, s in enumerate(scores) if s > -np.inf]
+        return got

@@ -1,0 +1,84 @@
+/*
+ * fie_decode.h -- C ABI of what a decode step needs around searching and adapters: beam
+ * search's selection, states reordered by their parents, pages of a cache, low-rank adapters.
+ * No counterpart on the reference's sampler path.
+ *
+ * Conventions are fie_sampler.h's: device pointers, work enqueued on `stream`, nothing
+ * synchronises or allocates, FIE_OK or a negative FIE_E* code, and
+ * fie_sampler_last_error() holds the message.
+ */
+#ifndef FIE_DECODE_H
+#define FIE_DECODE_H
+
+#include "fie_sampler.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define FIE_MAX_BEAMS 64
+#define FIE_MAX_EOS 16
+
+/* One step of a beam search over `requests` requests of `beams` beams; row b of request r is
+   r * beams + b.  With x the logits (a NaN counts as -inf, +inf as FLT_MAX):
+     total[b, v] = scores[b] + log_softmax(x[b])[v]              in 64 bits, rounded once
+   A request's continuations rank by (total descending, lower beam, larger logit, lower token);
+   those of total -inf do not exist.  The best `beams` that are no eos go on.  An eos
+   continuation among the best `beams` of all joins the pool, the request's `beams` best ended
+   ones, at total / (length + 1)^length_penalty; on ties the older stays in front.
+   Requests that are done, and beams of score -inf, are not read.  A request is done when its
+   pool is full and (early_stopping, or the best that goes on is no better than the pool's worst
+   at the same length), or when nothing goes on. */
+typedef struct fie_beam_args {
+    const void* logits;         /* [requests * beams, vocab], rows row_stride elements apart */
+    const float* scores;        /* [requests, beams]; -inf: no such beam */
+    const int32_t* lengths;     /* [requests] tokens chosen so far */
+    const uint8_t* done;        /* [requests] 0 or 1 */
+    const float* pool;          /* [requests, beams], -inf where empty */
+    const int32_t* ends;        /* [requests, beams, 3]: length, parent row, eos token */
+    float* next_scores;         /* these five may be the ones above */
+    int32_t* next_lengths;      /* lengths + 1, of requests that were not done */
+    uint8_t* next_done;
+    float* next_pool;
+    int32_t* next_ends;
+    int64_t* tokens;            /* [requests * beams]; `pad` where no beam goes on */
+    int32_t* parents;           /* [requests * beams] rows; the row itself where none goes on */
+    int32_t* history_tokens;    /* [history_steps, requests * beams], or NULL: the step's tokens and */
+    int32_t* history_parents;   /* parents are kept at [lengths[r]] too */
+    int64_t row_stride;
+    void* workspace;            /* fie_beam_workspace_size() bytes, 16-byte aligned */
+    size_t workspace_bytes;
+    double length_penalty;
+    int32_t requests, beams, vocab, dtype;
+    int32_t early_stopping, min_tokens, pad, history_steps;   /* before min_tokens no eos exists */
+    int32_t eos_count;
+    int32_t eos[FIE_MAX_EOS];
+    int32_t max_tokens;         /* continuations of so many tokens end, whatever their token; 0: none */
+} fie_beam_args;
+
+size_t fie_beam_workspace_size(const fie_beam_args* args);
+
+int fie_beam_step(const fie_beam_args* args, void* stream);
+
+/* Rows of up to FIE_MAX_STATES tensors gathered: dst row i is src row parents[i]; a parent
+   outside [0, rows) stands for i.  Outputs do not overlap their inputs. */
+#define FIE_MAX_STATES 48
+typedef struct fie_state {
+    const void* src;            /* [rows], row_bytes each, src_stride bytes apart */
+    void* dst;                  /* [n] likewise, n <= rows */
+    int64_t src_stride, dst_stride, row_bytes, rows;
+} fie_state;
+
+typedef struct fie_states_args {
+    const int32_t* parents;     /* [n] */
+    int32_t n, count;           /* rows that are written; tensors */
+    fie_state state[FIE_MAX_STATES];        /* those past count need not be there */
+} fie_states_args;
+
+int fie_reorder_states(const fie_states_args* args, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* FIE_DECODE_H */
