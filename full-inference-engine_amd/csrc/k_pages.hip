@@ -1,0 +1,148 @@
+// Pages of a cache behind the C ABI of include/fie_decode.h.
+#include <algorithm>
+
+#include "launchers.h"
+#include "pages.h"
+
+namespace fie {
+
+static PageState page_state(const fie_pages_args& a)
+{
+    PageState s;
+    s.pages = a.pages;
+    s.page = a.page;
+    s.rows = a.rows;
+    s.wide = a.wide;
+    s.nblocks = (a.pages + kPageBlock - 1) / kPageBlock;
+    s.table = a.state;
+    s.lengths = s.table + (int64_t)a.rows * a.wide;
+    s.refs = s.lengths + a.rows;
+    s.blocks = s.refs + a.pages;
+    return s;
+}
+
+static PageScratch page_scratch(void* p, int64_t pages, int64_t rows, size_t* bytes)
+{
+    PageScratch w;
+    w.mark = (uint64_t*)p;
+    w.writers = (int32_t*)(w.mark + pages);
+    w.list = w.writers + pages;
+    w.movers = w.list + pages;
+    w.order = w.movers + pages;
+    w.copies = (PageCopy*)(w.order + pages);
+    w.count = (int32_t*)(w.copies + rows);
+    if (bytes) *bytes = ((size_t)((uintptr_t)(w.count + 4) - (uintptr_t)p) + 15) & ~(size_t)15;
+    return w;
+}
+
+static int64_t chunks_of(const fie_pages_args& a, const fie_cache_group& g)
+{
+    return ((g.whole ? 1 : a.page) * g.token_bytes + 15 + kCopyChunk - 1) / kCopyChunk;
+}
+
+static int pages_check(const fie_pages_args* a, bool table)
+{
+    if (!a) return fail(FIE_E_ARG, "args is NULL");
+    if (a->pages < 1 || a->pages > FIE_MAX_PAGES) return fail(FIE_E_ARG, "pages out of range [1, 4194304]");
+    if (a->page < 1 || a->page > 65536) return fail(FIE_E_ARG, "page out of range [1, 65536]");
+    if (a->group_count < 0 || a->group_count > FIE_MAX_CACHE_GROUPS) return fail(FIE_E_ARG, "group_count out of range [0, 8]");
+    for (int i = 0; i < a->group_count; ++i) {
+        const fie_cache_group& g = a->group[i];
+        if (g.count < 0 || g.outer < 1 || g.token_bytes < 1 || g.token_bytes > 1 << 30 || (g.count && !g.base))
+            return fail(FIE_E_ARG, "a cache group's layout is out of range");
+        if (g.outer * chunks_of(*a, g) > 1 << 24)
+            return fail(FIE_E_ARG, "a cache group's pages are too large");
+    }
+    if (!table) return FIE_OK;
+    if (a->rows < 1 || a->rows > FIE_MAX_PAGE_ROWS) return fail(FIE_E_ARG, "rows out of range [1, 4096]");
+    if (a->wide < 1 || a->wide > a->pages) return fail(FIE_E_ARG, "wide out of range [1, pages]");
+    if (!a->state) return fail(FIE_E_ARG, "state is NULL");
+    size_t need;
+    page_scratch(nullptr, a->pages, a->rows, &need);
+    if (!a->scratch || a->scratch_bytes < need) return fail(FIE_E_WORKSPACE, "scratch too small");
+    if (((uintptr_t)a->scratch & 15) != 0) return fail(FIE_E_WORKSPACE, "scratch not 16-byte aligned");
+    return FIE_OK;
+}
+
+// Copies of at most `most` pages, whose number may be known to the device alone.
+static hipError_t copy_pages(const fie_pages_args& a, const PageList& l, int64_t most, hipStream_t st)
+{
+    for (int i = 0; i < a.group_count; ++i) {
+        const fie_cache_group& g = a.group[i];
+        if (!g.count || !most) continue;
+        const int chunks = (int)chunks_of(a, g);
+        const int64_t items = most * g.count * g.outer * chunks;
+        k_pages_copy<<<(unsigned)std::min<int64_t>(items, 8 * std::max(cu_count(), 1)), kCopyThreads, 0, st>>>(l, g, a.page, chunks);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+static hipError_t pages_step(const fie_pages_args& a, hipStream_t st)
+{
+    const PageState s = page_state(a);
+    const PageScratch w = page_scratch(a.scratch, a.pages, a.rows, nullptr);
+    const size_t fork = (size_t)a.rows * (4 * kForkCols + 4 + 2);
+    k_pages_fork<<<(unsigned)((a.wide + kForkCols - 1) / kForkCols), kForkThreads, fork, st>>>(s, a.parents, a.lengths);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    k_pages_grow<<<1, kGrowThreads, (size_t)(2 * a.rows + s.nblocks) * 4, st>>>(s, w, a.parents, a.lengths, a.granted);
+    e = hipGetLastError();
+    if (e != hipSuccess || !a.lengths) return e;
+    return copy_pages(a, PageList{w.copies, nullptr, nullptr, w.count, 0, a.pages}, a.rows, st);
+}
+
+static hipError_t pages_compact(const fie_pages_args& a, hipStream_t st)
+{
+    const PageState s = page_state(a);
+    const PageScratch w = page_scratch(a.scratch, a.pages, a.rows, nullptr);
+    k_pages_holes<<<(unsigned)s.nblocks, kGrowThreads, 0, st>>>(s, w, a.live);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const int64_t entries = std::max((int64_t)a.rows * a.wide, (int64_t)a.pages / 2);
+    k_pages_rename<<<(unsigned)std::min<int64_t>((entries + 255) / 256, 8 * std::max(cu_count(), 1)), 256, 0, st>>>(s, w);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    return copy_pages(a, PageList{nullptr, w.movers, w.list, w.count, 0, a.pages}, a.pages / 2, st);
+}
+
+}  // namespace fie
+
+using namespace fie;
+
+extern "C" size_t fie_pages_state_ints(int32_t pages, int32_t rows, int32_t wide)
+{
+    if (pages < 1 || pages > FIE_MAX_PAGES || rows < 1 || rows > FIE_MAX_PAGE_ROWS || wide < 1 || wide > pages) return 0;
+    return (size_t)rows * wide + rows + pages + (pages + kPageBlock - 1) / kPageBlock;
+}
+
+extern "C" size_t fie_pages_scratch_bytes(int32_t pages, int32_t rows)
+{
+    if (pages < 1 || pages > FIE_MAX_PAGES || rows < 1 || rows > FIE_MAX_PAGE_ROWS) return 0;
+    size_t bytes;
+    page_scratch(nullptr, pages, rows, &bytes);
+    return bytes;
+}
+
+extern "C" int fie_pages_step(const fie_pages_args* a, void* stream)
+{
+    if (const int rc = pages_check(a, true); rc != FIE_OK) return rc;
+    if (!a->granted) return fail(FIE_E_ARG, "granted is NULL");
+    return launch_status(pages_step(*a, (hipStream_t)stream), "k_pages_step");
+}
+
+extern "C" int fie_pages_compact(const fie_pages_args* a, void* stream)
+{
+    if (const int rc = pages_check(a, true); rc != FIE_OK) return rc;
+    return launch_status(pages_compact(*a, (hipStream_t)stream), "k_pages_compact");
+}
+
+extern "C" int fie_pages_copy(const fie_pages_args* a, void* stream)
+{
+    if (const int rc = pages_check(a, false); rc != FIE_OK) return rc;
+    if (a->copies < 0) return fail(FIE_E_ARG, "copies < 0");
+    if (a->copies == 0) return FIE_OK;
+    if (!a->src || !a->dst) return fail(FIE_E_ARG, "src or dst is NULL");
+    return launch_status(copy_pages(*a, PageList{nullptr, a->src, a->dst, nullptr, a->copies, a->pages}, a->copies, (hipStream_t)stream),
+                         "k_pages_copy");
+}

@@ -77,6 +77,59 @@ typedef struct fie_states_args {
 
 int fie_reorder_states(const fie_states_args* args, void* stream);
 
+/* Pages of a cache: `rows` sequences, each with up to `wide` pages of `page` tokens out of a pool
+   of `pages`.  A page may be in several rows' tables, always at the same place of a row.
+   The state is one array of int32 (fie_pages_state_ints):
+     table  [rows][wide]    page ids, -1 past a row's pages
+     lengths [rows]         tokens
+     refs   [pages]         table entries that hold the page; 0: free
+     blocks [ceil(pages / 1024)]   free pages among each 1024
+   The scratch (fie_pages_scratch_bytes, 16-byte aligned) is zeroed once by the caller; calls
+   leave it so. */
+#define FIE_MAX_PAGE_ROWS 4096
+#define FIE_MAX_PAGES (1 << 22)
+
+/* Cache tensors of one layout: a page is `outer` pieces, outer_stride bytes apart, of `page`
+   tokens of token_bytes one after another; with `whole` of token_bytes that go with the whole page. */
+typedef struct fie_cache_group {
+    void* const* base;          /* [count] on the device */
+    int64_t page_stride, outer_stride, token_bytes;
+    int32_t count, outer, whole, reserved;
+} fie_cache_group;
+
+#define FIE_MAX_CACHE_GROUPS 8
+typedef struct fie_pages_args {
+    int32_t* state;
+    void* scratch;
+    size_t scratch_bytes;
+    int32_t pages, page, rows, wide;
+    const int32_t* parents;     /* [rows] or NULL: each its own; outside [0, rows): the row is emptied */
+    const int32_t* lengths;     /* [rows] or NULL: its parent's */
+    uint8_t* granted;           /* [rows]: 0 where pages did not suffice */
+    int32_t* live;              /* fie_pages_compact: pages in use */
+    const int32_t* src;         /* fie_pages_copy: [copies] pages */
+    const int32_t* dst;
+    int32_t copies, group_count;
+    fie_cache_group group[FIE_MAX_CACHE_GROUPS];
+} fie_pages_args;
+
+size_t fie_pages_state_ints(int32_t pages, int32_t rows, int32_t wide);
+size_t fie_pages_scratch_bytes(int32_t pages, int32_t rows);
+
+/* Row i takes its parent's pages, as many as min(lengths[i], the parent's length) tokens need;
+   what no row holds any more is free.  Where lengths[i] is more, the row grows to it, in the rows'
+   order and by the lowest free pages; a last page that is not full and that other rows hold is
+   replaced by a copy first, but for the longest (then lowest) row where all its holders grow.  A
+   row whose pages, with those of the rows before it, are more than are free, or more than `wide`,
+   does not grow. */
+int fie_pages_step(const fie_pages_args* args, void* stream);
+
+/* The i-th used page at or past the count of used pages moves to the i-th free page below it. */
+int fie_pages_compact(const fie_pages_args* args, void* stream);
+
+/* Pages dst[i] become copies of src[i] (those outside [0, pages) are left out); no table changes. */
+int fie_pages_copy(const fie_pages_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
