@@ -61,6 +61,8 @@ class VerifyArgs(ctypes.Structure):
 NORM_ARGS = "@10P6q9i3f0q"
 INT8_ARGS = "@6P4q4iPN0q"
 BEAM_ARGS = "@15PqPNd8i18i0q"
+ADAPTER_ARGS = "@10PN3q12i0q"
+ADAPTER_PLAN_ARGS = "@2P4i0q"
 PAGES_ARGS, GROUP_ARGS = "@PPN4i6P2i", "P3q4i"          # the head, and eight groups
 STATES_ARGS, STATE_ARGS = "@P2i", "2P4q"        # the head, and as many states as there are
 
@@ -83,7 +85,8 @@ EXPORTS = (
 OPS_EXPORTS = ("fie_block_norm", "fie_int8_linear", "fie_int8_workspace_size")
 # Every symbol include/fie_decode.h declares.
 DECODE_EXPORTS = ("fie_beam_workspace_size", "fie_beam_step", "fie_reorder_states", "fie_pages_state_ints",
-                  "fie_pages_scratch_bytes", "fie_pages_step", "fie_pages_compact", "fie_pages_copy")
+                  "fie_pages_scratch_bytes", "fie_pages_step", "fie_pages_compact", "fie_pages_copy", "fie_adapter_plan_ints",
+                  "fie_adapter_plan", "fie_adapter_workspace_size", "fie_adapter_linear")
 SCRATCH_BYTES = 64 << 20
 
 _lib = None
@@ -133,13 +136,17 @@ def bind(lib) -> None:
     lib.fie_sampler_last_error.restype = ctypes.c_char_p
     lib.fie_block_norm.argtypes = [ctypes.c_char_p, _vp]
     lib.fie_int8_linear.argtypes = [ctypes.c_char_p, _vp]
-    for name in ("fie_beam_step", "fie_reorder_states", "fie_pages_step", "fie_pages_compact", "fie_pages_copy"):
+    for name in ("fie_beam_step", "fie_reorder_states", "fie_pages_step", "fie_pages_compact", "fie_pages_copy",
+                 "fie_adapter_plan", "fie_adapter_linear"):
         getattr(lib, name).argtypes = [ctypes.c_char_p, _vp]
     for name in EXPORTS + OPS_EXPORTS + DECODE_EXPORTS:
         if name not in ("fie_sampler_workspace_size", "fie_sampler_last_error"):
             getattr(lib, name).restype = ctypes.c_int
     lib.fie_beam_workspace_size.argtypes = [ctypes.c_char_p]
     lib.fie_beam_workspace_size.restype = ctypes.c_size_t
+    lib.fie_adapter_plan_ints.argtypes = [ctypes.c_int32] * 3
+    lib.fie_adapter_workspace_size.argtypes = [ctypes.c_char_p]
+    lib.fie_adapter_plan_ints.restype = lib.fie_adapter_workspace_size.restype = ctypes.c_size_t
     lib.fie_pages_state_ints.argtypes = [ctypes.c_int32] * 3
     lib.fie_pages_scratch_bytes.argtypes = [ctypes.c_int32] * 2
     lib.fie_pages_state_ints.restype = lib.fie_pages_scratch_bytes.restype = ctypes.c_size_t

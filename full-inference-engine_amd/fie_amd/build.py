@@ -2,7 +2,7 @@
 
 The kernels live in several translation units (the C ABI and small kernels in
 sampler.hip; k_scan, k_finish per dtype, k_lmhead, k_verify, k_norm, k_int8,
-k_beam and k_pages in their own files), compiled
+k_beam, k_pages and k_adapter in their own files), compiled
 to objects in parallel and linked into one shared library."""
 
 from __future__ import annotations
@@ -21,7 +21,7 @@ OBJ_DIR = os.path.join(_HERE, "_native", "obj")
 
 SOURCES = ("sampler.hip", "k_scan.hip", "k_finish_f32.hip", "k_finish_f16.hip", "k_finish_bf16.hip",
            "k_lmhead.hip", "k_verify.hip", "k_norm.hip", "k_int8.hip",
-           "k_beam.hip", "k_pages.hip")
+           "k_beam.hip", "k_pages.hip", "k_adapter.hip")
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",

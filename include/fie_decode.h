@@ -10,7 +10,7 @@
 #ifndef FIE_DECODE_H
 #define FIE_DECODE_H
 
-#include "fie_sampler.h"
+#include "fie_ops.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -129,6 +129,50 @@ int fie_pages_compact(const fie_pages_args* args, void* stream);
 
 /* Pages dst[i] become copies of src[i] (those outside [0, pages) are left out); no table changes. */
 int fie_pages_copy(const fie_pages_args* args, void* stream);
+
+/* Low-rank adapters of many tokens: with i = ids[t],
+     y[t] = base[t] + scale[i] * b[i] (a[i] x[t])          (ids[t] outside [0, adapters): base[t])
+   Products of x and a are exact and their sums fp32.  With fp16 and bf16 adapters a[i] x[t] enters
+   the second product as the sum of two numbers of their type, off by 2^-16 of it (bf16) or less; its
+   sums are fp32, and y is rounded once.  An adapter of rank 0 gives base. */
+#define FIE_MAX_RANK 256
+#define FIE_MAX_ADAPTERS 4096
+#define FIE_ADAPTER_K 64        /* rows of a are padded with zeros to a multiple of so many */
+#define FIE_ADAPTER_RANK 16     /* ranks likewise, in a and b */
+
+/* Whose tokens are whose: tokens by adapter, cut into tiles of `tile` (16 or 64) tokens.  plan is
+   fie_adapter_plan_ints() of int32. */
+typedef struct fie_adapter_plan_args {
+    const int32_t* ids;         /* [tokens] */
+    int32_t* plan;
+    int32_t tokens, adapters, tile, reserved;
+} fie_adapter_plan_args;
+
+size_t fie_adapter_plan_ints(int32_t tokens, int32_t adapters, int32_t tile);
+int fie_adapter_plan(const fie_adapter_plan_args* args, void* stream);
+
+typedef struct fie_adapter_args {
+    const void* x;              /* [tokens, k] in dtype, or int8 with x_scale */
+    const float* x_scale;       /* [tokens] */
+    const void* a;              /* [adapters, rank, k_pad], zeros past each adapter's rank and past k */
+    const void* b;              /* [adapters, n, rank], likewise */
+    const float* scale;         /* [adapters] */
+    const int32_t* ranks;       /* [adapters], 0..rank */
+    const int32_t* plan;        /* of these tokens and so many adapters */
+    const void* base;           /* [tokens, n] in y_dtype or fp32, or NULL: 0; may be y */
+    void* y;                    /* [tokens, n] */
+    void* workspace;            /* fie_adapter_workspace_size() bytes, 16-byte aligned */
+    size_t workspace_bytes;
+    int64_t x_stride, base_stride, y_stride;        /* elements between rows */
+    int32_t tokens, k, n, adapters;
+    int32_t rank, k_pad, tile;  /* rank a multiple of FIE_ADAPTER_RANK, k_pad of FIE_ADAPTER_K */
+    int32_t dtype, x_dtype;     /* the adapters' type; x's: that or FIE_I8 */
+    int32_t y_dtype, base_dtype;        /* dtype or FIE_F32; y_dtype or FIE_F32 */
+    int32_t reserved;
+} fie_adapter_args;
+
+size_t fie_adapter_workspace_size(const fie_adapter_args* args);
+int fie_adapter_linear(const fie_adapter_args* args, void* stream);
 
 #ifdef __cplusplus
 }
