@@ -45,11 +45,9 @@ template <int DT> struct Operand {
     }
 };
 
-// The plan: [0] the number of tiles, then each tile's adapter (-1: none), first place and tokens,
-// then the tokens in places.
-constexpr int kPlanHead = 4, kPlanTile = 4;
-
-FIE_DEV int plan_tiles_of(int tokens, int adapters, int tile) { return tokens / tile + min(tokens, adapters + 1); }
+// The plan: [0] the number of tiles, then each tile's adapter (-1: none), first place and tokens (16 at
+// most), then the tokens in places.
+constexpr int kPlanHead = 4, kPlanTile = 4, kTileTokens = 16;
 
 constexpr int kPlanThreads = 1024;
 
@@ -74,7 +72,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_adapter_plan(const fie_adapter
     int sum = 0, cut = 0;
     for (int i = first; i < last; ++i) {
         sum += count[i];
-        cut += (count[i] + a.tile - 1) / a.tile;
+        cut += (count[i] + kTileTokens - 1) / kTileTokens;
     }
     const int s = (int)wave_incl_scan_u32((uint32_t)sum), c = (int)wave_incl_scan_u32((uint32_t)cut);
     if (lane == 63) {
@@ -90,10 +88,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_adapter_plan(const fie_adapter
     if (tid == kPlanThreads - 1) a.plan[0] = tile + cut;
     for (int i = first; i < last; ++i) {
         next[i] = at;
-        for (int n = 0; n < count[i]; n += a.tile, ++tile) {
+        for (int n = 0; n < count[i]; n += kTileTokens, ++tile) {
             tiles[tile * kPlanTile] = i - 1;
             tiles[tile * kPlanTile + 1] = at + n;
-            tiles[tile * kPlanTile + 2] = min(a.tile, count[i] - n);
+            tiles[tile * kPlanTile + 2] = min(kTileTokens, count[i] - n);
         }
         at += count[i];
     }
@@ -102,7 +100,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_adapter_plan(const fie_adapter
 }
 
 struct AdapterWork {
-    float* h;                   // [splits][tokens in places][rank]
+    float* h;                   // [splits][places][rank], the first product by parts of k
     int splits, most;           // of k; tiles of the plan
 };
 
@@ -178,235 +176,292 @@ template <int DX, int DT, bool ALIGNED> struct TokenLoad {
     }
 };
 
-constexpr int kDownWaves = 4, kDownSteps = 4;           // steps of k of a wave at a time
+constexpr int kDownWaves = 4;
 
-// h = A x: grid (splits, tiles), 16 MT tokens by 16 RT ranks a workgroup, whose waves and the splits
-// take k in turn.  Operands come straight from memory: a row of A is read once for its tile's
-// tokens, x once.
-template <int DX, int DT, int MT, int RT, bool ALIGNED>
+// h = A x: grid (splits, tiles), 16 tokens of one adapter a workgroup.  The splits and their waves take k
+// in turn, U steps each, straight from memory to the matrix instructions, 16 RT ranks at a time; a
+// workgroup's sums meet in LDS, the splits' in the second product.  (One workgroup a tile, of 16 waves:
+// 1 x 4096 6.8 us against 3.8, 250 tokens of 64 adapters 9.3 against 5.3: a CU alone is slow to
+// bring in a whole A.)  Bound by A's way from memory for few tokens an adapter, by x's for many.
+template <int DX, int DT, int RT, int U, bool ALIGNED>
 __global__ __launch_bounds__(64 * kDownWaves) void k_adapter_down(const fie_adapter_args a, const AdapterWork w)
 {
     using Op = Operand<DT>;
     using Tok = TokenLoad<DX, DT, ALIGNED>;
     constexpr int XS = Tok::XS;
-    __shared__ f32x4_t red[kDownWaves][MT * RT][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ f32x4_t red[kDownWaves][RT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane >> 4;
     if ((int)blockIdx.y >= a.plan[0]) return;
     const int32_t* tile = a.plan + kPlanHead + blockIdx.y * kPlanTile;
     const int32_t* order = a.plan + kPlanHead + (int64_t)w.most * kPlanTile;
     const int id = tile[0], first = tile[1], count = tile[2];
     if (id < 0) return;
     const int rank = a.ranks[id];
-    const uint8_t* row[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int t = order[first + min(16 * m + (lane & 15), count - 1)];
-        row[m] = (const uint8_t*)a.x + (int64_t)t * a.x_stride * XS;
-    }
-    const int group = lane >> 4;
+    const uint8_t* const row = (const uint8_t*)a.x + (int64_t)order[first + min(lane & 15, count - 1)] * a.x_stride * XS;
     const int full = a.k / Op::STEP, steps = (a.k + Op::STEP - 1) / Op::STEP;
     for (int r0 = 0; r0 < rank; r0 += 16 * RT) {
         const uint8_t* ar[RT];
 #pragma unroll
         for (int r = 0; r < RT; ++r)
             ar[r] = (const uint8_t*)a.a + ((int64_t)id * a.rank + min(r0 + 16 * r, a.rank - 16) + (lane & 15)) * a.k_pad * Op::SIZE + 16 * group;
-        f32x4_t acc[MT][RT];
+        f32x4_t acc[RT];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int r = 0; r < RT; ++r) acc[r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = (blockIdx.x * kDownWaves + wave) * U; c < steps; c += gridDim.x * kDownWaves * U) {
+            if (c + U <= full) {
+                u32x4_t fa[U][RT];
+                Tok fx[U];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) acc[m][r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int c = (blockIdx.x * kDownWaves + wave) * kDownSteps; c < steps; c += gridDim.x * kDownWaves * kDownSteps) {
-            if (c + kDownSteps <= full) {
-                u32x4_t fa[kDownSteps][RT];
-                Tok fx[kDownSteps][MT];
-#pragma unroll
-                for (int u = 0; u < kDownSteps; ++u) {
+                for (int u = 0; u < U; ++u) {
 #pragma unroll
                     for (int r = 0; r < RT; ++r) fa[u][r] = *(const u32x4_t*)(ar[r] + (int64_t)(c + u) * 64);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) fx[u][m].load(row[m] + ((c + u) * Op::STEP + group * Op::EACH) * XS);
+                    fx[u].load(row + ((c + u) * Op::STEP + group * Op::EACH) * XS);
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int u = 0; u < kDownSteps; ++u)
+                for (int u = 0; u < U; ++u) {
+                    const u32x4_t x = fx[u].get(row + ((c + u) * Op::STEP + group * Op::EACH) * XS);
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        const u32x4_t x = fx[u][m].get(row[m] + ((c + u) * Op::STEP + group * Op::EACH) * XS);
-#pragma unroll
-                        for (int r = 0; r < RT; ++r) acc[m][r] = Op::mul(fa[u][r], x, acc[m][r]);
-                    }
+                    for (int r = 0; r < RT; ++r) acc[r] = Op::mul(fa[u][r], x, acc[r]);
+                }
             } else
 #pragma unroll 1
-                for (int u = c; u < min(c + kDownSteps, steps); ++u)
+                for (int u = c; u < min(c + U, steps); ++u) {
+                    const u32x4_t x = Tok::last(row, u * Op::STEP + group * Op::EACH, a.k);
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        const u32x4_t x = Tok::last(row[m], u * Op::STEP + group * Op::EACH, a.k);
-#pragma unroll
-                        for (int r = 0; r < RT; ++r) acc[m][r] = Op::mul(*(const u32x4_t*)(ar[r] + (int64_t)u * 64), x, acc[m][r]);
-                    }
+                    for (int r = 0; r < RT; ++r) acc[r] = Op::mul(*(const u32x4_t*)(ar[r] + (int64_t)u * 64), x, acc[r]);
+                }
         }
-        __syncthreads();
+        if (r0) __syncthreads();                        // the sums before are read
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int r = 0; r < RT; ++r) red[wave][m * RT + r][lane] = acc[m][r];
+        for (int r = 0; r < RT; ++r) red[wave][r][lane] = acc[r];
         __syncthreads();
-        for (int f = wave; f < MT * RT; f += kDownWaves) {
+        for (int f = wave; f < RT; f += kDownWaves) {
             f32x4_t t = red[0][f][lane];
 #pragma unroll
             for (int i = 1; i < kDownWaves; ++i) t += red[i][f][lane];
-            const int m = 16 * (f / RT) + (lane & 15), r = r0 + 16 * (f % RT) + 4 * group;
-            if (m < count && r < a.rank) *(f32x4_t*)(w.h + ((int64_t)blockIdx.x * a.tokens + first + m) * a.rank + r) = t;
+            const int r = r0 + 16 * f + 4 * group;
+            if ((lane & 15) < count && r < a.rank) *(f32x4_t*)(w.h + ((int64_t)blockIdx.x * a.tokens + first + (lane & 15)) * a.rank + r) = t;
         }
     }
 }
 
-constexpr int kUpWaves = 4, kUpCols = 4;                // 16-channel blocks of a wave
-constexpr int kUpChannels = 16 * kUpCols * kUpWaves;
-
-template <int DT> FIE_DEV void load4(const void* p, int64_t at, bool wide, int left, float* v)
-{
-    using Op = Operand<DT>;
-    if (wide && left >= 4) {
+// One and four elements as they are in memory (four: at an address aligned to four).
+template <int DT> struct Raw {
+    typedef typename std::conditional<DT == FIE_F32, float, uint16_t>::type one_t;
+    typedef typename std::conditional<DT == FIE_F32, f32x4_t, uint2>::type four_t;
+    static FIE_DEV float value(one_t r)
+    {
+        if constexpr (DT == FIE_F32) return r;
+        else return Operand<DT>::value(r);
+    }
+    static FIE_DEV void open(const four_t& r, float* v)
+    {
         if constexpr (DT == FIE_F32) {
-            const float4 f = *(const float4*)((const float*)p + at);
-            v[0] = f.x;
-            v[1] = f.y;
-            v[2] = f.z;
-            v[3] = f.w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = r[i];
         } else {
-            const uint2 u = *(const uint2*)((const uint16_t*)p + at);
-            v[0] = Op::value(u.x & 0xFFFFu);
-            v[1] = Op::value(u.x >> 16);
-            v[2] = Op::value(u.y & 0xFFFFu);
-            v[3] = Op::value(u.y >> 16);
+            v[0] = value((uint16_t)r.x);
+            v[1] = value((uint16_t)(r.x >> 16));
+            v[2] = value((uint16_t)r.y);
+            v[3] = value((uint16_t)(r.y >> 16));
         }
-    } else
+    }
+    static FIE_DEV one_t close(float v)
+    {
+        if constexpr (DT == FIE_F32) return v;
+        else return (uint16_t)Operand<DT>::bits(v);
+    }
+    static FIE_DEV four_t close(const float* v)
+    {
+        if constexpr (DT == FIE_F32) return f32x4_t{v[0], v[1], v[2], v[3]};
+        else return make_uint2(close(v[0]) | ((uint32_t)close(v[1]) << 16), close(v[2]) | ((uint32_t)close(v[3]) << 16));
+    }
+};
+
+constexpr int kUpWaves = 4, kUpCols = 4, kUpChannels = 16 * kUpCols;
+
+// The second product's operand of 16 ranks, for 16 tokens: a lane's numbers of its token, summed
+// over the splits.  With two-byte adapters lanes of groups 0 and 1 give the leading parts of 16 ranks
+// and groups 2 and 3 the trailing parts, both against the same 16 of B.
+template <int DT> struct UpOperand {
+    static constexpr int N = DT == FIE_F32 ? 4 : 8;
+    float v[N];
+    FIE_DEV void load(const float* h, int64_t part, int splits)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = 0.0f;
+        for (int p = 0; p < splits; p += 4) {           // four on their way together
+            f32x4_t t[4][N / 4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < N / 4; ++i) t[u][i] = *(const f32x4_t*)(h + (int64_t)min(p + u, splits - 1) * part + 4 * i);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] += p + u < splits ? t[u][i / 4][i % 4] : 0.0f;
+        }
+    }
+    FIE_DEV float most(float m) const
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = __builtin_fmaxf(m, __builtin_fabsf(v[i]));
+        return m;
+    }
+    FIE_DEV u32x4_t get(int e, bool trailing) const     // times 2^e
+    {
+        using Op = Operand<DT>;
+        u32x4_t o;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (i >= left) continue;
-            if constexpr (DT == FIE_F32) v[i] = ((const float*)p)[at + i];
-            else v[i] = Op::value(((const uint16_t*)p)[at + i]);
-        }
-}
-
-template <int DT> FIE_DEV void store4(void* p, int64_t at, bool wide, int left, const float* v)
-{
-    using Op = Operand<DT>;
-    if (wide && left >= 4) {
-        if constexpr (DT == FIE_F32) *(float4*)((float*)p + at) = make_float4(v[0], v[1], v[2], v[3]);
-        else *(uint2*)((uint16_t*)p + at) = make_uint2(Op::bits(v[0]) | (Op::bits(v[1]) << 16), Op::bits(v[2]) | (Op::bits(v[3]) << 16));
-    } else
+            if constexpr (DT == FIE_F32) o[i] = __float_as_uint(v[i]);
+            else {
+                uint32_t b[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (i >= left) continue;
-            if constexpr (DT == FIE_F32) ((float*)p)[at + i] = v[i];
-            else ((uint16_t*)p)[at + i] = (uint16_t)Op::bits(v[i]);
+                for (int j = 0; j < 2; ++j) {
+                    const float x = DT == FIE_F16 ? __builtin_ldexpf(v[2 * i + j], e) : v[2 * i + j];
+                    const uint32_t lead = Op::bits(x);
+                    const float back = Op::value(lead); // (an infinity has no rest)
+                    b[j] = trailing ? Op::bits(__builtin_fabsf(back) <= 3.4e38f ? x - back : 0.0f) : lead;
+                }
+                o[i] = b[0] | (b[1] << 16);
+            }
         }
-}
+        return o;
+    }
+};
 
-// y = base + scale B h: grid (blocks of kUpChannels channels, tiles).  h goes into LDS summed over the
-// splits, in fp32; with two-byte adapters each 16 ranks of it are taken as 16 leading and 16 trailing
-// parts against the same 16 of B, one instruction.  fp16 tokens are brought to an exponent of their
-// own first, so that no part overflows.  Bound by base and y.
-template <int DT, int DY, int DB, int MT>
-__global__ __launch_bounds__(64 * kUpWaves) void k_adapter_up(const fie_adapter_args a, const AdapterWork w, int wide)
+// y = base + scale B h: a wave a tile of 16 tokens and `steps` times 64 channels next to each other, on
+// its own; the four of a workgroup take four tiles, which mostly share their B.  h stays in registers as
+// the matrix instructions take it (CH times 16 ranks; CH 0: any number, built anew for each step).  fp16
+// tokens are brought to an exponent of their own first, so that no part overflows.  Results cross LDS
+// within the wave, so that base and y are read and written along their rows whatever these begin at.
+// Bound by base and y for many tokens an adapter, by B for few.
+template <int DT, int DY, int DB, int CH>
+__global__ __launch_bounds__(64 * kUpWaves) void k_adapter_up(const fie_adapter_args a, const AdapterWork w, int wide, int steps)
 {
     using Op = Operand<DT>;
-    extern __shared__ float H[];                        // [16 MT][rank + 4]
-    __shared__ float factor[16 * MT];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = lane >> 4;
-    if ((int)blockIdx.y >= a.plan[0]) return;
-    const int32_t* tile = a.plan + kPlanHead + blockIdx.y * kPlanTile;
+    using Part = UpOperand<DT>;
+    constexpr int kPitch = kUpChannels + 4, HELD = CH ? CH : 1;
+    __shared__ float stage[kUpWaves][16 * kPitch];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane >> 4, col = lane & 15;
+    const int t0 = blockIdx.y * kUpWaves + wave;
+    if (t0 >= a.plan[0]) return;
+    const int32_t* tile = a.plan + kPlanHead + (int64_t)t0 * kPlanTile;
     const int32_t* order = a.plan + kPlanHead + (int64_t)w.most * kPlanTile;
     const int id = tile[0], first = tile[1], count = tile[2];
-    const int rank = id < 0 ? 0 : a.ranks[id], pitch = a.rank + 4;
+    const int rank = id < 0 ? 0 : a.ranks[id];
     if (rank == 0 && a.base == a.y) return;
-    const int ranks = (rank + 15) / 16 * 16;
+    const int chunks = (rank + 15) / 16;
+    const int place = first + min(col, count - 1), mine = order[place];
+    float factor = rank ? a.scale[id] : 0.0f;
+    const bool trailing = group >= 2;
+    const float* const h = w.h + (int64_t)place * a.rank + (DT == FIE_F32 ? 4 * group : 8 * (group & 1));
+    const int64_t part = (int64_t)a.tokens * a.rank;
+    int e = 0;
+    u32x4_t fh[HELD];
     if (rank) {
-        const float s = a.scale[id];
-        for (int i = tid; i < 16 * MT * ranks; i += 64 * kUpWaves) {
-            const int m = i / ranks, r = i - m * ranks;
-            float v = 0.0f;
-            if (m < count)
-                for (int p = 0; p < w.splits; ++p) v += w.h[((int64_t)p * a.tokens + first + m) * a.rank + r];
-            H[m * pitch + r] = v;
-        }
-        __syncthreads();
-        if (tid < 16 * MT) {
-            float f = s;
-            if (a.x_scale && tid < count) f *= a.x_scale[order[first + tid]];
-            if constexpr (DT == FIE_F16) {
-                float most = 0.0f;
-                for (int r = 0; r < ranks; ++r) most = __builtin_fmaxf(most, __builtin_fabsf(H[tid * pitch + r]));
-                const int e = most > 0.0f && most <= 3.4e38f ? (int)((__float_as_uint(most) >> 23) & 255u) - 127 : 0;
-                for (int r = 0; r < ranks; ++r) H[tid * pitch + r] = __builtin_ldexpf(H[tid * pitch + r], -e);
-                f = __builtin_ldexpf(f, e);
+        if (a.x_scale) factor *= a.x_scale[mine];
+        Part p[HELD];
+        float most = 0.0f;
+        if constexpr (CH > 0) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                if (c < chunks) p[c].load(h + 16 * c, part, w.splits);
+                if (c < chunks) most = p[c].most(most);
             }
-            factor[tid] = f;
+        } else if constexpr (DT == FIE_F16)
+            for (int c = 0; c < chunks; ++c) {
+                p[0].load(h + 16 * c, part, w.splits);
+                most = p[0].most(most);
+            }
+        if constexpr (DT == FIE_F16) {
+            most = __builtin_fmaxf(most, __shfl_xor(most, 16, 64));
+            e = most > 0.0f && most <= 3.4e38f ? 127 - (int)((__float_as_uint(most) >> 23) & 255u) : 0;
+            factor = __builtin_ldexpf(factor, -e);
         }
-        __syncthreads();
+        if constexpr (CH > 0)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) fh[c] = c < chunks ? p[c].get(e, trailing) : u32x4_t{0, 0, 0, 0};
     }
-    const int n0 = (blockIdx.x * kUpWaves + wave) * (16 * kUpCols);
-    if (n0 >= a.n) return;
-    f32x4_t acc[MT][kUpCols];
+    float* const room = stage[wave];
+    const uint8_t* const b0 = (const uint8_t*)a.b + (int64_t)max(id, 0) * a.n * a.rank * Op::SIZE + 16 * (DT == FIE_F32 ? group : group & 1);
+    for (int s = 0; s < steps; ++s) {
+        const int n0 = (blockIdx.x * steps + s) * kUpChannels;
+        if (n0 >= a.n) return;
+        // base first, then B: both are on their way before anything is used.  Rows past the tile's tokens
+        // repeat its last one's, channels past n the last
+        const bool four = wide && n0 + kUpChannels <= a.n;
+        const int nw = n0 + 4 * col, nl = min(n0 + lane, a.n - 1);
+        typename Raw<DB>::four_t r4[4];
+        typename Raw<DB>::one_t r1[16];
+        if (a.base) {
+            if (four) {                                 // 4 channels a lane of 4 tokens
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+                for (int i = 0; i < 4; ++i)
+                    r4[i] = *(const typename Raw<DB>::four_t*)((const typename Raw<DB>::one_t*)a.base + (int64_t)__shfl(mine, 4 * i + group, 64) * a.base_stride + nw);
+            } else                                      // a channel a lane of 16
 #pragma unroll
-        for (int q = 0; q < kUpCols; ++q) acc[m][q] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    const uint8_t* br[kUpCols];
-    const int inner = DT == FIE_F32 ? 16 * group : 16 * (group & 1);
+                for (int r = 0; r < 16; ++r)
+                    r1[r] = ((const typename Raw<DB>::one_t*)a.base + (int64_t)__builtin_amdgcn_readlane(mine, r) * a.base_stride)[nl];
+        }
+        if (rank) {
+            f32x4_t acc[kUpCols];
 #pragma unroll
-    for (int q = 0; q < kUpCols; ++q)
-        br[q] = (const uint8_t*)a.b + ((int64_t)max(id, 0) * a.n + min(n0 + 16 * q + (lane & 15), a.n - 1)) * a.rank * Op::SIZE + inner;
-    for (int r0 = 0; r0 < ranks; r0 += 16) {
-        u32x4_t fb[kUpCols];
+            for (int q = 0; q < kUpCols; ++q) acc[q] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            const uint8_t* br[kUpCols];
 #pragma unroll
-        for (int q = 0; q < kUpCols; ++q) fb[q] = *(const u32x4_t*)(br[q] + r0 * Op::SIZE);
+            for (int q = 0; q < kUpCols; ++q) br[q] = b0 + (int64_t)min(n0 + 16 * q + col, a.n - 1) * a.rank * Op::SIZE;
+            if constexpr (CH > 0) {
+                u32x4_t fb[CH][kUpCols];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            if (16 * m >= count) continue;
-            const float* h = H + (16 * m + (lane & 15)) * pitch + r0 + (DT == FIE_F32 ? 4 * group : 8 * (group & 1));
-            u32x4_t fh;
-            if constexpr (DT == FIE_F32) {
+                for (int c = 0; c < CH; ++c)
+                    if (c < chunks)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) fh[i] = __float_as_uint(h[i]);
-            } else {
+                        for (int q = 0; q < kUpCols; ++q) fb[c][q] = *(const u32x4_t*)(br[q] + c * 16 * Op::SIZE);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t part[2];
+                for (int c = 0; c < CH; ++c)
+                    if (c < chunks)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float v = h[2 * i + j];
-                        const uint32_t lead = Op::bits(v);
-                        const float rest = v - Op::value(lead);
-                        // (an infinity has no rest)
-                        part[j] = group < 2 ? lead : Op::bits(__builtin_fabsf(Op::value(lead)) <= 3.4e38f ? rest : 0.0f);
-                    }
-                    fh[i] = part[0] | (part[1] << 16);
+                        for (int q = 0; q < kUpCols; ++q) acc[q] = Op::mul(fb[c][q], fh[c], acc[q]);
+            } else
+                for (int c = 0; c < chunks; ++c) {
+                    Part p;
+                    p.load(h + 16 * c, part, w.splits);
+                    const u32x4_t f = p.get(e, trailing);
+#pragma unroll
+                    for (int q = 0; q < kUpCols; ++q) acc[q] = Op::mul(*(const u32x4_t*)(br[q] + c * 16 * Op::SIZE), f, acc[q]);
                 }
+#pragma unroll
+            for (int q = 0; q < kUpCols; ++q) *(f32x4_t*)&room[col * kPitch + 16 * q + 4 * group] = acc[q] * factor;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        typename Raw<DY>::one_t* const y = (typename Raw<DY>::one_t*)a.y;
+        if (four) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 4 * i + group;
+                const int64_t t = __shfl(mine, r, 64);
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (a.base) Raw<DB>::open(r4[i], v);
+                if (rank) {
+                    const f32x4_t d = *(const f32x4_t*)&room[r * kPitch + 4 * col];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] += d[j];
+                }
+                if (r < count) *(typename Raw<DY>::four_t*)(y + t * a.y_stride + nw) = Raw<DY>::close(v);
             }
+        } else
 #pragma unroll
-            for (int q = 0; q < kUpCols; ++q) acc[m][q] = Op::mul(fb[q], fh, acc[m][q]);
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int c = 16 * m + (lane & 15);
-        if (c >= count) continue;
-        const int64_t t = order[first + c];
-        const float f = rank ? factor[c] : 0.0f;
-#pragma unroll
-        for (int q = 0; q < kUpCols; ++q) {
-            const int n = n0 + 16 * q + 4 * group, left = a.n - n;
-            if (left <= 0) continue;
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (a.base) load4<DB>(a.base, t * a.base_stride + n, wide & 1, left, v);
-            if (rank)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] += f * acc[m][q][i];
-            store4<DY>(a.y, t * a.y_stride + n, wide & 2, left, v);
-        }
+            for (int r = 0; r < 16; ++r) {
+                const int64_t t = __builtin_amdgcn_readlane(mine, r);
+                float v = a.base ? Raw<DB>::value(r1[r]) : 0.0f;
+                if (rank) v += room[r * kPitch + lane];
+                if (r < count && n0 + lane < a.n) y[t * a.y_stride + n0 + lane] = Raw<DY>::close(v);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 

@@ -5,31 +5,31 @@
 
 namespace fie {
 
-static int plan_most(int64_t tokens, int64_t adapters, int tile) { return (int)(tokens / tile + std::min(tokens, adapters + 1)); }
+static int64_t plan_most(int64_t tokens, int64_t adapters) { return tokens / kTileTokens + std::min(tokens, adapters + 1); }
+
+constexpr int kDownSteps = 4;                           // of a wave at a time; 2 from 33 ranks on
 
 static AdapterWork adapter_work(const fie_adapter_args& a)
 {
     AdapterWork w;
     w.h = (float*)a.workspace;
-    w.most = plan_most(a.tokens, a.adapters, a.tile);
-    // enough workgroups to fill the CUs; each wave has its steps of k
-    const int step = (a.dtype == FIE_F32 ? 16 : 32) * kDownSteps * kDownWaves;
-    w.splits = std::max(1, std::min({(a.k + step - 1) / step, 512 / std::max(w.most, 1), 32}));
+    w.most = (int)plan_most(a.tokens, a.adapters);
+    // enough workgroups to fill the CUs, as long as each wave has its steps of k
+    const int step = (a.dtype == FIE_F32 ? 16 : 32) * (a.rank > 32 ? 2 : kDownSteps) * kDownWaves;
+    w.splits = std::max(1, std::min({(a.k + step - 1) / step, 1024 / std::max(w.most, 1), 16}));
     return w;
 }
 
-static size_t adapter_bytes(const fie_adapter_args& a)
-{
-    return (size_t)adapter_work(a).splits * a.tokens * a.rank * 4;
-}
+static size_t adapter_bytes(const fie_adapter_args& a) { return (size_t)adapter_work(a).splits * a.tokens * a.rank * 4; }
 
-template <int DX, int DT, int MT, bool ALIGNED>
+template <int DX, int DT, bool ALIGNED>
 static hipError_t down_of(const fie_adapter_args& a, const AdapterWork& w, hipStream_t st)
 {
     const dim3 grid((unsigned)w.splits, (unsigned)w.most);
-    if (a.rank <= 16) k_adapter_down<DX, DT, MT, 1, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
-    else if (a.rank <= 32) k_adapter_down<DX, DT, MT, 2, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
-    else k_adapter_down<DX, DT, MT, 4, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
+    if (a.rank <= 16) k_adapter_down<DX, DT, 1, kDownSteps, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
+    else if (a.rank <= 32) k_adapter_down<DX, DT, 2, kDownSteps, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
+    else if (a.rank <= 48) k_adapter_down<DX, DT, 3, 2, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
+    else k_adapter_down<DX, DT, 4, 2, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
     return hipGetLastError();
 }
 
@@ -38,19 +38,25 @@ static hipError_t down(const fie_adapter_args& a, const AdapterWork& w, hipStrea
 {
     constexpr int XS = DX == FIE_I8 ? 1 : Operand<DT>::SIZE, BYTES = XS * Operand<DT>::EACH;
     const bool aligned = (uintptr_t)a.x % BYTES == 0 && a.x_stride * XS % BYTES == 0;
-    if (a.tile == 16) return aligned ? down_of<DX, DT, 1, true>(a, w, st) : down_of<DX, DT, 1, false>(a, w, st);
-    return aligned ? down_of<DX, DT, 4, true>(a, w, st) : down_of<DX, DT, 4, false>(a, w, st);
+    return aligned ? down_of<DX, DT, true>(a, w, st) : down_of<DX, DT, false>(a, w, st);
 }
 
 template <int DT, int DY, int DB>
 static hipError_t up(const fie_adapter_args& a, const AdapterWork& w, hipStream_t st)
 {
     constexpr int YB = DY == FIE_F32 ? 16 : 8, BB = DB == FIE_F32 ? 16 : 8;
-    const int wide = ((uintptr_t)a.base % BB == 0 && a.base_stride % 4 == 0 ? 1 : 0) | ((uintptr_t)a.y % YB == 0 && a.y_stride % 4 == 0 ? 2 : 0);
-    const dim3 grid((unsigned)((a.n + kUpChannels - 1) / kUpChannels), (unsigned)w.most);
-    const size_t lds = (size_t)a.tile * (a.rank + 4) * 4;
-    if (a.tile == 16) k_adapter_up<DT, DY, DB, 1><<<grid, 64 * kUpWaves, lds, st>>>(a, w, wide);
-    else k_adapter_up<DT, DY, DB, 4><<<grid, 64 * kUpWaves, lds, st>>>(a, w, wide);
+    const int wide = (uintptr_t)a.base % BB == 0 && a.base_stride % 4 == 0 && (uintptr_t)a.y % YB == 0 && a.y_stride % 4 == 0;
+    const int blocks = (a.n + kUpChannels - 1) / kUpChannels;
+    // as many waves as the CUs hold (16 each), and then more steps each
+    const int steps = (int)std::max<int64_t>(1, std::min<int64_t>(8, (int64_t)blocks * w.most / (16 * std::max(cu_count(), 1))));
+    const dim3 grid((unsigned)((blocks + steps - 1) / steps), (unsigned)((w.most + kUpWaves - 1) / kUpWaves));
+    switch (a.rank / 16) {
+    case 1: k_adapter_up<DT, DY, DB, 1><<<grid, 64 * kUpWaves, 0, st>>>(a, w, wide, steps); break;
+    case 2: k_adapter_up<DT, DY, DB, 2><<<grid, 64 * kUpWaves, 0, st>>>(a, w, wide, steps); break;
+    case 3: k_adapter_up<DT, DY, DB, 3><<<grid, 64 * kUpWaves, 0, st>>>(a, w, wide, steps); break;
+    case 4: k_adapter_up<DT, DY, DB, 4><<<grid, 64 * kUpWaves, 0, st>>>(a, w, wide, steps); break;
+    default: k_adapter_up<DT, DY, DB, 0><<<grid, 64 * kUpWaves, 0, st>>>(a, w, wide, steps); break;
+    }
     return hipGetLastError();
 }
 
@@ -65,19 +71,18 @@ static hipError_t adapter_dt(const fie_adapter_args& a, hipStream_t st)
     return hipSuccess;
 }
 
-static int plan_check(int64_t tokens, int64_t adapters, int tile)
+static int plan_check(int64_t tokens, int64_t adapters)
 {
     if (tokens < 0 || tokens > 1 << 24) return fail(FIE_E_ARG, "tokens out of range [0, 16777216]");
     if (adapters < 1 || adapters > FIE_MAX_ADAPTERS) return fail(FIE_E_ARG, "adapters out of range [1, 4096]");
-    if (tile != 16 && tile != 64) return fail(FIE_E_ARG, "tile is 16 or 64");
-    if (plan_most(tokens, adapters, tile) > 65535) return fail(FIE_E_ARG, "more tiles than a launch holds");
+    if (plan_most(tokens, adapters) > 65535) return fail(FIE_E_ARG, "more tiles than a launch holds");
     return FIE_OK;
 }
 
 static int adapter_check(const fie_adapter_args* a)
 {
     if (!a) return fail(FIE_E_ARG, "args is NULL");
-    if (const int rc = plan_check(a->tokens, a->adapters, a->tile); rc != FIE_OK) return rc;
+    if (const int rc = plan_check(a->tokens, a->adapters); rc != FIE_OK) return rc;
     if (a->dtype < FIE_F32 || a->dtype > FIE_BF16 || (a->x_dtype != a->dtype && a->x_dtype != FIE_I8))
         return fail(FIE_E_ARG, "x is in the adapters' type or int8");
     if ((a->y_dtype != a->dtype && a->y_dtype != FIE_F32) || (a->base && a->base_dtype != a->y_dtype && a->base_dtype != FIE_F32))
@@ -101,24 +106,24 @@ static int adapter_check(const fie_adapter_args* a)
 
 using namespace fie;
 
-extern "C" size_t fie_adapter_plan_ints(int32_t tokens, int32_t adapters, int32_t tile)
+extern "C" size_t fie_adapter_plan_ints(int32_t tokens, int32_t adapters)
 {
-    if (plan_check(tokens, adapters, tile) != FIE_OK) return 0;
-    return kPlanHead + (size_t)plan_most(tokens, adapters, tile) * kPlanTile + tokens;
+    if (plan_check(tokens, adapters) != FIE_OK) return 0;
+    return kPlanHead + (size_t)plan_most(tokens, adapters) * kPlanTile + tokens;
 }
 
 extern "C" int fie_adapter_plan(const fie_adapter_plan_args* a, void* stream)
 {
     if (!a) return fail(FIE_E_ARG, "args is NULL");
-    if (const int rc = plan_check(a->tokens, a->adapters, a->tile); rc != FIE_OK) return rc;
+    if (const int rc = plan_check(a->tokens, a->adapters); rc != FIE_OK) return rc;
     if (!a->plan || (a->tokens && !a->ids)) return fail(FIE_E_ARG, "ids or plan is NULL");
-    k_adapter_plan<<<1, kPlanThreads, 0, (hipStream_t)stream>>>(*a, plan_most(a->tokens, a->adapters, a->tile));
+    k_adapter_plan<<<1, kPlanThreads, 0, (hipStream_t)stream>>>(*a, (int)plan_most(a->tokens, a->adapters));
     return launch_status(hipGetLastError(), "k_adapter_plan");
 }
 
 extern "C" size_t fie_adapter_workspace_size(const fie_adapter_args* a)
 {
-    return a && a->tokens > 0 && a->k > 0 && a->rank > 0 && (a->tile == 16 || a->tile == 64) ? adapter_bytes(*a) : 0;
+    return a && a->tokens > 0 && a->k > 0 && a->rank > 0 && a->adapters > 0 ? adapter_bytes(*a) : 0;
 }
 
 extern "C" int fie_adapter_linear(const fie_adapter_args* a, void* stream)

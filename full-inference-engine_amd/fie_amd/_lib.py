@@ -61,8 +61,8 @@ class VerifyArgs(ctypes.Structure):
 NORM_ARGS = "@10P6q9i3f0q"
 INT8_ARGS = "@6P4q4iPN0q"
 BEAM_ARGS = "@15PqPNd8i18i0q"
-ADAPTER_ARGS = "@10PN3q12i0q"
-ADAPTER_PLAN_ARGS = "@2P4i0q"
+ADAPTER_ARGS = "@10PN3q10i0q"
+ADAPTER_PLAN_ARGS = "@2P2i0q"
 PAGES_ARGS, GROUP_ARGS = "@PPN4i6P2i", "P3q4i"          # the head, and eight groups
 STATES_ARGS, STATE_ARGS = "@P2i", "2P4q"        # the head, and as many states as there are
 
@@ -144,7 +144,7 @@ def bind(lib) -> None:
             getattr(lib, name).restype = ctypes.c_int
     lib.fie_beam_workspace_size.argtypes = [ctypes.c_char_p]
     lib.fie_beam_workspace_size.restype = ctypes.c_size_t
-    lib.fie_adapter_plan_ints.argtypes = [ctypes.c_int32] * 3
+    lib.fie_adapter_plan_ints.argtypes = [ctypes.c_int32] * 2
     lib.fie_adapter_workspace_size.argtypes = [ctypes.c_char_p]
     lib.fie_adapter_plan_ints.restype = lib.fie_adapter_workspace_size.restype = ctypes.c_size_t
     lib.fie_pages_state_ints.argtypes = [ctypes.c_int32] * 3

@@ -37,18 +37,16 @@ class AdapterPlan:
         if self.index < 0:
             raise ValueError("adapters run on a HIP device")
         self.tokens, self.adapters = ids.shape[0], adapters
-        # tiles of a decode step's few tokens an adapter, or of a prompt's many
-        self.tile = 16 if self.tokens <= 16 * adapters or self.tokens <= 512 else 64
         ids = ids.contiguous()
         lib = _lib.load()
-        n = lib.fie_adapter_plan_ints(self.tokens, adapters, self.tile)
+        n = lib.fie_adapter_plan_ints(self.tokens, adapters)
         if not n:
             raise ValueError(f"{self.tokens} tokens of {adapters} adapters are more than one call takes")
         self.data = torch.empty(n, dtype=torch.int32, device=ids.device)
         global _run_plan
         if _run_plan is None:
             _run_plan = _lib.launcher("fie_adapter_plan")
-        _run_plan(self.index, _pack_plan(ids.data_ptr(), self.data.data_ptr(), self.tokens, adapters, self.tile, 0))
+        _run_plan(self.index, _pack_plan(ids.data_ptr(), self.data.data_ptr(), self.tokens, adapters))
         self._made_on = torch._C._cuda_getCurrentRawStream(self.index)
 
     def on_stream(self) -> None:
@@ -164,7 +162,7 @@ def adapter_linear(x: torch.Tensor, bank: AdapterBank, plan: AdapterPlan, *, x_s
             b_stride = y_stride
         args = [x.data_ptr(), xs, bank.a.data_ptr(), bank.b.data_ptr(), bank.scale.data_ptr(), bank.ranks.data_ptr(),
                 plan.data.data_ptr(), bp, yp, 0, 0, x.stride(0), b_stride, y_stride, tokens, k, n, bank.adapters, bank.rank_pad,
-                bank.k_pad, plan.tile, code, x_code, _DTYPES[dtype], b_code, 0]
+                bank.k_pad, code, x_code, _DTYPES[dtype], b_code]
         args[10] = _size(_pack(*args))
         room = torch.empty(args[10], dtype=torch.uint8, device=y.device)
         args[9] = room.data_ptr()

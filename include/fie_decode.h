@@ -140,15 +140,15 @@ int fie_pages_copy(const fie_pages_args* args, void* stream);
 #define FIE_ADAPTER_K 64        /* rows of a are padded with zeros to a multiple of so many */
 #define FIE_ADAPTER_RANK 16     /* ranks likewise, in a and b */
 
-/* Whose tokens are whose: tokens by adapter, cut into tiles of `tile` (16 or 64) tokens.  plan is
+/* Whose tokens are whose: tokens by adapter, in tiles of up to 16.  plan is
    fie_adapter_plan_ints() of int32. */
 typedef struct fie_adapter_plan_args {
     const int32_t* ids;         /* [tokens] */
     int32_t* plan;
-    int32_t tokens, adapters, tile, reserved;
+    int32_t tokens, adapters;
 } fie_adapter_plan_args;
 
-size_t fie_adapter_plan_ints(int32_t tokens, int32_t adapters, int32_t tile);
+size_t fie_adapter_plan_ints(int32_t tokens, int32_t adapters);
 int fie_adapter_plan(const fie_adapter_plan_args* args, void* stream);
 
 typedef struct fie_adapter_args {
@@ -165,10 +165,9 @@ typedef struct fie_adapter_args {
     size_t workspace_bytes;
     int64_t x_stride, base_stride, y_stride;        /* elements between rows */
     int32_t tokens, k, n, adapters;
-    int32_t rank, k_pad, tile;  /* rank a multiple of FIE_ADAPTER_RANK, k_pad of FIE_ADAPTER_K */
+    int32_t rank, k_pad;        /* rank a multiple of FIE_ADAPTER_RANK, k_pad of FIE_ADAPTER_K */
     int32_t dtype, x_dtype;     /* the adapters' type; x's: that or FIE_I8 */
     int32_t y_dtype, base_dtype;        /* dtype or FIE_F32; y_dtype or FIE_F32 */
-    int32_t reserved;
 } fie_adapter_args;
 
 size_t fie_adapter_workspace_size(const fie_adapter_args* args);
