@@ -1,6 +1,7 @@
 // Beam search's selection (fie_beam_step): the best continuations of a request's beams.
 #pragma once
 
+#include "copy.h"
 #include "launchers.h"
 #include "fie_decode.h"
 
@@ -32,7 +33,7 @@ FIE_DEV float beam_clean(float x) { return x != x ? -__builtin_inff() : __builti
 
 template <int DT> struct BeamVec {                      // 16 bytes of logits
     static constexpr int N = DT == FIE_F32 ? 4 : 8;
-    static FIE_DEV void open(const uint4& r, float* x)
+    static FIE_DEV void open(const vec4_t& r, float* x)
     {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -70,27 +71,27 @@ FIE_DEV bool beam_dead(const fie_beam_args& a, int row)
 // are outside the row count as -inf (no vector without some of the row is touched).
 template <int DT> struct BeamRow {
     static constexpr int N = BeamVec<DT>::N, LOADS = kBeamEach / N;
-    const uint4* base;
+    const vec4_t* base;
     int shift, vocab, vecs;
     FIE_DEV BeamRow(const fie_beam_args& a, int row)
     {
         constexpr int SZ = 16 / N;
         const uintptr_t p = (uintptr_t)a.logits + (uintptr_t)((int64_t)row * a.row_stride * SZ);
-        base = (const uint4*)(p & ~(uintptr_t)15);
+        base = (const vec4_t*)(p & ~(uintptr_t)15);
         shift = (int)(p & 15) / SZ;
         vocab = a.vocab;
         vecs = (shift + vocab + N - 1) / N;
     }
-    FIE_DEV void load(int tile, uint4 (&r)[LOADS]) const
+    FIE_DEV void load(int tile, vec4_t (&r)[LOADS]) const
     {
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) r[j] = base[min((tile * LOADS + j) * kBeamThreads + (int)threadIdx.x, vecs - 1)];
+        for (int j = 0; j < LOADS; ++j) r[j] = global_get<vec4_t>(base + min((tile * LOADS + j) * kBeamThreads + (int)threadIdx.x, vecs - 1));
     }
     FIE_DEV int index(int tile, int e) const            // of the thread's e-th logit of a tile
     {
         return ((tile * LOADS + e / N) * kBeamThreads + (int)threadIdx.x) * N + e % N - shift;
     }
-    FIE_DEV void open(int tile, const uint4 (&r)[LOADS], float (&x)[kBeamEach]) const
+    FIE_DEV void open(int tile, const vec4_t (&r)[LOADS], float (&x)[kBeamEach]) const
     {
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) BeamVec<DT>::open(r[j], x + j * N);
@@ -125,7 +126,7 @@ __device__ __noinline__ int beam_deep(const BeamRow<DT>& row, int first, int las
         for (int j = first * LOADS; j < min(last * LOADS, (row.vecs + kBeamThreads - 1) / kBeamThreads); ++j) {
             const int v = j * kBeamThreads + tid;
             float x[N];
-            BeamVec<DT>::open(row.base[min(v, row.vecs - 1)], x);
+            BeamVec<DT>::open(global_get<vec4_t>(row.base + min(v, row.vecs - 1)), x);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const int i = v * N + e - row.shift;
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_scan(const fie_beam_args 
     const int rank = (w.most + kBeamWaves - 1) / kBeamWaves;
     float top = -kLargest, bound = -__builtin_inff();
     double sum = 0.0;
-    uint4 raw[LOADS];
+    vec4_t raw[LOADS];
     row.load(first, raw);
     for (int t = first; t < last; ++t) {
         float x[kBeamEach];

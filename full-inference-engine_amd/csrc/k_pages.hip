@@ -37,7 +37,9 @@ static PageScratch page_scratch(void* p, int64_t pages, int64_t rows, size_t* by
 
 static int64_t chunks_of(const fie_pages_args& a, const fie_cache_group& g)
 {
-    return ((g.whole ? 1 : a.page) * g.token_bytes + 15 + kCopyChunk - 1) / kCopyChunk;
+    const int64_t bytes = (g.whole ? 1 : a.page) * g.token_bytes;
+    // pieces that begin at 16-byte blocks need no chunk more than their bytes
+    return (bytes + (g.shift ? 15 : 0) + kCopyChunk - 1) / kCopyChunk;
 }
 
 static int pages_check(const fie_pages_args* a, bool table)
@@ -50,7 +52,7 @@ static int pages_check(const fie_pages_args* a, bool table)
         const fie_cache_group& g = a->group[i];
         if (g.count < 0 || g.outer < 1 || g.token_bytes < 1 || g.token_bytes > 1 << 30 || (g.count && !g.base))
             return fail(FIE_E_ARG, "a cache group's layout is out of range");
-        if (g.outer * chunks_of(*a, g) > 1 << 24)
+        if (g.count * g.outer * chunks_of(*a, g) > 1 << 24)
             return fail(FIE_E_ARG, "a cache group's pages are too large");
     }
     if (!table) return FIE_OK;
@@ -71,8 +73,10 @@ static hipError_t copy_pages(const fie_pages_args& a, const PageList& l, int64_t
         const fie_cache_group& g = a.group[i];
         if (!g.count || !most) continue;
         const int chunks = (int)chunks_of(a, g);
-        const int64_t items = most * g.count * g.outer * chunks;
-        k_pages_copy<<<(unsigned)std::min<int64_t>(items, 8 * std::max(cu_count(), 1)), kCopyThreads, 0, st>>>(l, g, a.page, chunks);
+        const int64_t pieces = (int64_t)g.count * g.outer * chunks;
+        // as many copies side by side as fill the CUs
+        const int64_t side = std::min<int64_t>({most, 65535, std::max<int64_t>(1, (8 * std::max(cu_count(), 1) + pieces - 1) / pieces)});
+        k_pages_copy<<<dim3((unsigned)pieces, (unsigned)side), kCopyThreads, 0, st>>>(l, g, a.page, chunks);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     return hipSuccess;

@@ -304,20 +304,17 @@ struct PageList {
     int n, pages;                   // so many
 };
 
-// Pieces of pages, `units` for each copy and cache of one layout, dealt to the grid's workgroups.
+// Pieces of pages of one layout: grid (pieces of a page in all caches, copies or fewer).
 __global__ __launch_bounds__(kCopyThreads) void k_pages_copy(const PageList l, const fie_cache_group g, int page, int chunks)
 {
     const int n = l.count ? *l.count : l.n;
     const int per = g.outer * chunks;
-    const int64_t items = (int64_t)n * g.count * per;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t one = item / per;
-        const int unit = (int)(item - one * per), i = (int)(one / g.count), c = (int)(one - (int64_t)i * g.count);
+    const int c = blockIdx.x / per, unit = blockIdx.x - c * per, piece = unit / chunks, chunk = unit - piece * chunks;
+    uint8_t* const base = (uint8_t*)g.base[c] + piece * g.outer_stride;
+    for (int i = blockIdx.y; i < n; i += gridDim.y) {
         const PageCopy p = l.copies ? l.copies[i] : PageCopy{l.src[i], l.dst[i], page};
-        if (p.src < 0 || p.src >= l.pages || p.dst < 0 || p.dst >= l.pages || p.src == p.dst) continue;
-        const int64_t bytes = g.whole ? g.token_bytes : p.fill * g.token_bytes;
-        uint8_t* base = (uint8_t*)g.base[c] + (unit / chunks) * g.outer_stride;
-        copy_chunk(base + p.dst * g.page_stride, base + p.src * g.page_stride, bytes, unit % chunks);
+        if ((uint32_t)p.src >= (uint32_t)l.pages || (uint32_t)p.dst >= (uint32_t)l.pages || p.src == p.dst) continue;
+        copy_chunk(base + p.dst * g.page_stride, base + p.src * g.page_stride, g.whole ? g.token_bytes : p.fill * g.token_bytes, chunk);
     }
 }
 

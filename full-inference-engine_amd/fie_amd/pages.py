@@ -113,7 +113,8 @@ class CachePages:
             raise ValueError(f"caches of more than {MAX_GROUPS} layouts")
         for (stride, outer_stride, token, outer, whole), tensors in groups.items():
             base = torch.tensor([t.data_ptr() for t in tensors], dtype=torch.int64).to(self.device)
-            self._groups.append(((stride, outer_stride, token, len(tensors), outer, whole, 0), tensors, base))
+            shift = int(any(v % 16 for v in (stride, outer_stride, *(t.data_ptr() for t in tensors))))
+            self._groups.append(((stride, outer_stride, token, len(tensors), outer, whole, shift), tensors, base))
         self._packed = None
 
     _packed: list | None = None

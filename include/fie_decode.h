@@ -94,7 +94,8 @@ int fie_reorder_states(const fie_states_args* args, void* stream);
 typedef struct fie_cache_group {
     void* const* base;          /* [count] on the device */
     int64_t page_stride, outer_stride, token_bytes;
-    int32_t count, outer, whole, reserved;
+    int32_t count, outer, whole;
+    int32_t shift;              /* 0: every base and stride is a multiple of 16 */
 } fie_cache_group;
 
 #define FIE_MAX_CACHE_GROUPS 8
