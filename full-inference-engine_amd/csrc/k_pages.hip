@@ -24,9 +24,7 @@ static PageState page_state(const fie_pages_args& a)
 static PageScratch page_scratch(void* p, int64_t pages, int64_t rows, size_t* bytes)
 {
     PageScratch w;
-    w.mark = (uint64_t*)p;
-    w.writers = (int32_t*)(w.mark + pages);
-    w.list = w.writers + pages;
+    w.list = (int32_t*)p;
     w.movers = w.list + pages;
     w.order = w.movers + pages;
     w.copies = (PageCopy*)(w.order + pages);
@@ -45,7 +43,7 @@ static int64_t chunks_of(const fie_pages_args& a, const fie_cache_group& g)
 static int pages_check(const fie_pages_args* a, bool table)
 {
     if (!a) return fail(FIE_E_ARG, "args is NULL");
-    if (a->pages < 1 || a->pages > FIE_MAX_PAGES) return fail(FIE_E_ARG, "pages out of range [1, 4194304]");
+    if (a->pages < 1 || a->pages > FIE_MAX_PAGES) return fail(FIE_E_ARG, "pages out of range [1, 2097152]");
     if (a->page < 1 || a->page > 65536) return fail(FIE_E_ARG, "page out of range [1, 65536]");
     if (a->group_count < 0 || a->group_count > FIE_MAX_CACHE_GROUPS) return fail(FIE_E_ARG, "group_count out of range [0, 8]");
     for (int i = 0; i < a->group_count; ++i) {
@@ -82,15 +80,28 @@ static hipError_t copy_pages(const fie_pages_args& a, const PageList& l, int64_t
     return hipSuccess;
 }
 
+constexpr int kSmallTable = 8192;       // entries of a table that one workgroup forks
+
 static hipError_t pages_step(const fie_pages_args& a, hipStream_t st)
 {
     const PageState s = page_state(a);
     const PageScratch w = page_scratch(a.scratch, a.pages, a.rows, nullptr);
-    const size_t fork = (size_t)a.rows * (4 * kForkCols + 4 + 2);
-    k_pages_fork<<<(unsigned)((a.wide + kForkCols - 1) / kForkCols), kForkThreads, fork, st>>>(s, a.parents, a.lengths);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    k_pages_grow<<<1, kGrowThreads, (size_t)(2 * a.rows + s.nblocks) * 4, st>>>(s, w, a.parents, a.lengths, a.granted);
+    const bool small = (int64_t)a.rows * a.wide <= kSmallTable;
+    const bool moves = a.parents || a.lengths;          // whether any entry may change
+    hipError_t e;
+    if (!small && moves) {
+        const int cols = a.rows <= 1024 ? 8 : 4;
+        const size_t lds = (size_t)a.rows * (4 * cols + 4 + 2) + 4 * (size_t)s.nblocks;
+        const unsigned grid = (unsigned)((a.wide + cols - 1) / cols);
+        if (cols == 8) k_pages_fork<8><<<grid, kPageThreads, lds, st>>>(s, a.parents, a.lengths);
+        else k_pages_fork<4><<<grid, kPageThreads, lds, st>>>(s, a.parents, a.lengths);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    const int bits = mark_bits(a.rows);
+    const size_t area = std::max<size_t>(small ? (size_t)a.rows * a.wide : 0, (size_t)3 << bits);
+    const size_t lds = ((size_t)3 * a.rows + s.nblocks + area) * 4;
+    if (small) k_pages_grow<true><<<1, kPageThreads, lds, st>>>(s, w, a.parents, a.lengths, a.granted, bits, (int)area);
+    else k_pages_grow<false><<<1, kPageThreads, lds, st>>>(s, w, a.parents, a.lengths, a.granted, bits, (int)area);
     e = hipGetLastError();
     if (e != hipSuccess || !a.lengths) return e;
     return copy_pages(a, PageList{w.copies, nullptr, nullptr, w.count, 0, a.pages}, a.rows, st);
@@ -100,7 +111,7 @@ static hipError_t pages_compact(const fie_pages_args& a, hipStream_t st)
 {
     const PageState s = page_state(a);
     const PageScratch w = page_scratch(a.scratch, a.pages, a.rows, nullptr);
-    k_pages_holes<<<(unsigned)s.nblocks, kGrowThreads, 0, st>>>(s, w, a.live);
+    k_pages_holes<<<(unsigned)s.nblocks, kPageThreads, 0, st>>>(s, w, a.live);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int64_t entries = std::max((int64_t)a.rows * a.wide, (int64_t)a.pages / 2);

@@ -8,8 +8,7 @@
 namespace fie {
 
 constexpr int kPageBlock = 1024;                        // pages of one count of free ones
-constexpr int kForkThreads = 1024, kForkCols = 8;
-constexpr int kGrowThreads = 1024;
+constexpr int kPageThreads = 1024;
 
 // The state's parts.
 struct PageState {
@@ -21,10 +20,7 @@ struct PageCopy {
     int32_t src, dst, fill;             // fill: tokens
 };
 
-// The scratch's: `mark` and `writers` are 0 between calls.
 struct PageScratch {
-    uint64_t* mark;             // [pages] a last page's longest writer, then lowest
-    int32_t* writers;           // [pages] rows that grow from it
     int32_t* list;              // [pages] free pages in order; compacting: holes
     int32_t* movers;            // [pages] compacting: used pages past the count, and
     int32_t* order;             // [pages] their numbers among those
@@ -45,162 +41,253 @@ FIE_DEV int page_held(const PageState& s, const int32_t* lengths, int i, int par
     return lengths ? max(0, min(lengths[i], have)) : have;
 }
 
-// A workgroup kForkCols columns of all rows: its table entries go through LDS, so that rows may
+// C columns from c0 on, or (C 0) all columns, of all rows' tables go through LDS (`tile`), so that rows may
 // take each other's.  A page is in one column of all rows that hold it, so one workgroup sees all
-// changes to its count: what is added first, then, behind a barrier, what is taken; a count
-// that gets to 0 is a page set free.  Dynamic LDS: [rows][kForkCols] entries, [rows] pages kept,
-// [rows] parents.
-__global__ __launch_bounds__(kForkThreads) void k_pages_fork(const PageState s, const int32_t* parents, const int32_t* lengths)
+// changes to its count: what is added first, then, behind a barrier, what is taken; a count that
+// gets to 0 is a page set free, counted by blocks in LDS (`freed`, [nblocks]).
+template <int C>
+FIE_DEV void fork_columns(const PageState& s, const int32_t* parents, const int32_t* lengths, int c0,
+                          int32_t* tile, int32_t* keep, uint16_t* from, int32_t* freed)
 {
-    extern __shared__ int32_t L[];
-    int32_t* const tile = L;
-    int32_t* const keep = L + s.rows * kForkCols;
-    uint16_t* const from = (uint16_t*)(keep + s.rows);
-    const int tid = threadIdx.x, c0 = blockIdx.x * kForkCols, n = s.rows * kForkCols;
-    for (int i = tid; i < n; i += kForkThreads) {
-        const int c = c0 + i % kForkCols;
-        tile[i] = c < s.wide ? s.table[(int64_t)(i / kForkCols) * s.wide + c] : -1;
-    }
-    for (int i = tid; i < s.rows; i += kForkThreads) {
+    const int tid = threadIdx.x, pitch = C ? C : s.wide;
+    auto each = [&](auto&& f) {                         // f(row, column)
+        if constexpr (C > 0) {
+#pragma unroll 2
+            for (int i = tid; i < s.rows * C; i += kPageThreads) f(i / C, i % C);
+        } else {
+#pragma unroll 1
+            for (int row = tid >> 6; row < s.rows; row += kPageThreads / 64)
+#pragma unroll 1
+                for (int c = tid & 63; c < s.wide; c += 64) f(row, c);
+        }
+    };
+    each([&](int row, int c) { tile[row * pitch + c] = c0 + c < s.wide ? s.table[(int64_t)row * s.wide + c0 + c] : -1; });
+#pragma unroll 1
+    for (int i = tid; i < s.rows; i += kPageThreads) {
         const int p = page_parent(parents, i, s.rows);
-        const int held = page_held(s, lengths, i, p);
-        keep[i] = (int)(((int64_t)held + s.page - 1) / s.page);
+        keep[i] = (int)(((uint32_t)page_held(s, lengths, i, p) + (uint32_t)s.page - 1u) / (uint32_t)s.page);
         from[i] = (uint16_t)(p < 0 ? i : p);            // without a parent nothing is kept
     }
+#pragma unroll 1
+    for (int i = tid; i < s.nblocks; i += kPageThreads) freed[i] = 0;
     __syncthreads();
-    auto fresh = [&](int i) {
-        const int row = i / kForkCols, c = i % kForkCols;
-        return c0 + c < keep[row] ? tile[(int)from[row] * kForkCols + c] : -1;
-    };
-    for (int i = tid; i < n; i += kForkThreads) {
-        const int was = tile[i], is = fresh(i);
-        if (was == is) continue;
-        s.table[(int64_t)(i / kForkCols) * s.wide + c0 + i % kForkCols] = is;
+    auto fresh = [&](int row, int c) { return c0 + c < keep[row] ? tile[(int)from[row] * pitch + c] : -1; };
+    each([&](int row, int c) {
+        const int is = fresh(row, c);
+        if (tile[row * pitch + c] == is) return;
+        s.table[(int64_t)row * s.wide + c0 + c] = is;
         if (is >= 0) atomicAdd(&s.refs[is], 1);
-    }
-    __threadfence();
-    __syncthreads();
-    for (int i = tid; i < n; i += kForkThreads) {
-        const int was = tile[i];
-        if (was == fresh(i) || was < 0) continue;
-        if (atomicAdd(&s.refs[was], -1) == 1) atomicAdd(&s.blocks[was / kPageBlock], 1);
-    }
+    });
+    __syncthreads();                                    // (a workgroup's own order is enough, and far cheaper than the device's)
+    each([&](int row, int c) {
+        const int was = tile[row * pitch + c];
+        if (was >= 0 && was != fresh(row, c) && atomicAdd(&s.refs[was], -1) == 1) atomicAdd(&freed[was / kPageBlock], 1);
+    });
 }
 
-FIE_DEV int32_t fresh_load(const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-FIE_DEV uint64_t fresh_load(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// A workgroup C columns of all rows.  Dynamic LDS: [rows][C] entries, [rows] pages kept, [nblocks],
+// [rows] parents.
+template <int C>
+__global__ __launch_bounds__(kPageThreads) void k_pages_fork(const PageState s, const int32_t* parents, const int32_t* lengths)
+{
+    extern __shared__ int32_t L[];
+    int32_t* const keep = L + s.rows * C;
+    int32_t* const freed = keep + s.rows;
+    fork_columns<C>(s, parents, lengths, blockIdx.x * C, L, keep, (uint16_t*)(freed + s.nblocks), freed);
+    __syncthreads();
+#pragma unroll 1
+    for (int b = threadIdx.x; b < s.nblocks; b += kPageThreads)
+        if (freed[b]) atomicAdd(&s.blocks[b], freed[b]);
+}
 
-// Exclusive prefix sum over the threads of a workgroup of 1024, sums past 2^30 as 2^30 (a wave's
-// own are below 2^31); *total the sum.  `part` [16].
+// Exclusive prefix sums over the threads of a workgroup of 1024, sums past 2^30 as 2^30 (a wave's
+// own are below 2^31); all the sums.  `part` [16].
 constexpr int kScanMost = 1 << 30;
-FIE_DEV int block_scan(int v, int32_t* part, int* total)
+FIE_DEV int block_scan(int v, int32_t* part, int* all)
 {
     const int wave = threadIdx.x >> 6;
     const int incl = (int)wave_incl_scan_u32((uint32_t)v);
     __syncthreads();                                    // part may still be read from before
     if ((threadIdx.x & 63) == 63) part[wave] = incl;
     __syncthreads();
-    int64_t before = 0, all = 0;
+    int64_t before = 0, sum = 0;
 #pragma unroll
     for (int w = 0; w < 16; ++w) {
         const int t = part[w];
         before += w < wave ? t : 0;
-        all += t;
+        sum += t;
     }
-    *total = (int)min(all, (int64_t)kScanMost);
+    *all = (int)min(sum, (int64_t)kScanMost);
     return (int)min(before + incl - v, (int64_t)kScanMost);
+}
+
+// Last pages that rows grow from and others hold, by their number: how many rows grow from each, and
+// the longest of these, then lowest (`slots` a power of two past 1.5 times the rows).
+struct PageMarks {
+    int32_t *key, *count;
+    uint32_t* best;
+    int bits;
+    FIE_DEV int slot(int p) const { return (int)(((uint32_t)p * 0x9E3779B1u) >> (32 - bits)); }
+    FIE_DEV void clear() const
+    {
+#pragma unroll 1
+        for (int i = threadIdx.x; i < 1 << bits; i += kPageThreads) {
+            key[i] = -1;
+            count[i] = 0;
+            best[i] = 0;
+        }
+    }
+    FIE_DEV void add(int p, uint32_t code) const
+    {
+        int i = slot(p);
+#pragma unroll 1
+        for (;; i = (i + 1) & ((1 << bits) - 1)) {
+            const int was = atomicCAS(&key[i], -1, p);
+            if (was == -1 || was == p) break;
+        }
+        atomicAdd(&count[i], 1);
+        atomicMax(&best[i], code);
+    }
+    FIE_DEV int find(int p) const
+    {
+        int i = slot(p);
+#pragma unroll 1
+        while (key[i] != p) i = (i + 1) & ((1 << bits) - 1);
+        return i;
+    }
+};
+
+// Dynamic LDS of k_pages_grow in ints: held, keep, end [rows], base [nblocks]; then the marks, and in
+// their place later the list of free pages (or, with FORK, the table's tile before them).
+static inline int mark_bits(int rows)
+{
+    int b = 4;
+    while ((1 << b) < rows + rows / 2) ++b;
+    return b;
 }
 
 // One workgroup: which rows grow, which last pages are copied, and which pages they get.  The free
 // pages are found by the counts of their blocks, so only blocks are read that have some of the
-// wanted.  Dynamic LDS: [rows] tokens held, [rows] pages wanted up to and with a row, [nblocks].
-__global__ __launch_bounds__(kGrowThreads) void k_pages_grow(const PageState s, const PageScratch w, const int32_t* parents,
-                                                             const int32_t* lengths, uint8_t* granted)
+// wanted.  FORK: a small table's rows take their parents' pages first, by the same workgroup (4 x 37: 6 us
+// and a launch less).  A chain of dependent steps through memory: parents, lengths, a row's last
+// page, its count, the blocks' pages.
+template <bool FORK>
+__global__ __launch_bounds__(kPageThreads) void k_pages_grow(const PageState s, const PageScratch w, const int32_t* parents,
+                                                             const int32_t* lengths, uint8_t* granted, int bits, int room)
 {
     extern __shared__ int32_t L[];
     __shared__ int32_t part[16];
     __shared__ int32_t copies;
     int32_t* const held = L;
-    int32_t* const end = held + s.rows;
+    int32_t* const keep = held + s.rows;
+    int32_t* const end = keep + s.rows;
     int32_t* const base = end + s.rows;
-    const int tid = threadIdx.x;
-    const int each = (s.rows + kGrowThreads - 1) / kGrowThreads, first = tid * each, last = min(first + each, s.rows);
+    int32_t* const area = base + s.nblocks;
+    const PageMarks marks{area, area + (1 << bits), (uint32_t*)(area + (2 << bits)), bits};
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int each = (s.rows + kPageThreads - 1) / kPageThreads, first = tid * each, last = min(first + each, s.rows);
     if (tid == 0) copies = 0;
-    for (int i = tid; i < s.rows; i += kGrowThreads) held[i] = page_held(s, lengths, i, page_parent(parents, i, s.rows));
-    __syncthreads();
-    auto wants = [&](int i) { return lengths ? max(lengths[i], held[i]) : held[i]; };
-    auto fits = [&](int want) { return (int64_t)want <= (int64_t)s.wide * s.page; };
-    auto up = [&](int tokens) { return (int)(((int64_t)tokens + s.page - 1) / s.page); };
-    auto part_page = [&](int i, int want) {             // a last page that is not full and is to be written
-        return want > held[i] && fits(want) && held[i] % s.page ? s.table[(int64_t)i * s.wide + held[i] / s.page] : -1;
-    };
-    auto key_of = [&](int i) { return ((uint64_t)(uint32_t)(held[i] % s.page) << 32) | (uint32_t)(s.rows - i); };
-    for (int i = first; i < last; ++i) {
-        const int p = part_page(i, wants(i));
-        if (p >= 0) {
-            atomicAdd(&w.writers[p], 1);
-            atomicMax((unsigned long long*)&w.mark[p], (unsigned long long)key_of(i));
-        }
+    if constexpr (FORK) {
+        fork_columns<0>(s, parents, lengths, 0, area, keep, (uint16_t*)end, base);
+        __syncthreads();
     }
-    __threadfence();
-    __syncthreads();
-    // what each row wants; end[] holds its sign bit for a copy until the rows' sums are there
-    int mine = 0;
+    const uint32_t page = (uint32_t)s.page;
+    auto wants = [&](int i) { return lengths ? max(lengths[i], held[i]) : held[i]; };
+    auto up = [&](int tokens) { return (int)(((uint32_t)tokens + page - 1u) / page); };
+    // each thread's rows: what is held, and a last page that is not full, is to be written and that
+    // others hold
+#pragma unroll 1
     for (int i = first; i < last; ++i) {
-        const int want = wants(i), p = part_page(i, want);
-        const bool copy = p >= 0 && !(fresh_load(&w.writers[p]) == fresh_load(&s.refs[p]) && fresh_load(&w.mark[p]) == key_of(i));
-        const int demand = want > held[i] && fits(want) ? up(want) - up(held[i]) + copy : 0;
+        const int h = page_held(s, lengths, i, page_parent(parents, i, s.rows));
+        held[i] = h;
+        keep[i] = up(h);
+    }
+    if (lengths) marks.clear();
+    __syncthreads();
+#pragma unroll 1
+    for (int i = first; i < last; ++i) {
+        const int h = held[i], want = wants(i), fill = h - max(keep[i] - 1, 0) * s.page;
+        int p = -1;
+        if (want > h && up(want) <= s.wide && fill < s.page && h) {
+            p = s.table[(int64_t)i * s.wide + keep[i] - 1];
+            if (s.refs[p] > 1) marks.add(p, ((uint32_t)fill << 13) | (uint32_t)(s.rows - i));
+            else p = -1;
+        }
+        end[i] = p;
+    }
+    __syncthreads();
+    // what each row wants, a copy in the sign bit
+    int mine = 0;
+#pragma unroll 1
+    for (int i = first; i < last; ++i) {
+        const int h = held[i], want = wants(i), fill = h - max(keep[i] - 1, 0) * s.page, p = end[i];
+        bool copy = false;
+        if (p >= 0) {
+            const int m = marks.find(p);
+            copy = !(marks.count[m] == s.refs[p] && marks.best[m] == (((uint32_t)fill << 13) | (uint32_t)(s.rows - i)));
+        }
+        const int demand = want > h && up(want) <= s.wide ? up(want) - keep[i] + copy : 0;
         end[i] = demand | (copy ? (int)0x80000000 : 0);
         mine += demand;
     }
-    int all;
-    int at = block_scan(mine, part, &all);
+    int sum;
+    int at = block_scan(mine, part, &sum);
     // where the free pages of each block begin
     int free = 0;
-    for (int b0 = 0; b0 < s.nblocks; b0 += kGrowThreads) {
+#pragma unroll 1
+    for (int b0 = 0; b0 < s.nblocks; b0 += kPageThreads) {
         const int b = b0 + tid;
-        const int v = b < s.nblocks ? fresh_load(&s.blocks[b]) : 0;
-        int sum;
+        const int v = b < s.nblocks ? s.blocks[b] + (FORK ? base[b] : 0) : 0;
         const int before = block_scan(v, part, &sum);
         if (b < s.nblocks) base[b] = free + before;
         free += sum;
     }
     int need = 0;                                       // pages that are given out
+#pragma unroll 1
     for (int i = first; i < last; ++i) {
         const int demand = end[i] & 0x7FFFFFFF;
         at += demand;
         if (demand && at <= free) need = at;
         end[i] = at | (end[i] & (int)0x80000000);
     }
-    for (int d = 32; d; d >>= 1) need = max(need, __shfl_xor(need, d, 64));
+    need = (int)wave_max_u32((uint32_t)need);
     __syncthreads();
-    if ((tid & 63) == 0) part[tid >> 6] = need;
+    if (lane == 0) part[tid >> 6] = need;
     __syncthreads();
 #pragma unroll
     for (int v = 0; v < 16; ++v) need = max(need, part[v]);
-    // the first `need` free pages, a wave a block
-    const int lane = tid & 63;
-    for (int b = __builtin_amdgcn_readfirstlane(tid >> 6); b < s.nblocks && base[b] < need; b += kGrowThreads / 64) {
+    // the first `need` free pages, a wave a block; the blocks' counts without them
+    int32_t* const list = need <= room ? area : w.list;
+#pragma unroll 1
+    for (int b = __builtin_amdgcn_readfirstlane(tid >> 6); b < s.nblocks && base[b] < need; b += kPageThreads / 64) {
         const int next = b + 1 < s.nblocks ? base[b + 1] : free;
         if (next == base[b]) continue;
         int rank = base[b];
         uint32_t is = 0;                                // bit j: page 64 j + lane is free
 #pragma unroll
+        for (int j = 0; j < kPageBlock / 64; ++j) is |= (uint32_t)(s.refs[min(b * kPageBlock + j * 64 + lane, s.pages - 1)] == 0) << j;
+#pragma unroll 1
         for (int j = 0; j < kPageBlock / 64; ++j) {
             const int p = b * kPageBlock + j * 64 + lane;
-            if (p < s.pages && fresh_load(&s.refs[p]) == 0) is |= 1u << j;
-        }
-#pragma unroll
-        for (int j = 0; j < kPageBlock / 64; ++j) {
-            const uint64_t m = __ballot((is >> j) & 1u);
+            const bool mine = ((is >> j) & 1u) && p < s.pages;
+            const uint64_t m = __ballot(mine);
             const int r = rank + (int)__popcll(m & ((1ull << lane) - 1ull));
-            if (((is >> j) & 1u) && r < need) w.list[r] = b * kPageBlock + j * 64 + lane;
+            if (mine && r < need) list[r] = p;
             rank += (int)__popcll(m);
+        }
+        if (!FORK && lane == 0) s.blocks[b] = next - min(next, need);
+    }
+    if constexpr (FORK) {
+#pragma unroll 1
+        for (int b = tid; b < s.nblocks; b += kPageThreads) {
+            const int next = b + 1 < s.nblocks ? base[b + 1] : free;
+            s.blocks[b] = next - max(base[b], min(next, need));
         }
     }
     __syncthreads();
     // a page for each that is wanted: the first row whose sum is past its number has it
-    for (int n = tid; n < need; n += kGrowThreads) {
+#pragma unroll 1
+    for (int n = tid; n < need; n += kPageThreads) {
         int lo = 0, hi = s.rows - 1;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
@@ -209,50 +296,40 @@ __global__ __launch_bounds__(kGrowThreads) void k_pages_grow(const PageState s, 
         }
         const int i = lo, before = i ? end[i - 1] & 0x7FFFFFFF : 0;
         const bool copy = end[i] < 0;
-        const int col = up(held[i]) + (n - before) - copy, p = w.list[n];
-        int32_t* to = s.table + (int64_t)i * s.wide + col;      // with a copy, the first is the last page itself
+        const int p = list[n];
+        int32_t* to = s.table + (int64_t)i * s.wide + keep[i] + (n - before) - copy;    // a copy's first is the last page itself
         if (copy && n == before) {
             const int was = *to;
-            atomicAdd(&s.refs[was], -1);                        // others hold it
-            w.copies[atomicAdd(&copies, 1)] = PageCopy{was, p, held[i] % s.page};
+            atomicAdd(&s.refs[was], -1);                // others hold it
+            w.copies[atomicAdd(&copies, 1)] = PageCopy{was, p, held[i] - (keep[i] - 1) * s.page};
         }
         *to = p;
         s.refs[p] = 1;
-        atomicAdd(&s.blocks[p / kPageBlock], -1);
     }
     __syncthreads();
-    // the marks go back to 0, the lengths out
+#pragma unroll 1
     for (int i = first; i < last; ++i) {
-        const int want = wants(i), sum = end[i] & 0x7FFFFFFF;
-        const bool copy = end[i] < 0, grow = want > held[i], fit = fits(want);
-        const bool gets = !grow || (fit && (sum <= free || up(want) - up(held[i]) + copy == 0));
-        if (grow && fit && held[i] % s.page && !(copy && gets)) {   // of a copied page the list has its number
-            const int p = s.table[(int64_t)i * s.wide + held[i] / s.page];
-            w.writers[p] = 0;
-            w.mark[p] = 0;
-        }
+        const int want = wants(i), u = up(want);
+        const bool grow = want > held[i];
+        const bool gets = !grow || (u <= s.wide && ((end[i] & 0x7FFFFFFF) <= free || u - keep[i] + (end[i] < 0) == 0));
         granted[i] = gets;
         s.lengths[i] = grow && gets ? want : held[i];
-    }
-    for (int n = tid; n < copies; n += kGrowThreads) {
-        w.writers[w.copies[n].src] = 0;
-        w.mark[w.copies[n].src] = 0;
     }
     if (tid == 0) *w.count = copies;
 }
 
 // A workgroup 1024 pages: free ones below the count of used pages are holes, used ones past it
 // move; both are numbered in order.
-__global__ __launch_bounds__(kGrowThreads) void k_pages_holes(const PageState s, const PageScratch w, int32_t* live)
+__global__ __launch_bounds__(kPageThreads) void k_pages_holes(const PageState s, const PageScratch w, int32_t* live)
 {
     __shared__ int32_t part[16];
     const int tid = threadIdx.x, block = blockIdx.x;
     int free = 0, before = 0;
-    for (int b = tid; b < s.nblocks; b += kGrowThreads) free += s.blocks[b];
+    for (int b = tid; b < s.nblocks; b += kPageThreads) free += s.blocks[b];
     block_scan(free, part, &free);
     const int used = s.pages - free, edge = used / kPageBlock;      // the block that the count falls into
     int below = 0;
-    for (int b = tid; b < s.nblocks; b += kGrowThreads) {
+    for (int b = tid; b < s.nblocks; b += kPageThreads) {
         before += b < block ? s.blocks[b] : 0;
         below += b < edge ? s.blocks[b] : 0;
     }

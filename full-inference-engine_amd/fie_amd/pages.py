@@ -26,7 +26,7 @@ _pack = struct.Struct(_lib.PAGES_ARGS + _lib.GROUP_ARGS * 8).pack
 _runs: dict[str, object] = {}           # the library's entries, loaded with the first call
 _raw_stream = torch._C._cuda_getCurrentRawStream
 MAX_ROWS = 4096
-MAX_PAGES = 1 << 22
+MAX_PAGES = 1 << 21
 MAX_GROUPS = 8
 
 
@@ -60,7 +60,7 @@ class CachePages:
         self.state = torch.zeros(lib.fie_pages_state_ints(pages, rows, max_pages), dtype=torch.int32, device=self.device)
         self.device, self._index = self.state.device, self.state.get_device()
         self.table, self.lengths, self.refs, self._blocks = self._parts(self.state)
-        self._scratch = torch.zeros(lib.fie_pages_scratch_bytes(pages, rows), dtype=torch.uint8, device=self.device)
+        self._scratch = torch.empty(lib.fie_pages_scratch_bytes(pages, rows), dtype=torch.uint8, device=self.device)
         self._made_on = _raw_stream(self._index)
         self._groups: list[tuple] = []          # (layout, tensors, their addresses on the device)
         self.table.fill_(-1)

@@ -84,10 +84,9 @@ int fie_reorder_states(const fie_states_args* args, void* stream);
      lengths [rows]         tokens
      refs   [pages]         table entries that hold the page; 0: free
      blocks [ceil(pages / 1024)]   free pages among each 1024
-   The scratch (fie_pages_scratch_bytes, 16-byte aligned) is zeroed once by the caller; calls
-   leave it so. */
+   The scratch (fie_pages_scratch_bytes, 16-byte aligned) holds nothing between calls. */
 #define FIE_MAX_PAGE_ROWS 4096
-#define FIE_MAX_PAGES (1 << 22)
+#define FIE_MAX_PAGES (1 << 21)
 
 /* Cache tensors of one layout: a page is `outer` pieces, outer_stride bytes apart, of `page`
    tokens of token_bytes one after another; with `whole` of token_bytes that go with the whole page. */
