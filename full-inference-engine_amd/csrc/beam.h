@@ -116,13 +116,15 @@ struct BeamShared {
 
 // The `need`-th best candidate of a span, exactly: radix passes over (key, index) that read the
 // span again, and at the end the `need` best into the list.  For spans whose candidates do not
-// fit the list (equal logits, or logits in rising order).
+// fit the list (equal logits, or logits in rising order).  (In line: a call takes stack in memory,
+// and with it 20 us between launches.)
 template <int DT>
-__device__ __noinline__ int beam_deep(const BeamRow<DT>& row, int first, int last, int most, BeamShared& S)
+FIE_DEV int beam_deep(const BeamRow<DT>& row, int first, int last, int most, BeamShared& S)
 {
     const int tid = threadIdx.x;
     auto each = [&](auto&& f) {
         constexpr int N = BeamRow<DT>::N, LOADS = BeamRow<DT>::LOADS;
+#pragma unroll 1
         for (int j = first * LOADS; j < min(last * LOADS, (row.vecs + kBeamThreads - 1) / kBeamThreads); ++j) {
             const int v = j * kBeamThreads + tid;
             float x[N];
@@ -148,6 +150,7 @@ __device__ __noinline__ int beam_deep(const BeamRow<DT>& row, int first, int las
     constexpr int kShift[5] = {53, 42, 32, 10, 0}, kBits[5] = {11, 11, 10, 10, 10};
     uint64_t prefix = 0;
     int left = need;
+#pragma unroll 1
     for (int p = 0; p < 5; ++p) {
         const int sh = kShift[p], bits = kBits[p], known = p == 3 ? 32 : sh + bits;     // bits 20..31 are the same in all
         if (p == 3) prefix |= 0xFFF00000u;
@@ -322,6 +325,15 @@ FIE_DEV double beam_value(uint64_t k)
     return __longlong_as_double((int64_t)((k >> 63) ? (k & 0x7FFFFFFFFFFFFFFFull) : ~k));
 }
 
+// length^penalty.  (The exponential and the logarithm as they are shared with a row's: a power's own code
+// takes longer to come in than to run.)
+FIE_DEV double beam_scale(int length, double penalty)
+{
+    if (penalty == 1.0) return (double)length;
+    if (penalty == 0.0) return 1.0;
+    return exp(penalty * log((double)length));
+}
+
 // A workgroup a request, a wave a row at first: the row's spans' lists are in order, so its best
 // candidates come off their heads one by one; then the request's, off its rows' lists, in one
 // wave with a beam a lane.  Bound by that chain: a few hundred cycles a candidate.
@@ -353,7 +365,7 @@ __global__ __launch_bounds__(1024) void k_beam_pick(const fie_beam_args a, const
         const BeamSpan sp = in ? w.span[(int64_t)row * w.spans + lane] : BeamSpan{0.0, -kLargest, 0};
         float m = sp.top;
         for (int d = 32; d; d >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d, 64));
-        double s = sp.sum > 0.0 ? sp.sum * exp((double)sp.top - (double)m) : 0.0;
+        double s = sp.sum * __builtin_amdgcn_exp2f((sp.top - m) * kLog2e);
         for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
         const uint64_t* from = w.cand + (int64_t)row * w.spans * most;
         for (int i = lane; i < w.spans * most; i += 64) heads[i] = from[i];
@@ -381,7 +393,7 @@ __global__ __launch_bounds__(1024) void k_beam_pick(const fie_beam_args a, const
         for (int i = 0; i < 3; ++i) old_end[threadIdx.x][i] = a.ends[(r * K + threadIdx.x) * 3 + i];
     }
     __syncthreads();
-    const double scale = pow((double)max(was ? length : length + 1, 1), a.length_penalty);
+    const double scale = beam_scale(max(was ? length : length + 1, 1), a.length_penalty);
     if (wave == 0) {
         const bool mine = lane < K && counts[lane] > 0;
         const double prior = mine ? (double)a.scores[r * K + lane] : 0.0;

@@ -22,10 +22,14 @@ _DTYPES = {torch.float32: FIE_F32, torch.float16: FIE_F16, torch.bfloat16: FIE_B
 _pack = struct.Struct(_lib.BEAM_ARGS).pack
 _run = None             # the library's entry, loaded with the first call
 _size = None
+_sizes: dict[tuple, int] = {}    # bytes of workspace by requests, beams, vocabulary and number of eos
+_F32, _I32 = torch.float32, torch.int32
 _reorder = None
 MAX_STATES = 48         # tensors of one launch
+_packs: dict[int, object] = {}
 MAX_BEAMS = 64
 MAX_EOS = 16
+_NO_EOS = (0,) * MAX_EOS
 MAX_ROWS = 65535
 
 
@@ -55,10 +59,6 @@ def first_beams(requests: int, beams: int, device: torch.device | str) -> Beams:
                  torch.full((requests, beams, 3), -1, dtype=torch.int32, device=device))
 
 
-_FIELDS = (("scores", torch.float32), ("lengths", torch.int32), ("done", torch.bool), ("pool", torch.float32),
-           ("ends", torch.int32))
-
-
 def beam_step(logits: torch.Tensor, beams: Beams, *, eos: Sequence[int] = (), length_penalty: float = 1.0,
               early_stopping: bool = False, min_tokens: int = 0, max_tokens: int = 0, pad: int = 0, inplace: bool = False,
               history: tuple[torch.Tensor, torch.Tensor] | None = None) -> BeamStep:
@@ -77,22 +77,22 @@ def beam_step(logits: torch.Tensor, beams: Beams, *, eos: Sequence[int] = (), le
     ``inplace`` writes the new beams over the old.  ``history``: int32 [steps, rows] tokens and
     parents; a step's are kept at its request's length.  Runs on the current stream; nothing waits
     for it."""
-    scores = beams.scores
+    scores, lengths, done, pool, ends = beams
     if scores.ndim != 2:
         raise ValueError("scores must be [requests, beams]")
-    requests, count = scores.shape
+    requests, count = shape = scores.shape
     rows = requests * count
     if not 1 <= count <= MAX_BEAMS or rows > MAX_ROWS:
         raise ValueError(f"beams must be in [1, {MAX_BEAMS}], rows at most {MAX_ROWS}")
     index = scores.get_device()
     if index < 0:
         raise ValueError("beam_step runs on a HIP device")
-    shapes = ((requests, count), (requests,), (requests,), (requests, count), (requests, count, 3))
-    for t, (name, dtype), shape in zip(beams, _FIELDS, shapes):
-        if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous {dtype} {list(shape)}")
-        if t.get_device() != index:
-            raise ValueError("every tensor must be on the scores' device")
+    if not (scores.dtype == pool.dtype == _F32 and lengths.dtype == ends.dtype == _I32 and done.dtype == torch.bool
+            and pool.shape == shape and lengths.shape == done.shape == (requests,) and ends.shape == (requests, count, 3)
+            and scores.is_contiguous() and lengths.is_contiguous() and done.is_contiguous() and pool.is_contiguous()
+            and ends.is_contiguous()):
+        raise ValueError(f"beams must be contiguous float32 scores and pool [{requests}, {count}], int32 lengths [{requests}], "
+                         f"bool done [{requests}] and int32 ends [{requests}, {count}, 3]")
     if logits.ndim != 2 or logits.shape[0] != rows:
         raise ValueError(f"logits must be [{rows}, vocab], a request's beams together")
     vocab = logits.shape[1]
@@ -101,10 +101,10 @@ def beam_step(logits: torch.Tensor, beams: Beams, *, eos: Sequence[int] = (), le
         raise ValueError("logits must be float32, float16 or bfloat16")
     if not 1 <= vocab <= _lib.MAX_VOCAB:
         raise ValueError(f"vocab must be in [1, {_lib.MAX_VOCAB}]")
-    if logits.get_device() != index:
+    if not (index == logits.get_device() == lengths.get_device() == done.get_device() == pool.get_device() == ends.get_device()):
         raise ValueError("every tensor must be on the scores' device")
-    eos = tuple(eos)
-    if len(eos) > MAX_EOS or any(not 0 <= e < vocab for e in eos):
+    stop = len(eos)
+    if stop > MAX_EOS or (stop and not 0 <= min(eos) <= max(eos) < vocab):
         raise ValueError(f"eos: at most {MAX_EOS} tokens of the vocabulary")
     if not length_penalty == length_penalty or not 0 <= pad < 1 << 31 or not 0 <= min_tokens < 1 << 31 \
             or not 0 <= max_tokens < 1 << 31:
@@ -112,26 +112,32 @@ def beam_step(logits: torch.Tensor, beams: Beams, *, eos: Sequence[int] = (), le
     h_tokens = h_parents = h_steps = 0
     if history is not None:
         for t in history:
-            if t.dtype != torch.int32 or t.ndim != 2 or t.shape[1] != rows or t.shape != history[0].shape \
+            if t.dtype != _I32 or t.ndim != 2 or t.shape[1] != rows or t.shape != history[0].shape \
                     or not t.is_contiguous() or t.get_device() != index:
                 raise ValueError(f"history must be two contiguous int32 [steps, {rows}] on the scores' device")
         h_tokens, h_parents, h_steps = history[0].data_ptr(), history[1].data_ptr(), history[0].shape[0]
-    if (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
-        logits = logits.contiguous()
-    device = scores.device
-    new = beams if inplace else Beams(*(torch.empty_like(t) for t in beams))
-    tokens = torch.empty(rows, dtype=torch.int64, device=device)
-    parents = torch.empty(rows, dtype=torch.int32, device=device)
+    stride, step = logits.stride()
+    if (vocab > 1 and step != 1) or (rows > 1 and stride < vocab):
+        logits, stride = logits.contiguous(), vocab
+    like = torch.empty_like
+    new = beams if inplace else Beams(like(scores), like(lengths), like(done), like(pool), like(ends))
+    tokens = scores.new_empty(rows, dtype=torch.int64)
+    parents = lengths.new_empty(rows)
     if rows:
         global _run, _size
         if _run is None:
             _run, _size = _lib.launcher("fie_beam_step"), _lib.load().fie_beam_workspace_size
-        args = [logits.data_ptr(), *(t.data_ptr() for t in beams), *(t.data_ptr() for t in new), tokens.data_ptr(),
-                parents.data_ptr(), h_tokens, h_parents, max(logits.stride(0), vocab), 0, 0, float(length_penalty), requests, count,
-                vocab, code, bool(early_stopping), min_tokens, pad, h_steps, len(eos), *eos, *(0,) * (MAX_EOS - len(eos)), max_tokens]
-        args[17] = _size(_pack(*args))
-        room = torch.empty(args[17], dtype=torch.uint8, device=device)
-        args[16] = room.data_ptr()
+        args = [logits.data_ptr(), scores.data_ptr(), lengths.data_ptr(), done.data_ptr(), pool.data_ptr(), ends.data_ptr(),
+                new.scores.data_ptr(), new.lengths.data_ptr(), new.done.data_ptr(), new.pool.data_ptr(), new.ends.data_ptr(),
+                tokens.data_ptr(), parents.data_ptr(), h_tokens, h_parents, max(stride, vocab), 0, 0, length_penalty, requests,
+                count, vocab, code, early_stopping, min_tokens, pad, h_steps, stop, *eos, *_NO_EOS[stop:], max_tokens]
+        size = _sizes.get((requests, count, vocab, stop))
+        if size is None:
+            if len(_sizes) > 256:
+                _sizes.clear()
+            size = _sizes[requests, count, vocab, stop] = _size(_pack(*args))
+        room = done.new_empty(size)
+        args[16], args[17] = room.data_ptr(), size
         _run(index, _pack(*args))
     return BeamStep(new, tokens, parents)
 
@@ -148,41 +154,46 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor,
     if index < 0:
         raise ValueError("reorder_states runs on a HIP device")
     n = parents.shape[0]
-    parents = parents.contiguous()
+    if not parents.is_contiguous():
+        parents = parents.contiguous()
     if out is not None and len(out) != len(states):
         raise ValueError("as many outputs as states")
-    got, parts, held = [], [], []                    # held: copies, until the launch
+    got, flat, held = [], [], []                    # held: copies, until the launch
     for i, s in enumerate(states):
         if s.ndim < 1 or s.get_device() != index:
             raise ValueError("states must be [rows, ...] on the parents' device")
-        rows = s.shape[0]
+        shape = s.shape
+        rows = shape[0]
         if n > rows:
             raise ValueError(f"{n} parents of {rows} rows")
-        if rows and not s[0].is_contiguous():
+        if not s.is_contiguous() and rows and not s[0].is_contiguous():
             s = s.contiguous()
             held.append(s)
         if out is None:
-            t = torch.empty((n, *s.shape[1:]), dtype=s.dtype, device=s.device)
+            t = s.new_empty((n, *shape[1:])) if n != rows or not s.is_contiguous() else torch.empty_like(s)
         else:
             t = out[i]
-            if t.dtype != s.dtype or t.shape != (n, *s.shape[1:]) or t.get_device() != index:
+            if t.dtype != s.dtype or t.shape != (n, *shape[1:]) or t.get_device() != index:
                 raise ValueError(f"output {i} must be [{n}, ...] as its state")
-            if n and not t[0].is_contiguous() or (n > 1 and t.numel() and t.stride(0) < t[0].numel()):
+            if not t.is_contiguous() and n and (not t[0].is_contiguous() or (n > 1 and t.numel() and t.stride(0) < t[0].numel())):
                 raise ValueError("outputs need contiguous rows that do not overlap")
             if s.numel() and t.numel() and _meet(s, t):
                 raise ValueError("an output overlaps its state")
         got.append(t)
-        size = s.element_size()
-        width = t[0].numel() * size if n else 0
-        if width:
-            parts.append((s.data_ptr(), t.data_ptr(), s.stride(0) * size, t.stride(0) * size, width, rows))
+        width = s.numel()
+        if width and n:
+            size = s.element_size()
+            flat += s.data_ptr(), t.data_ptr(), s.stride(0) * size, t.stride(0) * size, width // rows * size, rows
     global _reorder
-    if parts and _reorder is None:
+    if flat and _reorder is None:
         _reorder = _lib.launcher("fie_reorder_states")
-    for at in range(0, len(parts), MAX_STATES):
-        some = parts[at:at + MAX_STATES]
-        flat = [v for p in some for v in p]
-        _reorder(index, struct.pack(_lib.STATES_ARGS + _lib.STATE_ARGS * len(some), parents.data_ptr(), n, len(some), *flat))
+    for at in range(0, len(flat), 6 * MAX_STATES):
+        some = flat[at:at + 6 * MAX_STATES]
+        count = len(some) // 6
+        pack = _packs.get(count)
+        if pack is None:
+            pack = _packs[count] = struct.Struct(_lib.STATES_ARGS + _lib.STATE_ARGS * count).pack
+        _reorder(index, pack(parents.data_ptr(), n, count, *some))
     return got
 
 
