@@ -50,12 +50,14 @@ template <int DT> struct BeamVec {                      // 16 bytes of logits
     }
 };
 
-// The largest key T, low 16 bits 0, that at least `rank` lanes of the wave reach.
-FIE_DEV uint32_t beam_reach(uint32_t key, int rank)
+// The largest key T, low LOW bits 0, that at least `rank` lanes of the wave reach.  (A logit's upper
+// half has 7 bits behind the point's; a total's upper word needs its lower bits: by 16 of them the
+// bound was 2 below totals about -40, and ten times the candidates were ranked.)
+template <int LOW> FIE_DEV uint32_t beam_reach(uint32_t key, int rank)
 {
     uint32_t t = 0;
 #pragma unroll
-    for (int bit = 31; bit >= 16; --bit) {
+    for (int bit = 31; bit >= LOW; --bit) {
         const uint32_t up = t | (1u << bit);
         if (__popcll(__ballot(key >= up)) >= rank) t = up;
     }
@@ -248,7 +250,7 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_scan(const fie_beam_args 
         top = up;
         if (t == first) {
             const uint32_t key = m > -__builtin_inff() ? fkey(m + 0.0f) : 0u;
-            const uint32_t reach = beam_reach(key, rank);
+            const uint32_t reach = beam_reach<16>(key, rank);
             if (lane == 0) S.wave[wave] = reach;
             __syncthreads();
             uint32_t least = S.wave[0];
@@ -282,7 +284,7 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_scan(const fie_beam_args 
     if (count > kBeamThreads && count <= kBeamList) {
         uint32_t best = 0;
         for (int i = tid; i < count; i += kBeamThreads) best = max(best, comp_k(S.list[i]));
-        const uint32_t reach = beam_reach(best, rank);
+        const uint32_t reach = beam_reach<16>(best, rank);
         if (lane == 0) S.wave[wave] = reach;
         __syncthreads();
         uint32_t least = S.wave[0];
@@ -334,129 +336,284 @@ FIE_DEV double beam_scale(int length, double penalty)
     return exp(penalty * log((double)length));
 }
 
-// A workgroup a request, a wave a row at first: the row's spans' lists are in order, so its best
-// candidates come off their heads one by one; then the request's, off its rows' lists, in one
-// wave with a beam a lane.  Bound by that chain: a few hundred cycles a candidate.
-// Dynamic LDS: [waves][spans][most] spans' lists, [beams][most] rows' lists.
-__global__ __launch_bounds__(1024) void k_beam_pick(const fie_beam_args a, const BeamWork w)
+// What a request's workgroup settles before the pool.
+struct BeamChoice {
+    double lse[FIE_MAX_BEAMS];                          // log of a row's sum, less its maximum
+    float top[FIE_MAX_BEAMS], prior[FIE_MAX_BEAMS];
+    int32_t count[FIE_MAX_BEAMS];
+    uint64_t live_key[FIE_MAX_BEAMS];
+    int32_t live_token[FIE_MAX_BEAMS], live_beam[FIE_MAX_BEAMS];
+    float end_value[FIE_MAX_BEAMS];
+    int32_t end_token[FIE_MAX_BEAMS], end_beam[FIE_MAX_BEAMS];
+    int32_t found, ended, listed;
+    uint32_t wave[16];
+};
+
+constexpr int kPickEach = 4;                            // candidates of a thread
+constexpr int kPickList = 1024;                         // those that are ranked
+
+// A thread's n-th candidate: the waves take turns, so that each has its share of the good beams' (wave
+// after wave, one of bad beams alone lowered the bound to all there were: 64 x 8 20 us).
+FIE_DEV int pick_index(int n)
 {
-    extern __shared__ uint64_t L[];
-    __shared__ double lse[FIE_MAX_BEAMS];               // log of a row's sum, less its maximum
-    __shared__ float top[FIE_MAX_BEAMS];
-    __shared__ int32_t counts[FIE_MAX_BEAMS];
-    __shared__ uint64_t live_key[FIE_MAX_BEAMS];
-    __shared__ int32_t live_token[FIE_MAX_BEAMS], live_beam[FIE_MAX_BEAMS];
-    __shared__ float end_value[FIE_MAX_BEAMS], old_value[FIE_MAX_BEAMS];
-    __shared__ int32_t end_token[FIE_MAX_BEAMS], end_beam[FIE_MAX_BEAMS], old_end[FIE_MAX_BEAMS][3];
-    __shared__ int32_t found, ended;
-    const int r = blockIdx.x, K = a.beams, lane = threadIdx.x & 63, most = w.most;
+    const int waves = blockDim.x >> 6;
+    return ((threadIdx.x & 63) + 64 * n) * waves + (threadIdx.x >> 6);
+}
+
+FIE_DEV bool is_eos(const fie_beam_args& a, int token)
+{
+    bool eos = false;
+    for (int i = 0; i < a.eos_count; ++i) eos |= token == a.eos[i];
+    return eos;
+}
+
+// A continuation in the request's order: `first` by its total, `then` on ties, by the lower beam, the
+// larger logit and the lower token (of 20 bits).
+FIE_DEV uint64_t pick_then(int beam, uint64_t cand)
+{
+    return ((uint64_t)(63 - beam) << 52) | ((uint64_t)comp_k(cand) << 20) | ((uint32_t)cand & 0xFFFFFu);
+}
+FIE_DEV int then_beam(uint64_t t) { return 63 - (int)(t >> 52); }
+FIE_DEV int then_token(uint64_t t) { return 0xFFFFF - (int)(t & 0xFFFFFu); }
+
+// All of a request's candidates at once: a bound on their totals as in the scan, what reaches it into a
+// list, the list by rank, and its places in order by a wave's ballots.  False where more reach it than
+// the list holds (many equal totals).  `wanted`: as many as may stand in front of the last that goes on.
+FIE_DEV bool pick_ranked(const fie_beam_args& a, const BeamWork& w, int r, int wanted, int length, double scale, uint64_t* L,
+                         const uint64_t (&cand)[kPickEach], BeamChoice& C)
+{
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    const int per = w.spans * w.most, all = a.beams * per;
+    uint64_t key[kPickEach];
+    uint32_t best = 0;
+#pragma unroll
+    for (int n = 0; n < kPickEach; ++n) {
+        const int i = pick_index(n), beam = i < all ? i / per : 0;
+        key[n] = 0;
+        if (cand[n]) key[n] = beam_order((double)C.prior[beam] + ((double)(key_to_float(comp_k(cand[n])) - C.top[beam]) - C.lse[beam]));
+        best = max(best, (uint32_t)(key[n] >> 32));
+    }
+    const uint32_t reach = beam_reach<4>(best, (wanted + waves - 1) / waves);
+    if (lane == 0) C.wave[wave] = reach;
+    __syncthreads();
+    uint32_t least = C.wave[0];
+    for (int i = 1; i < waves; ++i) least = min(least, C.wave[i]);
+    uint64_t* const first = L;
+    uint64_t* const then = L + kPickList;
+#pragma unroll
+    for (int n = 0; n < kPickEach; ++n)
+        if (key[n] && (uint32_t)(key[n] >> 32) >= least) {
+            const int at = atomicAdd(&C.listed, 1), i = pick_index(n);
+            if (at < kPickList) {
+                first[at] = key[n];
+                then[at] = pick_then(i / per, cand[n]);
+            }
+        }
+    __syncthreads();
+    const int count = C.listed;
+    if (count > kPickList) return false;
+    uint64_t* const first_s = then + kPickList;         // in order
+    uint64_t* const then_s = first_s + kPickList;
+#pragma unroll 1
+    for (int i = tid; i < count; i += blockDim.x) {
+        const uint64_t f = first[i], t = then[i];
+        int place = 0;
+#pragma unroll 8
+        for (int j = 0; j < count; ++j) place += first[j] > f || (first[j] == f && then[j] > t);
+        first_s[place] = f;
+        then_s[place] = t;
+    }
+    __syncthreads();
+    if (wave) return true;
+    const bool last = a.max_tokens > 0 && length + 1 >= a.max_tokens;           // all end
+    const uint64_t below = (1ull << lane) - 1ull;
+    int live = 0, ends = 0, rank = 0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < count && live < a.beams && !(last && rank >= a.beams); i0 += 64) {
+        const int i = i0 + lane;
+        const uint64_t f = i < count ? first_s[i] : 0, t = i < count ? then_s[i] : 0;
+        const int token = then_token(t);
+        const bool eos = f && is_eos(a, token), exists = f && !(eos && length + 1 < a.min_tokens), goes = exists && !eos && !last;
+        const uint64_t any = __ballot(exists), on = __ballot(goes);
+        const int my_rank = rank + (int)__popcll(any & below), my_live = live + (int)__popcll(on & below);
+        const bool stops = exists && !goes && my_rank < a.beams;
+        const uint64_t off = __ballot(stops);
+        if (goes && my_live < a.beams) {
+            C.live_key[my_live] = f;
+            C.live_token[my_live] = token;
+            C.live_beam[my_live] = then_beam(t);
+        }
+        if (stops) {
+            const int at = ends + (int)__popcll(off & below);
+            C.end_value[at] = (float)(beam_value(f) / scale);
+            C.end_token[at] = token;
+            C.end_beam[at] = then_beam(t);
+        }
+        rank += (int)__popcll(any);
+        live += (int)__popcll(on);
+        ends += (int)__popcll(off);
+    }
+    if (lane == 0) {
+        C.found = min(live, a.beams);
+        C.ended = ends;
+    }
+    return true;
+}
+
+// The same one by one, for any number: a wave a row at first, whose spans' lists are in order, so that
+// its best candidates come off their heads; then the request's, off its rows' lists, in one wave
+// with a beam a lane.  A few hundred cycles a candidate.  LDS: [waves][spans][most], [beams][most].
+FIE_DEV void pick_one_by_one(const fie_beam_args& a, const BeamWork& w, int r, int length, double scale, uint64_t* L, BeamChoice& C)
+{
+    const int K = a.beams, lane = threadIdx.x & 63, most = w.most;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int length = a.lengths[r];
-    const bool was = a.done[r] != 0;
     uint64_t* heads = L + (int64_t)wave * w.spans * most;
     uint64_t* rows = L + (int64_t)waves * w.spans * most;
+#pragma unroll 1
     for (int b = wave; b < K; b += waves) {
-        const int row = r * K + b;
-        if (beam_dead(a, row)) {
-            if (lane == 0) counts[b] = 0;
-            continue;
-        }
-        const bool in = lane < w.spans;
-        const BeamSpan sp = in ? w.span[(int64_t)row * w.spans + lane] : BeamSpan{0.0, -kLargest, 0};
-        float m = sp.top;
-        for (int d = 32; d; d >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d, 64));
-        double s = sp.sum * __builtin_amdgcn_exp2f((sp.top - m) * kLog2e);
-        for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
-        const uint64_t* from = w.cand + (int64_t)row * w.spans * most;
+        if (C.count[b] == 0) continue;
+        const int64_t row = (int64_t)r * K + b;
+        const int held = lane < w.spans ? w.span[row * w.spans + lane].count : 0;
+        const uint64_t* from = w.cand + row * w.spans * most;
         for (int i = lane; i < w.spans * most; i += 64) heads[i] = from[i];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         int at = 0, n = 0;
-        uint64_t head = sp.count > 0 ? heads[lane * most] : 0;
+        uint64_t head = held > 0 ? heads[lane * most] : 0;
+#pragma unroll 1
         for (; n < most; ++n) {
             const uint64_t best = dwave_max_u64(head);
             if (best == 0) break;
             if (lane == 0) rows[b * most + n] = best;
             if (head == best) {
                 ++at;
-                head = at < sp.count ? heads[lane * most + at] : 0;
+                head = at < held ? heads[lane * most + at] : 0;
             }
         }
-        if (lane == 0) {
-            counts[b] = n;
-            top[b] = m;
-            lse[b] = log(s);
-        }
-    }
-    if ((int)threadIdx.x < K) {
-        const float p = a.pool[r * K + threadIdx.x];
-        old_value[threadIdx.x] = p == p ? p : -__builtin_inff();
-        for (int i = 0; i < 3; ++i) old_end[threadIdx.x][i] = a.ends[(r * K + threadIdx.x) * 3 + i];
+        if (lane == 0) C.count[b] = n;
     }
     __syncthreads();
-    const double scale = beam_scale(max(was ? length : length + 1, 1), a.length_penalty);
-    if (wave == 0) {
-        const bool mine = lane < K && counts[lane] > 0;
-        const double prior = mine ? (double)a.scores[r * K + lane] : 0.0;
-        const int n = mine ? counts[lane] : 0;
-        int at = 0;
-        auto look = [&]() {
-            if (at >= n) return (uint64_t)0;
-            const float x = key_to_float(comp_k(rows[lane * most + at]));
-            return beam_order(prior + ((double)(x - top[lane]) - lse[lane]));
-        };
-        uint64_t head = look();
-        int live = 0, ends = 0, rank = 0;
-        const bool last = a.max_tokens > 0 && length + 1 >= a.max_tokens;     // all end
-        while (live < K && !(last && rank >= K)) {
-            const uint64_t best = dwave_max_u64(head);
-            if (best == 0) break;
-            const int who = (int)__builtin_ctzll(__ballot(head == best));     // ties: the lower beam
-            const int token = (int)comp_idx(rows[who * most + __builtin_amdgcn_readlane(at, who)]);
-            bool eos = false;
-            for (int i = 0; i < a.eos_count; ++i) eos |= token == a.eos[i];
-            if (lane == who) {
-                ++at;
-                head = look();
-            }
-            if (eos && length + 1 < a.min_tokens) continue;                   // does not exist
-            eos |= last;
-            if (lane == 0) {
-                if (!eos) {
-                    live_key[live] = best;
-                    live_token[live] = token;
-                    live_beam[live] = who;
-                } else if (rank < K) {
-                    end_value[ends] = (float)(beam_value(best) / scale);
-                    end_token[ends] = token;
-                    end_beam[ends] = who;
-                }
-            }
-            if (!eos) ++live;
-            else if (rank < K) ++ends;
-            ++rank;
+    if (wave) return;
+    const int n = lane < K ? C.count[lane] : 0;
+    int at = 0;
+    auto look = [&]() {
+        if (at >= n) return (uint64_t)0;
+        const float x = key_to_float(comp_k(rows[lane * most + at]));
+        return beam_order((double)C.prior[lane] + ((double)(x - C.top[lane]) - C.lse[lane]));
+    };
+    uint64_t head = look();
+    int live = 0, ends = 0, rank = 0;
+    const bool last = a.max_tokens > 0 && length + 1 >= a.max_tokens;           // all end
+#pragma unroll 1
+    while (live < K && !(last && rank >= K)) {
+        const uint64_t best = dwave_max_u64(head);
+        if (best == 0) break;
+        const int who = (int)__builtin_ctzll(__ballot(head == best));           // ties: the lower beam
+        const int token = (int)comp_idx(rows[who * most + __builtin_amdgcn_readlane(at, who)]);
+        bool eos = is_eos(a, token);
+        if (lane == who) {
+            ++at;
+            head = look();
         }
+        if (eos && length + 1 < a.min_tokens) continue;                         // does not exist
+        eos |= last;
         if (lane == 0) {
-            found = live;
-            ended = ends;
+            if (!eos) {
+                C.live_key[live] = best;
+                C.live_token[live] = token;
+                C.live_beam[live] = who;
+            } else if (rank < K) {
+                C.end_value[ends] = (float)(beam_value(best) / scale);
+                C.end_token[ends] = token;
+                C.end_beam[ends] = who;
+            }
         }
+        if (!eos) ++live;
+        else if (rank < K) ++ends;
+        ++rank;
+    }
+    if (lane == 0) {
+        C.found = live;
+        C.ended = ends;
+    }
+}
+
+// A workgroup a request: its rows' logarithms, a wave each, then its best continuations, then the pool.
+// Bound by the chain of these steps.
+__global__ __launch_bounds__(1024) void k_beam_pick(const fie_beam_args a, const BeamWork w, int wanted)
+{
+    extern __shared__ uint64_t L[];
+    __shared__ BeamChoice C;
+    __shared__ float old_value[FIE_MAX_BEAMS];
+    __shared__ int32_t old_end[FIE_MAX_BEAMS][3];
+    const int r = blockIdx.x, K = a.beams, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
+    const int per = w.spans * w.most;
+    // every load at once: what a row that is not there left in the workspace is looked at by no one
+    uint64_t cand[kPickEach];
+    int32_t held[kPickEach];
+    if (wanted)
+#pragma unroll
+        for (int n = 0; n < kPickEach; ++n) {
+            const int i = pick_index(n), at = min(i, K * per - 1), list = at / w.most;
+            cand[n] = w.cand[(int64_t)r * K * per + at];
+            held[n] = i < K * per ? w.span[(int64_t)r * K * w.spans + list].count - (at - list * w.most) : 0;
+        }
+    const int length = a.lengths[r];
+    const bool was = a.done[r] != 0;
+    if (tid < K) {
+        const float p = a.pool[r * K + tid], s = a.scores[r * K + tid];
+        old_value[tid] = p == p ? p : -__builtin_inff();
+        for (int i = 0; i < 3; ++i) old_end[tid][i] = a.ends[(r * K + tid) * 3 + i];
+        C.prior[tid] = s;
+        C.count[tid] = !was && s > -__builtin_inff();
+    }
+    if (tid == 0) C.listed = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int b = wave; b < K; b += waves) {
+        if (C.count[b] == 0) continue;
+        const BeamSpan sp = lane < w.spans ? w.span[((int64_t)r * K + b) * w.spans + lane] : BeamSpan{0.0, -kLargest, 0};
+        float m = sp.top;
+        for (int d = 32; d; d >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d, 64));
+        double s = sp.sum * __builtin_amdgcn_exp2f((sp.top - m) * kLog2e);
+        for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
+        if (lane == 0) {
+            C.top[b] = m;
+            C.lse[b] = log(s);
+        }
+    }
+    const double scale = beam_scale(max(was ? length : length + 1, 1), a.length_penalty);
+    __syncthreads();
+    bool ranked = wanted > 0;
+    if (ranked) {
+#pragma unroll
+        for (int n = 0; n < kPickEach; ++n) {
+            const int i = pick_index(n);
+            if (held[n] <= 0 || C.count[min(i / per, K - 1)] == 0) cand[n] = 0;
+        }
+        ranked = pick_ranked(a, w, r, wanted, length, scale, L, cand, C);
+    }
+    if (!ranked) {
+        __syncthreads();
+        pick_one_by_one(a, w, r, length, scale, L, C);
     }
     __syncthreads();
     if (wave) return;
     // the pool: its own and the new ones by value, the older first; both are held before the writes
-    const int E = ended, live = found;
+    const int E = C.ended, live = C.found;
     const float mine = lane < K ? old_value[lane] : -__builtin_inff();
     int place = 64;
     if (lane < K) {
         place = 0;
         for (int j = 0; j < K; ++j) place += old_value[j] > mine || (old_value[j] == mine && j < lane);
-        for (int j = 0; j < E; ++j) place += end_value[j] > mine;
+        for (int j = 0; j < E; ++j) place += C.end_value[j] > mine;
     }
     int fresh = 64;
     if (lane < E) {
         fresh = 0;
-        const float v = end_value[lane];
+        const float v = C.end_value[lane];
         for (int j = 0; j < K; ++j) fresh += old_value[j] >= v;
-        for (int j = 0; j < E; ++j) fresh += end_value[j] > v || (end_value[j] == v && j < lane);
+        for (int j = 0; j < E; ++j) fresh += C.end_value[j] > v || (C.end_value[j] == v && j < lane);
     }
     auto put = [&](int to, float v, int e0, int e1, int e2) {
         a.next_pool[r * K + to] = v;
@@ -466,19 +623,19 @@ __global__ __launch_bounds__(1024) void k_beam_pick(const fie_beam_args a, const
         e[2] = e2;
     };
     if (place < K) put(place, mine, old_end[lane][0], old_end[lane][1], old_end[lane][2]);
-    if (fresh < K) put(fresh, end_value[lane], length + 1, r * K + end_beam[lane], end_token[lane]);
+    if (fresh < K) put(fresh, C.end_value[lane], length + 1, r * K + C.end_beam[lane], C.end_token[lane]);
     // the pool's worst
     float worst = __builtin_inff();
     if (place == K - 1) worst = mine;
-    if (fresh == K - 1) worst = end_value[lane];
+    if (fresh == K - 1) worst = C.end_value[lane];
     for (int d = 32; d; d >>= 1) worst = __builtin_fminf(worst, __shfl_xor(worst, d, 64));
     bool done = was || live == 0;
-    if (!done && worst > -__builtin_inff()) done = a.early_stopping || worst >= (float)(beam_value(live_key[0]) / scale);
+    if (!done && worst > -__builtin_inff()) done = a.early_stopping || worst >= (float)(beam_value(C.live_key[0]) / scale);
     if (lane < K) {
         const int row = r * K + lane;
         const bool goes = !done && lane < live;
-        const int token = goes ? live_token[lane] : a.pad, parent = goes ? r * K + live_beam[lane] : row;
-        a.next_scores[row] = goes ? (float)beam_value(live_key[lane]) : -__builtin_inff();
+        const int token = goes ? C.live_token[lane] : a.pad, parent = goes ? r * K + C.live_beam[lane] : row;
+        a.next_scores[row] = goes ? (float)beam_value(C.live_key[lane]) : -__builtin_inff();
         a.tokens[row] = token;
         a.parents[row] = parent;
         if (a.history_tokens && !was && length >= 0 && length < a.history_steps) {
