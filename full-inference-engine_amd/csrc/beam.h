@@ -10,7 +10,8 @@ namespace fie {
 constexpr int kBeamThreads = 256, kBeamWaves = kBeamThreads / 64;
 constexpr int kBeamEach = 32;                           // logits of a thread a tile
 constexpr int kBeamTile = kBeamThreads * kBeamEach;
-constexpr int kBeamList = 2048;                         // candidates a workgroup holds
+constexpr int kBeamList = 1024;                         // candidates a workgroup holds,
+constexpr int kBeamShare = kBeamList / kBeamWaves;      // and a wave
 constexpr int kBeamSpans = 32;                          // most spans of a row
 constexpr float kLog2e = 1.44269502f;
 constexpr float kLargest = 3.40282347e38f;
@@ -106,13 +107,18 @@ template <int DT> struct BeamRow {
     }
 };
 
+// Workgroups of a CU at a time.
+template <int DT> constexpr int kBeamHold = DT == FIE_BF16 ? 5 : 4;
+
 struct BeamShared {
-    uint64_t list[kBeamList];
-    uint32_t hist[2048];
+    union {
+        uint64_t list[kBeamList];
+        uint32_t hist[2048];        // of radix passes, before the list is made
+    };
     uint32_t wave[kBeamWaves];
     double sum[kBeamWaves];
     float top[kBeamWaves];
-    int32_t count;
+    int32_t count, held[kBeamWaves];
     uint32_t above, bin;
 };
 
@@ -197,10 +203,10 @@ FIE_DEV int beam_deep(const BeamRow<DT>& row, int first, int last, int most, Bea
 // grid (spans, rows): a span's largest logit, its sum of exp, and its best candidates in order.
 // One pass over the logits.  The first tile gives a bound: every wave finds what a quarter of the
 // wanted candidates reach among its 64 lanes' maxima, and the least of the four waves' bounds is
-// reached by all of them.  What reaches it is listed, in later tiles too; the list is ranked at
-// the end.
+// reached by all of them.  What reaches it is listed, in later tiles too; at the end the lists
+// are cut by such a bound of their own and ranked.
 template <int DT>
-__global__ __launch_bounds__(kBeamThreads) void k_beam_scan(const fie_beam_args a, const BeamWork w)
+__global__ __launch_bounds__(kBeamThreads, kBeamHold<DT>) void k_beam_scan(const fie_beam_args a, const BeamWork w)
 {
     __shared__ BeamShared S;
     const int row_id = blockIdx.y, span = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -215,6 +221,8 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_scan(const fie_beam_args 
         return;
     }
     if (tid == 0) S.count = 0;
+    uint64_t* const mine = S.list + wave * kBeamShare;
+    int held = 0;
     const int rank = (w.most + kBeamWaves - 1) / kBeamWaves;
     float top = -kLargest, bound = -__builtin_inff();
     double sum = 0.0;
@@ -224,22 +232,28 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_scan(const fie_beam_args 
         float x[kBeamEach];
         row.open(t, raw, x);
         if (t + 1 < last) row.load(t + 1, raw);
-        float m = x[0];
+        float part[4];                                  // maxima of eight logits each
 #pragma unroll
-        for (int e = 1; e < kBeamEach; ++e) m = __builtin_fmaxf(m, x[e]);
-        const float high = __builtin_fmaxf(top, m);
+        for (int g = 0; g < 4; ++g) {
+            part[g] = x[8 * g];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) part[g] = __builtin_fmaxf(part[g], x[8 * g + e]);
+        }
+        float m = __builtin_fmaxf(__builtin_fmaxf(part[0], part[1]), __builtin_fmaxf(part[2], part[3]));
+        float up = __builtin_fmaxf(top, m);
         float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int e = 0; e < kBeamEach; ++e) s[e & 3] += __builtin_amdgcn_exp2f((x[e] - high) * kLog2e);
+        for (int e = 0; e < kBeamEach; ++e) s[e & 3] += __builtin_amdgcn_exp2f((x[e] - up) * kLog2e);
         float here = (s[0] + s[1]) + (s[2] + s[3]);
-        float up = high;
-        if (!(here == here) || high > kLargest) {       // a NaN or an infinity among them
+        if (__any(!(here == here) || up > kLargest)) {  // a NaN or an infinity among them
             m = -__builtin_inff();
 #pragma unroll
             for (int e = 0; e < kBeamEach; ++e) {
                 x[e] = beam_clean(x[e]);
                 m = __builtin_fmaxf(m, x[e]);
             }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) part[g] = m;
             up = __builtin_fmaxf(top, m);
             here = 0.0f;
 #pragma unroll
@@ -259,13 +273,19 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_scan(const fie_beam_args 
             // a bound that some wave's lanes do not reach: everything is listed
             bound = least > kKeyNegInf ? key_to_float(least) : -kLargest;
         }
-        if (m >= bound)
+        // (places by ballot: with a counter in LDS a wave waited for it at each logit that was listed)
+        if (__any(m >= bound))
 #pragma unroll
-            for (int e = 0; e < kBeamEach; ++e)
-                if (x[e] >= bound) {
-                    const int at = atomicAdd(&S.count, 1);
-                    if (at < kBeamList) S.list[at] = comp_key(fkey(x[e] + 0.0f), (uint32_t)row.index(t, e));
-                }
+            for (int g = 0; g < 4; ++g)
+                if (__any(part[g] >= bound))
+#pragma unroll
+                    for (int e = 8 * g; e < 8 * g + 8; ++e) {
+                        const uint64_t hits = __ballot(x[e] >= bound);
+                        if (!hits) continue;
+                        const int at = held + (int)__popcll(hits & ((1ull << lane) - 1ull));
+                        if (x[e] >= bound && at < kBeamShare) mine[at] = comp_key(fkey(x[e] + 0.0f), (uint32_t)row.index(t, e));
+                        held += (int)__popcll(hits);
+                    }
     }
     // the span's maximum and sum
     float all = top;
@@ -278,30 +298,30 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_scan(const fie_beam_args 
     sum *= __builtin_amdgcn_exp2f((top - all) * kLog2e);
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
     if (lane == 0) S.sum[wave] = sum;
-    int count = S.count;
-    __syncthreads();
-    // a long list: a bound among what is listed, every lane holding some of it
-    if (count > kBeamThreads && count <= kBeamList) {
-        uint32_t best = 0;
-        for (int i = tid; i < count; i += kBeamThreads) best = max(best, comp_k(S.list[i]));
-        const uint32_t reach = beam_reach<16>(best, rank);
-        if (lane == 0) S.wave[wave] = reach;
-        __syncthreads();
-        uint32_t least = S.wave[0];
+    if (lane == 0) S.held[wave] = held;
+    // a bound among what the waves listed, and what reaches it together
+    uint64_t keep[kBeamShare / 64];
+    uint32_t best = 0;
 #pragma unroll
-        for (int i = 1; i < kBeamWaves; ++i) least = min(least, S.wave[i]);
-        uint64_t keep[kBeamList / kBeamThreads];
-#pragma unroll
-        for (int i = 0; i < kBeamList / kBeamThreads; ++i) keep[i] = tid + i * kBeamThreads < count ? S.list[tid + i * kBeamThreads] : 0;
-        if (tid == 0) S.count = 0;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kBeamList / kBeamThreads; ++i)
-            if (keep[i] && comp_k(keep[i]) >= least) S.list[atomicAdd(&S.count, 1)] = keep[i];
-        __syncthreads();
-        count = S.count;
-        __syncthreads();
+    for (int i = 0; i < kBeamShare / 64; ++i) {
+        keep[i] = lane + i * 64 < held ? mine[lane + i * 64] : 0;
+        best = max(best, comp_k(keep[i]));
     }
+    const uint32_t reach = beam_reach<16>(best, rank);
+    if (lane == 0) S.wave[wave] = reach;
+    __syncthreads();
+    uint32_t least = S.wave[0];
+    bool over = false;
+#pragma unroll
+    for (int i = 0; i < kBeamWaves; ++i) {
+        least = min(least, S.wave[i]);
+        over |= S.held[i] > kBeamShare;
+    }
+#pragma unroll
+    for (int i = 0; i < kBeamShare / 64; ++i)
+        if (keep[i] && comp_k(keep[i]) >= least) S.list[atomicAdd(&S.count, 1)] = keep[i];
+    __syncthreads();
+    int count = over ? kBeamList + 1 : S.count;
     if (count > 2 * kBeamThreads) count = beam_deep<DT>(row, first, last, w.most, S);
     // each entry's place
     uint64_t* cand = w.cand + ((int64_t)row_id * w.spans + span) * w.most;

@@ -7,7 +7,7 @@ namespace fie {
 
 static int64_t plan_most(int64_t tokens, int64_t adapters) { return tokens / kTileTokens + std::min(tokens, adapters + 1); }
 
-constexpr int kDownSteps = 4;                           // of a wave at a time; 2 from 33 ranks on
+constexpr int kDownSteps = 4;                           // of a wave at a time
 
 static AdapterWork adapter_work(const fie_adapter_args& a)
 {
@@ -15,7 +15,7 @@ static AdapterWork adapter_work(const fie_adapter_args& a)
     w.h = (float*)a.workspace;
     w.most = (int)plan_most(a.tokens, a.adapters);
     // enough workgroups to fill the CUs, as long as each wave has its steps of k
-    const int step = (a.dtype == FIE_F32 ? 16 : 32) * (a.rank > 32 ? 2 : kDownSteps) * kDownWaves;
+    const int step = (a.dtype == FIE_F32 ? 16 : 32) * kDownSteps * kDownWaves;
     w.splits = std::max(1, std::min({(a.k + step - 1) / step, 1024 / std::max(w.most, 1), 16}));
     return w;
 }
@@ -28,8 +28,8 @@ static hipError_t down_of(const fie_adapter_args& a, const AdapterWork& w, hipSt
     const dim3 grid((unsigned)w.splits, (unsigned)w.most);
     if (a.rank <= 16) k_adapter_down<DX, DT, 1, kDownSteps, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
     else if (a.rank <= 32) k_adapter_down<DX, DT, 2, kDownSteps, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
-    else if (a.rank <= 48) k_adapter_down<DX, DT, 3, 2, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
-    else k_adapter_down<DX, DT, 4, 2, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
+    else if (a.rank <= 48) k_adapter_down<DX, DT, 3, kDownSteps, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
+    else k_adapter_down<DX, DT, 4, kDownSteps, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
     return hipGetLastError();
 }
 

@@ -12,7 +12,10 @@ static BeamWork beam_work(const fie_beam_args& a)
     const int rows = a.requests * a.beams;
     // 7 elements more: rows need not begin at 16 bytes
     const int tiles = (a.vocab + 7 + kBeamTile - 1) / kBeamTile;
-    const int spans = std::min({kBeamSpans, tiles, std::max(1, 2048 / std::max(rows, 1))});
+    // as many workgroups as the CUs hold at a time, each with one long span: the rest would be a second
+    // round of few
+    const int hold = (a.dtype == FIE_BF16 ? kBeamHold<FIE_BF16> : kBeamHold<FIE_F32>) * std::max(cu_count(), 1);
+    const int spans = std::min({kBeamSpans, tiles, std::max(1, hold / std::max(rows, 1))});
     w.tiles = (tiles + spans - 1) / spans;
     w.spans = (tiles + w.tiles - 1) / w.tiles;
     w.most = std::min(a.vocab, a.beams + a.eos_count);

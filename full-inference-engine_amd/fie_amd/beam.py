@@ -22,7 +22,7 @@ _DTYPES = {torch.float32: FIE_F32, torch.float16: FIE_F16, torch.bfloat16: FIE_B
 _pack = struct.Struct(_lib.BEAM_ARGS).pack
 _run = None             # the library's entry, loaded with the first call
 _size = None
-_sizes: dict[tuple, int] = {}    # bytes of workspace by requests, beams, vocabulary and number of eos
+_sizes: dict[tuple, int] = {}    # bytes of workspace by a call's device, type and sizes
 _F32, _I32 = torch.float32, torch.int32
 _reorder = None
 MAX_STATES = 48         # tensors of one launch
@@ -131,11 +131,12 @@ def beam_step(logits: torch.Tensor, beams: Beams, *, eos: Sequence[int] = (), le
                 new.scores.data_ptr(), new.lengths.data_ptr(), new.done.data_ptr(), new.pool.data_ptr(), new.ends.data_ptr(),
                 tokens.data_ptr(), parents.data_ptr(), h_tokens, h_parents, max(stride, vocab), 0, 0, length_penalty, requests,
                 count, vocab, code, early_stopping, min_tokens, pad, h_steps, stop, *eos, *_NO_EOS[stop:], max_tokens]
-        size = _sizes.get((requests, count, vocab, stop))
+        key = index, code, requests, count, vocab, stop
+        size = _sizes.get(key)
         if size is None:
             if len(_sizes) > 256:
                 _sizes.clear()
-            size = _sizes[requests, count, vocab, stop] = _size(_pack(*args))
+            size = _sizes[key] = _size(_pack(*args))
         room = done.new_empty(size)
         args[16], args[17] = room.data_ptr(), size
         _run(index, _pack(*args))
