@@ -167,11 +167,12 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor,
         rows = shape[0]
         if n > rows:
             raise ValueError(f"{n} parents of {rows} rows")
-        if not s.is_contiguous() and rows and not s[0].is_contiguous():
-            s = s.contiguous()
+        dense = s.is_contiguous()
+        if not dense and rows and not s[0].is_contiguous():
+            s, dense = s.contiguous(), True
             held.append(s)
         if out is None:
-            t = s.new_empty((n, *shape[1:])) if n != rows or not s.is_contiguous() else torch.empty_like(s)
+            t = torch.empty_like(s) if dense and n == rows else s.new_empty((n, *shape[1:]))
         else:
             t = out[i]
             if t.dtype != s.dtype or t.shape != (n, *shape[1:]) or t.get_device() != index:
@@ -184,7 +185,9 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor,
         width = s.numel()
         if width and n:
             size = s.element_size()
-            flat += s.data_ptr(), t.data_ptr(), s.stride(0) * size, t.stride(0) * size, width // rows * size, rows
+            width = width // rows * size
+            flat += (s.data_ptr(), t.data_ptr(), width if dense else s.stride(0) * size,
+                     width if out is None else t.stride(0) * size, width, rows)
     global _reorder
     if flat and _reorder is None:
         _reorder = _lib.launcher("fie_reorder_states")
