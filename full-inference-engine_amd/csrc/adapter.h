@@ -196,7 +196,7 @@ __global__ __launch_bounds__(64 * kDownWaves) void k_adapter_down(const fie_adap
     const int32_t* order = a.plan + kPlanHead + (int64_t)w.most * kPlanTile;
     const int id = tile[0], first = tile[1], count = tile[2];
     if (id < 0) return;
-    const int rank = a.ranks[id];
+    const int rank = min(a.ranks[id], a.rank);
     const uint8_t* const row = (const uint8_t*)a.x + (int64_t)order[first + min(lane & 15, count - 1)] * a.x_stride * XS;
     const int full = a.k / Op::STEP, steps = (a.k + Op::STEP - 1) / Op::STEP;
     for (int r0 = 0; r0 < rank; r0 += 16 * RT) {
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void k_adapter_up(const fie_adapter_
     const int32_t* tile = a.plan + kPlanHead + (int64_t)t0 * kPlanTile;
     const int32_t* order = a.plan + kPlanHead + (int64_t)w.most * kPlanTile;
     const int id = tile[0], first = tile[1], count = tile[2];
-    const int rank = id < 0 ? 0 : a.ranks[id];
+    const int rank = id < 0 ? 0 : min(max(a.ranks[id], 0), a.rank);
     if (rank == 0 && a.base == a.y) return;
     const int chunks = (rank + 15) / 16;
     const int place = first + min(col, count - 1), mine = order[place];

@@ -230,6 +230,35 @@ def test_ending(alpha, early):
     assert got.beams.done[b.lengths >= 19].all()
 
 
+@pytest.mark.parametrize("R, K, V, E", [(1, 64, 151936, 0), (1, 64, 151936, 16), (2, 40, 100001, 3), (1, 33, 524288, 16)])
+def test_more_candidates_than_are_ranked_at_once(R, K, V, E):
+    """Lists of many spans and beams, taken one by one; and lists of equal totals, which no bound cuts."""
+    print(f"  case: {R} x {K} x {V}, {E} eos", flush=True)
+    eos = [V // 3 + i for i in range(E)]
+    x = rows(V + K, R * K, V, torch.bfloat16)
+    if E:
+        x[:, eos] = x.amax(1, keepdim=True) - torch.rand(R * K, E, device=DEV).bfloat16()
+    b = some_beams(V, R, K)
+    check(x, b, eos=eos)
+    b.scores.fill_(-2.0)
+    check(x[:1].expand(R * K, V), b, eos=eos, max_tokens=60)
+    check(torch.zeros(R * K, V, device=DEV), b, eos=eos)
+
+
+def test_equal_beams_past_the_ranked_list():
+    """As many equal totals as a request has candidates: by beam, then token."""
+    for K, V in ((16, 60000), (30, 20001)):
+        b = some_beams(2, 3, K)
+        b.scores.fill_(-1.0)
+        x = rows(5, 1, V, torch.float16).expand(3 * K, V)
+        got = check(x, b, eos=[4])
+        if V % 8 == 0:
+            # (rows that begin at other addresses are summed in another order: their logarithms are
+            # equal within the bound above, and check() has looked at that)
+            assert (got.parents.view(3, K)[:, :2] - torch.tensor([[0], [K], [2 * K]], device=DEV) == torch.tensor([0, 1], device=DEV)).all()
+        check(torch.ones(3 * K, V, device=DEV), b, eos=[0, 2])
+
+
 def test_many_eos_and_a_vocabulary_of_nothing_else():
     got = check(rows(13, 8, 16), some_beams(13, 2, 4), eos=range(16))
     assert got.beams.done.all()
