@@ -181,8 +181,9 @@ constexpr int kDownWaves = 4;
 // h = A x: grid (splits, tiles), 16 tokens of one adapter a workgroup.  The splits and their waves take k
 // in turn, U steps each, straight from memory to the matrix instructions, 16 RT ranks at a time; a
 // workgroup's sums meet in LDS, the splits' in the second product.  (One workgroup a tile, of 16 waves:
-// 1 x 4096 6.8 us against 3.8, 250 tokens of 64 adapters 9.3 against 5.3: a CU alone is slow to
-// bring in a whole A.)  Bound by A's way from memory for few tokens an adapter, by x's for many.
+// 1 x 4096 6.8 us against 3.8, 250 tokens of 64 adapters 9.3 against 4.6: a CU alone is slow to
+// bring in a whole A.)  Bound by A's way from memory for few tokens an adapter; for many by x's, and
+// with more ranks by A's from the L2 (4001 x 4097: rank 16 11 us, rank 48 20).
 template <int DX, int DT, int RT, int U, bool ALIGNED>
 __global__ __launch_bounds__(64 * kDownWaves) void k_adapter_down(const fie_adapter_args a, const AdapterWork w)
 {
@@ -337,7 +338,9 @@ template <int DT> struct UpOperand {
 // the matrix instructions take it (CH times 16 ranks; CH 0: any number, built anew for each step).  fp16
 // tokens are brought to an exponent of their own first, so that no part overflows.  Results cross LDS
 // within the wave, so that base and y are read and written along their rows whatever these begin at.
-// Bound by base and y for many tokens an adapter, by B for few.
+// Bound by base and y for many tokens an adapter (4001 x 4096, rank 16: 16 us, 4.1 TB/s; rank 48 29,
+// B's way from the L2; at 4099 channels, a channel a lane, 40), by B for few (250 x 16384 of 64 adapters
+// 15.7 us, 3.7 TB/s).  Two tiles a wave that share B's registers took longer, 43 and 60: half the waves.
 template <int DT, int DY, int DB, int CH>
 __global__ __launch_bounds__(64 * kUpWaves) void k_adapter_up(const fie_adapter_args a, const AdapterWork w, int wide, int steps)
 {

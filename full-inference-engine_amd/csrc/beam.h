@@ -204,7 +204,9 @@ FIE_DEV int beam_deep(const BeamRow<DT>& row, int first, int last, int most, Bea
 // One pass over the logits.  The first tile gives a bound: every wave finds what a quarter of the
 // wanted candidates reach among its 64 lanes' maxima, and the least of the four waves' bounds is
 // reached by all of them.  What reaches it is listed, in later tiles too; at the end the lists
-// are cut by such a bound of their own and ranked.
+// are cut by such a bound of their own and ranked.  Four instructions a logit and the exponential;
+// 512 rows of 151936 in bf16 35 us (4.4 TB/s, a large copy has 4.9), 4 rows 6.7, 80 rows of 50001 in
+// fp32 8.
 template <int DT>
 __global__ __launch_bounds__(kBeamThreads, kBeamHold<DT>) void k_beam_scan(const fie_beam_args a, const BeamWork w)
 {
@@ -558,7 +560,8 @@ FIE_DEV void pick_one_by_one(const fie_beam_args& a, const BeamWork& w, int r, i
 }
 
 // A workgroup a request: its rows' logarithms, a wave each, then its best continuations, then the pool.
-// Bound by the chain of these steps.
+// Bound by the chain of these steps, and by how much code each of them has to bring in: 1 request of 4
+// beams 9 us, 64 of 8 beams 11 (one candidate after the other 9 and 14).
 __global__ __launch_bounds__(1024) void k_beam_pick(const fie_beam_args a, const BeamWork w, int wanted)
 {
     extern __shared__ uint64_t L[];

