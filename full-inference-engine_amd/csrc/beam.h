@@ -351,6 +351,7 @@ FIE_DEV double beam_value(uint64_t k)
 
 // length^penalty.  (The exponential and the logarithm as they are shared with a row's: a power's own code
 // takes longer to come in than to run.)
+__host__ FIE_DEV bool beam_power(double penalty) { return penalty != 0.0 && penalty != 1.0; }
 FIE_DEV double beam_scale(int length, double penalty)
 {
     if (penalty == 1.0) return (double)length;
@@ -361,6 +362,7 @@ FIE_DEV double beam_scale(int length, double penalty)
 // What a request's workgroup settles before the pool.
 struct BeamChoice {
     double lse[FIE_MAX_BEAMS];                          // log of a row's sum, less its maximum
+    double scale;                                       // of an answer that ends here
     float top[FIE_MAX_BEAMS], prior[FIE_MAX_BEAMS];
     int32_t count[FIE_MAX_BEAMS];
     uint64_t live_key[FIE_MAX_BEAMS];
@@ -374,12 +376,13 @@ struct BeamChoice {
 constexpr int kPickEach = 4;                            // candidates of a thread
 constexpr int kPickList = 1024;                         // those that are ranked
 
-// A thread's n-th candidate: the waves take turns, so that each has its share of the good beams' (wave
-// after wave, one of bad beams alone lowered the bound to all there were: 64 x 8 20 us).
+// A thread's n-th candidate: the waves take turns, another first each time, so that each has its share of
+// the good beams' and of the lists' heads (a wave of bad beams alone, or of each list's last
+// alone where as many are listed as there are waves, lowers the bound to all there are: 20 us for 10).
 FIE_DEV int pick_index(int n)
 {
-    const int waves = blockDim.x >> 6;
-    return ((threadIdx.x & 63) + 64 * n) * waves + (threadIdx.x >> 6);
+    const int waves = blockDim.x >> 6, turn = (threadIdx.x & 63) + 64 * n;
+    return turn * waves + ((threadIdx.x >> 6) + turn) % waves;
 }
 
 FIE_DEV bool is_eos(const fie_beam_args& a, int token)
@@ -592,9 +595,10 @@ __global__ __launch_bounds__(1024) void k_beam_pick(const fie_beam_args a, const
     }
     if (tid == 0) C.listed = 0;
     __syncthreads();
+    const int workers = beam_power(a.length_penalty) ? waves - 1 : waves;       // (the last wave has the length's power)
 #pragma unroll 1
-    for (int b = wave; b < K; b += waves) {
-        if (C.count[b] == 0) continue;
+    for (int b = wave; b < K; b += workers) {
+        if (wave >= workers || C.count[b] == 0) continue;
         const BeamSpan sp = lane < w.spans ? w.span[((int64_t)r * K + b) * w.spans + lane] : BeamSpan{0.0, -kLargest, 0};
         float m = sp.top;
         for (int d = 32; d; d >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d, 64));
@@ -605,8 +609,12 @@ __global__ __launch_bounds__(1024) void k_beam_pick(const fie_beam_args a, const
             C.lse[b] = log(s);
         }
     }
-    const double scale = beam_scale(max(was ? length : length + 1, 1), a.length_penalty);
+    if (wave == waves - 1) {                            // (where it is none, at no cost)
+        const double scale = beam_scale(max(was ? length : length + 1, 1), a.length_penalty);
+        if (lane == 0) C.scale = scale;
+    }
     __syncthreads();
+    const double scale = C.scale;
     bool ranked = wanted > 0;
     if (ranked) {
 #pragma unroll

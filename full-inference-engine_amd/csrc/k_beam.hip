@@ -47,8 +47,8 @@ static hipError_t beam_run(const fie_beam_args& a, hipStream_t st)
     const int all = a.beams * w.spans * w.most, wanted = a.beams * (1 + a.eos_count);
     const size_t lists = (size_t)w.spans * w.most * 8, own = (size_t)a.beams * w.most * 8;
     const bool ranked = all <= 1024 * kPickEach && wanted <= kPickList / 4;
-    const int fits = (int)std::max<size_t>(1, (((size_t)140 << 10) - own) / lists);
-    const int waves = std::min(fits, ranked ? std::max(4, std::min(16, (all + 127) / 128)) : std::min(a.beams, 16));
+    const int fits = (int)std::max<size_t>(2, (((size_t)140 << 10) - own) / lists);
+    const int waves = std::min(fits, (ranked ? std::max(4, std::min(15, (all + 127) / 128)) : std::min(a.beams, 15)) + beam_power(a.length_penalty));
     const bool at_once = ranked && all <= 64 * waves * kPickEach;
     const size_t lds = std::max(waves * lists + own, at_once ? (size_t)kPickList * 32 : 0);
     k_beam_pick<<<(unsigned)a.requests, 64 * waves, lds, st>>>(a, w, at_once ? wanted : 0);
