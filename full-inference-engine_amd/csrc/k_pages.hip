@@ -100,8 +100,9 @@ static hipError_t pages_step(const fie_pages_args& a, hipStream_t st)
     const int bits = mark_bits(a.rows);
     const size_t area = std::max<size_t>(small ? (size_t)a.rows * a.wide : 0, (size_t)3 << bits);
     const size_t lds = ((size_t)3 * a.rows + s.nblocks + area) * 4;
-    if (small) k_pages_grow<true><<<1, kPageThreads, lds, st>>>(s, w, a.parents, a.lengths, a.granted, bits, (int)area);
-    else k_pages_grow<false><<<1, kPageThreads, lds, st>>>(s, w, a.parents, a.lengths, a.granted, bits, (int)area);
+    if (small && a.rows <= 64) k_pages_grow<true, 256><<<1, 256, lds, st>>>(s, w, a.parents, a.lengths, a.granted, bits, (int)area);
+    else if (small) k_pages_grow<true, kPageThreads><<<1, kPageThreads, lds, st>>>(s, w, a.parents, a.lengths, a.granted, bits, (int)area);
+    else k_pages_grow<false, kPageThreads><<<1, kPageThreads, lds, st>>>(s, w, a.parents, a.lengths, a.granted, bits, (int)area);
     e = hipGetLastError();
     if (e != hipSuccess || !a.lengths) return e;
     return copy_pages(a, PageList{w.copies, nullptr, nullptr, w.count, 0, a.pages}, a.rows, st);
@@ -111,13 +112,17 @@ static hipError_t pages_compact(const fie_pages_args& a, hipStream_t st)
 {
     const PageState s = page_state(a);
     const PageScratch w = page_scratch(a.scratch, a.pages, a.rows, nullptr);
-    k_pages_holes<<<(unsigned)s.nblocks, kPageThreads, 0, st>>>(s, w, a.live);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    const int64_t entries = std::max((int64_t)a.rows * a.wide, (int64_t)a.pages / 2);
-    k_pages_rename<<<(unsigned)std::min<int64_t>((entries + 255) / 256, 8 * std::max(cu_count(), 1)), 256, 0, st>>>(s, w);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    hipError_t e;
+    if (s.nblocks <= 2 && (int64_t)a.rows * a.wide <= kSmallTable) {
+        k_pages_holes<true><<<1, kPageThreads, 0, st>>>(s, w, a.live);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    } else {
+        k_pages_holes<false><<<(unsigned)s.nblocks, kPageThreads, 0, st>>>(s, w, a.live);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        const int64_t entries = std::max((int64_t)a.rows * a.wide, (int64_t)a.pages / 2);
+        k_pages_rename<<<(unsigned)std::min<int64_t>((entries + 255) / 256, 8 * std::max(cu_count(), 1)), 256, 0, st>>>(s, w);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
     return copy_pages(a, PageList{nullptr, w.movers, w.list, w.count, 0, a.pages}, a.pages / 2, st);
 }
 

@@ -45,7 +45,7 @@ FIE_DEV int page_held(const PageState& s, const int32_t* lengths, int i, int par
 // take each other's.  A page is in one column of all rows that hold it, so one workgroup sees all
 // changes to its count: what is added first, then, behind a barrier, what is taken; a count that
 // gets to 0 is a page set free, counted by blocks in LDS (`freed`, [nblocks]).
-template <int C>
+template <int C, int T>
 FIE_DEV void fork_columns(const PageState& s, const int32_t* parents, const int32_t* lengths, int c0,
                           int32_t* tile, int32_t* keep, uint16_t* from, int32_t* freed)
 {
@@ -53,23 +53,23 @@ FIE_DEV void fork_columns(const PageState& s, const int32_t* parents, const int3
     auto each = [&](auto&& f) {                         // f(row, column)
         if constexpr (C > 0) {
 #pragma unroll 2
-            for (int i = tid; i < s.rows * C; i += kPageThreads) f(i / C, i % C);
+            for (int i = tid; i < s.rows * C; i += T) f(i / C, i % C);
         } else {
 #pragma unroll 1
-            for (int row = tid >> 6; row < s.rows; row += kPageThreads / 64)
+            for (int row = tid >> 6; row < s.rows; row += T / 64)
 #pragma unroll 1
                 for (int c = tid & 63; c < s.wide; c += 64) f(row, c);
         }
     };
     each([&](int row, int c) { tile[row * pitch + c] = c0 + c < s.wide ? s.table[(int64_t)row * s.wide + c0 + c] : -1; });
 #pragma unroll 1
-    for (int i = tid; i < s.rows; i += kPageThreads) {
+    for (int i = tid; i < s.rows; i += T) {
         const int p = page_parent(parents, i, s.rows);
         keep[i] = (int)(((uint32_t)page_held(s, lengths, i, p) + (uint32_t)s.page - 1u) / (uint32_t)s.page);
         from[i] = (uint16_t)(p < 0 ? i : p);            // without a parent nothing is kept
     }
 #pragma unroll 1
-    for (int i = tid; i < s.nblocks; i += kPageThreads) freed[i] = 0;
+    for (int i = tid; i < s.nblocks; i += T) freed[i] = 0;
     __syncthreads();
     auto fresh = [&](int row, int c) { return c0 + c < keep[row] ? tile[(int)from[row] * pitch + c] : -1; };
     each([&](int row, int c) {
@@ -94,17 +94,17 @@ __global__ __launch_bounds__(kPageThreads) void k_pages_fork(const PageState s, 
     extern __shared__ int32_t L[];
     int32_t* const keep = L + s.rows * C;
     int32_t* const freed = keep + s.rows;
-    fork_columns<C>(s, parents, lengths, blockIdx.x * C, L, keep, (uint16_t*)(freed + s.nblocks), freed);
+    fork_columns<C, kPageThreads>(s, parents, lengths, blockIdx.x * C, L, keep, (uint16_t*)(freed + s.nblocks), freed);
     __syncthreads();
 #pragma unroll 1
     for (int b = threadIdx.x; b < s.nblocks; b += kPageThreads)
         if (freed[b]) atomicAdd(&s.blocks[b], freed[b]);
 }
 
-// Exclusive prefix sums over the threads of a workgroup of 1024, sums past 2^30 as 2^30 (a wave's
-// own are below 2^31); all the sums.  `part` [16].
+// Exclusive prefix sums over the threads of a workgroup of T, sums past 2^30 as 2^30 (a wave's
+// own are below 2^31); all the sums.  `part` [T / 64].
 constexpr int kScanMost = 1 << 30;
-FIE_DEV int block_scan(int v, int32_t* part, int* all)
+template <int T> FIE_DEV int block_scan(int v, int32_t* part, int* all)
 {
     const int wave = threadIdx.x >> 6;
     const int incl = (int)wave_incl_scan_u32((uint32_t)v);
@@ -113,7 +113,7 @@ FIE_DEV int block_scan(int v, int32_t* part, int* all)
     __syncthreads();
     int64_t before = 0, sum = 0;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) {
+    for (int w = 0; w < T / 64; ++w) {
         const int t = part[w];
         before += w < wave ? t : 0;
         sum += t;
@@ -129,10 +129,10 @@ struct PageMarks {
     uint32_t* best;
     int bits;
     FIE_DEV int slot(int p) const { return (int)(((uint32_t)p * 0x9E3779B1u) >> (32 - bits)); }
-    FIE_DEV void clear() const
+    template <int T> FIE_DEV void clear() const
     {
 #pragma unroll 1
-        for (int i = threadIdx.x; i < 1 << bits; i += kPageThreads) {
+        for (int i = threadIdx.x; i < 1 << bits; i += T) {
             key[i] = -1;
             count[i] = 0;
             best[i] = 0;
@@ -173,8 +173,8 @@ static inline int mark_bits(int rows)
 // and a launch less).  A chain of dependent steps through memory: parents, lengths, a row's last
 // page, its count, the blocks' pages.  512 rows 10 us (marks in memory, unrolled loops: 22), 4 rows with
 // their table 9.8.
-template <bool FORK>
-__global__ __launch_bounds__(kPageThreads) void k_pages_grow(const PageState s, const PageScratch w, const int32_t* parents,
+template <bool FORK, int T>
+__global__ __launch_bounds__(T) void k_pages_grow(const PageState s, const PageScratch w, const int32_t* parents,
                                                              const int32_t* lengths, uint8_t* granted, int bits, int room)
 {
     extern __shared__ int32_t L[];
@@ -187,10 +187,10 @@ __global__ __launch_bounds__(kPageThreads) void k_pages_grow(const PageState s, 
     int32_t* const area = base + s.nblocks;
     const PageMarks marks{area, area + (1 << bits), (uint32_t*)(area + (2 << bits)), bits};
     const int tid = threadIdx.x, lane = tid & 63;
-    const int each = (s.rows + kPageThreads - 1) / kPageThreads, first = tid * each, last = min(first + each, s.rows);
+    const int each = (s.rows + T - 1) / T, first = tid * each, last = min(first + each, s.rows);
     if (tid == 0) copies = 0;
     if constexpr (FORK) {
-        fork_columns<0>(s, parents, lengths, 0, area, keep, (uint16_t*)end, base);
+        fork_columns<0, T>(s, parents, lengths, 0, area, keep, (uint16_t*)end, base);
         __syncthreads();
     }
     const uint32_t page = (uint32_t)s.page;
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kPageThreads) void k_pages_grow(const PageState s, 
         held[i] = h;
         keep[i] = up(h);
     }
-    if (lengths) marks.clear();
+    if (lengths) marks.template clear<T>();
     __syncthreads();
 #pragma unroll 1
     for (int i = first; i < last; ++i) {
@@ -233,14 +233,14 @@ __global__ __launch_bounds__(kPageThreads) void k_pages_grow(const PageState s, 
         mine += demand;
     }
     int sum;
-    int at = block_scan(mine, part, &sum);
+    int at = block_scan<T>(mine, part, &sum);
     // where the free pages of each block begin
     int free = 0;
 #pragma unroll 1
-    for (int b0 = 0; b0 < s.nblocks; b0 += kPageThreads) {
+    for (int b0 = 0; b0 < s.nblocks; b0 += T) {
         const int b = b0 + tid;
         const int v = b < s.nblocks ? s.blocks[b] + (FORK ? base[b] : 0) : 0;
-        const int before = block_scan(v, part, &sum);
+        const int before = block_scan<T>(v, part, &sum);
         if (b < s.nblocks) base[b] = free + before;
         free += sum;
     }
@@ -257,11 +257,11 @@ __global__ __launch_bounds__(kPageThreads) void k_pages_grow(const PageState s, 
     if (lane == 0) part[tid >> 6] = need;
     __syncthreads();
 #pragma unroll
-    for (int v = 0; v < 16; ++v) need = max(need, part[v]);
+    for (int v = 0; v < T / 64; ++v) need = max(need, part[v]);
     // the first `need` free pages, a wave a block; the blocks' counts without them
     int32_t* const list = need <= room ? area : w.list;
 #pragma unroll 1
-    for (int b = __builtin_amdgcn_readfirstlane(tid >> 6); b < s.nblocks && base[b] < need; b += kPageThreads / 64) {
+    for (int b = __builtin_amdgcn_readfirstlane(tid >> 6); b < s.nblocks && base[b] < need; b += T / 64) {
         const int next = b + 1 < s.nblocks ? base[b + 1] : free;
         if (next == base[b]) continue;
         int rank = base[b];
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(kPageThreads) void k_pages_grow(const PageState s, 
     }
     if constexpr (FORK) {
 #pragma unroll 1
-        for (int b = tid; b < s.nblocks; b += kPageThreads) {
+        for (int b = tid; b < s.nblocks; b += T) {
             const int next = b + 1 < s.nblocks ? base[b + 1] : free;
             s.blocks[b] = next - max(base[b], min(next, need));
         }
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(kPageThreads) void k_pages_grow(const PageState s, 
     __syncthreads();
     // a page for each that is wanted: the first row whose sum is past its number has it
 #pragma unroll 1
-    for (int n = tid; n < need; n += kPageThreads) {
+    for (int n = tid; n < need; n += T) {
         int lo = 0, hi = s.rows - 1;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
@@ -320,59 +320,81 @@ __global__ __launch_bounds__(kPageThreads) void k_pages_grow(const PageState s, 
     if (tid == 0) *w.count = copies;
 }
 
-// A workgroup 1024 pages: free ones below the count of used pages are holes, used ones past it
-// move; both are numbered in order.
-__global__ __launch_bounds__(kPageThreads) void k_pages_holes(const PageState s, const PageScratch w, int32_t* live)
+// Moved pages and used pages of a compaction.
+struct PageMoves {
+    int moved, used;
+};
+
+// The block's 1024 pages: free ones below the count of used pages are holes, used ones past it move;
+// both are numbered in order.
+FIE_DEV PageMoves number_block(const PageState& s, const PageScratch& w, int block, int32_t* part)
 {
-    __shared__ int32_t part[16];
-    const int tid = threadIdx.x, block = blockIdx.x;
-    int free = 0, before = 0;
+    const int tid = threadIdx.x;
+    int free = 0, before = 0, below = 0;
     for (int b = tid; b < s.nblocks; b += kPageThreads) free += s.blocks[b];
-    block_scan(free, part, &free);
+    block_scan<kPageThreads>(free, part, &free);
     const int used = s.pages - free, edge = used / kPageBlock;      // the block that the count falls into
-    int below = 0;
     for (int b = tid; b < s.nblocks; b += kPageThreads) {
         before += b < block ? s.blocks[b] : 0;
         below += b < edge ? s.blocks[b] : 0;
     }
     const int q = edge * kPageBlock + tid;
     below += q < used && s.refs[q] == 0;
-    block_scan(before, part, &before);
-    block_scan(below, part, &below);                                // free pages below the count
+    block_scan<kPageThreads>(before, part, &before);
+    block_scan<kPageThreads>(below, part, &below);                  // free pages below the count
     const int p = block * kPageBlock + tid;
     const bool in = p < s.pages, is_free = in && s.refs[p] == 0;
     int sum;
-    const int rank = before + block_scan(is_free, part, &sum);     // of free pages below p
+    const int rank = before + block_scan<kPageThreads>(is_free, part, &sum);    // of free pages below p
     if (is_free && p < used) w.list[rank] = p;
     if (in && !is_free && p >= used) {
         const int n = (p - rank) - (used - below);                  // used pages below p, less those below the count
         w.movers[n] = p;
         w.order[p] = n;
     }
-    if (block == 0 && tid == 0) {
-        w.count[0] = below;
-        w.count[1] = used;
-        if (live) *live = used;
-    }
+    return PageMoves{below, used};
 }
 
-// Table entries, counts and blocks after the move.
-__global__ __launch_bounds__(256) void k_pages_rename(const PageState s, const PageScratch w)
+// Table entries, counts and blocks after the move: every `step`-th from `at` on.
+FIE_DEV void rename_pages(const PageState& s, const PageScratch& w, PageMoves m, int64_t at, int64_t step)
 {
-    const int moved = w.count[0], used = w.count[1];
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)s.rows * s.wide, step = (int64_t)gridDim.x * 256;
+    const int64_t n = (int64_t)s.rows * s.wide;
     for (int64_t i = at; i < n; i += step) {
         const int p = s.table[i];
-        if (p >= used) s.table[i] = w.list[w.order[p]];
+        if (p >= m.used) s.table[i] = w.list[w.order[p]];
     }
-    for (int64_t i = at; i < moved; i += step) {
+    for (int64_t i = at; i < m.moved; i += step) {
         s.refs[w.list[i]] = s.refs[w.movers[i]];
         s.refs[w.movers[i]] = 0;
     }
     for (int64_t b = at; b < s.nblocks; b += step) {
         const int size = min(kPageBlock, s.pages - (int)b * kPageBlock);
-        s.blocks[b] = max(0, min(size, (int)(b + 1) * kPageBlock - used - (kPageBlock - size)));
+        s.blocks[b] = max(0, min(size, (int)b * kPageBlock + size - m.used));
     }
+}
+
+// A workgroup a block; ALL: one workgroup all of a small pool's, and its table (8 rows: 2 us and a
+// launch less).
+template <bool ALL>
+__global__ __launch_bounds__(kPageThreads) void k_pages_holes(const PageState s, const PageScratch w, int32_t* live)
+{
+    __shared__ int32_t part[16];
+    PageMoves m{0, 0};
+    if constexpr (ALL) {
+        for (int b = 0; b < s.nblocks; ++b) m = number_block(s, w, b, part);
+        __syncthreads();
+        rename_pages(s, w, m, threadIdx.x, kPageThreads);
+    } else m = number_block(s, w, blockIdx.x, part);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        w.count[0] = m.moved;
+        w.count[1] = m.used;
+        if (live) *live = m.used;
+    }
+}
+
+__global__ __launch_bounds__(256) void k_pages_rename(const PageState s, const PageScratch w)
+{
+    rename_pages(s, w, PageMoves{w.count[0], w.count[1]}, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
 }
 
 // Where a call's copies stand: k_pages_grow's, lists of two arrays, or the caller's.
