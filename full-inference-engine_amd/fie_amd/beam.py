@@ -252,15 +252,21 @@ class BeamSearch:
         """One step of every request (``beam_step``); the beams are written over."""
         return beam_step(logits, self.beams, inplace=True, history=self._history, **self._settings)
 
-    def restart(self, requests: Sequence[int]) -> None:
-        """These requests' slots begin anew."""
-        if not len(requests):
-            return
+    def _slots(self, requests: Sequence[int]) -> torch.Tensor:
         if any(not 0 <= r < self.requests for r in requests):
             raise ValueError(f"requests must be in [0, {self.requests})")
-        at = torch.tensor(list(requests), dtype=torch.int64).to(self.device)
+        return torch.tensor(list(requests), dtype=torch.int64).to(self.device)
+
+    def restart(self, requests: Sequence[int]) -> None:
+        """These requests' slots begin anew."""
+        at = self._slots(requests)
         for t, fresh in zip(self.beams, first_beams(len(requests), self.count, self.device)):
             t[at] = fresh
+
+    def stop(self, requests: Sequence[int]) -> None:
+        """These requests are done as they are, or were never begun (slots that only fill up the batch): their
+        logits are not read until ``restart``.  Beams that had not ended are dropped."""
+        self.beams.done[self._slots(requests)] = True
 
     def all_done(self) -> bool:
         """Whether every request is done (waits for the device)."""

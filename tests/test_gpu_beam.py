@@ -276,6 +276,15 @@ def test_strides_and_alignment(at, pad, dtype):
     check(wide[:, at:at + V].t().contiguous().t(), some_beams(16, R, K), eos=[0])
 
 
+def test_past_32_bit_offsets():
+    """Rows more than 2^32 bytes apart."""
+    R, K, V, step = 2, 2, 5000, 3 * (1 << 30) // 2 + 1
+    room = torch.empty(3 * step + V, dtype=torch.bfloat16, device=DEV)
+    x = room.as_strided((R * K, V), (step, 1))
+    x.copy_(rows(21, R * K, V, torch.bfloat16))
+    check(x, some_beams(21, R, K), eos=[7])
+
+
 def test_inplace_and_history():
     R, K, V, T = 3, 4, 700, 5
     rows_ = R * K

@@ -127,6 +127,26 @@ def test_a_whole_search(beams, alpha):
     assert (memory[:, 0] == torch.arange(5, 5 + R, device=DEV).repeat_interleave(beams)).all()
 
 
+def test_slots_that_fill_up_the_batch():
+    """Stopped slots are not read, change nothing, and begin when they are asked to."""
+    V, beams = 50, 3
+    x = torch.randn(3 * beams, V, device=DEV, generator=torch.Generator(device=DEV).manual_seed(3))
+    alone, search = BeamSearch(DEV, 1, beams, max_tokens=5, eos=[1]), BeamSearch(DEV, 3, beams, max_tokens=5, eos=[1])
+    search.stop([0, 2])
+    x[:beams] = x[2 * beams:] = float("nan")
+    for _ in range(3):
+        got, want = search.step(x), alone.step(x[beams:2 * beams].clone())
+        assert got.parents[:beams].tolist() == list(range(beams)) and (got.tokens[2 * beams:] == 0).all()
+        assert torch.equal(got.tokens[beams:2 * beams], want.tokens) and torch.equal(got.parents[beams:2 * beams] - beams, want.parents)
+    assert search.answers(0) == [] and search.beams.lengths.tolist() == [0, 3, 0]
+    search.restart([2])
+    x[2 * beams:] = 0.0
+    assert search.step(x).parents[2 * beams:].tolist() == [2 * beams] * beams
+    search.stop([])
+    search.stop([1])
+    assert not [a for a in search.answers(1) if not a.ended]
+
+
 def test_slots_begin_anew():
     V, steps, beams = 30, 6, 3
     t = tables(9, V, steps)
@@ -155,7 +175,8 @@ def test_slots_begin_anew():
     assert search.beams.done[0]                         # six tokens
     search.restart([])
     for bad in ([2], [-1]):
-        with pytest.raises(ValueError):
-            search.restart(bad)
+        for call in (search.restart, search.stop):
+            with pytest.raises(ValueError):
+                call(bad)
     with pytest.raises(ValueError):
         search.answers(2)
