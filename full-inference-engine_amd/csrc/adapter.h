@@ -338,11 +338,12 @@ template <int DT> struct UpOperand {
 // the matrix instructions take it (CH times 16 ranks; CH 0: any number, built anew for each step).  fp16
 // tokens are brought to an exponent of their own first, so that no part overflows.  Results cross LDS
 // within the wave, so that base and y are read and written along their rows whatever these begin at.
-// Bound by base and y for many tokens an adapter (4001 x 4096, rank 16: 16 us, 4.1 TB/s; rank 48 29,
-// B's way from the L2; at 4099 channels, a channel a lane, 40), by B for few (250 x 16384 of 64 adapters
-// 15.7 us, 3.7 TB/s).  Two tiles a wave that share B's registers took longer, 43 and 60: half the waves.
+// Bound by base and y for many tokens an adapter (4001 x 4096, rank 16: 16 us, 4.1 TB/s; rank 48 24 and
+// rank 64 37, B's way from the L2; rank 48 at 4099 channels, a channel a lane, 36), by B for few (250 x
+// 16384 of 64 adapters 15 us, 3.8 TB/s).  Held to four waves a SIMD (rank 48 29 us with three, two tiles a
+// wave that share B's registers 43 with two); B's channels at every 128 bytes cost rank 64 52 us.
 template <int DT, int DY, int DB, int CH>
-__global__ __launch_bounds__(64 * kUpWaves) void k_adapter_up(const fie_adapter_args a, const AdapterWork w, int wide, int steps)
+__global__ __launch_bounds__(64 * kUpWaves, 4) void k_adapter_up(const fie_adapter_args a, const AdapterWork w, int wide, int steps)
 {
     using Op = Operand<DT>;
     using Part = UpOperand<DT>;
@@ -389,7 +390,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void k_adapter_up(const fie_adapter_
             for (int c = 0; c < CH; ++c) fh[c] = c < chunks ? p[c].get(e, trailing) : u32x4_t{0, 0, 0, 0};
     }
     float* const room = stage[wave];
-    const uint8_t* const b0 = (const uint8_t*)a.b + (int64_t)max(id, 0) * a.n * a.rank * Op::SIZE + 16 * (DT == FIE_F32 ? group : group & 1);
+    const uint8_t* const b0 = (const uint8_t*)a.b + (int64_t)max(id, 0) * a.n * a.b_pitch * Op::SIZE + 16 * (DT == FIE_F32 ? group : group & 1);
     for (int s = 0; s < steps; ++s) {
         const int n0 = (blockIdx.x * steps + s) * kUpChannels;
         if (n0 >= a.n) return;
@@ -397,17 +398,24 @@ __global__ __launch_bounds__(64 * kUpWaves) void k_adapter_up(const fie_adapter_
         // repeat its last one's, channels past n the last
         const bool four = wide && n0 + kUpChannels <= a.n;
         const int nw = n0 + 4 * col, nl = min(n0 + lane, a.n - 1);
-        typename Raw<DB>::four_t r4[4];
-        typename Raw<DB>::one_t r1[16];
+        typedef typename Raw<DB>::one_t base_t;
+        typedef typename Raw<DB>::four_t base4_t;
+        constexpr int W = sizeof(base4_t) / 4;          // words of four
+        uint32_t raw[16];                               // of either kind, in the same registers
         if (a.base) {
             if (four) {                                 // 4 channels a lane of 4 tokens
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    r4[i] = *(const typename Raw<DB>::four_t*)((const typename Raw<DB>::one_t*)a.base + (int64_t)__shfl(mine, 4 * i + group, 64) * a.base_stride + nw);
+                for (int i = 0; i < 4; ++i) {
+                    const base4_t v = *(const base4_t*)((const base_t*)a.base + (int64_t)__shfl(mine, 4 * i + group, 64) * a.base_stride + nw);
+                    __builtin_memcpy(&raw[W * i], &v, sizeof v);
+                }
             } else                                      // a channel a lane of 16
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    r1[r] = ((const typename Raw<DB>::one_t*)a.base + (int64_t)__builtin_amdgcn_readlane(mine, r) * a.base_stride)[nl];
+                for (int r = 0; r < 16; ++r) {
+                    const base_t v = ((const base_t*)a.base + (int64_t)__builtin_amdgcn_readlane(mine, r) * a.base_stride)[nl];
+                    if constexpr (DB == FIE_F32) raw[r] = __float_as_uint(v);
+                    else raw[r] = v;
+                }
         }
         if (rank) {
             f32x4_t acc[kUpCols];
@@ -415,20 +423,24 @@ __global__ __launch_bounds__(64 * kUpWaves) void k_adapter_up(const fie_adapter_
             for (int q = 0; q < kUpCols; ++q) acc[q] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
             const uint8_t* br[kUpCols];
 #pragma unroll
-            for (int q = 0; q < kUpCols; ++q) br[q] = b0 + (int64_t)min(n0 + 16 * q + col, a.n - 1) * a.rank * Op::SIZE;
+            for (int q = 0; q < kUpCols; ++q) br[q] = b0 + (int64_t)min(n0 + 16 * q + col, a.n - 1) * a.b_pitch * Op::SIZE;
             if constexpr (CH > 0) {
-                u32x4_t fb[CH][kUpCols];
+                constexpr int Q = CH == 4 ? 2 : kUpCols;        // blocks at a time, as far as registers go
 #pragma unroll
-                for (int c = 0; c < CH; ++c)
-                    if (c < chunks)
+                for (int q0 = 0; q0 < kUpCols; q0 += Q) {
+                    u32x4_t fb[CH][Q];
 #pragma unroll
-                        for (int q = 0; q < kUpCols; ++q) fb[c][q] = *(const u32x4_t*)(br[q] + c * 16 * Op::SIZE);
-                __builtin_amdgcn_sched_barrier(0);
+                    for (int c = 0; c < CH; ++c)
+                        if (c == 0 || c < chunks)
 #pragma unroll
-                for (int c = 0; c < CH; ++c)
-                    if (c < chunks)
+                            for (int q = 0; q < Q; ++q) fb[c][q] = *(const u32x4_t*)(br[q0 + q] + c * 16 * Op::SIZE);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int q = 0; q < kUpCols; ++q) acc[q] = Op::mul(fb[c][q], fh[c], acc[q]);
+                    for (int c = 0; c < CH; ++c)
+                        if (c == 0 || c < chunks)
+#pragma unroll
+                            for (int q = 0; q < Q; ++q) acc[q0 + q] = Op::mul(fb[c][q], fh[c], acc[q0 + q]);
+                }
             } else
                 for (int c = 0; c < chunks; ++c) {
                     Part p;
@@ -448,7 +460,11 @@ __global__ __launch_bounds__(64 * kUpWaves) void k_adapter_up(const fie_adapter_
                 const int r = 4 * i + group;
                 const int64_t t = __shfl(mine, r, 64);
                 float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (a.base) Raw<DB>::open(r4[i], v);
+                if (a.base) {
+                    base4_t b;
+                    __builtin_memcpy(&b, &raw[W * i], sizeof b);
+                    Raw<DB>::open(b, v);
+                }
                 if (rank) {
                     const f32x4_t d = *(const f32x4_t*)&room[r * kPitch + 4 * col];
 #pragma unroll
@@ -460,7 +476,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void k_adapter_up(const fie_adapter_
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int64_t t = __builtin_amdgcn_readlane(mine, r);
-                float v = a.base ? Raw<DB>::value(r1[r]) : 0.0f;
+                float v = a.base ? Operand<DB>::value(raw[r]) : 0.0f;
                 if (rank) v += room[r * kPitch + lane];
                 if (r < count && n0 + lane < a.n) y[t * a.y_stride + n0 + lane] = Raw<DY>::close(v);
             }

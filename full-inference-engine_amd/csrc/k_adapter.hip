@@ -7,7 +7,7 @@ namespace fie {
 
 static int64_t plan_most(int64_t tokens, int64_t adapters) { return tokens / kTileTokens + std::min(tokens, adapters + 1); }
 
-constexpr int kDownSteps = 4;                           // of a wave at a time
+constexpr int kDownSteps = 4;                           // of a wave at a time; 2 of 64 ranks (4001 x 4096 22 us, 24 with 4)
 
 static AdapterWork adapter_work(const fie_adapter_args& a)
 {
@@ -29,7 +29,7 @@ static hipError_t down_of(const fie_adapter_args& a, const AdapterWork& w, hipSt
     if (a.rank <= 16) k_adapter_down<DX, DT, 1, kDownSteps, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
     else if (a.rank <= 32) k_adapter_down<DX, DT, 2, kDownSteps, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
     else if (a.rank <= 48) k_adapter_down<DX, DT, 3, kDownSteps, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
-    else k_adapter_down<DX, DT, 4, kDownSteps, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
+    else k_adapter_down<DX, DT, 4, 2, ALIGNED><<<grid, 64 * kDownWaves, 0, st>>>(a, w);
     return hipGetLastError();
 }
 
@@ -91,6 +91,7 @@ static int adapter_check(const fie_adapter_args* a)
     if (a->k_pad < a->k || a->k_pad % FIE_ADAPTER_K) return fail(FIE_E_ARG, "k_pad is k's next multiple of 64");
     if (a->rank < FIE_ADAPTER_RANK || a->rank > FIE_MAX_RANK || a->rank % FIE_ADAPTER_RANK)
         return fail(FIE_E_ARG, "rank is a multiple of 16 in [16, 256]");
+    if (a->b_pitch < a->rank || a->b_pitch % (a->dtype == FIE_F32 ? 4 : 8)) return fail(FIE_E_ARG, "b_pitch is rank or more, a multiple of 16 bytes");
     if (a->x_stride < 0 || a->y_stride < a->n) return fail(FIE_E_ARG, "a row stride is shorter than its row");
     if (a->tokens == 0) return FIE_OK;
     if (!a->x || !a->a || !a->b || !a->scale || !a->ranks || !a->plan || !a->y || (a->x_dtype == FIE_I8) != (a->x_scale != nullptr))

@@ -172,7 +172,7 @@ static inline int mark_bits(int rows)
 // wanted.  FORK: a small table's rows take their parents' pages first, by the same workgroup (4 x 37: 6 us
 // and a launch less).  A chain of dependent steps through memory: parents, lengths, a row's last
 // page, its count, the blocks' pages.  512 rows 10 us (marks in memory, unrolled loops: 22), 4 rows with
-// their table 9.8.
+// their table 8.4 (1024 threads 9.6).
 template <bool FORK, int T>
 __global__ __launch_bounds__(T) void k_pages_grow(const PageState s, const PageScratch w, const int32_t* parents,
                                                              const int32_t* lengths, uint8_t* granted, int bits, int room)

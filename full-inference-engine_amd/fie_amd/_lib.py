@@ -61,7 +61,7 @@ class VerifyArgs(ctypes.Structure):
 NORM_ARGS = "@10P6q9i3f0q"
 INT8_ARGS = "@6P4q4iPN0q"
 BEAM_ARGS = "@15PqPNd8i18i0q"
-ADAPTER_ARGS = "@10PN3q10i0q"
+ADAPTER_ARGS = "@10PN3q12i0q"
 ADAPTER_PLAN_ARGS = "@2P2i0q"
 PAGES_ARGS, GROUP_ARGS = "@PPN4i6P2i", "P3q4i"          # the head, and eight groups
 STATES_ARGS, STATE_ARGS = "@P2i", "2P4q"        # the head, and as many states as there are

@@ -71,7 +71,10 @@ class AdapterBank:
         self.adapters, self.k, self.n, self.rank, self.dtype = adapters, k, n, rank, dtype
         self.rank_pad, self.k_pad = -(-rank // 16) * 16, -(-k // 64) * 64
         self.a = torch.zeros((adapters, self.rank_pad, self.k_pad), dtype=dtype, device=device)
-        self.b = torch.zeros((adapters, n, self.rank_pad), dtype=dtype, device=device)
+        # channels that begin at every 128 bytes come in at half the rate (rank 64 in bf16)
+        size = self.a.element_size()
+        self.b_pitch = self.rank_pad + (16 // size if self.rank_pad * size % 128 == 0 else 0)
+        self.b = torch.zeros((adapters, n, self.b_pitch), dtype=dtype, device=device)
         self.scale = torch.zeros(adapters, dtype=torch.float32, device=device)
         self.ranks = torch.zeros(adapters, dtype=torch.int32, device=device)
         self.device, self.index = self.a.device, self.a.get_device()
@@ -162,7 +165,7 @@ def adapter_linear(x: torch.Tensor, bank: AdapterBank, plan: AdapterPlan, *, x_s
             b_stride = y_stride
         args = [x.data_ptr(), xs, bank.a.data_ptr(), bank.b.data_ptr(), bank.scale.data_ptr(), bank.ranks.data_ptr(),
                 plan.data.data_ptr(), bp, yp, 0, 0, x.stride(0), b_stride, y_stride, tokens, k, n, bank.adapters, bank.rank_pad,
-                bank.k_pad, code, x_code, _DTYPES[dtype], b_code]
+                bank.k_pad, bank.b_pitch, code, x_code, _DTYPES[dtype], b_code, 0]
         args[10] = _size(_pack(*args))
         room = torch.empty(args[10], dtype=torch.uint8, device=y.device)
         args[9] = room.data_ptr()

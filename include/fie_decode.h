@@ -156,7 +156,7 @@ typedef struct fie_adapter_args {
     const void* x;              /* [tokens, k] in dtype, or int8 with x_scale */
     const float* x_scale;       /* [tokens] */
     const void* a;              /* [adapters, rank, k_pad], zeros past each adapter's rank and past k */
-    const void* b;              /* [adapters, n, rank], likewise */
+    const void* b;              /* [adapters, n, rank], likewise, b_pitch elements between channels */
     const float* scale;         /* [adapters] */
     const int32_t* ranks;       /* [adapters], 0..rank */
     const int32_t* plan;        /* of these tokens and so many adapters */
@@ -167,8 +167,10 @@ typedef struct fie_adapter_args {
     int64_t x_stride, base_stride, y_stride;        /* elements between rows */
     int32_t tokens, k, n, adapters;
     int32_t rank, k_pad;        /* rank a multiple of FIE_ADAPTER_RANK, k_pad of FIE_ADAPTER_K */
+    int32_t b_pitch;            /* rank or more; a multiple of 16 bytes, best none of 128 */
     int32_t dtype, x_dtype;     /* the adapters' type; x's: that or FIE_I8 */
     int32_t y_dtype, base_dtype;        /* dtype or FIE_F32; y_dtype or FIE_F32 */
+    int32_t reserved;
 } fie_adapter_args;
 
 size_t fie_adapter_workspace_size(const fie_adapter_args* args);

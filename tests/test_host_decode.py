@@ -35,7 +35,7 @@ BEAM = ("logits scores lengths done pool ends next_scores next_lengths next_done
         "history_steps eos_count").split() + [f"eos[{i}]" for i in range(16)] + ["max_tokens"]
 PLAN = "ids plan tokens adapters".split()
 ADAPTER = ("x x_scale a b scale ranks plan base y workspace workspace_bytes x_stride base_stride y_stride tokens k n adapters rank k_pad "
-           "dtype x_dtype y_dtype base_dtype").split()
+           "b_pitch dtype x_dtype y_dtype base_dtype reserved").split()
 GROUP = "base page_stride outer_stride token_bytes count outer whole shift".split()
 PAGES = ("state scratch scratch_bytes pages page rows wide parents lengths granted live src dst copies group_count").split()
 STATE = "src dst src_stride dst_stride row_bytes rows".split()
@@ -171,7 +171,7 @@ def test_page_sizes_and_copies():
 
 def adapter_args(**kw):
     a = {n: 256 for n in ADAPTER}
-    a.update(x_scale=0, base=0, workspace_bytes=1 << 30, x_stride=64, base_stride=32, y_stride=32, tokens=4, k=64, n=32, adapters=2, rank=16, k_pad=64,
+    a.update(x_scale=0, base=0, workspace_bytes=1 << 30, x_stride=64, base_stride=32, y_stride=32, tokens=4, k=64, n=32, adapters=2, rank=16, k_pad=64, b_pitch=16, reserved=0,
              dtype=_lib.FIE_BF16, x_dtype=_lib.FIE_BF16, y_dtype=_lib.FIE_BF16, base_dtype=_lib.FIE_F32)
     assert set(kw) <= set(a)
     return struct.pack(_lib.ADAPTER_ARGS, *{**a, **kw}.values())
@@ -184,7 +184,7 @@ def adapter_args(**kw):
     (dict(x_dtype=_lib.FIE_F16), _lib.FIE_E_ARG, b"x is in"), (dict(y_dtype=_lib.FIE_F16), _lib.FIE_E_ARG, b"y is in"),
     (dict(base=512, base_dtype=_lib.FIE_F16), _lib.FIE_E_ARG, b"y is in"), (dict(n=0), _lib.FIE_E_ARG, b"n or k"),
     (dict(k=0), _lib.FIE_E_ARG, b"n or k"), (dict(k=131072, k_pad=131072), _lib.FIE_E_ARG, b"n or k"), (dict(k_pad=65), _lib.FIE_E_ARG, b"k_pad"),
-    (dict(k=65), _lib.FIE_E_ARG, b"k_pad"), (dict(rank=8), _lib.FIE_E_ARG, b"rank"), (dict(rank=272), _lib.FIE_E_ARG, b"rank"),
+    (dict(k=65), _lib.FIE_E_ARG, b"k_pad"), (dict(rank=8), _lib.FIE_E_ARG, b"rank"), (dict(rank=272), _lib.FIE_E_ARG, b"rank"), (dict(b_pitch=8), _lib.FIE_E_ARG, b"b_pitch"), (dict(b_pitch=20), _lib.FIE_E_ARG, b"b_pitch"),
     (dict(x_stride=-1), _lib.FIE_E_ARG, b"stride"), (dict(y_stride=31), _lib.FIE_E_ARG, b"stride"), (dict(x=0), _lib.FIE_E_ARG, b"NULL"),
     (dict(plan=0), _lib.FIE_E_ARG, b"NULL"), (dict(x_scale=256), _lib.FIE_E_ARG, b"x_scale"), (dict(x_dtype=_lib.FIE_I8), _lib.FIE_E_ARG, b"x_scale"),
     (dict(b=264), _lib.FIE_E_ARG, b"16-byte"), (dict(base=256), _lib.FIE_E_ARG, b"place"),
