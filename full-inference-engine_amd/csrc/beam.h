@@ -373,6 +373,13 @@ struct BeamChoice {
     uint32_t wave[16];
 };
 
+// The order of a beam's continuation by a token of logit x.  (In fp32 x - top would be off by 2^-24 of
+// it: tokens far below the top would tie across beams.)
+FIE_DEV uint64_t beam_total(const BeamChoice& C, int beam, float x)
+{
+    return beam_order((double)C.prior[beam] + (((double)x - (double)C.top[beam]) - C.lse[beam]));
+}
+
 constexpr int kPickEach = 4;                            // candidates of a thread
 constexpr int kPickList = 1024;                         // those that are ranked
 
@@ -415,7 +422,7 @@ FIE_DEV bool pick_ranked(const fie_beam_args& a, const BeamWork& w, int r, int w
     for (int n = 0; n < kPickEach; ++n) {
         const int i = pick_index(n), beam = i < all ? i / per : 0;
         key[n] = 0;
-        if (cand[n]) key[n] = beam_order((double)C.prior[beam] + ((double)(key_to_float(comp_k(cand[n])) - C.top[beam]) - C.lse[beam]));
+        if (cand[n]) key[n] = beam_total(C, beam, key_to_float(comp_k(cand[n])));
         best = max(best, (uint32_t)(key[n] >> 32));
     }
     const uint32_t reach = beam_reach<4>(best, (wanted + waves - 1) / waves);
@@ -522,8 +529,7 @@ FIE_DEV void pick_one_by_one(const fie_beam_args& a, const BeamWork& w, int r, i
     int at = 0;
     auto look = [&]() {
         if (at >= n) return (uint64_t)0;
-        const float x = key_to_float(comp_k(rows[lane * most + at]));
-        return beam_order((double)C.prior[lane] + ((double)(x - C.top[lane]) - C.lse[lane]));
+        return beam_total(C, lane, key_to_float(comp_k(rows[lane * most + at])));
     };
     uint64_t head = look();
     int live = 0, ends = 0, rank = 0;

@@ -64,14 +64,16 @@ def beam_step(logits: torch.Tensor, beams: Beams, *, eos: Sequence[int] = (), le
               history: tuple[torch.Tensor, torch.Tensor] | None = None) -> BeamStep:
     """One step of beam search: ``logits`` [requests * beams, vocab] (float32, float16, bfloat16).
 
-    A continuation's score is its beam's and the token's log-probability, in 64 bits and rounded
-    once; continuations rank by score, then lower beam, larger logit, lower token.  The best
-    ``beams`` of a request that are not in ``eos`` go on.  An ending one among its best ``beams``
-    of all joins the request's pool at score / (length + 1) ** ``length_penalty``; before
-    ``min_tokens`` tokens none exists, and with ``max_tokens`` those of that many tokens all end.  A request is done when its pool is full and, unless
-    ``early_stopping``, the best that goes on is no better than the pool's worst; or when nothing
-    goes on.  Rows of a request that is done, and rows beside its last beam, come out with score
-    -inf, token ``pad`` and themselves as parent, and their logits are not read at the next step.
+    A continuation's score is its beam's and the token's log-probability, added in 64 bits and
+    rounded once (a row's sum of exponentials alone has terms in fp32: its logarithm is off by about
+    1e-7).  Continuations rank by their totals, then lower beam, larger logit, lower token.  The
+    best ``beams`` of a request that are not in ``eos`` go on.  An ending one among its best
+    ``beams`` of all joins the request's pool at total / (length + 1) ** ``length_penalty``; before
+    ``min_tokens`` tokens none exists, and with ``max_tokens`` those of that many tokens all end.
+    A request is done when its pool is full and, unless ``early_stopping``, the best that goes on
+    is no better than the pool's worst; or when nothing goes on.  Rows of a request that is done,
+    and rows beside its last beam, come out with score -inf, token ``pad`` and themselves as parent,
+    and their logits are not read at the next step.
 
     A NaN logit counts as -inf, +inf as the largest float32; tokens masked with -inf do not exist.
     ``inplace`` writes the new beams over the old.  ``history``: int32 [steps, rows] tokens and

@@ -21,7 +21,9 @@ extern "C" {
 
 /* One step of a beam search over `requests` requests of `beams` beams; row b of request r is
    r * beams + b.  With x the logits (a NaN counts as -inf, +inf as FLT_MAX):
-     total[b, v] = scores[b] + log_softmax(x[b])[v]              in 64 bits, rounded once
+     total[b, v] = scores[b] + ((x[b, v] - m) - log(sum exp(x[b] - m)))      m = max x[b]
+   in 64 bits and rounded once to a score, but for the sum: its terms and sums of 32 of them are fp32,
+   so its logarithm is off by 2^-24 (6 mean(m - x) + 16) at most, the mean over the terms' weights.
    A request's continuations rank by (total descending, lower beam, larger logit, lower token);
    those of total -inf do not exist.  The best `beams` that are no eos go on.  An eos
    continuation among the best `beams` of all joins the pool, the request's `beams` best ended
