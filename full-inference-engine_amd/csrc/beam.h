@@ -349,6 +349,9 @@ FIE_DEV double beam_value(uint64_t k)
     return __longlong_as_double((int64_t)((k >> 63) ? (k & 0x7FFFFFFFFFFFFFFFull) : ~k));
 }
 
+// A score or an answer's value: none is -inf, which says that nothing is there.
+FIE_DEV float beam_held(double v) { return __builtin_fmaxf((float)v, -kLargest); }
+
 // length^penalty.  (The exponential and the logarithm as they are shared with a row's: a power's own code
 // takes longer to come in than to run.)
 __host__ FIE_DEV bool beam_power(double penalty) { return penalty != 0.0 && penalty != 1.0; }
@@ -477,7 +480,7 @@ FIE_DEV bool pick_ranked(const fie_beam_args& a, const BeamWork& w, int r, int w
         }
         if (stops) {
             const int at = ends + (int)__popcll(off & below);
-            C.end_value[at] = (float)(beam_value(f) / scale);
+            C.end_value[at] = beam_held(beam_value(f) / scale);
             C.end_token[at] = token;
             C.end_beam[at] = then_beam(t);
         }
@@ -553,7 +556,7 @@ FIE_DEV void pick_one_by_one(const fie_beam_args& a, const BeamWork& w, int r, i
                 C.live_token[live] = token;
                 C.live_beam[live] = who;
             } else if (rank < K) {
-                C.end_value[ends] = (float)(beam_value(best) / scale);
+                C.end_value[ends] = beam_held(beam_value(best) / scale);
                 C.end_token[ends] = token;
                 C.end_beam[ends] = who;
             }
@@ -667,12 +670,12 @@ __global__ __launch_bounds__(1024) void k_beam_pick(const fie_beam_args a, const
     if (fresh == K - 1) worst = C.end_value[lane];
     for (int d = 32; d; d >>= 1) worst = __builtin_fminf(worst, __shfl_xor(worst, d, 64));
     bool done = was || live == 0;
-    if (!done && worst > -__builtin_inff()) done = a.early_stopping || worst >= (float)(beam_value(C.live_key[0]) / scale);
+    if (!done && worst > -__builtin_inff()) done = a.early_stopping || worst >= beam_held(beam_value(C.live_key[0]) / scale);
     if (lane < K) {
         const int row = r * K + lane;
         const bool goes = !done && lane < live;
         const int token = goes ? C.live_token[lane] : a.pad, parent = goes ? r * K + C.live_beam[lane] : row;
-        a.next_scores[row] = goes ? (float)beam_value(C.live_key[lane]) : -__builtin_inff();
+        a.next_scores[row] = goes ? beam_held(beam_value(C.live_key[lane])) : -__builtin_inff();
         a.tokens[row] = token;
         a.parents[row] = parent;
         if (a.history_tokens && !was && length >= 0 && length < a.history_steps) {

@@ -76,6 +76,7 @@ def beam_step(logits: torch.Tensor, beams: Beams, *, eos: Sequence[int] = (), le
     and their logits are not read at the next step.
 
     A NaN logit counts as -inf, +inf as the largest float32; tokens masked with -inf do not exist.
+    Scores and values below the least float32 are held at it.
     ``inplace`` writes the new beams over the old.  ``history``: int32 [steps, rows] tokens and
     parents; a step's are kept at its request's length.  Runs on the current stream; nothing waits
     for it."""

@@ -25,9 +25,10 @@ extern "C" {
    in 64 bits and rounded once to a score, but for the sum: its terms and sums of 32 of them are fp32,
    so its logarithm is off by 2^-24 (6 mean(m - x) + 16) at most, the mean over the terms' weights.
    A request's continuations rank by (total descending, lower beam, larger logit, lower token);
-   those of total -inf do not exist.  The best `beams` that are no eos go on.  An eos
-   continuation among the best `beams` of all joins the pool, the request's `beams` best ended
-   ones, at total / (length + 1)^length_penalty; on ties the older stays in front.
+   those of logit -inf do not exist.  Scores and values below -FLT_MAX are held at it, so that none
+   is -inf.  The best `beams` that are no eos go on.  An eos continuation among the best `beams` of
+   all joins the pool, the request's `beams` best ended ones, at total / (length + 1)^length_penalty;
+   on ties the older stays in front.
    Requests that are done, and beams of score -inf, are not read.  A request is done when its
    pool is full and (early_stopping, or the best that goes on is no better than the pool's worst
    at the same length), or when nothing goes on. */
