@@ -362,6 +362,10 @@ FIE_DEV double beam_scale(int length, double penalty)
     return exp(penalty * log((double)length));
 }
 
+// An answer's value.  (A power out of a double's range is 0 or an infinity: no total but 0 is left
+// undefined by that, and it is 0 at any length.)
+FIE_DEV float beam_ended(double total, double scale) { return total != 0.0 ? beam_held(total / scale) : 0.0f; }
+
 // What a request's workgroup settles before the pool.
 struct BeamChoice {
     double lse[FIE_MAX_BEAMS];                          // log of a row's sum, less its maximum
@@ -480,7 +484,7 @@ FIE_DEV bool pick_ranked(const fie_beam_args& a, const BeamWork& w, int r, int w
         }
         if (stops) {
             const int at = ends + (int)__popcll(off & below);
-            C.end_value[at] = beam_held(beam_value(f) / scale);
+            C.end_value[at] = beam_ended(beam_value(f), scale);
             C.end_token[at] = token;
             C.end_beam[at] = then_beam(t);
         }
@@ -556,7 +560,7 @@ FIE_DEV void pick_one_by_one(const fie_beam_args& a, const BeamWork& w, int r, i
                 C.live_token[live] = token;
                 C.live_beam[live] = who;
             } else if (rank < K) {
-                C.end_value[ends] = beam_held(beam_value(best) / scale);
+                C.end_value[ends] = beam_ended(beam_value(best), scale);
                 C.end_token[ends] = token;
                 C.end_beam[ends] = who;
             }
@@ -670,7 +674,7 @@ __global__ __launch_bounds__(1024) void k_beam_pick(const fie_beam_args a, const
     if (fresh == K - 1) worst = C.end_value[lane];
     for (int d = 32; d; d >>= 1) worst = __builtin_fminf(worst, __shfl_xor(worst, d, 64));
     bool done = was || live == 0;
-    if (!done && worst > -__builtin_inff()) done = a.early_stopping || worst >= beam_held(beam_value(C.live_key[0]) / scale);
+    if (!done && worst > -__builtin_inff()) done = a.early_stopping || worst >= beam_ended(beam_value(C.live_key[0]), scale);
     if (lane < K) {
         const int row = r * K + lane;
         const bool goes = !done && lane < live;

@@ -1,5 +1,6 @@
 // Beam search's selection behind the C ABI of include/fie_decode.h.
 #include <algorithm>
+#include <cmath>
 
 #include "beam.h"
 #include "states.h"
@@ -64,7 +65,7 @@ static int beam_check(const fie_beam_args* a)
     if (a->dtype < FIE_F32 || a->dtype > FIE_BF16) return fail(FIE_E_ARG, "unknown dtype");
     if (a->row_stride < a->vocab) return fail(FIE_E_ARG, "row_stride < vocab");
     if (a->eos_count < 0 || a->eos_count > FIE_MAX_EOS) return fail(FIE_E_ARG, "eos_count out of range [0, 16]");
-    if (a->length_penalty != a->length_penalty) return fail(FIE_E_ARG, "length_penalty is NaN");
+    if (!std::isfinite(a->length_penalty)) return fail(FIE_E_ARG, "length_penalty is not finite");
     if (a->requests == 0) return FIE_OK;
     if (!a->logits || !a->scores || !a->lengths || !a->done || !a->pool || !a->ends || !a->next_scores || !a->next_lengths ||
         !a->next_done || !a->next_pool || !a->next_ends || !a->tokens || !a->parents)

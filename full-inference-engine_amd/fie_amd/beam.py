@@ -24,6 +24,7 @@ _run = None             # the library's entry, loaded with the first call
 _size = None
 _sizes: dict[tuple, int] = {}    # bytes of workspace by a call's device, type and sizes
 _F32, _I32 = torch.float32, torch.int32
+_INF = float("inf")
 _reorder = None
 MAX_STATES = 48         # tensors of one launch
 _packs: dict[int, object] = {}
@@ -109,9 +110,9 @@ def beam_step(logits: torch.Tensor, beams: Beams, *, eos: Sequence[int] = (), le
     stop = len(eos)
     if stop > MAX_EOS or (stop and not 0 <= min(eos) <= max(eos) < vocab):
         raise ValueError(f"eos: at most {MAX_EOS} tokens of the vocabulary")
-    if not length_penalty == length_penalty or not 0 <= pad < 1 << 31 or not 0 <= min_tokens < 1 << 31 \
+    if not -_INF < length_penalty < _INF or not 0 <= pad < 1 << 31 or not 0 <= min_tokens < 1 << 31 \
             or not 0 <= max_tokens < 1 << 31:
-        raise ValueError("length_penalty must be a number, pad, min_tokens and max_tokens whole numbers of 31 bits")
+        raise ValueError("length_penalty must be a finite number, pad, min_tokens and max_tokens whole numbers of 31 bits")
     h_tokens = h_parents = h_steps = 0
     if history is not None:
         for t in history:
@@ -295,6 +296,8 @@ class BeamSearch:
         got = [Answer(float(v), way(int(p) - rows.start, int(n) - 1) + [int(t)], True)
                for v, (n, p, t) in zip(pool, ends) if v > -np.inf]
         if not done and length:
-            scale = float(length) ** self._settings["length_penalty"]
-            got += [Answer(float(s) / scale, way(b, steps), False) for b, s in enumerate(scores) if s > -np.inf]
+            with np.errstate(all="ignore"):             # (as the kernel: a power out of range is 0 or an infinity)
+                scale = np.float64(length) ** self._settings["length_penalty"]
+                values = np.where(scores != 0.0, np.maximum(scores / scale, np.finfo(np.float32).min), 0.0)
+            got += [Answer(float(v), way(b, steps), False) for b, (s, v) in enumerate(zip(scores, values)) if s > -np.inf]
         return got
