@@ -336,7 +336,7 @@ template <int DT> struct UpOperand {
 // y = base + scale B h: a wave a tile of 16 tokens and `steps` times 64 channels next to each other, on
 // its own; the four of a workgroup take four tiles, which mostly share their B.  h stays in registers as
 // the matrix instructions take it (CH times 16 ranks; CH 0: any number, built anew for each step).  fp16
-// tokens are brought to an exponent of their own first, so that no part overflows.  Results cross LDS
+// tokens are brought to an exponent of their own first, so that no part overflows or loses bits.  Results cross LDS
 // within the wave, so that base and y are read and written along their rows whatever these begin at.
 // Bound by base and y for many tokens an adapter (4001 x 4096, rank 16: 16 us, 4.1 TB/s; rank 48 24 and
 // rank 64 37, B's way from the L2; rank 48 at 4099 channels, a channel a lane, 36), by B for few (250 x
@@ -382,7 +382,10 @@ __global__ __launch_bounds__(64 * kUpWaves, 4) void k_adapter_up(const fie_adapt
             }
         if constexpr (DT == FIE_F16) {
             most = __builtin_fmaxf(most, __shfl_xor(most, 16, 64));
-            e = most > 0.0f && most <= 3.4e38f ? 127 - (int)((__float_as_uint(most) >> 23) & 255u) : 0;
+            // the largest to [2^14, 2^15), so that trailing parts of numbers far below it are normal, too (with
+            // it at [1, 2) one 2^-11 of the largest was off by 2^-14 of itself).  Products of fp16 numbers are
+            // multiples of 2^-48 and their sums below 2^49, so factor keeps its bits
+            e = most > 0.0f && most <= 3.4e38f ? 127 + 14 - (int)((__float_as_uint(most) >> 23) & 255u) : 0;
             factor = __builtin_ldexpf(factor, -e);
         }
         if constexpr (CH > 0)

@@ -109,9 +109,10 @@ def adapter_linear(x: torch.Tensor, bank: AdapterBank, plan: AdapterPlan, *, x_s
 
     The output is in ``out_dtype``, the bank's type or float32; by default the bank's.  ``out`` [tokens, n] is
     written instead of a new tensor (unit element stride, any row stride); it may be ``base`` itself.
-    A[i] x[t] is summed in fp32 and, with two-byte adapters, enters the second product as two numbers
-    of their type, together off by 2^-16 of it (bf16) or 2^-22 (fp16); that product's sums are fp32,
-    and the result is rounded once.  Runs on the current stream; nothing waits for it."""
+    A[i] x[t] is summed in fp32 and, with two-byte adapters, each of its numbers enters the second
+    product as two of their type, together off by 2^-16 of it (bf16) or by 2^-22 of it and 2^-39 of the
+    token's largest, whichever is more (fp16); that product's sums are fp32, and the result is rounded
+    once.  Runs on the current stream; nothing waits for it."""
     shape, k, n, tokens, index = x.shape, bank.k, bank.n, plan.tokens, bank.index
     if not shape or shape[-1] != k or x.numel() != tokens * k:
         raise ValueError(f"x must be [..., {k}] of the plan's {tokens} tokens")
