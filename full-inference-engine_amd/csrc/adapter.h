@@ -242,6 +242,8 @@ __global__ __launch_bounds__(64 * kDownWaves) void k_adapter_down(const fie_adap
 #pragma unroll
             for (int i = 1; i < kDownWaves; ++i) t += red[i][f][lane];
             const int r = r0 + 16 * f + 4 * group;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = r + i < rank ? t[i] : 0.0f;      // (ranks of padding: an infinite x times 0)
             if ((lane & 15) < count && r < a.rank) *(f32x4_t*)(w.h + ((int64_t)blockIdx.x * a.tokens + first + (lane & 15)) * a.rank + r) = t;
         }
     }

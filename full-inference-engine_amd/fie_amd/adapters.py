@@ -112,7 +112,8 @@ def adapter_linear(x: torch.Tensor, bank: AdapterBank, plan: AdapterPlan, *, x_s
     A[i] x[t] is summed in fp32 and, with two-byte adapters, each of its numbers enters the second
     product as two of their type, together off by 2^-16 of it (bf16) or by 2^-22 of it and 2^-39 of the
     token's largest, whichever is more (fp16); that product's sums are fp32, and the result is rounded
-    once.  Runs on the current stream; nothing waits for it."""
+    once.  Infinite and NaN activations give what the formula gives, for their token alone; adapters
+    themselves are finite numbers.  Runs on the current stream; nothing waits for it."""
     shape, k, n, tokens, index = x.shape, bank.k, bank.n, plan.tokens, bank.index
     if not shape or shape[-1] != k or x.numel() != tokens * k:
         raise ValueError(f"x must be [..., {k}] of the plan's {tokens} tokens")

@@ -139,7 +139,9 @@ int fie_pages_copy(const fie_pages_args* args, void* stream);
    Products of x and a are exact and their sums fp32.  With fp16 and bf16 adapters each number of
    a[i] x[t] enters the second product as the sum of two of their type, off by 2^-16 of itself (bf16) or
    by 2^-22 of itself or 2^-39 of the token's largest, whichever is more (fp16); that product's sums are
-   fp32, and y is rounded once.  An adapter of rank 0 gives base. */
+   fp32, and y is rounded once.  An adapter of rank 0 gives base.
+   Infinite and NaN numbers of x give what the formula gives, for their token alone; those of a and b are
+   for the adapter's tokens NaN as a rule. */
 #define FIE_MAX_RANK 256
 #define FIE_MAX_ADAPTERS 4096
 #define FIE_ADAPTER_K 64        /* rows of a are padded with zeros to a multiple of so many */
