@@ -151,8 +151,8 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor,
                    out: Sequence[torch.Tensor] | None = None) -> list[torch.Tensor]:
     """``[s[parents] for s in states]`` in one launch: states [rows, ...] of any types, ``parents`` int32
     [n] rows (one outside [0, rows) stands for the row's own number, which has to be one of the
-    states').  ``out``: as many tensors [n, ...] to write into, apart from the states.  Runs on the
-    current stream; nothing waits for it."""
+    states').  ``out``: as many tensors [n, ...] to write into, apart from all states and from each
+    other.  Runs on the current stream; nothing waits for it."""
     if parents.dtype != torch.int32 or parents.ndim != 1:
         raise ValueError("parents must be int32 [rows]")
     index = parents.get_device()
@@ -183,8 +183,6 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor,
                 raise ValueError(f"output {i} must be [{n}, ...] as its state")
             if not t.is_contiguous() and n and (not t[0].is_contiguous() or (n > 1 and t.numel() and t.stride(0) < t[0].numel())):
                 raise ValueError("outputs need contiguous rows that do not overlap")
-            if s.numel() and t.numel() and _meet(s, t):
-                raise ValueError("an output overlaps its state")
         got.append(t)
         width = s.numel()
         if width and n:
@@ -192,6 +190,8 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor,
             width = width // rows * size
             flat += (s.data_ptr(), t.data_ptr(), width if dense else s.stride(0) * size,
                      width if out is None else t.stride(0) * size, width, rows)
+    if out is not None and flat and _cross(flat, n, parents.data_ptr()):
+        raise ValueError("an output overlaps a state, the parents or another output")
     global _reorder
     if flat and _reorder is None:
         _reorder = _lib.launcher("fie_reorder_states")
@@ -205,13 +205,52 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor,
     return got
 
 
-def _meet(s: torch.Tensor, t: torch.Tensor) -> bool:
-    """Whether the memory from the first to the last element of one has any of the other's."""
-    def span(x):
-        last = sum((n - 1) * st for n, st in zip(x.shape, x.stride()))
-        return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
-    (a, b), (c, d) = span(s), span(t)
-    return a < d and c < b
+def _cross(flat: list, n: int, parents: int) -> bool:
+    """Whether an output (of n rows) has memory of a state's, another output's or the parents': ``flat`` has (state, output, their
+    strides, width, rows of the state) in bytes.  Rows of one stride may lie between each other's."""
+    # first byte and end, stride (0: one piece), width, an output
+    parts = [(parents, parents + 4 * n, 0, 4 * n, False)]
+    for i in range(0, len(flat), 6):
+        s, t, s_stride, t_stride, width, rows = flat[i:i + 6]
+        parts.append((s, s + (rows - 1) * s_stride + width, s_stride if rows > 1 else 0, width, False))
+        parts.append((t, t + (n - 1) * t_stride + width, t_stride if n > 1 else 0, width, True))
+    parts.sort()
+    some: list = []                                 # that meet in a chain
+    end = 0
+    for p in parts:
+        if p[0] >= end:                             # apart from all before it
+            if len(some) > 1 and _meet(some):
+                return True
+            some = []
+        some.append(p)
+        end = max(end, p[1])
+    return len(some) > 1 and _meet(some)
+
+
+def _meet(parts: list) -> bool:
+    stride = max(p[2] for p in parts)
+    if stride and len(parts) > 8 and all(p[2] == stride for p in parts):
+        # columns of one buffer: two rounds of their places in a row
+        at = sorted((p[0] % stride, p[3], p[4]) for p in parts)
+        every = outs = 0
+        for first, width, out in at + [(first + stride, width, out) for first, width, out in at]:
+            if first < (every if out else outs):
+                break
+            every = max(every, first + width)
+            outs = max(outs, first + width) if out else outs
+        else:
+            return False
+    return any(_shared(q, p) for i, p in enumerate(parts) for q in parts[:i] if p[4] or q[4])
+
+
+def _shared(a: tuple, b: tuple) -> bool:
+    if a[1] <= b[0] or b[1] <= a[0]:
+        return False
+    if a[2] and b[2] and a[2] != b[2]:
+        return True                                 # (rows of two strides that miss each other are not looked for)
+    stride = a[2] or b[2]
+    at = (b[0] - a[0]) % stride if stride else 0
+    return at < a[3] or stride - at < b[3]
 
 
 class Answer(NamedTuple):
