@@ -15,6 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import FIE_BF16, FIE_F16, FIE_F32, FIE_I8
+from .beam import _shared
 
 _DTYPES = {torch.float32: FIE_F32, torch.float16: FIE_F16, torch.bfloat16: FIE_BF16}
 _pack = struct.Struct(_lib.ADAPTER_ARGS).pack
@@ -108,7 +109,8 @@ def adapter_linear(x: torch.Tensor, bank: AdapterBank, plan: AdapterPlan, *, x_s
     (float32, one a token); base [..., n] in the output's type or float32 (None: 0).
 
     The output is in ``out_dtype``, the bank's type or float32; by default the bank's.  ``out`` [tokens, n] is
-    written instead of a new tensor (unit element stride, any row stride); it may be ``base`` itself.
+    written instead of a new tensor (unit element stride, any row stride); it may be ``base`` itself,
+    else it is apart from it.
     A[i] x[t] is summed in fp32 and, with two-byte adapters, each of its numbers enters the second
     product as two of their type, together off by 2^-16 of it (bf16) or by 2^-22 of it and 2^-39 of the
     token's largest, whichever is more (fp16); that product's sums are fp32, and the result is rounded
@@ -165,6 +167,12 @@ def adapter_linear(x: torch.Tensor, bank: AdapterBank, plan: AdapterPlan, *, x_s
             raise ValueError("base and out in one place must be the same tensor")
         if bp == yp:
             b_stride = y_stride
+        elif bp and out is not None:
+            def part(p, stride, size):
+                return p, p + ((tokens - 1) * stride + n) * size, stride * size if tokens > 1 else 0, n * size
+
+            if _shared(part(bp, b_stride, base.element_size()), part(yp, y_stride, y.element_size())):
+                raise ValueError("out must be base itself or apart from it")
         args = [x.data_ptr(), xs, bank.a.data_ptr(), bank.b.data_ptr(), bank.scale.data_ptr(), bank.ranks.data_ptr(),
                 plan.data.data_ptr(), bp, yp, 0, 0, x.stride(0), b_stride, y_stride, tokens, k, n, bank.adapters, bank.rank_pad,
                 bank.k_pad, bank.b_pitch, code, x_code, _DTYPES[dtype], b_code, 0]

@@ -244,6 +244,7 @@ def _meet(parts: list) -> bool:
 
 
 def _shared(a: tuple, b: tuple) -> bool:
+    """Whether rows of (first byte, end, stride or 0 for one piece, width) have memory in common."""
     if a[1] <= b[0] or b[1] <= a[0]:
         return False
     if a[2] and b[2] and a[2] != b[2]:
