@@ -189,17 +189,19 @@ class CachePages:
     def load(self, table: torch.Tensor, lengths: torch.Tensor) -> None:
         """Begins with these rows' pages (waits for the device).  Entries past a row's pages are taken as -1;
         rows that share a page have it at the same place."""
-        table = table.to(self.device, torch.int32)
-        lengths = lengths.to(self.device, torch.int32)
+        # 64 bits: a cut to 32 could make a page or a length of what is none
+        table, lengths = (t.to(self.device) if t.is_floating_point() else t.to(self.device, torch.int64) for t in (table, lengths))
         if table.shape != self.table.shape or lengths.shape != self.lengths.shape:
             raise ValueError(f"table must be [{self.rows}, {self.max_pages}], lengths [{self.rows}]")
-        if bool((lengths < 0).any()) or bool((lengths.long() > self.max_pages * self.page_size).any()):
-            raise ValueError("lengths must be in [0, max_pages * page_size]")
+        most = min(self.max_pages * self.page_size, (1 << 31) - 1)
+        if not bool(((lengths >= 0) & (lengths <= most)).all()):
+            raise ValueError("lengths must be in [0, max_pages * page_size], 31 bits at most")
         col = torch.arange(self.max_pages, device=self.device)
         used = col < ((lengths.long() + self.page_size - 1) // self.page_size)[:, None]
-        ids = table[used].long()
+        ids = table[used]
         if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= self.pages):
             raise ValueError(f"a row's pages must be in [0, {self.pages})")
+        ids = ids.long()
         at = col.expand_as(table)[used]
         place = torch.full((self.pages,), -1, dtype=torch.int64, device=self.device).scatter_reduce_(0, ids, at, "amax")
         if bool((place[ids] != at).any()):
