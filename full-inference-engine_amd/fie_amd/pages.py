@@ -81,7 +81,8 @@ class CachePages:
     def add_caches(self, caches: Sequence[torch.Tensor], token_dim: int | None = 1) -> None:
         """Tensors [pages, ...] that go along when pages are copied.  ``token_dim`` is the dimension of a page's
         tokens, everything past it contiguous: 1 for [pages, page_size, heads, dim], 2 for [pages, heads,
-        page_size, dim]; None where a page has values for all its tokens together (scales)."""
+        page_size, dim]; None where a page has values for all its tokens together (scales).  Pages may lie
+        between each other ([heads, pages, page_size, dim], transposed)."""
         groups: dict[tuple, list[torch.Tensor]] = {}
         for t in caches:
             if t.get_device() != self._index:
@@ -104,10 +105,12 @@ class CachePages:
                 for n in t.shape[at + 1:]:
                     inner *= n
                 outer, outer_stride, token = *_pieces(t, at), inner * size
-            span = (outer - 1) * outer_stride * size + token * (1 if token_dim is None else self.page_size)
-            if self.pages > 1 and t.stride(0) * size < span:
+            piece, step, pitch = token * (1 if token_dim is None else self.page_size), t.stride(0) * size, outer_stride * size
+            # a page's pieces lie together, or all pages' first pieces do, then all second ones
+            if self.pages > 1 and step < (outer - 1) * pitch + piece \
+                    and not (step >= piece and pitch >= (self.pages - 1) * step + piece):
                 raise ValueError("a cache's pages overlap")
-            key = (t.stride(0) * size, outer_stride * size, token, outer, int(token_dim is None))
+            key = (step, pitch, token, outer, int(token_dim is None))
             groups.setdefault(key, []).append(t)
         if len(self._groups) + len(groups) > MAX_GROUPS:
             raise ValueError(f"caches of more than {MAX_GROUPS} layouts")
