@@ -8,7 +8,7 @@ namespace fie {
 constexpr int kCopyThreads = 256;
 constexpr int kCopyUnroll = 4;                                      // 16-byte pieces of a thread on their way together
 constexpr int kCopyChunk = kCopyThreads * kCopyUnroll * 16;         // bytes of a workgroup
-constexpr int kMostBlocks = 1 << 24;                                // a launch holds fewer than 2^32 threads
+constexpr int kMostBlocks = (1 << 24) - 1;                          // a launch holds fewer than 2^32 threads
 
 // Memory of the device by an address of any make: without the address space the compiler has to
 // take it for LDS as well, and waits for each access before the next.

@@ -50,7 +50,7 @@ static int pages_check(const fie_pages_args* a, bool table)
         const fie_cache_group& g = a->group[i];
         if (g.count < 0 || g.outer < 1 || g.token_bytes < 1 || g.token_bytes > 1 << 30 || (g.count && !g.base))
             return fail(FIE_E_ARG, "a cache group's layout is out of range");
-        if (g.count * g.outer * chunks_of(*a, g) > 1 << 24)
+        if ((int64_t)g.count * g.outer > kMostBlocks || chunks_of(*a, g) > kMostBlocks || (int64_t)g.count * g.outer * chunks_of(*a, g) > kMostBlocks)
             return fail(FIE_E_ARG, "a cache group's pages are too large");
     }
     if (!table) return FIE_OK;
