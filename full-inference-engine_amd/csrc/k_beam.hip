@@ -56,15 +56,21 @@ static hipError_t beam_run(const fie_beam_args& a, hipStream_t st)
     return hipGetLastError();
 }
 
-static int beam_check(const fie_beam_args* a)
+static int beam_sizes(const fie_beam_args* a)
 {
-    if (!a) return fail(FIE_E_ARG, "args is NULL");
     if (a->beams < 1 || a->beams > FIE_MAX_BEAMS) return fail(FIE_E_ARG, "beams out of range [1, 64]");
     if (a->requests < 0 || (int64_t)a->requests * a->beams > 65535) return fail(FIE_E_ARG, "more than 65535 rows");
     if (a->vocab < 1 || a->vocab > kMaxTiles * kTile) return fail(FIE_E_ARG, "vocab out of range [1, 524288]");
     if (a->dtype < FIE_F32 || a->dtype > FIE_BF16) return fail(FIE_E_ARG, "unknown dtype");
-    if (a->row_stride < a->vocab) return fail(FIE_E_ARG, "row_stride < vocab");
     if (a->eos_count < 0 || a->eos_count > FIE_MAX_EOS) return fail(FIE_E_ARG, "eos_count out of range [0, 16]");
+    return FIE_OK;
+}
+
+static int beam_check(const fie_beam_args* a)
+{
+    if (!a) return fail(FIE_E_ARG, "args is NULL");
+    if (const int rc = beam_sizes(a); rc != FIE_OK) return rc;
+    if (a->row_stride < a->vocab) return fail(FIE_E_ARG, "row_stride < vocab");
     if (!std::isfinite(a->length_penalty)) return fail(FIE_E_ARG, "length_penalty is not finite");
     if (a->requests == 0) return FIE_OK;
     if (!a->logits || !a->scores || !a->lengths || !a->done || !a->pool || !a->ends || !a->next_scores || !a->next_lengths ||
@@ -85,7 +91,7 @@ using namespace fie;
 
 extern "C" size_t fie_beam_workspace_size(const fie_beam_args* a)
 {
-    return a && a->requests > 0 && a->beams > 0 && a->beams <= FIE_MAX_BEAMS && a->vocab > 0 && a->eos_count >= 0 ? beam_bytes(*a) : 0;
+    return a && a->requests > 0 && beam_sizes(a) == FIE_OK ? beam_bytes(*a) : 0;
 }
 
 extern "C" int fie_beam_step(const fie_beam_args* a, void* stream)
