@@ -21,11 +21,19 @@ _DTYPES = {torch.float32: FIE_F32, torch.float16: FIE_F16, torch.bfloat16: FIE_B
 _pack = struct.Struct(_lib.ADAPTER_ARGS).pack
 _pack_plan = struct.Struct(_lib.ADAPTER_PLAN_ARGS).pack
 _run = _run_plan = _size = None         # the library's entries, loaded with the first call
+_raw_stream = torch._C._cuda_getCurrentRawStream
 MAX_RANK = 256
 MAX_ADAPTERS = 4096
 MAX_TOKENS = 1 << 20
 MAX_K = 131071
 MAX_CHANNELS = 0x7FFFFF00
+
+
+def _keep(index: int, made_on: int, *tensors: torch.Tensor) -> None:
+    if _raw_stream(index) != made_on and not torch.cuda.is_current_stream_capturing():
+        stream = torch.cuda.current_stream(index)
+        for t in tensors:
+            t.record_stream(stream)
 
 
 class AdapterPlan:
@@ -48,12 +56,11 @@ class AdapterPlan:
         if _run_plan is None:
             _run_plan = _lib.launcher("fie_adapter_plan")
         _run_plan(self.index, _pack_plan(ids.data_ptr(), self.data.data_ptr(), self.tokens, adapters))
-        self._made_on = torch._C._cuda_getCurrentRawStream(self.index)
+        self._made_on = _raw_stream(self.index)
 
     def on_stream(self) -> None:
         """Memory made on another stream is kept for this one (which waits for that one itself)."""
-        if torch._C._cuda_getCurrentRawStream(self.index) != self._made_on and not torch.cuda.is_current_stream_capturing():
-            self.data.record_stream(torch.cuda.current_stream(self.index))
+        _keep(self.index, self._made_on, self.data)
 
 
 class AdapterBank:
@@ -79,6 +86,11 @@ class AdapterBank:
         self.scale = torch.zeros(adapters, dtype=torch.float32, device=device)
         self.ranks = torch.zeros(adapters, dtype=torch.int32, device=device)
         self.device, self.index = self.a.device, self.a.get_device()
+        self._made_on = _raw_stream(self.index)
+
+    def on_stream(self) -> None:
+        """Memory made on another stream is kept for this one (which waits for that one itself)."""
+        _keep(self.index, self._made_on, self.a, self.b, self.scale, self.ranks)
 
     def load(self, i: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
         """Adapter i: a [rank, k], b [n, rank], rank up to the bank's (0: it does nothing).  On the current
@@ -88,6 +100,7 @@ class AdapterBank:
         if a.ndim != 2 or b.ndim != 2 or a.shape[1] != self.k or b.shape != (self.n, a.shape[0]) or a.shape[0] > self.rank:
             raise ValueError(f"a must be [rank, {self.k}], b [{self.n}, rank], rank at most {self.rank}")
         r = a.shape[0]
+        self.on_stream()
         self.a[i].zero_()
         self.b[i].zero_()
         self.a[i, :r, :self.k] = a
@@ -180,5 +193,6 @@ def adapter_linear(x: torch.Tensor, bank: AdapterBank, plan: AdapterPlan, *, x_s
         room = torch.empty(args[10], dtype=torch.uint8, device=y.device)
         args[9] = room.data_ptr()
         plan.on_stream()
+        bank.on_stream()
         _run(index, _pack(*args))
     return y.view(*shape[:-1], n) if out is None and len(shape) != 2 else y

@@ -26,6 +26,7 @@ _sizes: dict[tuple, int] = {}    # bytes of workspace by a call's device, type a
 _F32, _I32 = torch.float32, torch.int32
 _INF = float("inf")
 _reorder = None
+_raw_stream = torch._C._cuda_getCurrentRawStream
 MAX_STATES = 48         # tensors of one launch
 _packs: dict[int, object] = {}
 MAX_BEAMS = 64
@@ -291,9 +292,19 @@ class BeamSearch:
         rows = requests * beams
         self._history = (torch.zeros((max_tokens, rows), dtype=torch.int32, device=self.device),
                          torch.zeros((max_tokens, rows), dtype=torch.int32, device=self.device))
+        self._index = self.beams.scores.get_device()
+        self._made_on = _raw_stream(self._index)
+
+    def _on_stream(self) -> None:
+        """Memory made on another stream is kept for this one."""
+        if _raw_stream(self._index) != self._made_on and not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(self._index)
+            for t in (*self.beams, *self._history):
+                t.record_stream(stream)
 
     def step(self, logits: torch.Tensor) -> BeamStep:
         """One step of every request (``beam_step``); the beams are written over."""
+        self._on_stream()
         return beam_step(logits, self.beams, inplace=True, history=self._history, **self._settings)
 
     def _slots(self, requests: Sequence[int]) -> torch.Tensor:
@@ -304,13 +315,16 @@ class BeamSearch:
     def restart(self, requests: Sequence[int]) -> None:
         """These requests' slots begin anew."""
         at = self._slots(requests)
+        self._on_stream()
         for t, fresh in zip(self.beams, first_beams(len(requests), self.count, self.device)):
             t[at] = fresh
 
     def stop(self, requests: Sequence[int]) -> None:
         """These requests are done as they are, or were never begun (slots that only fill up the batch): their
         logits are not read until ``restart``.  Beams that had not ended are dropped."""
-        self.beams.done[self._slots(requests)] = True
+        at = self._slots(requests)
+        self._on_stream()
+        self.beams.done[at] = True
 
     def all_done(self) -> bool:
         """Whether every request is done (waits for the device)."""

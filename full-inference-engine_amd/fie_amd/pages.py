@@ -118,9 +118,11 @@ class CachePages:
             base = torch.tensor([t.data_ptr() for t in tensors], dtype=torch.int64).to(self.device)
             shift = int(any(v % 16 for v in (stride, outer_stride, *(t.data_ptr() for t in tensors))))
             self._groups.append(((stride, outer_stride, token, len(tensors), outer, whole, shift), tensors, base))
+        self._mixed |= bool(groups) and _raw_stream(self._index) != self._made_on
         self._packed = None
 
     _packed: list | None = None
+    _mixed = False                      # addresses of caches made on another stream than the state
 
     def _args(self, parents: int, lengths: int, granted: int, live: int, src: int, dst: int, copies: int) -> bytes:
         p = self._packed
@@ -132,7 +134,7 @@ class CachePages:
 
     def _on_stream(self) -> None:
         """Memory made on another stream is kept for this one."""
-        if _raw_stream(self._index) != self._made_on and not torch.cuda.is_current_stream_capturing():
+        if (self._mixed or _raw_stream(self._index) != self._made_on) and not torch.cuda.is_current_stream_capturing():
             stream = torch.cuda.current_stream(self._index)
             for t in (self.state, self._scratch, *(base for _, _, base in self._groups)):
                 t.record_stream(stream)
