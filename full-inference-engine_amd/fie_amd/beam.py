@@ -53,11 +53,11 @@ class BeamStep(NamedTuple):
 
 def first_beams(requests: int, beams: int, device: torch.device | str) -> Beams:
     """Before the first step: a request's first row is its only beam."""
-    scores = torch.full((requests, beams), float("-inf"), device=device)
+    scores = torch.full((requests, beams), -_INF, dtype=_F32, device=device)
     scores[:, :1] = 0.0
     return Beams(scores, torch.zeros(requests, dtype=torch.int32, device=device),
                  torch.zeros(requests, dtype=torch.bool, device=device),
-                 torch.full((requests, beams), float("-inf"), device=device),
+                 torch.full((requests, beams), -_INF, dtype=_F32, device=device),
                  torch.full((requests, beams, 3), -1, dtype=torch.int32, device=device))
 
 
