@@ -29,8 +29,8 @@ MAX_K = 131071
 MAX_CHANNELS = 0x7FFFFF00
 
 
-def _keep(index: int, made_on: int, *tensors: torch.Tensor) -> None:
-    if _raw_stream(index) != made_on and not torch.cuda.is_current_stream_capturing():
+def _keep(index: int, *tensors: torch.Tensor) -> None:
+    if not torch.cuda.is_current_stream_capturing():
         stream = torch.cuda.current_stream(index)
         for t in tensors:
             t.record_stream(stream)
@@ -60,7 +60,8 @@ class AdapterPlan:
 
     def on_stream(self) -> None:
         """Memory made on another stream is kept for this one (which waits for that one itself)."""
-        _keep(self.index, self._made_on, self.data)
+        if _raw_stream(self.index) != self._made_on:
+            _keep(self.index, self.data)
 
 
 class AdapterBank:
@@ -90,7 +91,8 @@ class AdapterBank:
 
     def on_stream(self) -> None:
         """Memory made on another stream is kept for this one (which waits for that one itself)."""
-        _keep(self.index, self._made_on, self.a, self.b, self.scale, self.ranks)
+        if _raw_stream(self.index) != self._made_on:
+            _keep(self.index, self.a, self.b, self.scale, self.ranks)
 
     def load(self, i: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
         """Adapter i: a [rank, k], b [n, rank], rank up to the bank's (0: it does nothing).  On the current
