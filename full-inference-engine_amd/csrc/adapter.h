@@ -52,7 +52,8 @@ constexpr int kPlanHead = 4, kPlanTile = 4, kTileTokens = 16;
 constexpr int kPlanThreads = 1024;
 
 // One workgroup: counts, where each adapter's tokens begin, and the tokens' places.  (In which
-// order an adapter's tokens stand changes no result: each is a column of its own.)
+// order an adapter's tokens stand changes no result: each is a column of its own.)  Once a batch: 1 and
+// 250 tokens 2.6 us, 4001 8.5, 65536 113 (two passes of one workgroup, LDS atomics on few counters).
 __global__ __launch_bounds__(kPlanThreads) void k_adapter_plan(const fie_adapter_plan_args a, int most)
 {
     __shared__ int32_t count[FIE_MAX_ADAPTERS + 1], next[FIE_MAX_ADAPTERS + 1];
@@ -181,9 +182,10 @@ constexpr int kDownWaves = 4;
 // h = A x: grid (splits, tiles), 16 tokens of one adapter a workgroup.  The splits and their waves take k
 // in turn, U steps each, straight from memory to the matrix instructions, 16 RT ranks at a time; a
 // workgroup's sums meet in LDS, the splits' in the second product.  (One workgroup a tile, of 16 waves:
-// 1 x 4096 6.8 us against 3.8, 250 tokens of 64 adapters 9.3 against 4.6: a CU alone is slow to
+// 1 x 4096 6.8 us against 3.7, 250 tokens of 64 adapters 9.3 against 4.8: a CU alone is slow to
 // bring in a whole A.)  Bound by A's way from memory for few tokens an adapter; for many by x's, and
-// with more ranks by A's from the L2 (4001 x 4097: rank 16 11 us, rank 48 20).
+// with more ranks by A's from the L2 (4001 x 4096: rank 16 11 us, rank 48 18, rank 64 22, rank 256 75; 4001
+// x 4097 of rank 48 20).
 template <int DX, int DT, int RT, int U, bool ALIGNED>
 __global__ __launch_bounds__(64 * kDownWaves) void k_adapter_down(const fie_adapter_args a, const AdapterWork w)
 {
@@ -340,10 +342,13 @@ template <int DT> struct UpOperand {
 // the matrix instructions take it (CH times 16 ranks; CH 0: any number, built anew for each step).  fp16
 // tokens are brought to an exponent of their own first, so that no part overflows or loses bits.  Results cross LDS
 // within the wave, so that base and y are read and written along their rows whatever these begin at.
-// Bound by base and y for many tokens an adapter (4001 x 4096, rank 16: 16 us, 4.1 TB/s; rank 48 24 and
-// rank 64 37, B's way from the L2; rank 48 at 4099 channels, a channel a lane, 36), by B for few (250 x
-// 16384 of 64 adapters 15 us, 3.8 TB/s).  Held to four waves a SIMD (rank 48 29 us with three, two tiles a
-// wave that share B's registers 43 with two); B's channels at every 128 bytes cost rank 64 52 us.
+// Bound by base and y for many tokens an adapter (4001 x 4096, rank 16: 17 us, 4.0 TB/s; rank 48 24 and
+// rank 64 37, B's way from the L2; rank 48 at 4099 channels, a channel a lane, 33), by B for few (250 x
+// 16384 of 64 adapters 16 us, 18 behind the 8-bit product with its fp32 base: 3.2 TB/s).  Ranks past 64 build
+// their operand anew for each 64 channels (rank 128 139 us, rank 256 266).  Held to four waves a SIMD (rank
+// 48 29 us with three, two tiles a wave that share B's registers 43 with two); that leaves CH 4 with an
+// fp32 base 32 bytes a lane in memory, which costs nothing to be seen (250 x 16384 at k 512, both products 41.9
+// us, with a bf16 base 41.4).  B's channels at every 128 bytes cost rank 64 52 us.
 template <int DT, int DY, int DB, int CH>
 __global__ __launch_bounds__(64 * kUpWaves, 4) void k_adapter_up(const fie_adapter_args a, const AdapterWork w, int wide, int steps)
 {

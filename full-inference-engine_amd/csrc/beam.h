@@ -124,7 +124,9 @@ struct BeamShared {
 
 // The `need`-th best candidate of a span, exactly: radix passes over (key, index) that read the
 // span again, and at the end the `need` best into the list.  For spans whose candidates do not
-// fit the list (equal logits, or logits in rising order).  (In line: a call takes stack in memory,
+// fit the list: equal logits, logits in rising order, and spans whose first tile leaves a wave without
+// logits, so that nothing bounds them.  With few rows a span is a tile, and a row's last tile of fewer
+// than 193 vectors is such a one: 4 rows of 50257 in bf16 19 us, of 57344 (7 whole tiles) 7.  (In line: a call takes stack in memory,
 // and with it 20 us between launches.)
 template <int DT>
 FIE_DEV int beam_deep(const BeamRow<DT>& row, int first, int last, int most, BeamShared& S)
@@ -205,8 +207,8 @@ FIE_DEV int beam_deep(const BeamRow<DT>& row, int first, int last, int most, Bea
 // wanted candidates reach among its 64 lanes' maxima, and the least of the four waves' bounds is
 // reached by all of them.  What reaches it is listed, in later tiles too; at the end the lists
 // are cut by such a bound of their own and ranked.  Four instructions a logit and the exponential;
-// 512 rows of 151936 in bf16 35 us (4.4 TB/s, a large copy has 4.9), 4 rows 6.7, 80 rows of 50001 in
-// fp32 8.
+// 512 rows of 151936 in bf16 36 to 38 us (4.2 TB/s, a large copy has 4.9), 4 rows 6.8, 80 rows of 50001
+// in fp32 8.3.
 template <int DT>
 __global__ __launch_bounds__(kBeamThreads, kBeamHold<DT>) void k_beam_scan(const fie_beam_args a, const BeamWork w)
 {
@@ -577,7 +579,8 @@ FIE_DEV void pick_one_by_one(const fie_beam_args& a, const BeamWork& w, int r, i
 
 // A workgroup a request: its rows' logarithms, a wave each, then its best continuations, then the pool.
 // Bound by the chain of these steps, and by how much code each of them has to bring in: 1 request of 4
-// beams 9 us, 64 of 8 beams 11 (one candidate after the other 9 and 14).
+// beams 9 us, 64 of 8 beams 11 (one candidate after the other 9 and 14); one by one for a request of 64
+// beams at 50257 166.
 __global__ __launch_bounds__(1024) void k_beam_pick(const fie_beam_args a, const BeamWork w, int wanted)
 {
     extern __shared__ uint64_t L[];

@@ -80,7 +80,10 @@ class AdapterBank:
         self.adapters, self.k, self.n, self.rank, self.dtype = adapters, k, n, rank, dtype
         self.rank_pad, self.k_pad = -(-rank // 16) * 16, -(-k // 64) * 64
         self.a = torch.zeros((adapters, self.rank_pad, self.k_pad), dtype=dtype, device=device)
-        # channels that begin at every 128 bytes come in at half the rate (rank 64 in bf16)
+        # Channels that begin at every 128 bytes come in slowly where tiles share them (the second product, us,
+        # with 16 bytes more a channel and without): 4001 x 4096 in bf16 rank 64 37 and 53, 128 138 and 179, 256
+        # 263 and 339; in fp32 rank 32 32 and 35, 64 47 and 53, 256 193 and 239.  250 x 16384 of 64 adapters, each
+        # read once or twice: bf16 36 and 49, 137 and 139, 272 and 278; fp32 35 and 35, 74 and 67, 366 and 293
         size = self.a.element_size()
         self.b_pitch = self.rank_pad + (16 // size if self.rank_pad * size % 128 == 0 else 0)
         self.b = torch.zeros((adapters, n, self.b_pitch), dtype=dtype, device=device)
