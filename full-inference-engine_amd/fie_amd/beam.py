@@ -172,6 +172,9 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor,
         rows = shape[0]
         if n > rows:
             raise ValueError(f"{n} parents of {rows} rows")
+        if s.is_conj() or s.is_neg():               # another's memory, to be read as such
+            s = s.resolve_conj().resolve_neg()
+            held.append(s)
         dense = s.is_contiguous()
         if not dense and rows and not s[0].is_contiguous():
             s, dense = s.contiguous(), True
@@ -180,7 +183,7 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor,
             t = torch.empty_like(s) if dense and n == rows else s.new_empty((n, *shape[1:]))
         else:
             t = out[i]
-            if t.dtype != s.dtype or t.shape != (n, *shape[1:]) or t.get_device() != index:
+            if t.dtype != s.dtype or t.shape != (n, *shape[1:]) or t.get_device() != index or t.is_conj() or t.is_neg():
                 raise ValueError(f"output {i} must be [{n}, ...] as its state")
             if not t.is_contiguous() and n and (not t[0].is_contiguous() or (n > 1 and t.numel() and t.stride(0) < t[0].numel())):
                 raise ValueError("outputs need contiguous rows that do not overlap")

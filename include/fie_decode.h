@@ -64,7 +64,7 @@ size_t fie_beam_workspace_size(const fie_beam_args* args);
 int fie_beam_step(const fie_beam_args* args, void* stream);
 
 /* Rows of up to FIE_MAX_STATES tensors gathered: dst row i is src row parents[i]; a parent
-   outside [0, rows) stands for i.  Outputs do not overlap their inputs.  One call takes fewer
+   outside [0, rows) stands for i.  Outputs have no memory of any input or each other.  One call takes fewer
    than 2^24 pieces of 16 KB, a row of each tensor at least one. */
 #define FIE_MAX_STATES 48
 typedef struct fie_state {
