@@ -295,7 +295,7 @@ class BeamSearch:
         rows = requests * beams
         self._history = (torch.zeros((max_tokens, rows), dtype=torch.int32, device=self.device),
                          torch.zeros((max_tokens, rows), dtype=torch.int32, device=self.device))
-        self._index = self.beams.scores.get_device()
+        self.device, self._index = self.beams.scores.device, self.beams.scores.get_device()
         self._made_on = _raw_stream(self._index)
 
     def _on_stream(self) -> None:
