@@ -195,7 +195,7 @@ class CachePages:
         """Begins with these rows' pages (waits for the device).  Entries past a row's pages are taken as -1;
         rows that share a page have it at the same place."""
         # 64 bits: a cut to 32 could make a page or a length of what is none
-        table, lengths = (t.to(self.device) if t.is_floating_point() else t.to(self.device, torch.int64) for t in (table, lengths))
+        table, lengths = (t.to(self.device, torch.float64 if t.is_floating_point() else torch.int64) for t in (table, lengths))
         if table.shape != self.table.shape or lengths.shape != self.lengths.shape:
             raise ValueError(f"table must be [{self.rows}, {self.max_pages}], lengths [{self.rows}]")
         most = min(self.max_pages * self.page_size, (1 << 31) - 1)

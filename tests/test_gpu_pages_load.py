@@ -38,3 +38,5 @@ def test_lengths_past_31_bits_of_large_pages():
         pool.load(table, torch.tensor([1 << 31]))
     with pytest.raises(ValueError):
         pool.load(table, torch.tensor([float("nan")]))
+    with pytest.raises(ValueError):
+        pool.load(table, torch.tensor([2.0 ** 31]))     # fp32 holds no 2^31 - 1 to compare it with
